@@ -5,12 +5,13 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libkleos_b200.so")
 DRIVER = os.path.join(HERE, "kleos_driver")
-SOURCES = ["kleos_api.cu"]
+SOURCES = ["kleos_api.cu", "operators.cu"]
 
 
 def _newest_source_mtime() -> float:
@@ -26,14 +27,20 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return LIB
     cmd = [
         "nvcc", "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
-        "-shared", "-Xcompiler", "-fPIC", "-ccbin", "g++",
+        "-Xcompiler", "-fPIC", "-ccbin", "g++",
         "-I", "/usr/include",  # nccl.h (types only; the library itself is dlopen'ed)
-        "-o", LIB,
-    ] + [os.path.join(CSRC, s) for s in SOURCES] + ["-ldl"]
+    ]
     if verbose:
-        cmd.insert(1, "-Xptxas")
-        cmd.insert(2, "-v")
-    subprocess.check_call(cmd)
+        cmd[1:1] = ["-Xptxas", "-v"]
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [os.path.join(tmp, s + ".o") for s in SOURCES]
+        running = [subprocess.Popen(cmd + ["-c", os.path.join(CSRC, s), "-o", o]) for s, o in zip(SOURCES, objects)]
+        for p in running:
+            p.wait()
+        for p in running:
+            if p.returncode:
+                raise subprocess.CalledProcessError(p.returncode, p.args)
+        subprocess.check_call(cmd + ["-shared", "-o", LIB] + objects + ["-ldl"])
     return LIB
 
 

@@ -1,0 +1,265 @@
+// The experts' products on the FP32 pipes, for floats and for what the tensor-core kernels cannot load (sizes, strides or
+// addresses that are no multiples of 16 bytes).
+//
+//   kForward  y[r]  = x[r] W[e]^T + b[e]      for the rows r of expert e, offsets[e] <= r < offsets[e + 1]
+//   kDx       dx[r] = dy[r] W[e]
+//   kDw       dW[e] = sum over r of dy[r]^T x[r]
+//
+// A block computes a 128 x 128 tile of one expert, a thread 8 x 8 of it, over slices of 16 that are loaded into registers
+// while the slice before them is multiplied.  Operands are converted when they are loaded, so products and sums are
+// fp32 multiply-adds whatever the type, two at a time (fma.rn.f32x2: half the instructions, the same rounding).
+#pragma once
+
+#include "ops_common.cuh"
+
+namespace kleos {
+namespace experts {
+using namespace ops;
+
+enum Mode { kForward, kDx, kDw };
+
+struct Args {
+    const void *x, *dy, *w, *bias;  // rows [rows][K] and [rows][N], weights [E][N][K]
+    void* out;
+    const int* offsets;
+    long long ldx, ldy, ldo;
+    int rows, E, N, K;
+    bool wide_out;  // dW as floats
+};
+
+// first[e] = tiles of `tile` rows of the experts before e, for e <= E; rows of nobody count as those of expert E, and
+// first[E + 1] is the total.  All threads of the block call it.
+__device__ __forceinline__ void tiles_of_groups(int* first, const int* offsets, int E, int rows, int tile) {
+    if (threadIdx.x < 32) {
+        int at = 0;
+        for (int e0 = 0; e0 <= E; e0 += 32) {
+            const int e = e0 + (int)threadIdx.x;
+            int n = 0;
+            if (e < E) {
+                const Group g = group_rows(offsets, e, rows);
+                n = (g.end - g.begin + tile - 1) / tile;
+            } else if (e == E) {
+                n = (rows - min(max(offsets[E], 0), rows) + tile - 1) / tile;
+            }
+            int upto = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if ((int)threadIdx.x >= o) upto += v;
+            }
+            if (e <= E) {
+                first[e] = at + upto - n;
+                if (e == E) first[E + 1] = at + upto;
+            }
+            at += __shfl_sync(0xffffffffu, upto, 31);
+        }
+    }
+    __syncthreads();
+}
+// The group that tile t belongs to: the last one that begins at or before it.
+__device__ __forceinline__ int group_of_tile(const int* first, int E, int t) {
+    int lo = 0, hi = E;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (first[mid] <= t) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+constexpr int kTile = 128, kSlice = 16, kPitch = kTile + 4;
+
+__device__ __forceinline__ unsigned long long pack2(float a, float b) {
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+
+// Eight elements of an operand for a thread.  kAlong: the slice's direction is the contiguous one in memory (thread
+// t holds 8 of the 16 steps of line t / 2), else the tile's is (thread t holds lines 8 (t % 16).. of step t / 16).
+template <typename T, bool kAlong, int V>
+struct Operand {
+    const T* p;      // line 0 of the tile, step 0
+    long long ld;
+    int lines, steps;  // that exist
+    float v[8];
+    __device__ __forceinline__ void load(int step0) {
+        const int line = kAlong ? threadIdx.x >> 1 : (threadIdx.x & 15) * 8;
+        const int step = step0 + (kAlong ? (threadIdx.x & 1) * 8 : threadIdx.x >> 4);
+        const T* q = p + (kAlong ? line * ld + step : step * ld + line);
+        const int room = kAlong ? (line < lines ? steps - step : 0) : (step < steps ? lines - line : 0);
+#pragma unroll
+        for (int i = 0; i < 8; i += V) {
+            if (i + V <= room) {
+                const auto u = load_vec<T, V>(q + i);
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[i + k] = Elem<T>::to_f(u.v[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[i + k] = 0.f;
+            }
+        }
+    }
+    __device__ __forceinline__ void put(float (*s)[kPitch]) const {
+        if constexpr (kAlong) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[(threadIdx.x & 1) * 8 + i][threadIdx.x >> 1] = v[i];
+        } else {
+            float4* d = reinterpret_cast<float4*>(&s[threadIdx.x >> 4][(threadIdx.x & 15) * 8]);
+            d[0] = make_float4(v[0], v[1], v[2], v[3]);
+            d[1] = make_float4(v[4], v[5], v[6], v[7]);
+        }
+    }
+};
+
+// V: elements of a load, 16 bytes' worth where every row begins on such a boundary and is a multiple of it, else 1.
+template <typename T, int kMode, int V>
+__global__ void __launch_bounds__(256, 2) product_kernel(Args a) {
+    __shared__ __align__(16) float sa[2][kSlice][kPitch], sb[2][kSlice][kPitch];
+    __shared__ int first[kMaxExperts + 2];
+    pdl_wait();
+    pdl_trigger();
+    const int tid = threadIdx.x;
+    const T *x = static_cast<const T*>(a.x), *dy = static_cast<const T*>(a.dy), *w = static_cast<const T*>(a.w);
+    const int cols = kMode == kForward ? a.N : a.K;  // of the result
+    const int c0 = blockIdx.y * kTile;
+    int e, m0, lines, steps;  // first line of the tile and how many it has; length of the sums
+    long long row0 = 0;
+    if constexpr (kMode == kDw) {
+        e = blockIdx.z;
+        const Group g = group_rows(a.offsets, e, a.rows);
+        row0 = g.begin;
+        steps = g.end - g.begin;
+        m0 = blockIdx.x * kTile;
+        lines = min(kTile, a.N - m0);
+    } else {
+        tiles_of_groups(first, a.offsets, a.E, a.rows, kTile);
+        const int t = blockIdx.x;
+        if (t >= first[a.E + 1]) return;
+        e = group_of_tile(first, a.E, t);
+        Group g;
+        if (e < a.E) g = group_rows(a.offsets, e, a.rows);
+        else g = Group{min(max(a.offsets[a.E], 0), a.rows), a.rows};
+        m0 = g.begin + (t - first[e]) * kTile;
+        lines = min(kTile, g.end - m0);
+        steps = e == a.E ? 0 : kMode == kForward ? a.K : a.N;  // rows of nobody: zeros
+    }
+    const size_t we = (size_t)e * a.N * a.K;
+    constexpr bool kA = kMode != kDw, kB = kMode == kForward;
+    Operand<T, kA, V> A;
+    Operand<T, kB, V> B;
+    A.lines = lines;
+    B.lines = min(kTile, cols - c0);
+    A.steps = B.steps = steps;
+    if constexpr (kMode == kForward) {
+        A.p = x + m0 * a.ldx;
+        A.ld = a.ldx;
+        B.p = w + we + (size_t)c0 * a.K;
+        B.ld = a.K;
+    } else if constexpr (kMode == kDx) {
+        A.p = dy + m0 * a.ldy;
+        A.ld = a.ldy;
+        B.p = w + we + c0;
+        B.ld = a.K;
+    } else {
+        A.p = dy + row0 * a.ldy + m0;
+        A.ld = a.ldy;
+        B.p = x + row0 * a.ldx + c0;
+        B.ld = a.ldx;
+    }
+    const int ty = tid >> 4, tx = tid & 15;  // lines 4 ty.. and 64 + 4 ty.., columns likewise
+    unsigned long long acc[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = 0;
+    A.load(0);
+    B.load(0);
+    A.put(sa[0]);
+    B.put(sb[0]);
+    __syncthreads();
+    int now = 0;
+    for (int s = 0; s < steps; s += kSlice, now ^= 1) {
+        const bool more = s + kSlice < steps;
+        if (more) {
+            A.load(s + kSlice);
+            B.load(s + kSlice);
+        }
+#pragma unroll
+        for (int k = 0; k < kSlice; ++k) {
+            float4 u[2];
+            ulonglong2 v[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                u[h] = *reinterpret_cast<const float4*>(&sa[now][k][64 * h + 4 * ty]);
+                v[h] = *reinterpret_cast<const ulonglong2*>(&sb[now][k][64 * h + 4 * tx]);
+            }
+            const float f[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
+            const unsigned long long g[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const unsigned long long ff = pack2(f[i], f[i]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[i][j]) : "l"(ff), "l"(g[j]));
+            }
+        }
+        if (more) {
+            A.put(sa[now ^ 1]);
+            B.put(sb[now ^ 1]);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int line = (i < 4 ? 0 : 60) + 4 * ty + i;
+        if (line >= lines) continue;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int c = c0 + (j < 4 ? 0 : 60) + 4 * tx + j;
+            if (c >= cols) continue;
+            float2 p;
+            asm("mov.b64 {%0, %1}, %2;" : "=f"(p.x), "=f"(p.y) : "l"(acc[i][j >> 1]));
+            float v = j & 1 ? p.y : p.x;
+            if (kMode == kForward && a.bias && e < a.E) v += Elem<T>::to_f(static_cast<const T*>(a.bias)[(size_t)e * a.N + c]);
+            const size_t at = kMode == kDw ? we + (size_t)(m0 + line) * a.K + c : (size_t)(m0 + line) * a.ldo + c;
+            if (kMode == kDw && a.wide_out) static_cast<float*>(a.out)[at] = v;
+            else static_cast<T*>(a.out)[at] = Elem<T>::from_f(v);
+        }
+    }
+}
+
+// db[e] = sum of the rows of dy of expert e.  A block sums 64 columns of an expert: 32 rows at a time, 8 columns a
+// thread, then over the 32 partial sums in their order.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) bias_kernel(Args a) {
+    __shared__ float s[32][65];
+    pdl_wait();
+    pdl_trigger();
+    const int e = blockIdx.y, c = blockIdx.x * 64 + (threadIdx.x & 7) * 8, part = threadIdx.x >> 3;
+    const Group g = group_rows(a.offsets, e, a.rows);
+    float v[8] = {};
+    for (long long r = g.begin + part; r < g.end; r += 32) {
+        const T* p = static_cast<const T*>(a.dy) + r * a.ldy + c;
+#pragma unroll
+        for (int i = 0; i < 8; i += V)
+            if (c + i < a.N) {
+                const auto u = load_vec<T, V>(p + i);
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[i + k] += Elem<T>::to_f(u.v[k]);
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[part][(threadIdx.x & 7) * 8 + i] = v[i];
+    __syncthreads();
+    const int col = blockIdx.x * 64 + threadIdx.x;
+    if (threadIdx.x < 64 && col < a.N) {
+        float t = s[0][threadIdx.x];
+        for (int k = 1; k < 32; ++k) t += s[k][threadIdx.x];
+        const size_t at = (size_t)e * a.N + col;
+        if (a.wide_out) static_cast<float*>(a.out)[at] = t;
+        else static_cast<T*>(a.out)[at] = Elem<T>::from_f(t);
+    }
+}
+
+}  // namespace experts
+}  // namespace kleos

@@ -1,0 +1,301 @@
+// C ABI of the operators around the experts: layer norm, the sort of tokens by expert with the rows there and back, and
+// the experts' products over the sorted rows, each with its gradients.  No counterpart in the reference, whose layer is
+// one fused forward.  None of them needs kleos_initialize, allocates, synchronises or keeps anything between calls.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <initializer_list>
+#include <type_traits>
+
+#include "expert_simt.cuh"
+#include "layer_norm.cuh"
+#include "sort_tokens.cuh"
+
+namespace kleos {
+namespace {
+using namespace ops;
+
+size_t bytes_of(int torch_dtype) { return torch_dtype == 0 ? 4 : 2; }
+bool known_type(int torch_dtype) { return torch_dtype == 0 || torch_dtype == 2 || torch_dtype == 3; }
+constexpr char kTypes[] = "torch_dtype must be 0 (float), 2 (bf16) or 3 (fp16)";
+
+// Whether every pointer (null ones too) is where an element of so many bytes may be.
+bool whole(size_t bytes, std::initializer_list<const void*> ptrs) {
+    for (const void* p : ptrs)
+        if (!aligned(p, bytes)) return false;
+    return true;
+}
+constexpr char kWhole[] = "a device pointer is no multiple of its element's size";
+
+// Whether all of it can be moved 16 bytes at a time.
+bool by_16(size_t elem, std::initializer_list<const void*> ptrs, std::initializer_list<long long> elems) {
+    for (const void* p : ptrs)
+        if (!aligned(p, 16)) return false;
+    for (const long long n : elems)
+        if (n * (long long)elem % 16) return false;
+    return true;
+}
+
+// ---------------------------------------------------------------- layer norm
+template <typename T>
+cudaError_t norm_forward(const norm::Args& a, cudaStream_t st) {
+    const int sms = sm_count();
+    cudaError_t rc = cudaSuccess;
+    auto run = [&](auto v, auto g, auto n) {
+        constexpr int V = decltype(v)::value, G = decltype(g)::value, N = decltype(n)::value;
+        constexpr int kThreads = G > 256 ? G : 256, per = kThreads / G;
+        const int blocks = std::min((a.rows + per - 1) / per, sms * (2048 / kThreads));
+        rc = launch(norm::forward_kernel<T, V, G, N>, dim3(blocks), kThreads, 0, 1, st, a);
+    };
+    constexpr int W = 16 / sizeof(T);
+    using std::integral_constant;
+    const bool wide = by_16(sizeof(T), {a.x, a.y}, {a.ldx, a.ldy, a.H});
+    const bool done = wide ? norm::with_shape<W>(a.H, [&](auto g, auto n) { run(integral_constant<int, W>(), g, n); })
+                           : norm::with_shape<1>(a.H, [&](auto g, auto n) { run(integral_constant<int, 1>(), g, n); });
+    if (!done) rc = launch(norm::forward_long_kernel<T>, dim3(std::min(a.rows, sms * 2)), 1024, 0, 1, st, a);
+    return rc;
+}
+
+template <typename T>
+cudaError_t norm_backward(const norm::Args& a, cudaStream_t st) {
+    const int sms = sm_count();
+    cudaError_t rc = cudaSuccess;
+    int partials = 0;
+    auto run = [&](auto v, auto g, auto n) {
+        constexpr int V = decltype(v)::value, G = decltype(g)::value, N = decltype(n)::value;
+        constexpr int kThreads = G > 256 ? G : 256, per = kThreads / G;
+        partials = std::min((a.rows + per - 1) / per, std::min(2 * sms, norm::kMaxPartials));
+        const size_t smem = G == 32 ? sizeof(float) * 2 * a.H : 0;
+        rc = launch(norm::backward_kernel<T, V, G, N>, dim3(partials), kThreads, smem, 1, st, a);
+    };
+    if (a.rows > 0) {
+        constexpr int W = 16 / sizeof(T);
+        using std::integral_constant;
+        const bool wide = by_16(sizeof(T), {a.x, a.dy, a.dx}, {a.ldx, a.lddy, a.lddx, a.H});
+        const bool done = wide ? norm::with_shape<W>(a.H, [&](auto g, auto n) { run(integral_constant<int, W>(), g, n); })
+                               : norm::with_shape<1>(a.H, [&](auto g, auto n) { run(integral_constant<int, 1>(), g, n); });
+        if (!done) {
+            rc = launch(norm::backward_long_kernel<T>, dim3(std::min(a.rows, sms * 2)), 1024, 0, 1, st, a);
+            partials = std::min(a.rows, norm::kMaxPartials);
+            if (rc == cudaSuccess && a.partial)
+                rc = launch(norm::column_kernel<T>, dim3((a.H + 255) / 256, partials), 256, 0, 1, st, a);
+        }
+    }
+    if (rc == cudaSuccess && a.partial) rc = launch(norm::finish_kernel<T>, dim3((2 * a.H + 31) / 32), 256, 0, 1, st, a, partials);
+    return rc;
+}
+
+// ---------------------------------------------------------------- sort, gather, combine
+template <template <typename, int> class Kernel>
+int move_rows(const char* call, const sorting::Move& m, int torch_dtype, std::initializer_list<const void*> ptrs, cudaStream_t st) {
+    return with_type(call, torch_dtype, [&](auto* null) {
+        using T = std::remove_pointer_t<decltype(null)>;
+        constexpr int W = 16 / sizeof(T);
+        const int grid = (int)std::min<long long>(std::max(m.T, 1), 148 * 64);
+        if (by_16(sizeof(T), ptrs, {m.ld, m.H})) return finish(call, launch(Kernel<T, W>::get(), dim3(grid), 256, 0, 1, st, m));
+        return finish(call, launch(Kernel<T, 1>::get(), dim3(grid), 256, 0, 1, st, m));
+    });
+}
+template <typename T, int V>
+struct Gather {
+    static auto get() { return sorting::gather_kernel<T, V>; }
+};
+template <typename T, int V>
+struct Combine {
+    static auto get() { return sorting::combine_kernel<T, V>; }
+};
+template <typename T, int V>
+struct CombineBack {
+    static auto get() { return sorting::combine_back_kernel<T, V>; }
+};
+
+const char* bad_places(int T, int K, int H, long long ld) {
+    if (T < 0 || K < 1 || K > kMaxTopK || (long long)T * K > 0x7fffff00LL) return "T must be 0 or more, K from 1 to 8, T * K below 2^31";
+    if (H < 1 || ld < H) return "H must be 1 or more, and no row longer than its stride";
+    return nullptr;
+}
+
+// ---------------------------------------------------------------- products
+template <int kMode>
+int products_simt(const char* call, const experts::Args& a, int torch_dtype, cudaStream_t st) {
+    return with_type(call, torch_dtype, [&](auto* null) {
+        using T = std::remove_pointer_t<decltype(null)>;
+        constexpr int W = 16 / sizeof(T);
+        const int tile = experts::kTile, cols = kMode == experts::kForward ? a.N : a.K;
+        const dim3 grid = kMode == experts::kDw ? dim3((a.N + tile - 1) / tile, (cols + tile - 1) / tile, a.E)
+                                                : dim3(a.rows / tile + a.E + 1, (cols + tile - 1) / tile);
+        const bool wide = by_16(sizeof(T), {a.x, a.dy, a.w}, {a.ldx, a.ldy, a.N, a.K});
+        if (wide) return finish(call, launch(experts::product_kernel<T, kMode, W>, grid, 256, 0, 1, st, a));
+        return finish(call, launch(experts::product_kernel<T, kMode, 1>, grid, 256, 0, 1, st, a));
+    });
+}
+
+const char* bad_products(int rows, int E, int N, int K, long long ld_n, long long ld_k) {
+    if (rows < 0 || rows > 0x7fff0000 || E < 1 || E > kMaxExperts) return "rows must be 0 or more, E from 1 to 1024";
+    if (N < 1 || K < 1 || N > 1 << 22 || K > 1 << 22) return "N and K must be from 1 to 2^22";
+    if (ld_n < N || ld_k < K) return "no row may be longer than its stride";
+    return nullptr;
+}
+
+}  // namespace
+}  // namespace kleos
+
+using namespace kleos;
+
+extern "C" {
+
+long long kleos_layer_norm_workspace(int H) { return H < 1 ? KLEOS_E_ARG : (long long)norm::kMaxPartials * 2 * H * (long long)sizeof(float); }
+
+int kleos_layer_norm(const void* x, long long ldx, const void* weight, const void* bias, int rows, int H, float eps,
+                     int torch_dtype, int param_dtype, void* y, long long ldy, float* mean, float* rstd, void* stream) {
+    const char* call = "kleos_layer_norm";
+    if (!known_type(torch_dtype)) return refuse(call, KLEOS_E_UNSUPPORTED, kTypes);
+    if (param_dtype != 0 && param_dtype != torch_dtype) return refuse(call, KLEOS_E_UNSUPPORTED, "param_dtype must be 0 (float) or the element type");
+    if (rows < 0 || H < 1 || ldx < H || ldy < H) return refuse(call, KLEOS_E_ARG, "rows must be 0 or more, H 1 or more, and no row longer than its stride");
+    if (!(eps >= 0.f)) return refuse(call, KLEOS_E_ARG, "eps must not be negative");
+    if (rows == 0) return KLEOS_OK;
+    if (!x || !y) return refuse(call, KLEOS_E_ARG, "null device pointer");
+    if (!whole(bytes_of(torch_dtype), {x, y}) || !whole(bytes_of(param_dtype), {weight, bias}) || !whole(4, {mean, rstd})) return refuse(call, KLEOS_E_ARG, kWhole);
+    if (!sm_count()) return refuse(call, KLEOS_E_CUDA, "no current CUDA device");
+    norm::Args a{};
+    a.x = x; a.weight = weight; a.bias = bias; a.y = y; a.mean = mean; a.rstd = rstd;
+    a.ldx = ldx; a.ldy = ldy; a.rows = rows; a.H = H; a.wide = param_dtype == 0; a.eps = eps;
+    return with_type(call, torch_dtype, [&](auto* null) { return finish(call, norm_forward<std::remove_pointer_t<decltype(null)>>(a, stream_of(stream))); });
+}
+
+int kleos_layer_norm_backward(const void* dy, long long lddy, const void* x, long long ldx, const void* weight, const float* mean,
+                              const float* rstd, int rows, int H, int torch_dtype, int param_dtype, void* dx, long long lddx,
+                              void* dweight, void* dbias, void* workspace, long long workspace_bytes, void* stream) {
+    const char* call = "kleos_layer_norm_backward";
+    if (!known_type(torch_dtype)) return refuse(call, KLEOS_E_UNSUPPORTED, kTypes);
+    if (param_dtype != 0 && param_dtype != torch_dtype) return refuse(call, KLEOS_E_UNSUPPORTED, "param_dtype must be 0 (float) or the element type");
+    if (rows < 0 || H < 1 || ldx < H || lddy < H || lddx < H) return refuse(call, KLEOS_E_ARG, "rows must be 0 or more, H 1 or more, and no row longer than its stride");
+    if (rows > 0 && (!dy || !x || !mean || !rstd || !dx)) return refuse(call, KLEOS_E_ARG, "null device pointer");
+    const bool sums = dweight || dbias;
+    if (sums && (!workspace || !aligned(workspace, 16) || workspace_bytes < kleos_layer_norm_workspace(H)))
+        return refuse(call, KLEOS_E_ARG, "dweight and dbias need a 16-byte aligned workspace of kleos_layer_norm_workspace(H) bytes");
+    if (!whole(bytes_of(torch_dtype), {dy, x, dx}) || !whole(bytes_of(param_dtype), {weight, dweight, dbias}) || !whole(4, {mean, rstd})) return refuse(call, KLEOS_E_ARG, kWhole);
+    if (!sm_count()) return refuse(call, KLEOS_E_CUDA, "no current CUDA device");
+    norm::Args a{};
+    a.x = x; a.dy = dy; a.weight = weight; a.dx = dx; a.dweight = dweight; a.dbias = dbias;
+    a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
+    a.partial = sums ? static_cast<float*>(workspace) : nullptr;
+    a.ldx = ldx; a.lddy = lddy; a.lddx = lddx; a.rows = rows; a.H = H; a.wide = param_dtype == 0;
+    return with_type(call, torch_dtype, [&](auto* null) { return finish(call, norm_backward<std::remove_pointer_t<decltype(null)>>(a, stream_of(stream))); });
+}
+
+int kleos_sort_tokens(const int32_t* topk, int T, int K, int E, int32_t* offsets, int32_t* row_of, int32_t* source, void* stream) {
+    const char* call = "kleos_sort_tokens";
+    if (const char* bad = bad_places(T, K, 1, 1)) return refuse(call, KLEOS_E_ARG, bad);
+    if (E < 1 || E > kMaxExperts) return refuse(call, KLEOS_E_ARG, "E must be from 1 to 1024");
+    if (!offsets || (T > 0 && (!topk || !row_of))) return refuse(call, KLEOS_E_ARG, "null device pointer");
+    if (!whole(4, {topk, offsets, row_of, source})) return refuse(call, KLEOS_E_ARG, kWhole);
+    if (!sm_count()) return refuse(call, KLEOS_E_CUDA, "no current CUDA device");
+    const size_t smem = sizeof(int) * sorting::kWarps * E;
+    cudaError_t rc = smem > 32768 ? cudaFuncSetAttribute(sorting::sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
+    const int cluster = (long long)T * K <= 4096 ? 1 : sorting::kCluster;
+    if (rc == cudaSuccess) rc = launch(sorting::sort_kernel, dim3(cluster), sorting::kThreads, smem, cluster, stream_of(stream), topk, T * K, E, offsets, row_of, source);
+    return finish(call, rc);
+}
+
+int kleos_gather_tokens(const void* x, long long ldx, const int32_t* row_of, const int32_t* offsets, int T, int K, int E, int H,
+                        int torch_dtype, void* rows, void* stream) {
+    const char* call = "kleos_gather_tokens";
+    if (!known_type(torch_dtype)) return refuse(call, KLEOS_E_UNSUPPORTED, kTypes);
+    if (const char* bad = bad_places(T, K, H, ldx)) return refuse(call, KLEOS_E_ARG, bad);
+    if (E < 1 || E > kMaxExperts) return refuse(call, KLEOS_E_ARG, "E must be from 1 to 1024");
+    if (T == 0) return KLEOS_OK;
+    if (!x || !row_of || !offsets || !rows) return refuse(call, KLEOS_E_ARG, "null device pointer");
+    if (!whole(bytes_of(torch_dtype), {x, rows}) || !whole(4, {row_of, offsets})) return refuse(call, KLEOS_E_ARG, kWhole);
+    if (!sm_count()) return refuse(call, KLEOS_E_CUDA, "no current CUDA device");
+    sorting::Move m{};
+    m.from = x; m.to = rows; m.row_of = row_of; m.offsets = offsets; m.ld = ldx; m.T = T; m.K = K; m.E = E; m.H = H; m.n = T * K;
+    return move_rows<Gather>(call, m, torch_dtype, {x, rows}, stream_of(stream));
+}
+
+int kleos_combine_tokens(const void* rows, const int32_t* row_of, const float* weights, int T, int K, int H, int torch_dtype,
+                         void* out, long long ldo, void* stream) {
+    const char* call = "kleos_combine_tokens";
+    if (!known_type(torch_dtype)) return refuse(call, KLEOS_E_UNSUPPORTED, kTypes);
+    if (const char* bad = bad_places(T, K, H, ldo)) return refuse(call, KLEOS_E_ARG, bad);
+    if (T == 0) return KLEOS_OK;
+    if (!rows || !row_of || !out) return refuse(call, KLEOS_E_ARG, "null device pointer");
+    if (!whole(bytes_of(torch_dtype), {rows, out}) || !whole(4, {row_of, weights})) return refuse(call, KLEOS_E_ARG, kWhole);
+    if (!sm_count()) return refuse(call, KLEOS_E_CUDA, "no current CUDA device");
+    sorting::Move m{};
+    m.from = rows; m.to = out; m.row_of = row_of; m.weights = weights; m.ld = ldo; m.T = T; m.K = K; m.H = H; m.n = T * K;
+    return move_rows<Combine>(call, m, torch_dtype, {rows, out}, stream_of(stream));
+}
+
+int kleos_combine_tokens_backward(const void* dout, long long ldd, const void* rows, const int32_t* row_of, const float* weights,
+                                  const int32_t* offsets, int T, int K, int E, int H, int torch_dtype, void* drows,
+                                  float* dweights, void* stream) {
+    const char* call = "kleos_combine_tokens_backward";
+    if (!known_type(torch_dtype)) return refuse(call, KLEOS_E_UNSUPPORTED, kTypes);
+    if (const char* bad = bad_places(T, K, H, ldd)) return refuse(call, KLEOS_E_ARG, bad);
+    if (E < 1 || E > kMaxExperts) return refuse(call, KLEOS_E_ARG, "E must be from 1 to 1024");
+    if (T == 0) return KLEOS_OK;
+    if (!dout || !rows || !row_of || !offsets || !drows) return refuse(call, KLEOS_E_ARG, "null device pointer");
+    if (!whole(bytes_of(torch_dtype), {dout, rows, drows}) || !whole(4, {row_of, weights, offsets, dweights})) return refuse(call, KLEOS_E_ARG, kWhole);
+    if (!sm_count()) return refuse(call, KLEOS_E_CUDA, "no current CUDA device");
+    sorting::Move m{};
+    m.from = dout; m.other = rows; m.to = drows; m.row_of = row_of; m.offsets = offsets; m.weights = weights; m.dweights = dweights;
+    m.ld = ldd; m.T = T; m.K = K; m.E = E; m.H = H; m.n = T * K;
+    return move_rows<CombineBack>(call, m, torch_dtype, {dout, rows, drows}, stream_of(stream));
+}
+
+int kleos_expert_products(const void* x, long long ldx, const int32_t* offsets, const void* w, const void* bias, int rows, int E,
+                          int N, int K, int torch_dtype, void* y, long long ldy, void* stream) {
+    const char* call = "kleos_expert_products";
+    if (!known_type(torch_dtype)) return refuse(call, KLEOS_E_UNSUPPORTED, kTypes);
+    if (const char* bad = bad_products(rows, E, N, K, ldy, ldx)) return refuse(call, KLEOS_E_ARG, bad);
+    if (rows == 0) return KLEOS_OK;
+    if (!x || !offsets || !w || !y) return refuse(call, KLEOS_E_ARG, "null device pointer");
+    if (!whole(bytes_of(torch_dtype), {x, w, bias, y}) || !whole(4, {offsets})) return refuse(call, KLEOS_E_ARG, kWhole);
+    if (!sm_count()) return refuse(call, KLEOS_E_CUDA, "no current CUDA device");
+    experts::Args a{};
+    a.x = x; a.w = w; a.bias = bias; a.out = y; a.offsets = offsets; a.ldx = ldx; a.ldo = ldy; a.rows = rows; a.E = E; a.N = N; a.K = K;
+    return products_simt<experts::kForward>(call, a, torch_dtype, stream_of(stream));
+}
+
+int kleos_expert_products_dx(const void* dy, long long lddy, const int32_t* offsets, const void* w, int rows, int E, int N, int K,
+                             int torch_dtype, void* dx, long long lddx, void* stream) {
+    const char* call = "kleos_expert_products_dx";
+    if (!known_type(torch_dtype)) return refuse(call, KLEOS_E_UNSUPPORTED, kTypes);
+    if (const char* bad = bad_products(rows, E, N, K, lddy, lddx)) return refuse(call, KLEOS_E_ARG, bad);
+    if (rows == 0) return KLEOS_OK;
+    if (!dy || !offsets || !w || !dx) return refuse(call, KLEOS_E_ARG, "null device pointer");
+    if (!whole(bytes_of(torch_dtype), {dy, w, dx}) || !whole(4, {offsets})) return refuse(call, KLEOS_E_ARG, kWhole);
+    if (!sm_count()) return refuse(call, KLEOS_E_CUDA, "no current CUDA device");
+    experts::Args a{};
+    a.dy = dy; a.w = w; a.out = dx; a.offsets = offsets; a.ldy = lddy; a.ldo = lddx; a.rows = rows; a.E = E; a.N = N; a.K = K;
+    return products_simt<experts::kDx>(call, a, torch_dtype, stream_of(stream));
+}
+
+int kleos_expert_products_dw(const void* dy, long long lddy, const void* x, long long ldx, const int32_t* offsets, int rows, int E,
+                             int N, int K, int torch_dtype, int grad_dtype, void* dw, void* dbias, void* stream) {
+    const char* call = "kleos_expert_products_dw";
+    if (!known_type(torch_dtype)) return refuse(call, KLEOS_E_UNSUPPORTED, kTypes);
+    if (grad_dtype != 0 && grad_dtype != torch_dtype) return refuse(call, KLEOS_E_UNSUPPORTED, "grad_dtype must be 0 (float) or the element type");
+    if (const char* bad = bad_products(rows, E, N, K, lddy, ldx)) return refuse(call, KLEOS_E_ARG, bad);
+    if (!offsets || !dw || (rows > 0 && (!x || !dy))) return refuse(call, KLEOS_E_ARG, "null device pointer");
+    if (!whole(bytes_of(torch_dtype), {dy, x}) || !whole(bytes_of(grad_dtype), {dw, dbias}) || !whole(4, {offsets})) return refuse(call, KLEOS_E_ARG, kWhole);
+    if (!sm_count()) return refuse(call, KLEOS_E_CUDA, "no current CUDA device");
+    experts::Args a{};
+    a.dy = dy; a.x = x; a.out = dw; a.offsets = offsets; a.ldy = lddy; a.ldx = ldx; a.rows = rows; a.E = E; a.N = N; a.K = K;
+    a.wide_out = grad_dtype == 0;
+    const cudaStream_t st = stream_of(stream);
+    if (const int rc = products_simt<experts::kDw>(call, a, torch_dtype, st)) return rc;
+    if (!dbias) return KLEOS_OK;
+    a.out = dbias;
+    return with_type(call, torch_dtype, [&](auto* null) {
+        using T = std::remove_pointer_t<decltype(null)>;
+        constexpr int W = 16 / sizeof(T);
+        const dim3 grid((N + 63) / 64, E);
+        if (by_16(sizeof(T), {dy}, {lddy, N})) return finish(call, launch(experts::bias_kernel<T, W>, grid, 256, 0, 1, st, a));
+        return finish(call, launch(experts::bias_kernel<T, 1>, grid, 256, 0, 1, st, a));
+    });
+}
+
+}  // extern "C"

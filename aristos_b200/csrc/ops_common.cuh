@@ -1,0 +1,107 @@
+// What the operators around the experts share (layer norm, sort by expert, rows there and back, products): vectors of
+// elements, sums over a warp, launches, refusals.
+#pragma once
+
+#include <cstdio>
+
+#include "common.cuh"
+
+namespace kleos {
+namespace ops {
+
+constexpr int kMaxExperts = 1024;  // experts of a sort or of products
+
+// N elements that are loaded and stored at once.
+template <typename T, int N>
+struct __align__(sizeof(T) * N) Vec {
+    T v[N];
+};
+
+// No read-only path here either: the kernel in front may still be writing what its successor's blocks wait for.
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> load_vec(const T* p) {
+    return *reinterpret_cast<const Vec<T, N>*>(p);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& v) {
+    *reinterpret_cast<Vec<T, N>*>(p) = v;
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// Offsets come from the caller's device memory, so no kernel trusts them: rows outside [0, rows) do not exist.
+struct Group {
+    int begin, end;
+};
+__device__ __forceinline__ Group group_rows(const int* offsets, int e, int rows) {
+    Group g;
+    g.begin = min(max(offsets[e], 0), rows);
+    g.end = max(min(offsets[e + 1], rows), g.begin);
+    return g;
+}
+
+inline int refuse(const char* call, int code, const char* what) {
+    std::fprintf(stderr, "[kleos_b200] %s: %s\n", call, what);
+    return code;
+}
+
+inline bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+inline cudaStream_t stream_of(void* stream) { return stream ? static_cast<cudaStream_t>(stream) : cudaStreamPerThread; }
+
+// Launched as the kernels of a forward are (see pdl_wait()): every kernel here calls pdl_wait() before it touches
+// global memory.
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st, const A&... args) {
+    cudaLaunchConfig_t lc{};
+    lc.gridDim = grid;
+    lc.blockDim = dim3((unsigned)threads);
+    lc.dynamicSmemBytes = smem;
+    lc.stream = st;
+    cudaLaunchAttribute at[2] = {};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    lc.attrs = at;
+    lc.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&lc, kernel, args...);
+}
+
+inline int finish(const char* call, cudaError_t e) {
+    if (e == cudaSuccess) return KLEOS_OK;
+    cudaGetLastError();  // (a refused launch is reported here and not to a later call)
+    std::fprintf(stderr, "[kleos_b200] %s: launch failed: %s\n", call, cudaGetErrorString(e));
+    return KLEOS_E_CUDA;
+}
+
+// Multiprocessors of the current device, 0 when there is none.
+inline int sm_count() {
+    static int known[64] = {};
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return 0;
+    if (dev < 64 && known[dev]) return known[dev];
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    if (dev < 64) known[dev] = n;
+    return n;
+}
+
+// Calls f with a null pointer of the element type of `torch_dtype` (0 float, 2 bf16, 3 fp16).
+template <typename F>
+int with_type(const char* call, int torch_dtype, F f) {
+    switch (torch_dtype) {
+        case 0: return f(static_cast<float*>(nullptr));
+        case 2: return f(static_cast<__nv_bfloat16*>(nullptr));
+        case 3: return f(static_cast<__half*>(nullptr));
+        default: return refuse(call, KLEOS_E_UNSUPPORTED, "torch_dtype must be 0 (float), 2 (bf16) or 3 (fp16)");
+    }
+}
+
+}  // namespace ops
+}  // namespace kleos

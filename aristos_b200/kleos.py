@@ -27,7 +27,10 @@ EXPORTS = (
     "kleos_forward", "kleos_forward_bench", "kleos_forward_host", "kleos_forward_host_async",
     "kleos_host_sync", "kleos_get_rank",
     "kleos_local_experts", "kleos_get_info", "kleos_last_status", "kleos_clear_status", "kleos_debug_routing",
-    "kleos_phase_times", "kleos_flow_timeline", "kleos_debug_flow_stamps", "kleos_debug_flow_stalls", "kleos_debug_tile_order", "kleos_launch_count", "kleos_debug_gemm_stats", "kleos_debug_suppress_return_flag", "kleos_gate_stats", "kleos_plan_placement", "kleos_placement_model", "kleos_route_static", "kleos_finalize", "kleos_error_string",
+    "kleos_phase_times", "kleos_flow_timeline", "kleos_debug_flow_stamps", "kleos_debug_flow_stalls", "kleos_debug_tile_order", "kleos_launch_count", "kleos_debug_gemm_stats", "kleos_debug_suppress_return_flag", "kleos_gate_stats", "kleos_plan_placement", "kleos_placement_model", "kleos_route_static",
+    "kleos_layer_norm", "kleos_layer_norm_workspace", "kleos_layer_norm_backward", "kleos_sort_tokens", "kleos_gather_tokens",
+    "kleos_combine_tokens", "kleos_combine_tokens_backward", "kleos_expert_products", "kleos_expert_products_dx",
+    "kleos_expert_products_dw", "kleos_finalize", "kleos_error_string",
 )
 
 PHASE_NAMES = ("route", "slots", "dispatch", "plan", "gemm1", "gemm2", "combine", "total")
@@ -50,6 +53,15 @@ class LayerInfo(ctypes.Structure):
                  "torch_dtype", "hidden_act", "elem_bytes")] + \
                [("input_elems", ctypes.c_int64), ("output_elems", ctypes.c_int64)]
 
+
+# argument types of the operators around the experts: p pointer, l long long, i int, f float
+_C = dict(p=ctypes.c_void_p, l=ctypes.c_longlong, i=ctypes.c_int, f=ctypes.c_float)
+_OPERATOR_ARGS = {
+    "kleos_layer_norm_workspace": "i", "kleos_layer_norm": "plppiifiiplppp", "kleos_layer_norm_backward": "plplpppiiiiplppplp",
+    "kleos_sort_tokens": "piiipppp", "kleos_gather_tokens": "plppiiiiipp", "kleos_combine_tokens": "pppiiiiplp",
+    "kleos_combine_tokens_backward": "plppppiiiiippp", "kleos_expert_products": "plpppiiiiiplp",
+    "kleos_expert_products_dx": "plppiiiiiplp", "kleos_expert_products_dw": "plplpiiiiiippp",
+}
 
 _lib = None
 
@@ -75,6 +87,9 @@ def load_library() -> ctypes.CDLL:
         lib.kleos_gate_stats.argtypes = [ctypes.c_void_p] * 3
         lib.kleos_phase_times.argtypes = [ctypes.POINTER(ctypes.c_float), ctypes.c_int]
         lib.kleos_get_unique_id.argtypes = [ctypes.c_void_p]
+        lib.kleos_layer_norm_workspace.restype = ctypes.c_longlong
+        for name, args in _OPERATOR_ARGS.items():
+            getattr(lib, name).argtypes = [_C[c] for c in args]
         _lib = lib
     return _lib
 
@@ -205,6 +220,238 @@ def route_static(A, Wg, gate_bias, S, H, E, K, torch_dtype, probs, topk, mcw, st
     _check(lib.kleos_route_static(_ptr(A), _ptr(Wg), _ptr(gate_bias), S, H, E, K, torch_dtype,
                                   _ptr(probs), _ptr(topk), _ptr(mcw), stream),
            "kleos_route_static")
+
+
+# ---------------------------------------------------------------------------- operators around the experts
+# Arguments are torch tensors on one GPU; sizes and row strides are read from them, and what does not fit together raises
+# KleosError (KLEOS_E_ARG, or KLEOS_E_UNSUPPORTED for an element type) before anything is launched.  They run on
+# `stream` (a cudaStream_t; None is the per-thread default stream, which other streams of the program do not wait for:
+# pass the stream that the tensors are used on).  See include/kleos_b200.h for what each computes.
+_ARG = -8
+_MOST_ROWS = 0x7fff0000  # sizes are C ints
+_codes = {}
+
+
+def _code(t) -> int:
+    if not _codes:
+        import torch
+        _codes.update({torch.float32: 0, torch.bfloat16: 2, torch.float16: 3})
+    return _codes.get(t.dtype, -1)
+
+
+def _require(ok, call: str, what: str) -> None:
+    if not ok:
+        raise KleosError(_ARG, f"{call}: {what}")
+
+
+def _rows(call, name, t, like=None, rows=None, cols=None) -> int:
+    """Row stride of a matrix whose rows are contiguous."""
+    if t.dim() != 2 or t.device.type != "cuda" or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
+        raise KleosError(_ARG, f"{call}: {name} must be a matrix on the GPU" + (f" of {rows} rows" if rows is not None else "") +
+                         (f" of {cols} columns" if cols is not None else ""))
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise KleosError(_ARG, f"{call}: {name} must have the element type and device of the input")
+    rs, cs = t.stride()
+    cols = t.shape[1]
+    _require(t.shape[0] <= _MOST_ROWS and cols <= _MOST_ROWS, call, f"{name} is too large")
+    if cols > 1 and cs != 1:
+        raise KleosError(_ARG, f"{call}: the rows of {name} must be contiguous")
+    if t.shape[0] < 2:
+        return max(cols, 1)
+    if rs < cols:
+        raise KleosError(_ARG, f"{call}: the rows of {name} must not overlap")
+    return rs
+
+
+def _whole(call, name, t, shape, dtypes, device) -> None:
+    if tuple(t.shape) != tuple(shape) or t.dtype not in dtypes or t.device != device or not t.is_contiguous():
+        raise KleosError(_ARG, f"{call}: {name} must be contiguous, of shape {tuple(shape)}, of type "
+                         f"{' or '.join(str(d) for d in dtypes)} and on {device}")
+
+
+def _launch(call, device, *args) -> None:
+    """Calls the entry point with the tensors' device as the current one."""
+    import torch
+    fn = getattr(load_library(), call)
+    if device.index == torch.cuda.current_device():
+        _check(fn(*args), call)
+    else:
+        with torch.cuda.device(device):
+            _check(fn(*args), call)
+
+
+def layer_norm_workspace(H: int) -> int:
+    """Bytes of workspace that layer_norm_backward needs for dweight and dbias."""
+    n = load_library().kleos_layer_norm_workspace(H)
+    if n < 0:
+        _check(n, "kleos_layer_norm_workspace")
+    return n
+
+
+def _params(call, x, named) -> int:
+    import torch
+    given = [(n, t) for n, t in named if t is not None]
+    for n, t in given:
+        _whole(call, n, t, (x.shape[1],), (torch.float32, x.dtype), x.device)
+        _require(t.dtype == given[0][1].dtype, call, "the parameters and their gradients must have one type")
+    return _code(given[0][1]) if given else 0
+
+
+def layer_norm(x, weight, bias, eps, y, mean=None, rstd=None, stream=None) -> None:
+    """y = layer norm of the rows of x; weight and bias may be None; mean and rstd (floats, one a row) are for the
+    backward pass."""
+    import torch
+    call = "kleos_layer_norm"
+    ldx = _rows(call, "x", x)
+    R, H = x.shape
+    ldy = _rows(call, "y", y, x, R, H)
+    code = _params(call, x, (("weight", weight), ("bias", bias)))
+    for n, t in (("mean", mean), ("rstd", rstd)):
+        if t is not None:
+            _whole(call, n, t, (R,), (torch.float32,), x.device)
+    _launch(call, x.device, x.data_ptr(), ldx, _ptr(weight), _ptr(bias), R, H, eps, _code(x), code, y.data_ptr(), ldy, _ptr(mean),
+            _ptr(rstd), stream)
+
+
+def layer_norm_backward(dy, x, weight, mean, rstd, dx, dweight=None, dbias=None, workspace=None, stream=None) -> None:
+    """Gradients of layer_norm.  dweight and dbias need a workspace of layer_norm_workspace(H) bytes."""
+    import torch
+    call = "kleos_layer_norm_backward"
+    ldx = _rows(call, "x", x)
+    R, H = x.shape
+    lddy, lddx = _rows(call, "dy", dy, x, R, H), _rows(call, "dx", dx, x, R, H)
+    code = _params(call, x, (("weight", weight), ("dweight", dweight), ("dbias", dbias)))
+    for n, t in (("mean", mean), ("rstd", rstd)):
+        _whole(call, n, t, (R,), (torch.float32,), x.device)
+    room = 0
+    if workspace is not None:
+        _require(workspace.device == x.device and workspace.is_contiguous(), call, "the workspace must be contiguous and on the input's device")
+        room = workspace.numel() * workspace.element_size()
+    _launch(call, x.device, dy.data_ptr(), lddy, x.data_ptr(), ldx, _ptr(weight), mean.data_ptr(), rstd.data_ptr(), R, H, _code(x),
+            code, dx.data_ptr(), lddx, _ptr(dweight), _ptr(dbias), _ptr(workspace), room, stream)
+
+
+def _ints(call, name, t, shape, device) -> None:
+    import torch
+    _whole(call, name, t, shape, (torch.int32,), device)
+
+
+def _places(call, row_of, device):
+    _require(row_of.dim() == 2, call, "row_of must have a row per token and a column per expert of it")
+    _ints(call, "row_of", row_of, row_of.shape, device)
+    return row_of.shape
+
+
+def _offsets(call, offsets, device) -> int:
+    E = offsets.shape[0] - 1 if offsets.dim() == 1 else 0
+    _require(E >= 1, call, "offsets must have an entry per expert and one more")
+    _ints(call, "offsets", offsets, (E + 1,), device)
+    return E
+
+
+def sort_tokens(topk, num_experts, offsets, row_of, source=None, stream=None) -> None:
+    """Rows of the tokens' experts, sorted by expert: offsets [E + 1], row_of [T, K], source [T * K], all int32."""
+    call = "kleos_sort_tokens"
+    _require(topk.dim() == 2 and topk.device.type == "cuda", call, "topk must be a matrix on the GPU")
+    T, K = topk.shape
+    _ints(call, "topk", topk, (T, K), topk.device)
+    _ints(call, "offsets", offsets, (num_experts + 1,), topk.device)
+    _ints(call, "row_of", row_of, (T, K), topk.device)
+    if source is not None:
+        _ints(call, "source", source, (T * K,), topk.device)
+    _launch(call, topk.device, topk.data_ptr(), T, K, num_experts, offsets.data_ptr(), row_of.data_ptr(), _ptr(source), stream)
+
+
+def _weights(call, name, t, T, K, device) -> None:
+    import torch
+    if t is not None:
+        _whole(call, name, t, (T, K), (torch.float32,), device)
+
+
+def gather_tokens(x, row_of, offsets, rows, stream=None) -> None:
+    """rows[row_of[t, k]] = x[t], zeros from offsets[E] on."""
+    call = "kleos_gather_tokens"
+    ldx = _rows(call, "x", x)
+    T, H = x.shape
+    K = _places(call, row_of, x.device)[1]
+    _require(row_of.shape[0] == T, call, "row_of must have a row per token")
+    E = _offsets(call, offsets, x.device)
+    _whole(call, "rows", rows, (T * K, H), (x.dtype,), x.device)
+    _launch(call, x.device, x.data_ptr(), ldx, row_of.data_ptr(), offsets.data_ptr(), T, K, E, H, _code(x), rows.data_ptr(), stream)
+
+
+def combine_tokens(rows, row_of, weights, out, stream=None) -> None:
+    """out[t] = sum over k of weights[t, k] * rows[row_of[t, k]]; weights None: ones."""
+    call = "kleos_combine_tokens"
+    T, K = _places(call, row_of, rows.device)
+    ldo = _rows(call, "out", out, rows, T)
+    _whole(call, "rows", rows, (T * K, out.shape[1]), (rows.dtype,), rows.device)
+    _weights(call, "weights", weights, T, K, rows.device)
+    _launch(call, rows.device, rows.data_ptr(), row_of.data_ptr(), _ptr(weights), T, K, out.shape[1], _code(rows), out.data_ptr(), ldo,
+            stream)
+
+
+def gather_tokens_backward(drows, row_of, dx, stream=None) -> None:
+    """Gradient of gather_tokens: dx[t] = sum over k of drows[row_of[t, k]]."""
+    combine_tokens(drows, row_of, None, dx, stream)
+
+
+def combine_tokens_backward(dout, rows, row_of, weights, offsets, drows, dweights=None, stream=None) -> None:
+    """Gradients of combine_tokens for the rows (zeros from offsets[E] on) and the weights."""
+    call = "kleos_combine_tokens_backward"
+    ldd = _rows(call, "dout", dout)
+    T, H = dout.shape
+    K = _places(call, row_of, dout.device)[1]
+    _require(row_of.shape[0] == T, call, "row_of must have a row per token")
+    E = _offsets(call, offsets, dout.device)
+    _whole(call, "rows", rows, (T * K, H), (dout.dtype,), dout.device)
+    _whole(call, "drows", drows, (T * K, H), (dout.dtype,), dout.device)
+    _weights(call, "weights", weights, T, K, dout.device)
+    _weights(call, "dweights", dweights, T, K, dout.device)
+    _launch(call, dout.device, dout.data_ptr(), ldd, rows.data_ptr(), row_of.data_ptr(), _ptr(weights), offsets.data_ptr(), T, K, E, H,
+            _code(dout), drows.data_ptr(), _ptr(dweights), stream)
+
+
+def expert_products(x, offsets, w, bias, y, stream=None) -> None:
+    """y[r] = x[r] W[e]^T + bias[e] for the rows of every expert, zeros from offsets[E] on; bias may be None."""
+    call = "kleos_expert_products"
+    ldx = _rows(call, "x", x)
+    R, K = x.shape
+    E = _offsets(call, offsets, x.device)
+    _require(w.dim() == 3, call, "w must be [experts, N, K]")
+    N = w.shape[1]
+    _whole(call, "w", w, (E, N, K), (x.dtype,), x.device)
+    if bias is not None:
+        _whole(call, "bias", bias, (E, N), (x.dtype,), x.device)
+    ldy = _rows(call, "y", y, x, R, N)
+    _launch(call, x.device, x.data_ptr(), ldx, offsets.data_ptr(), w.data_ptr(), _ptr(bias), R, E, N, K, _code(x), y.data_ptr(), ldy, stream)
+
+
+def expert_products_dx(dy, offsets, w, dx, stream=None) -> None:
+    """dx[r] = dy[r] W[e] for the rows of every expert, zeros from offsets[E] on."""
+    call = "kleos_expert_products_dx"
+    lddy = _rows(call, "dy", dy)
+    R, N = dy.shape
+    E = _offsets(call, offsets, dy.device)
+    _require(w.dim() == 3, call, "w must be [experts, N, K]")
+    K = w.shape[2]
+    _whole(call, "w", w, (E, N, K), (dy.dtype,), dy.device)
+    lddx = _rows(call, "dx", dx, dy, R, K)
+    _launch(call, dy.device, dy.data_ptr(), lddy, offsets.data_ptr(), w.data_ptr(), R, E, N, K, _code(dy), dx.data_ptr(), lddx, stream)
+
+
+def expert_products_dw(dy, x, offsets, dw, dbias=None, stream=None) -> None:
+    """dw[e] = sum over the rows of expert e of dy[r]^T x[r], dbias[e] = sum of dy[r]; in the element type or floats."""
+    import torch
+    call = "kleos_expert_products_dw"
+    lddy, ldx = _rows(call, "dy", dy), _rows(call, "x", x, dy, dy.shape[0])
+    (R, N), K = dy.shape, x.shape[1]
+    E = _offsets(call, offsets, dy.device)
+    _whole(call, "dw", dw, (E, N, K), (dy.dtype, torch.float32), dy.device)
+    if dbias is not None:
+        _whole(call, "dbias", dbias, (E, N), (dw.dtype,), dy.device)
+    _launch(call, dy.device, dy.data_ptr(), lddy, x.data_ptr(), ldx, offsets.data_ptr(), R, E, N, K, _code(dy), _code(dw), dw.data_ptr(),
+            _ptr(dbias), stream)
 
 
 FLOW_MILESTONES = ("start", "planned", "first_tile", "last_gemm1_tile", "last_tile", "dispatched",

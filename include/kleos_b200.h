@@ -258,6 +258,76 @@ int kleos_plan_placement(const kleos_placement_request* request, kleos_placement
 int kleos_placement_model(const char* config_json_path, uint32_t* moe_stages, uint32_t* p2p_buffer_mb,
                           uint32_t* grad_buffer_mb);
 
+/* ------------------------------------------------------------------------------------------------
+ * Operators around the experts, for programs that train an MoE block, or serve one whose experts
+ * kleos_forward does not compute: layer norm, the sort of tokens by expert with the rows there and
+ * back, and the experts' products over the sorted rows, each with its gradients.  No counterpart
+ * in the reference, whose layer is one fused forward.
+ *
+ * None of them needs kleos_initialize, allocates, synchronises with the host or keeps anything
+ * from one call to the next, so they may be captured and calls may overlap on different streams.
+ * They run on the current device, asynchronously on `stream` (NULL = per-thread default stream);
+ * every pointer is a DEVICE pointer owned by the caller, and no output may overlap an input.
+ * torch_dtype is 0 (float), 2 (bf16) or 3 (fp16); anything else is KLEOS_E_UNSUPPORTED.  A row
+ * stride (ld...) counts elements and is at least the row's length.  Sums are kept in 32 bits and
+ * rounded once, in a fixed order: the same call gives the same bits.  Where addresses, strides and
+ * lengths are multiples of 16 bytes the kernels move 16 bytes at a time; others are taken too, more slowly. */
+
+/* y = (x - mean) * rstd * weight + bias of every row, rstd = 1 / sqrt(var + eps), var the mean square of
+ * x - mean.  x [rows, H] and y of torch_dtype; weight [H] and bias [H] of param_dtype, 0 (float) or
+ * torch_dtype, NULL for ones and zeros.  mean [rows] and rstd [rows] are floats for the backward pass and
+ * may be NULL. */
+int kleos_layer_norm(const void* x, long long ldx, const void* weight, const void* bias, int rows, int H, float eps,
+                     int torch_dtype, int param_dtype, void* y, long long ldy, float* mean, float* rstd, void* stream);
+
+/* Gradients of kleos_layer_norm: dx [rows, H] of torch_dtype, dweight [H] and dbias [H] of param_dtype (each may be
+ * NULL), from dy and the mean and rstd that the forward pass gave.  dweight and dbias are overwritten (zeros when
+ * rows is 0) and need a 16-byte aligned workspace of kleos_layer_norm_workspace(H) bytes, whose contents do not
+ * matter: 296 partial sums of two rows of floats. */
+long long kleos_layer_norm_workspace(int H);
+int kleos_layer_norm_backward(const void* dy, long long lddy, const void* x, long long ldx, const void* weight,
+                              const float* mean, const float* rstd, int rows, int H, int torch_dtype, int param_dtype,
+                              void* dx, long long lddx, void* dweight, void* dbias, void* workspace,
+                              long long workspace_bytes, void* stream);
+
+/* Where the rows of each expert lie.  topk [T, K] holds the experts of every token (as kleos_route_static gives them);
+ * an id outside 0 .. E - 1 is a place without an expert.
+ *   offsets [E + 1]   rows of expert e: offsets[e] .. offsets[e + 1] - 1; offsets[E] = places with an expert
+ *   row_of [T, K]     row of every place, in the order of the tokens within an expert; -1 without an expert
+ *   source [T * K]    t * K + k of every row, -1 from offsets[E] on; may be NULL
+ * K from 1 to 8, E from 1 to 1024. */
+int kleos_sort_tokens(const int32_t* topk, int T, int K, int E, int32_t* offsets, int32_t* row_of, int32_t* source,
+                      void* stream);
+
+/* rows[row_of[t, k]] = x[t]: rows [T * K, H] sorted by expert, zeros from offsets[E] on. */
+int kleos_gather_tokens(const void* x, long long ldx, const int32_t* row_of, const int32_t* offsets, int T, int K, int E,
+                        int H, int torch_dtype, void* rows, void* stream);
+
+/* out[t] = sum over k of weights[t, k] * rows[row_of[t, k]], places without an expert left out (zeros for a token that
+ * has none).  weights [T, K] are floats; NULL for ones, which makes it the gradient of kleos_gather_tokens. */
+int kleos_combine_tokens(const void* rows, const int32_t* row_of, const float* weights, int T, int K, int H, int torch_dtype,
+                         void* out, long long ldo, void* stream);
+
+/* Gradients of kleos_combine_tokens: drows[row_of[t, k]] = weights[t, k] * dout[t], zeros from offsets[E] on, and
+ * dweights[t, k] = <dout[t], rows[row_of[t, k]]>, 0 without an expert; dweights may be NULL. */
+int kleos_combine_tokens_backward(const void* dout, long long ldd, const void* rows, const int32_t* row_of,
+                                  const float* weights, const int32_t* offsets, int T, int K, int E, int H,
+                                  int torch_dtype, void* drows, float* dweights, void* stream);
+
+/* y[r] = x[r] W[e]^T + bias[e] for the rows r of expert e, offsets[e] <= r < offsets[e + 1]; zeros for rows from
+ * offsets[E] on.  x [rows, K], W [E, N, K], bias [E, N] or NULL, y [rows, N].  offsets is ascending from 0; what it says
+ * beyond `rows` is not read.  E from 1 to 1024. */
+int kleos_expert_products(const void* x, long long ldx, const int32_t* offsets, const void* w, const void* bias, int rows,
+                          int E, int N, int K, int torch_dtype, void* y, long long ldy, void* stream);
+
+/* Gradients of kleos_expert_products: dx[r] = dy[r] W[e], zeros for rows from offsets[E] on; dW[e] = sum over the rows
+ * of expert e of dy[r]^T x[r] and dbias[e] = sum of dy[r], zeros for an expert without rows.  dW [E, N, K] and
+ * dbias [E, N] (or NULL) of grad_dtype, 0 (float) or torch_dtype. */
+int kleos_expert_products_dx(const void* dy, long long lddy, const int32_t* offsets, const void* w, int rows, int E, int N,
+                             int K, int torch_dtype, void* dx, long long lddx, void* stream);
+int kleos_expert_products_dw(const void* dy, long long lddy, const void* x, long long ldx, const int32_t* offsets, int rows,
+                             int E, int N, int K, int torch_dtype, int grad_dtype, void* dw, void* dbias, void* stream);
+
 /* Test hook for the failure path: while on, the expert FFN does not raise its "results
  * returned" flags, so the combine's bounded wait runs out, the forward records
  * {KLEOS_E_DEVICE, KLEOS_AT_COMBINE_WAIT} and returns with the context intact.  Nothing is

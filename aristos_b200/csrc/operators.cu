@@ -9,6 +9,7 @@
 #include <type_traits>
 
 #include "expert_simt.cuh"
+#include "expert_tc.cuh"
 #include "layer_norm.cuh"
 #include "sort_tokens.cuh"
 
@@ -129,6 +130,93 @@ int products_simt(const char* call, const experts::Args& a, int torch_dtype, cud
         if (wide) return finish(call, launch(experts::product_kernel<T, kMode, W>, grid, 256, 0, 1, st, a));
         return finish(call, launch(experts::product_kernel<T, kMode, 1>, grid, 256, 0, 1, st, a));
     });
+}
+
+// Tensor of up to three dimensions (sizes and strides from the innermost, which is contiguous), copied in boxes of 128
+// bytes by `lines` lines, 128-byte swizzle.
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+bool encode(CUtensorMap* map, int torch_dtype, const void* base, int dims, const cuuint64_t* sizes, const long long* strides, int lines) {
+    static const EncodeTiledFn fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(f);
+    }();
+    if (!fn) return false;
+    const size_t elem = bytes_of(torch_dtype);
+    const CUtensorMapDataType type = torch_dtype == 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : torch_dtype == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const cuuint64_t pitch[2] = {(cuuint64_t)strides[0] * elem, dims > 2 ? (cuuint64_t)strides[1] * elem : 0};
+    const cuuint32_t box[3] = {(cuuint32_t)(128 / elem), (cuuint32_t)lines, 1}, one[3] = {1, 1, 1};
+    return fn(map, type, (cuuint32_t)dims, const_cast<void*>(base), sizes, pitch, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool encode_rows(CUtensorMap* map, int torch_dtype, const void* base, int rows, int cols, long long ld, int lines) {
+    const cuuint64_t sizes[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    return encode(map, torch_dtype, base, 2, sizes, &ld, lines);
+}
+bool encode_weights(CUtensorMap* map, int torch_dtype, const void* base, int E, int N, int K, int lines) {
+    const cuuint64_t sizes[3] = {(cuuint64_t)K, (cuuint64_t)N, (cuuint64_t)E};
+    const long long strides[2] = {K, (long long)N * K};
+    return encode(map, torch_dtype, base, 3, sizes, strides, lines);
+}
+
+constexpr long long kWaitCycles = 20000000000LL;  // about ten seconds: nothing but a copy or an MMA is waited for
+
+// Pairs of blocks for so many tiles at most.
+int pair_grid(long long tiles) { return 2 * (int)std::max<long long>(1, std::min<long long>(sm_count() / 2, tiles)); }
+
+template <typename TE, bool kDx>
+int products_tc(const char* call, const experts::Args& a, int torch_dtype, cudaStream_t st) {
+    using namespace experts::tcp;
+    TcArgs g{};
+    g.offsets = a.offsets; g.bias = a.bias; g.out = a.out; g.ldo = a.ldo; g.rows = a.rows; g.E = a.E; g.wait_cycles = kWaitCycles;
+    g.M = kDx ? a.K : a.N;
+    g.len = kDx ? a.N : a.K;
+    RowMaps rows;
+    CUtensorMap w;
+    bool ok = encode_weights(&w, torch_dtype, a.w, a.E, a.N, a.K, kDx ? 64 : 128);
+    for (int i = 0; i < kBoxes; ++i) ok = ok && encode_rows(&rows.box[i], torch_dtype, kDx ? a.dy : a.x, a.rows, g.len, kDx ? a.ldy : a.ldx, box_rows(i));
+    if (!ok) return refuse(call, KLEOS_E_CUDA, "cuTensorMapEncodeTiled failed");
+    static bool done[64];
+    cudaError_t rc = allow_smem(product_tc_kernel<TE, kDx>, done, SMEM_BYTES);
+    const long long tiles = (long long)((g.M + 2 * BM - 1) / (2 * BM)) * (a.rows / 256 + std::min(a.E, a.rows));
+    if (rc == cudaSuccess) rc = launch(product_tc_kernel<TE, kDx>, dim3(pair_grid(tiles)), kThreads, SMEM_BYTES, 1, st, rows, w, g);
+    return finish(call, rc);
+}
+
+template <typename TE, bool kWideOut>
+int weights_tc(const char* call, const experts::Args& a, int torch_dtype, cudaStream_t st) {
+    using namespace experts::tcp;
+    TcArgs g{};
+    g.offsets = a.offsets; g.out = a.out; g.rows = a.rows; g.E = a.E; g.M = a.N; g.len = a.K; g.wait_cycles = kWaitCycles;
+    CUtensorMap dy, x, dw;
+    const bool ok = encode_rows(&dy, torch_dtype, a.dy, a.rows, a.N, a.ldy, BK) && encode_rows(&x, torch_dtype, a.x, a.rows, a.K, a.ldx, BK) &&
+                    encode_weights(&dw, kWideOut ? 0 : torch_dtype, a.out, a.E, a.N, a.K, 32);
+    if (!ok) return refuse(call, KLEOS_E_CUDA, "cuTensorMapEncodeTiled failed");
+    static bool done[64];
+    cudaError_t rc = allow_smem(weight_tc_kernel<TE, kWideOut>, done, wg::SMEM_BYTES);
+    const long long tiles = (long long)a.E * ((a.N + 255) / 256) * ((a.K + 255) / 256);
+    if (rc == cudaSuccess) rc = launch(weight_tc_kernel<TE, kWideOut>, dim3(pair_grid(tiles)), kThreads, wg::SMEM_BYTES, 1, st, dy, x, dw, g);
+    return finish(call, rc);
+}
+
+// The tensor cores' kernels load 16-bit elements by TMA, whose rows begin and end on 16-byte boundaries; floats (whose
+// sums are fp32 multiply-adds) and everything else go to the FP32 pipes.
+template <int kMode>
+int products(const char* call, const experts::Args& a, int torch_dtype, cudaStream_t st) {
+    if (torch_dtype != 0 && a.rows > 0 && by_16(2, {a.x, a.dy, a.w, a.out}, {a.ldx, a.ldy, a.ldo, a.N, a.K})) {
+        if constexpr (kMode != experts::kDw) {
+            return torch_dtype == 2 ? products_tc<__nv_bfloat16, kMode == experts::kDx>(call, a, torch_dtype, st)
+                                    : products_tc<__half, kMode == experts::kDx>(call, a, torch_dtype, st);
+        } else if (a.wide_out) {
+            return torch_dtype == 2 ? weights_tc<__nv_bfloat16, true>(call, a, torch_dtype, st) : weights_tc<__half, true>(call, a, torch_dtype, st);
+        } else {
+            return torch_dtype == 2 ? weights_tc<__nv_bfloat16, false>(call, a, torch_dtype, st) : weights_tc<__half, false>(call, a, torch_dtype, st);
+        }
+    }
+    return products_simt<kMode>(call, a, torch_dtype, st);
 }
 
 const char* bad_products(int rows, int E, int N, int K, long long ld_n, long long ld_k) {
@@ -256,7 +344,7 @@ int kleos_expert_products(const void* x, long long ldx, const int32_t* offsets, 
     if (!sm_count()) return refuse(call, KLEOS_E_CUDA, "no current CUDA device");
     experts::Args a{};
     a.x = x; a.w = w; a.bias = bias; a.out = y; a.offsets = offsets; a.ldx = ldx; a.ldo = ldy; a.rows = rows; a.E = E; a.N = N; a.K = K;
-    return products_simt<experts::kForward>(call, a, torch_dtype, stream_of(stream));
+    return products<experts::kForward>(call, a, torch_dtype, stream_of(stream));
 }
 
 int kleos_expert_products_dx(const void* dy, long long lddy, const int32_t* offsets, const void* w, int rows, int E, int N, int K,
@@ -270,7 +358,7 @@ int kleos_expert_products_dx(const void* dy, long long lddy, const int32_t* offs
     if (!sm_count()) return refuse(call, KLEOS_E_CUDA, "no current CUDA device");
     experts::Args a{};
     a.dy = dy; a.w = w; a.out = dx; a.offsets = offsets; a.ldy = lddy; a.ldo = lddx; a.rows = rows; a.E = E; a.N = N; a.K = K;
-    return products_simt<experts::kDx>(call, a, torch_dtype, stream_of(stream));
+    return products<experts::kDx>(call, a, torch_dtype, stream_of(stream));
 }
 
 int kleos_expert_products_dw(const void* dy, long long lddy, const void* x, long long ldx, const int32_t* offsets, int rows, int E,
@@ -286,7 +374,7 @@ int kleos_expert_products_dw(const void* dy, long long lddy, const void* x, long
     a.dy = dy; a.x = x; a.out = dw; a.offsets = offsets; a.ldy = lddy; a.ldx = ldx; a.rows = rows; a.E = E; a.N = N; a.K = K;
     a.wide_out = grad_dtype == 0;
     const cudaStream_t st = stream_of(stream);
-    if (const int rc = products_simt<experts::kDw>(call, a, torch_dtype, st)) return rc;
+    if (const int rc = products<experts::kDw>(call, a, torch_dtype, st)) return rc;
     if (!dbias) return KLEOS_OK;
     a.out = dbias;
     return with_type(call, torch_dtype, [&](auto* null) {

@@ -92,6 +92,17 @@ inline int sm_count() {
     return n;
 }
 
+// Lets a kernel have more than 48 KiB of dynamic shared memory, once per device.
+template <typename... P>
+cudaError_t allow_smem(void (*kernel)(P...), bool (&done)[64], int bytes) {
+    int dev = -1;
+    cudaError_t rc = cudaGetDevice(&dev);
+    if (rc != cudaSuccess || (dev < 64 && done[dev])) return rc;
+    rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (rc == cudaSuccess && dev < 64) done[dev] = true;
+    return rc;
+}
+
 // Calls f with a null pointer of the element type of `torch_dtype` (0 float, 2 bf16, 3 fp16).
 template <typename F>
 int with_type(const char* call, int torch_dtype, F f) {

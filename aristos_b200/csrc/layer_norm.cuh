@@ -11,6 +11,7 @@
 #include <type_traits>
 
 #include "ops_common.cuh"
+#include "tc_common.cuh"
 
 namespace kleos {
 namespace norm {
@@ -23,8 +24,9 @@ struct Args {
     void *y, *dx, *dweight, *dbias;
     float *mean, *rstd, *partial;
     long long ldx, lddy, ldy, lddx;
-    int rows, H;
-    bool wide;  // parameters are floats, whatever the element type
+    int rows, H, depth;  // depth: stages of the ring
+    bool wide;       // parameters are floats, whatever the element type
+    bool param_vec;  // ... and can be loaded as vectors
     float eps;
 };
 
@@ -38,73 +40,240 @@ __device__ __forceinline__ void put_param(void* p, int j, bool wide, float v) {
     else static_cast<T*>(p)[j] = Elem<T>::from_f(v);
 }
 
-// Sum of (a, b) over the G threads of a row, the same in all of them: a warp, or a whole block of G threads.
+// V parameters from column j on, as floats.
+template <typename T, int V>
+__device__ __forceinline__ void load_params(const void* p, int j, bool wide, bool vec, float otherwise, float (&f)[V]) {
+    if (p && vec) {
+        if (wide) {
+#pragma unroll
+            for (int k = 0; k < V; k += 4) {
+                const auto u = load_vec<float, (V < 4 ? V : 4)>(static_cast<const float*>(p) + j + k);
+#pragma unroll
+                for (int i = 0; i < (V < 4 ? V : 4); ++i) f[k + i] = u.v[i];
+            }
+        } else {
+            const auto u = load_vec<T, V>(static_cast<const T*>(p) + j);
+#pragma unroll
+            for (int k = 0; k < V; ++k) f[k] = Elem<T>::to_f(u.v[k]);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) f[k] = param<T>(p, j + k, wide, otherwise);
+    }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void load_params(const void* p, int j, bool wide, bool vec, float otherwise, F2 (&f)[V / 2]) {
+    float v[V];
+    load_params<T, V>(p, j, wide, vec, otherwise, v);
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) f[k] = pair(v[2 * k], v[2 * k + 1]);
+}
+
+// Sum over the W lanes of a group of a warp (W a power of two), the same in all of them.
+template <int W>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// Sum of (a, b) over the G threads of a row, the same in all of them: a warp, or a whole block of G threads, which
+// meets once (`turn` alternates between the two halves of `shared`).
 template <int G>
-__device__ __forceinline__ float2 row_sum(float a, float b, float2* shared) {
+__device__ __forceinline__ float2 row_sum(float a, float b, float2 (*shared)[32], int turn) {
     a = warp_sum(a);
     b = warp_sum(b);
     if constexpr (G > 32) {
         constexpr int W = G / 32;
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        __syncthreads();  // (the sums of the row before have been read)
-        if (lane == 0) shared[warp] = make_float2(a, b);
+        if (lane == 0) shared[turn & 1][warp] = make_float2(a, b);
         __syncthreads();
-        const float2 v = lane < W ? shared[lane] : make_float2(0.f, 0.f);
-        a = warp_sum(v.x);
-        b = warp_sum(v.y);
+        a = b = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float2 v = shared[turn & 1][w];
+            a += v.x;
+            b += v.y;
+        }
     }
     return make_float2(a, b);
 }
 
-template <typename T, int V, int N>
-__device__ __forceinline__ void load_row(const T* row, int H, int G, int at, Vec<T, V> (&v)[N]) {
+// Rows on their way to shared memory: tiles of `per` rows of one or two matrices (row i of matrix m of a stage is the
+// stage's row m * per + i), kDepth of them in flight, each filled by bulk copies that one thread issues.
+constexpr int kMostDepth = 8;
+template <typename T, int kMatrices>
+struct Ring {
+    T* rows;
+    unsigned long long* full;  // [depth]
+    const T* from[kMatrices];
+    long long ld[kMatrices];
+    int depth, per, H, total;  // total: rows of the matrices
+    // One thread: rows r0 .. r0 + per - 1 to stage s.
+    __device__ __forceinline__ void issue(long long r0, int s) const {
+        if (r0 >= total) return;
+        const int n = (int)min((long long)per, total - r0);
+        const uint32_t bytes = (uint32_t)(H * sizeof(T));
+        tc::mbar_expect_tx(&full[s], kMatrices * n * bytes);
+        for (int m = 0; m < kMatrices; ++m)
+            for (int k = 0; k < n; ++k)
+                tc::bulk_load(rows + (size_t)((s * kMatrices + m) * per + k) * H, from[m] + (r0 + k) * ld[m], bytes, &full[s]);
+    }
+    __device__ __forceinline__ const T* row(int s, int m, int k) const { return rows + (s * kMatrices + m) * per * H + k * H; }
+    // False when the copies did not come in about ten seconds: the caller's results are NaN then.
+    __device__ __forceinline__ bool wait(int s, uint32_t parity) const {
+        if (tc::mbar_try_wait(&full[s], parity)) return true;
+        const long long t0 = clock64();
+        while (!tc::mbar_try_wait(&full[s], parity))
+            if (clock64() - t0 > 20000000000LL) return false;
+        return true;
+    }
+};
+template <typename T, int kMatrices>
+__device__ __forceinline__ Ring<T, kMatrices> make_ring(void* smem, unsigned long long* full, const Args& a, int depth, int per, bool first) {
+    Ring<T, kMatrices> r;
+    r.rows = static_cast<T*>(smem);
+    r.full = full;
+    r.depth = depth;
+    r.per = per;
+    r.H = a.H;
+    r.total = a.rows;
+    r.from[0] = static_cast<const T*>(a.x);
+    r.ld[0] = a.ldx;
+    if constexpr (kMatrices == 2) {
+        r.from[1] = static_cast<const T*>(a.dy);
+        r.ld[1] = a.lddy;
+    }
+    if (first) {
+        for (int i = 0; i < depth; ++i) tc::mbar_init(&full[i], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    return r;
+}
+
+// What a thread has of a row: N vectors of V elements, G threads a row.
+template <int V, int G, int N, typename F>
+__device__ __forceinline__ void each_vector(int at, int H, F f) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int j = (at + i * G) * V;
-        if (j < H) v[i] = load_vec<T, V>(row + j);
+    for (int i = 0; i < N; ++i)
+        if ((at + i * G) * V < H) f(i, (at + i * G) * V);
+}
+
+// Rows that can be copied in bulk.  G threads a row, N vectors of V elements each; rows of a tile = blockDim / G.  The
+// block meets once a tile: every warp sums the squares around its own mean, and what the warps' means differ by from
+// the row's is added when they meet (the same sum, without a second round).
+template <typename T, int V, int G, int N>
+__global__ void __launch_bounds__(G > 256 ? G : 256, G > 256 ? 1 : 2) forward_kernel(Args a) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ unsigned long long full[kMostDepth];
+    __shared__ float2 shared[2][16];
+    __shared__ float share[16];  // values of a row that a warp holds
+    constexpr int W = G / 32;
+    const int at = threadIdx.x % G, group = threadIdx.x / G, per = blockDim.x / G, H = a.H, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const auto ring = make_ring<T, 1>(smem, full, a, a.depth, per, threadIdx.x == 0);
+    const long long step = (long long)gridDim.x * per, first = (long long)blockIdx.x * per;
+    pdl_wait();
+    pdl_trigger();
+    if (threadIdx.x == 0)
+        for (int i = 0; i < a.depth; ++i) ring.issue(first + i * step, i);
+    const float inv = 1.f / (float)H;
+    F2 w[N][V / 2], b[N][V / 2];
+    float mine = 0.f;
+    each_vector<V, G, N>(at, H, [&](int i, int j) {
+        mine += V;
+        load_params<T, V>(a.weight, j, a.wide, a.param_vec, 1.f, w[i]);
+        load_params<T, V>(a.bias, j, a.wide, a.param_vec, 0.f, b[i]);
+    });
+    const float n = warp_sum(mine), inv_n = n > 0.f ? 1.f / n : 0.f;
+    if (lane == 0) share[warp] = n;
+    __syncthreads();
+    const float my_share = share[group * W + lane % W];  // of the warp that this lane answers for
+    int stage = 0;
+    uint32_t parity = 0;
+    long long r = first + group;
+    for (int tile = 0; r - group < a.rows; r += step, ++tile) {
+        const bool came = ring.wait(stage, parity), real = r < a.rows;
+        F2 x[N][V / 2], s = both(0.f);
+        if (real)
+            each_vector<V, G, N>(at, H, [&](int i, int j) {
+                to_pairs<T, V>(load_vec<T, V>(ring.row(stage, 0, group) + j), x[i]);
+#pragma unroll
+                for (int k = 0; k < V / 2; ++k) s = add2(s, x[i][k]);
+            });
+        float m = warp_sum(sum2(s)) * inv_n;
+        F2 q2 = both(0.f);
+        const F2 minus = both(-m);
+        if (real)
+            each_vector<V, G, N>(at, H, [&](int i, int) {
+#pragma unroll
+                for (int k = 0; k < V / 2; ++k) {
+                    const F2 d = add2(x[i][k], minus);
+                    q2 = fma2(d, d, q2);
+                }
+            });
+        float q = warp_sum(sum2(q2));
+        if (W > 1 && lane == 0) shared[tile & 1][warp] = make_float2(m, q);
+        __syncthreads();  // ... and the tile is in registers
+        if (threadIdx.x == 0) ring.issue(r - group + a.depth * step, stage);
+        if (++stage == a.depth) stage = 0, parity ^= 1;
+        if constexpr (W > 1) {
+            const float2 v = shared[tile & 1][group * W + lane % W];
+            m = lanes_sum<W>(v.x * my_share) * inv;
+            const float d = v.x - m;
+            q = lanes_sum<W>(fmaf(my_share * d, d, v.y));
+        }
+        if (!real) continue;
+        const float rs = came ? rsqrtf(q * inv + a.eps) : __uint_as_float(0x7fffffffu);
+        T* y = static_cast<T*>(a.y) + r * a.ldy;
+        const F2 rs2 = both(rs), m2 = both(-m);
+        each_vector<V, G, N>(at, H, [&](int i, int j) {
+            F2 o[V / 2];
+#pragma unroll
+            for (int k = 0; k < V / 2; ++k) o[k] = fma2(mul2(add2(x[i][k], m2), rs2), w[i][k], b[i][k]);
+            store_vec<T, V>(y + j, from_pairs<T, V>(o));
+        });
+        if (at == 0) {
+            if (a.mean) a.mean[r] = m;
+            if (a.rstd) a.rstd[r] = rs;
+        }
     }
 }
 
-// G threads a row, N vectors of V elements each; rows / block = blockDim / G.
-template <typename T, int V, int G, int N>
-__global__ void __launch_bounds__(G > 256 ? G : 256) forward_kernel(Args a) {
-    __shared__ float2 shared[32];
+// Any other row of up to G * N elements, a block a row, loaded one by one while the row before is added up.
+template <typename T, int G, int N>
+__global__ void __launch_bounds__(G) forward_odd_kernel(Args a) {
+    __shared__ float2 shared[2][32];
     pdl_wait();
     pdl_trigger();
-    const int at = threadIdx.x % G, per = blockDim.x / G, H = a.H;
+    const int at = threadIdx.x, H = a.H;
     const float inv = 1.f / (float)H;
-    for (long long r = (long long)blockIdx.x * per + threadIdx.x / G; r < a.rows; r += (long long)gridDim.x * per) {
-        Vec<T, V> x[N];
-        load_row<T, V, N>(static_cast<const T*>(a.x) + r * a.ldx, H, G, at, x);
+    float next[N], x[N];
+    auto fetch = [&](long long r) {
+        const T* row = static_cast<const T*>(a.x) + r * a.ldx;
+        each_vector<1, G, N>(at, H, [&](int i, int j) { next[i] = Elem<T>::to_f(row[j]); });
+    };
+    long long r = blockIdx.x;
+    if (r < a.rows) fetch(r);
+    for (int turn = 0; r < a.rows; r += gridDim.x, turn += 2) {
         float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if ((at + i * G) * V < H)
-#pragma unroll
-                for (int k = 0; k < V; ++k) s += Elem<T>::to_f(x[i].v[k]);
-        const float m = row_sum<G>(s, 0.f, shared).x * inv;
+        each_vector<1, G, N>(at, H, [&](int i, int) {
+            x[i] = next[i];
+            s += x[i];
+        });
+        if (r + gridDim.x < a.rows) fetch(r + gridDim.x);
+        const float m = row_sum<G>(s, 0.f, shared, turn).x * inv;
         s = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if ((at + i * G) * V < H)
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    const float d = Elem<T>::to_f(x[i].v[k]) - m;
-                    s = fmaf(d, d, s);
-                }
-        const float rs = 1.f / sqrtf(row_sum<G>(s, 0.f, shared).x * inv + a.eps);
+        each_vector<1, G, N>(at, H, [&](int i, int) {
+            const float d = x[i] - m;
+            s = fmaf(d, d, s);
+        });
+        const float rs = rsqrtf(row_sum<G>(s, 0.f, shared, turn + 1).x * inv + a.eps);
         T* y = static_cast<T*>(a.y) + r * a.ldy;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int j = (at + i * G) * V;
-            if (j >= H) continue;
-            Vec<T, V> o;
-#pragma unroll
-            for (int k = 0; k < V; ++k)
-                o.v[k] = Elem<T>::from_f(fmaf((Elem<T>::to_f(x[i].v[k]) - m) * rs, param<T>(a.weight, j + k, a.wide, 1.f),
-                                              param<T>(a.bias, j + k, a.wide, 0.f)));
-            store_vec<T, V>(y + j, o);
-        }
+        each_vector<1, G, N>(at, H, [&](int i, int j) {
+            y[j] = Elem<T>::from_f(fmaf((x[i] - m) * rs, param<T>(a.weight, j, a.wide, 1.f), param<T>(a.bias, j, a.wide, 0.f)));
+        });
         if (at == 0) {
             if (a.mean) a.mean[r] = m;
             if (a.rstd) a.rstd[r] = rs;
@@ -115,22 +284,23 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) forward_kernel(Args a) {
 // Rows too long for registers: a block reads its row three times.
 template <typename T>
 __global__ void __launch_bounds__(1024) forward_long_kernel(Args a) {
-    __shared__ float2 shared[32];
+    __shared__ float2 shared[2][32];
     pdl_wait();
     pdl_trigger();
     const float inv = 1.f / (float)a.H;
+    int turn = 0;
     for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T* x = static_cast<const T*>(a.x) + r * a.ldx;
         T* y = static_cast<T*>(a.y) + r * a.ldy;
         float s = 0.f;
         for (int j = threadIdx.x; j < a.H; j += 1024) s += Elem<T>::to_f(x[j]);
-        const float m = row_sum<1024>(s, 0.f, shared).x * inv;
+        const float m = row_sum<1024>(s, 0.f, shared, turn++).x * inv;
         s = 0.f;
         for (int j = threadIdx.x; j < a.H; j += 1024) {
             const float d = Elem<T>::to_f(x[j]) - m;
             s = fmaf(d, d, s);
         }
-        const float rs = 1.f / sqrtf(row_sum<1024>(s, 0.f, shared).x * inv + a.eps);
+        const float rs = rsqrtf(row_sum<1024>(s, 0.f, shared, turn++).x * inv + a.eps);
         for (int j = threadIdx.x; j < a.H; j += 1024)
             y[j] = Elem<T>::from_f(fmaf((Elem<T>::to_f(x[j]) - m) * rs, param<T>(a.weight, j, a.wide, 1.f), param<T>(a.bias, j, a.wide, 0.f)));
         if (threadIdx.x == 0) {
@@ -140,97 +310,187 @@ __global__ void __launch_bounds__(1024) forward_long_kernel(Args a) {
     }
 }
 
-// dx of the block's rows, and its sums over them for dw and db: partial[block][0] and [1].
+// Sum over a warp of a (returned in lanes 0..15) and of b (in lanes 16..31).
+__device__ __forceinline__ float warp_sums(float a, float b) {
+    const bool high = threadIdx.x & 16;
+    float v = (high ? b : a) + __shfl_xor_sync(0xffffffffu, high ? a : b, 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// dx of the block's rows, and its sums over them for dw and db: partial[block][0] and [1].  G threads have a row, N
+// vectors of V elements each, 32 elements where the row is long enough: what a row costs beside its elements (two sums
+// over the group, a barrier, addresses) is as many instructions as 16 elements.  A thread's columns are the same
+// in every row, so their sums stay in its registers; the weights, which would take as many again, are in shared
+// memory.  The groups of G threads go through rows of their own, each with a ring and a barrier, and add up at the end.
+template <int G>
+constexpr int kGroups = 512 / G;
+
+// V floats of shared memory as pairs.
+template <int V>
+__device__ __forceinline__ void weights_at(const float* p, F2 (&w)[V / 2]) {
+#pragma unroll
+    for (int k = 0; k < V; k += 4) {
+        const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(p + k);
+        w[k / 2].v = u.x;
+        w[k / 2 + 1].v = u.y;
+    }
+}
 template <typename T, int V, int G, int N>
-__global__ void __launch_bounds__(G > 256 ? G : 256) backward_kernel(Args a) {
-    extern __shared__ float sums[];  // G == 32: [2 * H]
-    __shared__ float2 shared[32];
+__global__ void __launch_bounds__(G * kGroups<G>, 1) backward_kernel(Args a) {
+    constexpr int P = kGroups<G>, W = G / 32;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ unsigned long long full[P][kMostDepth];
+    __shared__ float shared[P][2][2][W];
+    const int at = threadIdx.x % G, group = threadIdx.x / G, H = a.H, warp = at >> 5, lane = threadIdx.x & 31;
+    // weights as floats, then the groups' rings
+    float* weight = reinterpret_cast<float*>(smem);
+    unsigned char* rings = smem + (size_t)(H * 4 + 127) / 128 * 128;
+    const auto ring = make_ring<T, 2>(rings + (size_t)group * a.depth * 2 * H * sizeof(T), full[group], a, a.depth, 1, at == 0);
+    const long long step = (long long)gridDim.x * P, first = blockIdx.x + (long long)group * gridDim.x;
     pdl_wait();
     pdl_trigger();
-    const int at = threadIdx.x % G, per = blockDim.x / G, H = a.H;
+    if (at == 0)
+        for (int i = 0; i < a.depth; ++i) ring.issue(first + i * step, i);
     const float inv = 1.f / (float)H;
-    float dw[N][V], db[N][V];
+    F2 dw[N][V / 2], db[N][V / 2];
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int k = 0; k < V; ++k) dw[i][k] = db[i][k] = 0.f;
-    for (long long r = (long long)blockIdx.x * per + threadIdx.x / G; r < a.rows; r += (long long)gridDim.x * per) {
-        Vec<T, V> x[N], dy[N];
-        load_row<T, V, N>(static_cast<const T*>(a.x) + r * a.ldx, H, G, at, x);
-        load_row<T, V, N>(static_cast<const T*>(a.dy) + r * a.lddy, H, G, at, dy);
-        const float m = a.mean[r], rs = a.rstd[r];
-        float sg = 0.f, sgh = 0.f;
+        for (int k = 0; k < V / 2; ++k) dw[i][k] = db[i][k] = both(0.f);
+    for (int j = threadIdx.x; j < H; j += G * P) weight[j] = param<T>(a.weight, j, a.wide, 1.f);
+    __syncthreads();
+    float next_m = 0.f, next_rs = 0.f;
+    if (first < a.rows) next_m = a.mean[first], next_rs = a.rstd[first];
+    int stage = 0;
+    uint32_t parity = 0;
+    long long turn = 0;
+    for (long long r = first; r < a.rows; r += step, ++turn) {
+        float m = next_m, rs = next_rs;
+        if (r + step < a.rows) next_m = a.mean[r + step], next_rs = a.rstd[r + step];
+        if (!ring.wait(stage, parity)) rs = __uint_as_float(0x7fffffffu);
+        const T *px = ring.row(stage, 0, 0), *pdy = ring.row(stage, 1, 0);
+        const F2 rs2 = both(rs), m2 = both(-m);
+        F2 h[N][V / 2], g[N][V / 2], sg2 = both(0.f), sgh2 = both(0.f);
+        each_vector<V, G, N>(at, H, [&](int i, int j) {
+            F2 d[V / 2], w[V / 2];
+            to_pairs<T, V>(load_vec<T, V>(px + j), h[i]);
+            to_pairs<T, V>(load_vec<T, V>(pdy + j), d);
+            weights_at<V>(weight + j, w);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int j = (at + i * G) * V;
-            if (j >= H) continue;
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float d = Elem<T>::to_f(dy[i].v[k]), h = (Elem<T>::to_f(x[i].v[k]) - m) * rs;
-                const float g = d * param<T>(a.weight, j + k, a.wide, 1.f);
-                sg += g;
-                sgh = fmaf(g, h, sgh);
-                dw[i][k] = fmaf(d, h, dw[i][k]);
-                db[i][k] += d;
+            for (int k = 0; k < V / 2; ++k) {
+                h[i][k] = mul2(add2(h[i][k], m2), rs2);
+                g[i][k] = mul2(d[k], w[k]);
+                sg2 = add2(sg2, g[i][k]);
+                sgh2 = fma2(g[i][k], h[i][k], sgh2);
+                dw[i][k] = fma2(d[k], h[i][k], dw[i][k]);
+                db[i][k] = add2(db[i][k], d[k]);
             }
+        });
+        const float mine = warp_sums(sum2(sg2), sum2(sgh2));
+        float sg, sgh;
+        if constexpr (W > 1) {
+            float (*s)[W] = shared[group][turn & 1];
+            if ((lane & 15) == 0) s[lane >> 4][warp] = mine;
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(G) : "memory");
+            sg = sgh = 0.f;
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                sg += s[0][i];
+                sgh += s[1][i];
+            }
+        } else {
+            sg = __shfl_sync(0xffffffffu, mine, 0);
+            sgh = __shfl_sync(0xffffffffu, mine, 16);
         }
-        const float2 s = row_sum<G>(sg, sgh, shared);
-        const float mg = s.x * inv, mgh = s.y * inv;
+        if (at == 0) ring.issue(r + a.depth * step, stage);  // (the group has met: the row is in registers)
+        const F2 c0 = both(-rs * sg * inv), c1 = both(-rs * sgh * inv);
         T* dx = static_cast<T*>(a.dx) + r * a.lddx;
+        each_vector<V, G, N>(at, H, [&](int i, int j) {
+            F2 o[V / 2];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int j = (at + i * G) * V;
-            if (j >= H) continue;
-            Vec<T, V> o;
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float h = (Elem<T>::to_f(x[i].v[k]) - m) * rs;
-                const float g = Elem<T>::to_f(dy[i].v[k]) * param<T>(a.weight, j + k, a.wide, 1.f);
-                o.v[k] = Elem<T>::from_f(rs * (g - mg - h * mgh));
-            }
-            store_vec<T, V>(dx + j, o);
-        }
+            for (int k = 0; k < V / 2; ++k) o[k] = fma2(h[i][k], c1, fma2(g[i][k], rs2, c0));
+            store_vec<T, V>(dx + j, from_pairs<T, V>(o));
+        });
+        if (++stage == a.depth) stage = 0, parity ^= 1;
     }
     if (!a.partial) return;
-    float* mine = a.partial + (size_t)blockIdx.x * 2 * H;
-    if constexpr (G == 32) {
-        // a warp's rows are its own: the warps' sums are added in their order
-        for (int warp = 0; warp < per; ++warp) {
-            if ((int)threadIdx.x >> 5 == warp)
+    float* out = a.partial + (size_t)blockIdx.x * 2 * H;
+    float* sums = reinterpret_cast<float*>(rings);  // [2 * H]: every row has been read
+    // the groups' sums, added in their order
+    for (int p = 0; p < P; ++p) {
+        __syncthreads();
+        if (group != p) continue;
+        float* to = p < P - 1 ? sums : out;
+        each_vector<V, G, N>(at, H, [&](int i, int j) {
 #pragma unroll
-                for (int i = 0; i < N; ++i)
-#pragma unroll
-                    for (int k = 0; k < V; ++k) {
-                        const int j = (at + i * G) * V + k;
-                        if (j < H) {
-                            sums[j] = warp ? sums[j] + dw[i][k] : dw[i][k];
-                            sums[H + j] = warp ? sums[H + j] + db[i][k] : db[i][k];
-                        }
-                    }
-            __syncthreads();
-        }
-        for (int j = threadIdx.x; j < 2 * H; j += blockDim.x) mine[j] = sums[j];
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const int j = (at + i * G) * V + k;
-                if (j < H) {
-                    mine[j] = dw[i][k];
-                    mine[H + j] = db[i][k];
-                }
+            for (int c = 0; c < V; ++c) {
+                const float2 u = split(dw[i][c / 2]), v = split(db[i][c / 2]);
+                const float f = c & 1 ? u.y : u.x, e = c & 1 ? v.y : v.x;
+                to[j + c] = p ? sums[j + c] + f : f;
+                to[H + j + c] = p ? sums[H + j + c] + e : e;
             }
+        });
     }
+}
+
+// ... of any other row of up to G * N elements
+template <typename T, int G, int N>
+__global__ void __launch_bounds__(G) backward_odd_kernel(Args a) {
+    __shared__ float2 shared[2][32];
+    pdl_wait();
+    pdl_trigger();
+    const int at = threadIdx.x, H = a.H;
+    const float inv = 1.f / (float)H;
+    float w[N], dw[N], db[N], x[N], dy[N], m = 0.f, rs = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) dw[i] = db[i] = 0.f;
+    each_vector<1, G, N>(at, H, [&](int i, int j) { w[i] = param<T>(a.weight, j, a.wide, 1.f); });
+    auto fetch = [&](long long r) {
+        const T *px = static_cast<const T*>(a.x) + r * a.ldx, *pdy = static_cast<const T*>(a.dy) + r * a.lddy;
+        each_vector<1, G, N>(at, H, [&](int i, int j) {
+            x[i] = Elem<T>::to_f(px[j]);
+            dy[i] = Elem<T>::to_f(pdy[j]);
+        });
+        m = a.mean[r];
+        rs = a.rstd[r];
+    };
+    long long r = blockIdx.x;
+    if (r < a.rows) fetch(r);
+    for (int turn = 0; r < a.rows; r += gridDim.x, ++turn) {
+        float h[N], g[N], sg = 0.f, sgh = 0.f;
+        const float rs_now = rs;
+        each_vector<1, G, N>(at, H, [&](int i, int) {
+            h[i] = (x[i] - m) * rs;
+            g[i] = dy[i] * w[i];
+            sg += g[i];
+            sgh = fmaf(g[i], h[i], sgh);
+            dw[i] = fmaf(dy[i], h[i], dw[i]);
+            db[i] += dy[i];
+        });
+        if (r + gridDim.x < a.rows) fetch(r + gridDim.x);
+        const float2 s = row_sum<G>(sg, sgh, shared, turn);
+        const float c0 = -rs_now * s.x * inv, c1 = -rs_now * s.y * inv;
+        T* dx = static_cast<T*>(a.dx) + r * a.lddx;
+        each_vector<1, G, N>(at, H, [&](int i, int j) { dx[j] = Elem<T>::from_f(fmaf(h[i], c1, fmaf(g[i], rs_now, c0))); });
+    }
+    if (!a.partial) return;
+    float* out = a.partial + (size_t)blockIdx.x * 2 * H;
+    each_vector<1, G, N>(at, H, [&](int i, int j) {
+        out[j] = dw[i];
+        out[H + j] = db[i];
+    });
 }
 
 // Rows too long for registers: dx, a block a row; dw and db by column_kernel.
 template <typename T>
 __global__ void __launch_bounds__(1024) backward_long_kernel(Args a) {
-    __shared__ float2 shared[32];
+    __shared__ float2 shared[2][32];
     pdl_wait();
     pdl_trigger();
     const float inv = 1.f / (float)a.H;
+    int turn = 0;
     for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T *x = static_cast<const T*>(a.x) + r * a.ldx, *dy = static_cast<const T*>(a.dy) + r * a.lddy;
         const float m = a.mean[r], rs = a.rstd[r];
@@ -240,7 +500,7 @@ __global__ void __launch_bounds__(1024) backward_long_kernel(Args a) {
             sg += g;
             sgh = fmaf(g, (Elem<T>::to_f(x[j]) - m) * rs, sgh);
         }
-        const float2 s = row_sum<1024>(sg, sgh, shared);
+        const float2 s = row_sum<1024>(sg, sgh, shared, turn++);
         T* dx = static_cast<T*>(a.dx) + r * a.lddx;
         for (int j = threadIdx.x; j < a.H; j += 1024) {
             const float g = Elem<T>::to_f(dy[j]) * param<T>(a.weight, j, a.wide, 1.f), h = (Elem<T>::to_f(x[j]) - m) * rs;
@@ -266,47 +526,61 @@ __global__ void __launch_bounds__(256) column_kernel(Args a) {
     mine[a.H + j] = db;
 }
 
-// dw and db: the blocks' sums, added up eight at a time by 8 threads a column in a fixed order.
+// dw and db: the blocks' sums, a 32nd of them by each of 32 threads a column, then those, in a fixed order.
 template <typename T>
-__global__ void __launch_bounds__(256) finish_kernel(Args a, int partials) {
-    __shared__ float s[8][33];
+__global__ void __launch_bounds__(1024) finish_kernel(Args a, int partials) {
+    __shared__ float s[32][33];
     pdl_wait();
     pdl_trigger();
     const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
     float v = 0.f;
     if (j < 2 * a.H)
-        for (int p = part; p < partials; p += 8) v += a.partial[(size_t)p * 2 * a.H + j];
+#pragma unroll 10
+        for (int p = part; p < partials; p += 32) v += a.partial[(size_t)p * 2 * a.H + j];
     s[part][lane] = v;
     __syncthreads();
-    if (part == 0 && j < 2 * a.H) {
-#pragma unroll
-        for (int k = 1; k < 8; ++k) v += s[k][lane];
-        if (j < a.H) {
-            if (a.dweight) put_param<T>(a.dweight, j, a.wide, v);
+    const float t = warp_sum(s[lane][part]);  // column `part` of the block
+    const int c = blockIdx.x * 32 + part;
+    if (lane == 0 && c < 2 * a.H) {
+        if (c < a.H) {
+            if (a.dweight) put_param<T>(a.dweight, c, a.wide, t);
         } else if (a.dbias) {
-            put_param<T>(a.dbias, j - a.H, a.wide, v);
+            put_param<T>(a.dbias, c - a.H, a.wide, t);
         }
     }
 }
 
-// Calls f with threads a row and vectors a thread for H elements in vectors of V: a warp where four vectors a lane hold
-// the row, else a block of 256 or 512 threads.  False where a row is too long for their registers.
+// Calls f with threads a row and vectors a thread for H elements in vectors of V: 16 elements a thread where the row is
+// longer than 256, 32 above 8192 elements.  False where a row is too long for registers.
 template <int V, typename F>
 bool with_shape(int H, F f) {
-    constexpr int kMost = V == 1 ? 16 : 4;
-    const int n = (H + V - 1) / V;
-    auto shape = [&](auto g, auto k) {
-        f(g, k);
+    constexpr int K = 16 / V;
+    auto shape = [&](auto g, auto n) {
+        f(g, n);
         return true;
     };
     using std::integral_constant;
-    if (n <= 32) return shape(integral_constant<int, 32>(), integral_constant<int, 1>());
-    if (n <= 64) return shape(integral_constant<int, 32>(), integral_constant<int, 2>());
-    if (n <= 128) return shape(integral_constant<int, 32>(), integral_constant<int, 4>());
-    if (n <= 256) return shape(integral_constant<int, 256>(), integral_constant<int, 1>());
-    if (n <= 512) return shape(integral_constant<int, 256>(), integral_constant<int, 2>());
-    if (n <= 1024) return shape(integral_constant<int, 256>(), integral_constant<int, 4>());
-    if (n <= 512 * kMost) return shape(integral_constant<int, 512>(), integral_constant<int, kMost>());
+    if (H <= 256) return shape(integral_constant<int, 32>(), integral_constant<int, K / 2>());
+    if (H <= 512) return shape(integral_constant<int, 32>(), integral_constant<int, K>());
+    if (H <= 1024) return shape(integral_constant<int, 64>(), integral_constant<int, K>());
+    if (H <= 2048) return shape(integral_constant<int, 128>(), integral_constant<int, K>());
+    if (H <= 4096) return shape(integral_constant<int, 256>(), integral_constant<int, K>());
+    if (H <= 8192) return shape(integral_constant<int, 512>(), integral_constant<int, K>());
+    if (H <= 16384) return shape(integral_constant<int, 512>(), integral_constant<int, 2 * K>());
+    return false;
+}
+// ... for elements one by one
+template <typename F>
+bool with_odd_shape(int H, F f) {
+    auto shape = [&](auto g, auto n) {
+        f(g, n);
+        return true;
+    };
+    using std::integral_constant;
+    if (H <= 256) return shape(integral_constant<int, 64>(), integral_constant<int, 4>());
+    if (H <= 1024) return shape(integral_constant<int, 256>(), integral_constant<int, 4>());
+    if (H <= 2048) return shape(integral_constant<int, 256>(), integral_constant<int, 8>());
+    if (H <= 8192) return shape(integral_constant<int, 512>(), integral_constant<int, 16>());
     return false;
 }
 

@@ -39,43 +39,66 @@ bool by_16(size_t elem, std::initializer_list<const void*> ptrs, std::initialize
 }
 
 // ---------------------------------------------------------------- layer norm
+// Stages of a ring, `bytes` each, for `most` bytes on their way: one at least.
+constexpr int kRingMost = 224 * 1024;
+int ring_depth(size_t bytes, int most) { return std::max(1, std::min(norm::kMostDepth, (int)(most / bytes))); }
+
 template <typename T>
-cudaError_t norm_forward(const norm::Args& a, cudaStream_t st) {
+cudaError_t norm_forward(norm::Args a, cudaStream_t st) {
     const int sms = sm_count();
-    cudaError_t rc = cudaSuccess;
-    auto run = [&](auto v, auto g, auto n) {
-        constexpr int V = decltype(v)::value, G = decltype(g)::value, N = decltype(n)::value;
-        constexpr int kThreads = G > 256 ? G : 256, per = kThreads / G;
-        const int blocks = std::min((a.rows + per - 1) / per, sms * (2048 / kThreads));
-        rc = launch(norm::forward_kernel<T, V, G, N>, dim3(blocks), kThreads, 0, 1, st, a);
-    };
     constexpr int W = 16 / sizeof(T);
-    using std::integral_constant;
-    const bool wide = by_16(sizeof(T), {a.x, a.y}, {a.ldx, a.ldy, a.H});
-    const bool done = wide ? norm::with_shape<W>(a.H, [&](auto g, auto n) { run(integral_constant<int, W>(), g, n); })
-                           : norm::with_shape<1>(a.H, [&](auto g, auto n) { run(integral_constant<int, 1>(), g, n); });
+    cudaError_t rc = cudaSuccess;
+    bool done;
+    if (by_16(sizeof(T), {a.x, a.y}, {a.ldx, a.ldy, a.H})) {
+        done = norm::with_shape<W>(a.H, [&](auto g, auto n) {
+            constexpr int G = decltype(g)::value, kThreads = G > 256 ? G : 256, per = kThreads / G;
+            const auto kernel = norm::forward_kernel<T, W, G, decltype(n)::value>;
+            const size_t stage = (size_t)per * a.H * sizeof(T);
+            const int tiles = (a.rows + per - 1) / per;
+            static bool allowed[64];
+            rc = allow_smem(kernel, allowed, kRingMost);
+            a.depth = ring_depth(stage, G > 256 ? 98304 : 49152);
+            const int blocks = tiles <= sms ? tiles : std::min(tiles, std::max(1, resident_blocks(kernel, kThreads, a.depth * stage)));
+            a.depth = std::min(a.depth, (tiles + blocks - 1) / blocks);
+            if (rc == cudaSuccess) rc = launch(kernel, dim3(blocks), kThreads, a.depth * stage, 1, st, a);
+        });
+    } else {
+        done = norm::with_odd_shape(a.H, [&](auto g, auto n) {
+            constexpr int G = decltype(g)::value;
+            rc = launch(norm::forward_odd_kernel<T, G, decltype(n)::value>, dim3(std::min(a.rows, sms * (2048 / G))), G, 0, 1, st, a);
+        });
+    }
     if (!done) rc = launch(norm::forward_long_kernel<T>, dim3(std::min(a.rows, sms * 2)), 1024, 0, 1, st, a);
     return rc;
 }
 
 template <typename T>
-cudaError_t norm_backward(const norm::Args& a, cudaStream_t st) {
+cudaError_t norm_backward(norm::Args a, cudaStream_t st) {
     const int sms = sm_count();
+    constexpr int W = 16 / sizeof(T);
     cudaError_t rc = cudaSuccess;
     int partials = 0;
-    auto run = [&](auto v, auto g, auto n) {
-        constexpr int V = decltype(v)::value, G = decltype(g)::value, N = decltype(n)::value;
-        constexpr int kThreads = G > 256 ? G : 256, per = kThreads / G;
-        partials = std::min((a.rows + per - 1) / per, std::min(2 * sms, norm::kMaxPartials));
-        const size_t smem = G == 32 ? sizeof(float) * 2 * a.H : 0;
-        rc = launch(norm::backward_kernel<T, V, G, N>, dim3(partials), kThreads, smem, 1, st, a);
-    };
     if (a.rows > 0) {
-        constexpr int W = 16 / sizeof(T);
-        using std::integral_constant;
-        const bool wide = by_16(sizeof(T), {a.x, a.dy, a.dx}, {a.ldx, a.lddy, a.lddx, a.H});
-        const bool done = wide ? norm::with_shape<W>(a.H, [&](auto g, auto n) { run(integral_constant<int, W>(), g, n); })
-                               : norm::with_shape<1>(a.H, [&](auto g, auto n) { run(integral_constant<int, 1>(), g, n); });
+        bool done;
+        if (by_16(sizeof(T), {a.x, a.dy, a.dx}, {a.ldx, a.lddy, a.lddx, a.H})) {
+            done = norm::with_shape<W>(a.H, [&](auto g, auto n) {
+                constexpr int G = decltype(g)::value, N = decltype(n)::value, P = norm::kGroups<G>;
+                const auto kernel = norm::backward_kernel<T, W, G, N>;
+                const size_t stage = 2 * (size_t)P * a.H * sizeof(T), least = P > 1 && a.partial ? 8 * (size_t)a.H : 0;
+                partials = std::min(a.rows, std::min(sms, norm::kMaxPartials));
+                const size_t weights = (size_t)(a.H * 4 + 127) / 128 * 128;
+                a.depth = std::min(ring_depth(stage, kRingMost - (int)weights), (a.rows + partials * P - 1) / (partials * P));
+                static bool allowed[64];
+                rc = allow_smem(kernel, allowed, kRingMost);
+                if (rc == cudaSuccess) rc = launch(kernel, dim3(partials), G * P, weights + std::max(a.depth * stage, least), 1, st, a);
+            });
+        } else {
+            done = norm::with_odd_shape(a.H, [&](auto g, auto n) {
+                constexpr int G = decltype(g)::value;
+                partials = std::min(a.rows, std::min(2 * sms, norm::kMaxPartials));
+                rc = launch(norm::backward_odd_kernel<T, G, decltype(n)::value>, dim3(partials), G, 0, 1, st, a);
+            });
+        }
         if (!done) {
             rc = launch(norm::backward_long_kernel<T>, dim3(std::min(a.rows, sms * 2)), 1024, 0, 1, st, a);
             partials = std::min(a.rows, norm::kMaxPartials);
@@ -83,7 +106,7 @@ cudaError_t norm_backward(const norm::Args& a, cudaStream_t st) {
                 rc = launch(norm::column_kernel<T>, dim3((a.H + 255) / 256, partials), 256, 0, 1, st, a);
         }
     }
-    if (rc == cudaSuccess && a.partial) rc = launch(norm::finish_kernel<T>, dim3((2 * a.H + 31) / 32), 256, 0, 1, st, a, partials);
+    if (rc == cudaSuccess && a.partial) rc = launch(norm::finish_kernel<T>, dim3((2 * a.H + 31) / 32), 1024, 0, 1, st, a, partials);
     return rc;
 }
 
@@ -249,6 +272,7 @@ int kleos_layer_norm(const void* x, long long ldx, const void* weight, const voi
     norm::Args a{};
     a.x = x; a.weight = weight; a.bias = bias; a.y = y; a.mean = mean; a.rstd = rstd;
     a.ldx = ldx; a.ldy = ldy; a.rows = rows; a.H = H; a.wide = param_dtype == 0; a.eps = eps;
+    a.param_vec = whole(16, {weight, bias});
     return with_type(call, torch_dtype, [&](auto* null) { return finish(call, norm_forward<std::remove_pointer_t<decltype(null)>>(a, stream_of(stream))); });
 }
 
@@ -270,6 +294,7 @@ int kleos_layer_norm_backward(const void* dy, long long lddy, const void* x, lon
     a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
     a.partial = sums ? static_cast<float*>(workspace) : nullptr;
     a.ldx = ldx; a.lddy = lddy; a.lddx = lddx; a.rows = rows; a.H = H; a.wide = param_dtype == 0;
+    a.param_vec = whole(16, {weight});
     return with_type(call, torch_dtype, [&](auto* null) { return finish(call, norm_backward<std::remove_pointer_t<decltype(null)>>(a, stream_of(stream))); });
 }
 

@@ -33,6 +33,72 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// Two floats in a register pair: one instruction for both, each rounded as the scalar one would (add, mul, fma .f32x2).
+struct F2 {
+    unsigned long long v;
+};
+__device__ __forceinline__ F2 pair(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ F2 both(float a) { return pair(a, a); }
+__device__ __forceinline__ float2 split(F2 a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ float sum2(F2 a) {
+    const float2 f = split(a);
+    return f.x + f.y;
+}
+
+// A vector of elements as pairs of floats, and back (one rounding).
+template <typename T, int V>
+__device__ __forceinline__ void to_pairs(const Vec<T, V>& v, F2 (&p)[V / 2]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) p[i] = pair(v.v[2 * i], v.v[2 * i + 1]);
+    } else {
+        const auto* h = reinterpret_cast<const typename Pack2<T>::type*>(v.v);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            const float2 f = Pack2<T>::to_f2(h[i]);
+            p[i] = pair(f.x, f.y);
+        }
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> from_pairs(const F2 (&p)[V / 2]) {
+    Vec<T, V> v;
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+        const float2 f = split(p[i]);
+        if constexpr (sizeof(T) == 4) {
+            v.v[2 * i] = f.x;
+            v.v[2 * i + 1] = f.y;
+        } else {
+            reinterpret_cast<typename Pack2<T>::type*>(v.v)[i] = Pack2<T>::from_f2(f.x, f.y);
+        }
+    }
+    return v;
+}
+
 // Offsets come from the caller's device memory, so no kernel trusts them: rows outside [0, rows) do not exist.
 struct Group {
     int begin, end;
@@ -101,6 +167,15 @@ cudaError_t allow_smem(void (*kernel)(P...), bool (&done)[64], int bytes) {
     rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (rc == cudaSuccess && dev < 64) done[dev] = true;
     return rc;
+}
+
+// Blocks of a kernel that all multiprocessors hold at once, which is what a kernel whose blocks share out their work
+// evenly is launched with.
+template <typename... P>
+int resident_blocks(void (*kernel)(P...), int threads, size_t smem) {
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess) return 0;
+    return n * sm_count();
 }
 
 // Calls f with a null pointer of the element type of `torch_dtype` (0 float, 2 bf16, 3 fp16).

@@ -229,55 +229,66 @@ def route_static(A, Wg, gate_bias, S, H, E, K, torch_dtype, probs, topk, mcw, st
 # pass the stream that the tensors are used on).  See include/kleos_b200.h for what each computes.
 _ARG = -8
 _MOST_ROWS = 0x7fff0000  # sizes are C ints
-_codes = {}
+_entry = {}              # entry points by name
+_torch = None
 
 
-def _code(t) -> int:
-    if not _codes:
-        import torch
-        _codes.update({torch.float32: 0, torch.bfloat16: 2, torch.float16: 3})
-    return _codes.get(t.dtype, -1)
-
-
-def _require(ok, call: str, what: str) -> None:
-    if not ok:
-        raise KleosError(_ARG, f"{call}: {what}")
-
-
-def _rows(call, name, t, like=None, rows=None, cols=None) -> int:
-    """Row stride of a matrix whose rows are contiguous."""
-    if t.dim() != 2 or t.device.type != "cuda" or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
-        raise KleosError(_ARG, f"{call}: {name} must be a matrix on the GPU" + (f" of {rows} rows" if rows is not None else "") +
-                         (f" of {cols} columns" if cols is not None else ""))
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
-        raise KleosError(_ARG, f"{call}: {name} must have the element type and device of the input")
-    rs, cs = t.stride()
-    cols = t.shape[1]
-    _require(t.shape[0] <= _MOST_ROWS and cols <= _MOST_ROWS, call, f"{name} is too large")
-    if cols > 1 and cs != 1:
-        raise KleosError(_ARG, f"{call}: the rows of {name} must be contiguous")
-    if t.shape[0] < 2:
-        return max(cols, 1)
-    if rs < cols:
-        raise KleosError(_ARG, f"{call}: the rows of {name} must not overlap")
-    return rs
-
-
-def _whole(call, name, t, shape, dtypes, device) -> None:
-    if tuple(t.shape) != tuple(shape) or t.dtype not in dtypes or t.device != device or not t.is_contiguous():
-        raise KleosError(_ARG, f"{call}: {name} must be contiguous, of shape {tuple(shape)}, of type "
-                         f"{' or '.join(str(d) for d in dtypes)} and on {device}")
-
-
-def _launch(call, device, *args) -> None:
-    """Calls the entry point with the tensors' device as the current one."""
+def _bind():
+    """torch and the entry points, at the first call (a small call is as fast as its checks)."""
+    global _torch, _codes
     import torch
-    fn = getattr(load_library(), call)
-    if device.index == torch.cuda.current_device():
-        _check(fn(*args), call)
+    lib = load_library()
+    _entry.update({name: getattr(lib, name) for name in _OPERATOR_ARGS})
+    _codes = {torch.float32: 0, torch.bfloat16: 2, torch.float16: 3}
+    _torch = torch
+    return torch
+
+
+def _refuse(call: str, what: str):
+    raise KleosError(_ARG, f"{call}: {what}")
+
+
+def _first(call, name, t):
+    """Shape, row stride, element type and device of the matrix that the others go by."""
+    if t.dim() != 2 or not t.is_cuda:
+        _refuse(call, f"{name} must be a matrix on the GPU")
+    return t.shape, _rows(call, name, t, t.shape[0], t.shape[1], t.dtype, t.get_device()), t.dtype, t.get_device()
+
+
+def _rows(call, name, t, rows, cols, dtype, dev) -> int:
+    """Row stride of a matrix whose rows are contiguous."""
+    if t.shape != (rows, cols) or t.dtype is not dtype or t.get_device() != dev:
+        _refuse(call, f"{name} must be {rows} x {cols}, {dtype}, on GPU {dev}")
+    if t.is_contiguous():
+        if rows > _MOST_ROWS or cols > _MOST_ROWS:
+            _refuse(call, f"{name} is too large")
+        return cols or 1
+    ld, one = t.stride()
+    if (cols > 1 and one != 1) or (rows > 1 and ld < cols) or rows > _MOST_ROWS or cols > _MOST_ROWS:
+        _refuse(call, f"the rows of {name} must be contiguous, and must not overlap")
+    return ld if rows > 1 else cols or 1
+
+
+def _whole(call, name, t, shape, dtype, dev) -> int:
+    """Address of a contiguous tensor of this shape, type and device."""
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+        _refuse(call, f"{name} must be contiguous, of shape {tuple(shape)}, {dtype}, on GPU {dev}")
+    return t.data_ptr()
+
+
+def _maybe(call, name, t, shape, dtype, dev):
+    return None if t is None else _whole(call, name, t, shape, dtype, dev)
+
+
+def _launch(call, dev, *args) -> None:
+    """Calls the entry point with the tensors' device as the current one."""
+    if dev == _torch.cuda.current_device():
+        rc = _entry[call](*args)
     else:
-        with torch.cuda.device(device):
-            _check(fn(*args), call)
+        with _torch.cuda.device(dev):
+            rc = _entry[call](*args)
+    if rc:
+        _check(rc, call)
 
 
 def layer_norm_workspace(H: int) -> int:
@@ -288,107 +299,89 @@ def layer_norm_workspace(H: int) -> int:
     return n
 
 
-def _params(call, x, named) -> int:
-    import torch
-    given = [(n, t) for n, t in named if t is not None]
-    for n, t in given:
-        _whole(call, n, t, (x.shape[1],), (torch.float32, x.dtype), x.device)
-        _require(t.dtype == given[0][1].dtype, call, "the parameters and their gradients must have one type")
-    return _code(given[0][1]) if given else 0
+def _param_type(call, dtype, *params):
+    """The one type of the parameters that are given: floats, or the element type."""
+    kind = None
+    for p in params:
+        if p is not None:
+            if kind is None:
+                kind = p.dtype
+                if kind is not dtype and kind is not _torch.float32:
+                    _refuse(call, f"the parameters must be floats or {dtype}")
+            elif p.dtype is not kind:
+                _refuse(call, "the parameters and their gradients must have one type")
+    return kind or _torch.float32
 
 
 def layer_norm(x, weight, bias, eps, y, mean=None, rstd=None, stream=None) -> None:
     """y = layer norm of the rows of x; weight and bias may be None; mean and rstd (floats, one a row) are for the
     backward pass."""
-    import torch
-    call = "kleos_layer_norm"
-    ldx = _rows(call, "x", x)
-    R, H = x.shape
-    ldy = _rows(call, "y", y, x, R, H)
-    code = _params(call, x, (("weight", weight), ("bias", bias)))
-    for n, t in (("mean", mean), ("rstd", rstd)):
-        if t is not None:
-            _whole(call, n, t, (R,), (torch.float32,), x.device)
-    _launch(call, x.device, x.data_ptr(), ldx, _ptr(weight), _ptr(bias), R, H, eps, _code(x), code, y.data_ptr(), ldy, _ptr(mean),
-            _ptr(rstd), stream)
+    call, torch = "kleos_layer_norm", _torch or _bind()
+    (R, H), ldx, dt, dev = _first(call, "x", x)
+    ldy = _rows(call, "y", y, R, H, dt, dev)
+    pt = _param_type(call, dt, weight, bias)
+    _launch(call, dev, x.data_ptr(), ldx, _maybe(call, "weight", weight, (H,), pt, dev), _maybe(call, "bias", bias, (H,), pt, dev), R, H, eps,
+            _codes.get(dt, -1), _codes[pt], y.data_ptr(), ldy, _maybe(call, "mean", mean, (R,), torch.float32, dev),
+            _maybe(call, "rstd", rstd, (R,), torch.float32, dev), stream)
 
 
 def layer_norm_backward(dy, x, weight, mean, rstd, dx, dweight=None, dbias=None, workspace=None, stream=None) -> None:
     """Gradients of layer_norm.  dweight and dbias need a workspace of layer_norm_workspace(H) bytes."""
-    import torch
-    call = "kleos_layer_norm_backward"
-    ldx = _rows(call, "x", x)
-    R, H = x.shape
-    lddy, lddx = _rows(call, "dy", dy, x, R, H), _rows(call, "dx", dx, x, R, H)
-    code = _params(call, x, (("weight", weight), ("dweight", dweight), ("dbias", dbias)))
-    for n, t in (("mean", mean), ("rstd", rstd)):
-        _whole(call, n, t, (R,), (torch.float32,), x.device)
-    room = 0
+    call, torch = "kleos_layer_norm_backward", _torch or _bind()
+    (R, H), ldx, dt, dev = _first(call, "x", x)
+    lddy, lddx = _rows(call, "dy", dy, R, H, dt, dev), _rows(call, "dx", dx, R, H, dt, dev)
+    pt = _param_type(call, dt, weight, dweight, dbias)
+    space, room = None, 0
     if workspace is not None:
-        _require(workspace.device == x.device and workspace.is_contiguous(), call, "the workspace must be contiguous and on the input's device")
-        room = workspace.numel() * workspace.element_size()
-    _launch(call, x.device, dy.data_ptr(), lddy, x.data_ptr(), ldx, _ptr(weight), mean.data_ptr(), rstd.data_ptr(), R, H, _code(x),
-            code, dx.data_ptr(), lddx, _ptr(dweight), _ptr(dbias), _ptr(workspace), room, stream)
+        space, room = _whole(call, "workspace", workspace, workspace.shape, workspace.dtype, dev), workspace.nbytes
+    _launch(call, dev, dy.data_ptr(), lddy, x.data_ptr(), ldx, _maybe(call, "weight", weight, (H,), pt, dev),
+            _whole(call, "mean", mean, (R,), torch.float32, dev), _whole(call, "rstd", rstd, (R,), torch.float32, dev), R, H,
+            _codes.get(dt, -1), _codes[pt], dx.data_ptr(), lddx, _maybe(call, "dweight", dweight, (H,), pt, dev),
+            _maybe(call, "dbias", dbias, (H,), pt, dev), space, room, stream)
 
 
-def _ints(call, name, t, shape, device) -> None:
-    import torch
-    _whole(call, name, t, shape, (torch.int32,), device)
+def _offsets(call, offsets, dev):
+    """Number of experts and address."""
+    if offsets.dim() != 1 or offsets.shape[0] < 2:
+        _refuse(call, "offsets must have an entry per expert and one more")
+    return offsets.shape[0] - 1, _whole(call, "offsets", offsets, offsets.shape, _torch.int32, dev)
 
 
-def _places(call, row_of, device):
-    _require(row_of.dim() == 2, call, "row_of must have a row per token and a column per expert of it")
-    _ints(call, "row_of", row_of, row_of.shape, device)
-    return row_of.shape
-
-
-def _offsets(call, offsets, device) -> int:
-    E = offsets.shape[0] - 1 if offsets.dim() == 1 else 0
-    _require(E >= 1, call, "offsets must have an entry per expert and one more")
-    _ints(call, "offsets", offsets, (E + 1,), device)
-    return E
+def _places(call, row_of, T, dev):
+    """Experts of a token and address."""
+    if row_of.dim() != 2 or row_of.shape[0] != T:
+        _refuse(call, "row_of must have a row per token and a column per expert of it")
+    return row_of.shape[1], _whole(call, "row_of", row_of, row_of.shape, _torch.int32, dev)
 
 
 def sort_tokens(topk, num_experts, offsets, row_of, source=None, stream=None) -> None:
     """Rows of the tokens' experts, sorted by expert: offsets [E + 1], row_of [T, K], source [T * K], all int32."""
-    call = "kleos_sort_tokens"
-    _require(topk.dim() == 2 and topk.device.type == "cuda", call, "topk must be a matrix on the GPU")
-    T, K = topk.shape
-    _ints(call, "topk", topk, (T, K), topk.device)
-    _ints(call, "offsets", offsets, (num_experts + 1,), topk.device)
-    _ints(call, "row_of", row_of, (T, K), topk.device)
-    if source is not None:
-        _ints(call, "source", source, (T * K,), topk.device)
-    _launch(call, topk.device, topk.data_ptr(), T, K, num_experts, offsets.data_ptr(), row_of.data_ptr(), _ptr(source), stream)
-
-
-def _weights(call, name, t, T, K, device) -> None:
-    import torch
-    if t is not None:
-        _whole(call, name, t, (T, K), (torch.float32,), device)
+    call, torch = "kleos_sort_tokens", _torch or _bind()
+    if topk.dim() != 2 or not topk.is_cuda:
+        _refuse(call, "topk must be a matrix on the GPU")
+    (T, K), i32, dev = topk.shape, torch.int32, topk.get_device()
+    _launch(call, dev, _whole(call, "topk", topk, (T, K), i32, dev), T, K, num_experts,
+            _whole(call, "offsets", offsets, (num_experts + 1,), i32, dev), _whole(call, "row_of", row_of, (T, K), i32, dev),
+            _maybe(call, "source", source, (T * K,), i32, dev), stream)
 
 
 def gather_tokens(x, row_of, offsets, rows, stream=None) -> None:
     """rows[row_of[t, k]] = x[t], zeros from offsets[E] on."""
     call = "kleos_gather_tokens"
-    ldx = _rows(call, "x", x)
-    T, H = x.shape
-    K = _places(call, row_of, x.device)[1]
-    _require(row_of.shape[0] == T, call, "row_of must have a row per token")
-    E = _offsets(call, offsets, x.device)
-    _whole(call, "rows", rows, (T * K, H), (x.dtype,), x.device)
-    _launch(call, x.device, x.data_ptr(), ldx, row_of.data_ptr(), offsets.data_ptr(), T, K, E, H, _code(x), rows.data_ptr(), stream)
+    _torch or _bind()
+    (T, H), ldx, dt, dev = _first(call, "x", x)
+    K, at = _places(call, row_of, T, dev)
+    E, off = _offsets(call, offsets, dev)
+    _launch(call, dev, x.data_ptr(), ldx, at, off, T, K, E, H, _codes.get(dt, -1), _whole(call, "rows", rows, (T * K, H), dt, dev), stream)
 
 
 def combine_tokens(rows, row_of, weights, out, stream=None) -> None:
     """out[t] = sum over k of weights[t, k] * rows[row_of[t, k]]; weights None: ones."""
-    call = "kleos_combine_tokens"
-    T, K = _places(call, row_of, rows.device)
-    ldo = _rows(call, "out", out, rows, T)
-    _whole(call, "rows", rows, (T * K, out.shape[1]), (rows.dtype,), rows.device)
-    _weights(call, "weights", weights, T, K, rows.device)
-    _launch(call, rows.device, rows.data_ptr(), row_of.data_ptr(), _ptr(weights), T, K, out.shape[1], _code(rows), out.data_ptr(), ldo,
-            stream)
+    call, torch = "kleos_combine_tokens", _torch or _bind()
+    (T, H), ldo, dt, dev = _first(call, "out", out)
+    K, at = _places(call, row_of, T, dev)
+    _launch(call, dev, _whole(call, "rows", rows, (T * K, H), dt, dev), at, _maybe(call, "weights", weights, (T, K), torch.float32, dev), T, K, H,
+            _codes.get(dt, -1), out.data_ptr(), ldo, stream)
 
 
 def gather_tokens_backward(drows, row_of, dx, stream=None) -> None:
@@ -398,60 +391,48 @@ def gather_tokens_backward(drows, row_of, dx, stream=None) -> None:
 
 def combine_tokens_backward(dout, rows, row_of, weights, offsets, drows, dweights=None, stream=None) -> None:
     """Gradients of combine_tokens for the rows (zeros from offsets[E] on) and the weights."""
-    call = "kleos_combine_tokens_backward"
-    ldd = _rows(call, "dout", dout)
-    T, H = dout.shape
-    K = _places(call, row_of, dout.device)[1]
-    _require(row_of.shape[0] == T, call, "row_of must have a row per token")
-    E = _offsets(call, offsets, dout.device)
-    _whole(call, "rows", rows, (T * K, H), (dout.dtype,), dout.device)
-    _whole(call, "drows", drows, (T * K, H), (dout.dtype,), dout.device)
-    _weights(call, "weights", weights, T, K, dout.device)
-    _weights(call, "dweights", dweights, T, K, dout.device)
-    _launch(call, dout.device, dout.data_ptr(), ldd, rows.data_ptr(), row_of.data_ptr(), _ptr(weights), offsets.data_ptr(), T, K, E, H,
-            _code(dout), drows.data_ptr(), _ptr(dweights), stream)
+    call, torch = "kleos_combine_tokens_backward", _torch or _bind()
+    (T, H), ldd, dt, dev = _first(call, "dout", dout)
+    K, at = _places(call, row_of, T, dev)
+    E, off = _offsets(call, offsets, dev)
+    _launch(call, dev, dout.data_ptr(), ldd, _whole(call, "rows", rows, (T * K, H), dt, dev), at,
+            _maybe(call, "weights", weights, (T, K), torch.float32, dev), off, T, K, E, H, _codes.get(dt, -1),
+            _whole(call, "drows", drows, (T * K, H), dt, dev), _maybe(call, "dweights", dweights, (T, K), torch.float32, dev), stream)
 
 
 def expert_products(x, offsets, w, bias, y, stream=None) -> None:
     """y[r] = x[r] W[e]^T + bias[e] for the rows of every expert, zeros from offsets[E] on; bias may be None."""
     call = "kleos_expert_products"
-    ldx = _rows(call, "x", x)
-    R, K = x.shape
-    E = _offsets(call, offsets, x.device)
-    _require(w.dim() == 3, call, "w must be [experts, N, K]")
-    N = w.shape[1]
-    _whole(call, "w", w, (E, N, K), (x.dtype,), x.device)
-    if bias is not None:
-        _whole(call, "bias", bias, (E, N), (x.dtype,), x.device)
-    ldy = _rows(call, "y", y, x, R, N)
-    _launch(call, x.device, x.data_ptr(), ldx, offsets.data_ptr(), w.data_ptr(), _ptr(bias), R, E, N, K, _code(x), y.data_ptr(), ldy, stream)
+    _torch or _bind()
+    (R, K), ldx, dt, dev = _first(call, "x", x)
+    E, off = _offsets(call, offsets, dev)
+    N = w.shape[1] if w.dim() == 3 else _refuse(call, "w must be [experts, N, K]")
+    ldy = _rows(call, "y", y, R, N, dt, dev)
+    _launch(call, dev, x.data_ptr(), ldx, off, _whole(call, "w", w, (E, N, K), dt, dev), _maybe(call, "bias", bias, (E, N), dt, dev), R, E, N, K,
+            _codes.get(dt, -1), y.data_ptr(), ldy, stream)
 
 
 def expert_products_dx(dy, offsets, w, dx, stream=None) -> None:
     """dx[r] = dy[r] W[e] for the rows of every expert, zeros from offsets[E] on."""
     call = "kleos_expert_products_dx"
-    lddy = _rows(call, "dy", dy)
-    R, N = dy.shape
-    E = _offsets(call, offsets, dy.device)
-    _require(w.dim() == 3, call, "w must be [experts, N, K]")
-    K = w.shape[2]
-    _whole(call, "w", w, (E, N, K), (dy.dtype,), dy.device)
-    lddx = _rows(call, "dx", dx, dy, R, K)
-    _launch(call, dy.device, dy.data_ptr(), lddy, offsets.data_ptr(), w.data_ptr(), R, E, N, K, _code(dy), dx.data_ptr(), lddx, stream)
+    _torch or _bind()
+    (R, N), lddy, dt, dev = _first(call, "dy", dy)
+    E, off = _offsets(call, offsets, dev)
+    K = w.shape[2] if w.dim() == 3 else _refuse(call, "w must be [experts, N, K]")
+    lddx = _rows(call, "dx", dx, R, K, dt, dev)
+    _launch(call, dev, dy.data_ptr(), lddy, off, _whole(call, "w", w, (E, N, K), dt, dev), R, E, N, K, _codes.get(dt, -1), dx.data_ptr(), lddx, stream)
 
 
 def expert_products_dw(dy, x, offsets, dw, dbias=None, stream=None) -> None:
     """dw[e] = sum over the rows of expert e of dy[r]^T x[r], dbias[e] = sum of dy[r]; in the element type or floats."""
-    import torch
-    call = "kleos_expert_products_dw"
-    lddy, ldx = _rows(call, "dy", dy), _rows(call, "x", x, dy, dy.shape[0])
-    (R, N), K = dy.shape, x.shape[1]
-    E = _offsets(call, offsets, dy.device)
-    _whole(call, "dw", dw, (E, N, K), (dy.dtype, torch.float32), dy.device)
-    if dbias is not None:
-        _whole(call, "dbias", dbias, (E, N), (dw.dtype,), dy.device)
-    _launch(call, dy.device, dy.data_ptr(), lddy, x.data_ptr(), ldx, offsets.data_ptr(), R, E, N, K, _code(dy), _code(dw), dw.data_ptr(),
-            _ptr(dbias), stream)
+    call, torch = "kleos_expert_products_dw", _torch or _bind()
+    (R, N), lddy, dt, dev = _first(call, "dy", dy)
+    K = x.shape[1] if x.dim() == 2 else _refuse(call, "x must be a matrix")
+    ldx = _rows(call, "x", x, R, K, dt, dev)
+    E, off = _offsets(call, offsets, dev)
+    gt = torch.float32 if dw.dtype is torch.float32 else dt
+    _launch(call, dev, dy.data_ptr(), lddy, x.data_ptr(), ldx, off, R, E, N, K, _codes.get(dt, -1), _codes.get(gt, -1),
+            _whole(call, "dw", dw, (E, N, K), gt, dev), _maybe(call, "dbias", dbias, (E, N), gt, dev), stream)
 
 
 FLOW_MILESTONES = ("start", "planned", "first_tile", "last_gemm1_tile", "last_tile", "dispatched",

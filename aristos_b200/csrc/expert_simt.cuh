@@ -75,8 +75,12 @@ __device__ __forceinline__ unsigned long long pack2(float a, float b) {
     return v;
 }
 
-// Eight elements of an operand for a thread.  kAlong: the slice's direction is the contiguous one in memory (thread
-// t holds 8 of the 16 steps of line t / 2), else the tile's is (thread t holds lines 8 (t % 16).. of step t / 16).
+// Where line l of step k of a slice lies: eights of lines change places every four steps, so that neither the stores of
+// operands that are contiguous along the steps nor the reads of four lines at once meet a bank conflict.
+__device__ __forceinline__ int place(int k, int l) { return l ^ ((k & 12) << 1); }
+
+// Eight elements of an operand for a thread.  kAlong: the slice's direction is the contiguous one in memory (thread t
+// holds four steps of lines t / 4 and 64 + t / 4), else the tile's is (thread t holds lines 8 (t % 16).. of step t / 16).
 template <typename T, bool kAlong, int V>
 struct Operand {
     const T* p;      // line 0 of the tile, step 0
@@ -84,35 +88,34 @@ struct Operand {
     int lines, steps;  // that exist
     float v[8];
     __device__ __forceinline__ void load(int step0) {
-        const int line = kAlong ? threadIdx.x >> 1 : (threadIdx.x & 15) * 8;
-        const int step = step0 + (kAlong ? (threadIdx.x & 1) * 8 : threadIdx.x >> 4);
-        const T* q = p + (kAlong ? line * ld + step : step * ld + line);
-        const int room = kAlong ? (line < lines ? steps - step : 0) : (step < steps ? lines - line : 0);
 #pragma unroll
         for (int i = 0; i < 8; i += V) {
-            if (i + V <= room) {
-                const auto u = load_vec<T, V>(q + i);
+            const int line = kAlong ? (threadIdx.x >> 2) + (i >> 2) * 64 : (threadIdx.x & 15) * 8 + i;
+            const int step = step0 + (kAlong ? (threadIdx.x & 3) * 4 + (i & 3) : threadIdx.x >> 4);
+            const bool in = kAlong ? line < lines && step + V <= steps : step < steps && line + V <= lines;
+            Vec<T, V> u;
+            if (in) u = load_vec<T, V>(p + (kAlong ? line * ld + step : step * ld + line));
 #pragma unroll
-                for (int k = 0; k < V; ++k) v[i + k] = Elem<T>::to_f(u.v[k]);
-            } else {
-#pragma unroll
-                for (int k = 0; k < V; ++k) v[i + k] = 0.f;
-            }
+            for (int k = 0; k < V; ++k) v[i + k] = in ? Elem<T>::to_f(u.v[k]) : 0.f;
         }
     }
     __device__ __forceinline__ void put(float (*s)[kPitch]) const {
         if constexpr (kAlong) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[(threadIdx.x & 1) * 8 + i][threadIdx.x >> 1] = v[i];
+            for (int i = 0; i < 8; ++i) {
+                const int k = (threadIdx.x & 3) * 4 + (i & 3);
+                s[k][place(k, (threadIdx.x >> 2) + (i >> 2) * 64)] = v[i];
+            }
         } else {
-            float4* d = reinterpret_cast<float4*>(&s[threadIdx.x >> 4][(threadIdx.x & 15) * 8]);
+            const int k = threadIdx.x >> 4;
+            float4* d = reinterpret_cast<float4*>(&s[k][place(k, (threadIdx.x & 15) * 8)]);
             d[0] = make_float4(v[0], v[1], v[2], v[3]);
             d[1] = make_float4(v[4], v[5], v[6], v[7]);
         }
     }
 };
 
-// V: elements of a load, 16 bytes' worth where every row begins on such a boundary and is a multiple of it, else 1.
+// V: elements of a load, four where every row begins on a 16-byte boundary and is a multiple of it, else 1.
 template <typename T, int kMode, int V>
 __global__ void __launch_bounds__(256, 2) product_kernel(Args a) {
     __shared__ __align__(16) float sa[2][kSlice][kPitch], sb[2][kSlice][kPitch];
@@ -191,8 +194,8 @@ __global__ void __launch_bounds__(256, 2) product_kernel(Args a) {
             ulonglong2 v[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                u[h] = *reinterpret_cast<const float4*>(&sa[now][k][64 * h + 4 * ty]);
-                v[h] = *reinterpret_cast<const ulonglong2*>(&sb[now][k][64 * h + 4 * tx]);
+                u[h] = *reinterpret_cast<const float4*>(&sa[now][k][place(k, 64 * h + 4 * ty)]);
+                v[h] = *reinterpret_cast<const ulonglong2*>(&sb[now][k][place(k, 64 * h + 4 * tx)]);
             }
             const float f[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
             const unsigned long long g[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
@@ -238,15 +241,21 @@ __global__ void __launch_bounds__(256) bias_kernel(Args a) {
     const int e = blockIdx.y, c = blockIdx.x * 64 + (threadIdx.x & 7) * 8, part = threadIdx.x >> 3;
     const Group g = group_rows(a.offsets, e, a.rows);
     float v[8] = {};
-    for (long long r = g.begin + part; r < g.end; r += 32) {
-        const T* p = static_cast<const T*>(a.dy) + r * a.ldy + c;
+    constexpr int kAhead = 8;  // rows on their way
+    for (long long r0 = g.begin + part; r0 < g.end; r0 += 32 * kAhead) {
+        Vec<T, V> u[kAhead][8 / V];
 #pragma unroll
-        for (int i = 0; i < 8; i += V)
-            if (c + i < a.N) {
-                const auto u = load_vec<T, V>(p + i);
+        for (int k = 0; k < kAhead; ++k) {
+            const T* p = static_cast<const T*>(a.dy) + (r0 + 32 * k) * a.ldy + c;
 #pragma unroll
-                for (int k = 0; k < V; ++k) v[i + k] += Elem<T>::to_f(u.v[k]);
-            }
+            for (int i = 0; i < 8; i += V)
+                if (r0 + 32 * k < g.end && c + i < a.N) u[k][i / V] = load_vec<T, V>(p + i);
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (r0 + 32 * k < g.end && c + i < a.N) v[i] += Elem<T>::to_f(u[k][i / V].v[i % V]);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[part][(threadIdx.x & 7) * 8 + i] = v[i];

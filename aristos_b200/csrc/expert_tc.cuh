@@ -5,15 +5,16 @@
 //   weight_tc_kernel              dW[e] = sum over the rows r of e of dy[r]^T x[r]
 //
 // Products: result columns (of W) on the MMA's M side, 256 a pair of blocks, the rows of an expert on its N side, 32 to
-// 256 of them: an expert may have any number of rows, and the weights are what a small batch has to stream.  For dx the
+// 288 of them: an expert may have any number of rows, and the weights are what a small batch has to stream.  For dx the
 // weights' other direction is summed over, so W is read in M-major tiles (64 columns of 64 rows, 128-byte swizzle)
 // instead of K-major ones; nothing is transposed in memory.
 // Weight gradients: both operands lie with the summed direction (the rows) outermost, so both are M-major / N-major
 // tiles of 64 rows.  An expert's last 64 rows may reach into the next expert's: only the steps of 16 rows that it has
 // are multiplied, and in the last of those a warp of each block clears the rows that are not its own before the MMA
 // reads them (a factor of zero would not do: the other expert's row may be infinite).
-// Sums are fp32 in tensor memory, two accumulators of 256 columns, so that the read-back of a tile runs beside the next
-// one's main loop.  No load is multicast; every wait is bounded, and a block that gives up stores NaN for what it owes.
+// Sums are fp32 in tensor memory: sixteen slots of 32 columns of which a tile of products takes as many as its rows need,
+// two accumulators of 256 columns for the weight gradients, so that the read-back of a tile runs beside the next one's main
+// loop.  No load is multicast; every wait is bounded, and a block that gives up stores NaN for what it owes.
 #pragma once
 
 #include <cuda.h>
@@ -27,17 +28,17 @@ namespace tcp {
 using namespace tc;
 
 constexpr int BM = 128, BK = 64;          // per block: M, elements of a slice of the sums
-constexpr int kMaxHalf = 128;             // rows of a tile, per block
-constexpr int HALF_BYTES = 128 * 128;     // one operand's slice of a block
-constexpr int SLICE_BYTES = 2 * HALF_BYTES;
+constexpr int kMaxHalf = 144;             // rows of a tile of products, per block
+constexpr int HALF_BYTES = 128 * 128;     // 128 lines' slice of an operand
 constexpr int kBackWarps = 8, kThreads = (4 + kBackWarps) * 32;
 constexpr int TMEM_COLS = 512, ACC_COLS = 256;
-constexpr int kBoxes = 5;
+constexpr int kSlotCols = 32, kSlots = TMEM_COLS / kSlotCols;
+constexpr int kBoxes = 6;
 
 struct RowMaps {
     CUtensorMap box[kBoxes];
 };
-__host__ __device__ constexpr int box_rows(int i) { return i == 0 ? 16 : i == 1 ? 32 : i == 2 ? 64 : i == 3 ? 96 : 128; }
+__host__ __device__ constexpr int box_rows(int i) { return i == 0 ? 16 : i == 1 ? 32 : i == 2 ? 64 : i == 3 ? 96 : i == 4 ? 128 : kMaxHalf; }
 __device__ __forceinline__ int box_of(int rows) {
     int i = 0;
     while (box_rows(i) < rows) ++i;
@@ -68,6 +69,13 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
         "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
         "[%0], [%1, {%2, %3, %4}], [%5];"
         ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar_cluster)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair_hint(void* smem_dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar_cluster, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint "
+        "[%0], [%1, {%2, %3, %4}], [%5], %6;"
+        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar_cluster), "l"(policy)
         : "memory");
 }
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t smem_src, int x, int y, int z) {
@@ -110,29 +118,28 @@ __device__ __forceinline__ bool all_of_group(bool yes, int barrier) {  // whethe
     return all != 0;
 }
 
-template <int kSlices>
+// kAccs accumulators are announced in turn, kFree parts of tensor memory given back.
+template <int kSlices, int kAccs, int kFree>
 struct Barriers {
     unsigned long long full[kSlices];   // used on the leader
     unsigned long long empty[kSlices];  // one per block
     unsigned long long tail[kSlices];   // one per block: a slice whose rows are not all the expert's (weight gradients)
-    unsigned long long acc_full[2];     // one per block
-    unsigned long long acc_empty[2];    // used on the leader: the read-back warps of both blocks
+    unsigned long long acc_full[kAccs];   // one per block
+    unsigned long long acc_empty[kFree];  // used on the leader: the read-back warps of both blocks
     uint32_t tmem_base;
     int abort;
 };
 // Barriers, tensor memory and the start of the block's life, the same in all kernels here.
-template <int kSlices>
-__device__ __forceinline__ void set_up(Barriers<kSlices>* b, int full_count) {
+template <int kSlices, int kAccs, int kFree>
+__device__ __forceinline__ void set_up(Barriers<kSlices, kAccs, kFree>* b, int full_count) {
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlices; ++i) {
             mbar_init(&b->full[i], full_count);
             mbar_init(&b->empty[i], 1);
             mbar_init(&b->tail[i], 1);
         }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&b->acc_full[i], 1);
-            mbar_init(&b->acc_empty[i], 2 * kBackWarps);
-        }
+        for (int i = 0; i < kAccs; ++i) mbar_init(&b->acc_full[i], 1);
+        for (int i = 0; i < kFree; ++i) mbar_init(&b->acc_empty[i], 2 * kBackWarps);
         b->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -142,8 +149,8 @@ __device__ __forceinline__ void set_up(Barriers<kSlices>* b, int full_count) {
     }
 }
 // Neither block may leave while its partner can still touch its shared memory, barriers or tensor memory.
-template <int kSlices>
-__device__ __forceinline__ void tear_down(Barriers<kSlices>* b) {
+template <int kSlices, int kAccs, int kFree>
+__device__ __forceinline__ void tear_down(Barriers<kSlices, kAccs, kFree>* b) {
     tc_fence_before();
     __syncthreads();
     if (*(volatile int*)&b->abort) settle_after_abort();
@@ -156,26 +163,56 @@ __device__ __forceinline__ void tear_down(Barriers<kSlices>* b) {
 
 // ---------------------------------------------------------------- products
 constexpr int kSlices = 6;
+constexpr int SLICE_BYTES = HALF_BYTES + kMaxHalf * 128;
 constexpr int STG_ROW = BM * 2 + 16;  // bytes of a staged row: padded, so that eight rows meet no bank conflict
+using ProductBarriers = Barriers<kSlices, kSlots, kSlots>;
 struct Control {
-    Barriers<kSlices> b;
+    ProductBarriers b;
     int first[kMaxExperts + 1];  // tiles before every expert
-    __align__(16) unsigned char stage[2][16 * STG_ROW];
+    __align__(16) unsigned char stage[2][2][16 * STG_ROW];  // per read-back group, two turns: 16 rows x 256 bytes
 };
 constexpr int SMEM_BYTES = kSlices * SLICE_BYTES + 1024 + (int)sizeof(Control);
 static_assert(SMEM_BYTES <= 232448, "227 KiB of shared memory per block");
+static_assert(SLICE_BYTES % 1024 == 0, "the swizzle repeats every 1024 bytes");
+
+// Tiles along the rows of an expert.  A K slice of a tile of n rows takes the larger of 2 n cycles of the tensor pipe and
+// n + 256 of shared memory; one of 288 rows is two instructions a step, which read the weights twice, 672 cycles.  Of the
+// two counts that come into question, fewest tiles of up to 288 rows or of up to 256, the cheaper one.
+__device__ __forceinline__ int split_cost(int units, int s) {  // units of 32 rows, shared out evenly
+    const int low = units / s, more = units - low * s;
+    auto cost = [](int u) { return u > 8 ? 672 : u > 7 ? 512 : 32 * u + 256; };
+    return more * cost(low + 1) + (s - more) * cost(low);
+}
+__device__ __forceinline__ int row_splits(int n) {
+    const int units = (n + 31) >> 5, a = (units + 8) / 9, b = (units + 7) >> 3;
+    return a == b || split_cost(units, a) <= split_cost(units, b) ? a : b;
+}
+
+// The slots of a tile that starts at ring position `at`: as one run, or as two when they wrap around or are more than the
+// 256 columns of an instruction.
+struct Runs {
+    int n0, n1, slot0, slot1;
+    __device__ __forceinline__ Runs(uint32_t at, int half) {
+        const int n = half >> 4, room = kSlots - (int)(at % kSlots);
+        slot0 = (int)(at % kSlots);
+        n0 = n > room ? room : n > 8 ? (n + 1) >> 1 : n;
+        n1 = n - n0;
+        slot1 = (slot0 + n0) % kSlots;
+    }
+};
 
 struct Tile {
     int e, col, row, n, half;  // expert, first column of the pair, first row, rows, rows per block in the MMA
+    bool once;                 // no other tile reads these weights
 };
 // Tiles in order of expert, columns, rows: those that run together read the same weights.  An expert's rows are split
-// evenly in units of 32 into as few tiles of up to 256 as hold them.  `at`: the caller's place in the list.
+// evenly in units of 32 into row_splits() tiles.  `at`: the caller's place in the list.
 __device__ __forceinline__ Tile tile_at(int t, const int* first, const TcArgs& g, int* at) {
     int e = *at;
     while (first[e + 1] <= t) ++e;
     *at = e;
     const Group rows = group_rows(g.offsets, e, g.rows);
-    const int n = rows.end - rows.begin, splits = (n + 255) >> 8, r = t - first[e];
+    const int n = rows.end - rows.begin, splits = row_splits(n), r = t - first[e];
     Tile x;
     x.e = e;
     const int mt = r / splits, j = r - mt * splits;
@@ -185,6 +222,7 @@ __device__ __forceinline__ Tile tile_at(int t, const int* first, const TcArgs& g
     x.row = rows.begin + 32 * u0;
     x.half = 16 * u;
     x.n = min(32 * u, n - 32 * u0);
+    x.once = splits == 1;
     return x;
 }
 
@@ -226,7 +264,7 @@ product_tc_kernel(const __grid_constant__ RowMaps map_x, const __grid_constant__
     set_up(&ctl->b, 1);
     pdl_wait();
     const int MT = (g.M + 2 * BM - 1) / (2 * BM);
-    count_tiles(ctl->first, g, [&](int n) { return ((n + 255) >> 8) * MT; });
+    count_tiles(ctl->first, g, [&](int n) { return row_splits(n) * MT; });
     __syncthreads();
     tc_fence_before();
     cluster_sync_all();
@@ -241,6 +279,10 @@ product_tc_kernel(const __grid_constant__ RowMaps map_x, const __grid_constant__
         // The leader announces the bytes of both blocks on its own barrier; a slice that lands before the
         // announcement only makes the barrier's byte count negative for a moment.
         if (lane == 0) {
+            // weights that one tile reads leave L2 first, those that others read too stay
+            uint64_t stream, keep;
+            asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(stream));
+            asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(keep));
             uint32_t it = 0;
             int at = 0;
             bool ok = true;
@@ -262,10 +304,10 @@ product_tc_kernel(const __grid_constant__ RowMaps map_x, const __grid_constant__
                         tma_load_2d_pair(dst + HALF_BYTES, &map_x.box[box], kb * BK, x.row + (int)rank * x.half, full);
                     } else if constexpr (kDx) {
                         const int col = x.col + (int)rank * BM;
-                        tma_load_3d_pair(dst, &map_w, col, kb * BK, x.e, full);
-                        tma_load_3d_pair(dst + 8192, &map_w, col + 64, kb * BK, x.e, full);
+                        tma_load_3d_pair_hint(dst, &map_w, col, kb * BK, x.e, full, x.once ? stream : keep);
+                        tma_load_3d_pair_hint(dst + 8192, &map_w, col + 64, kb * BK, x.e, full, x.once ? stream : keep);
                     } else {
-                        tma_load_3d_pair(dst, &map_w, kb * BK, x.col + (int)rank * BM, x.e, full);
+                        tma_load_3d_pair_hint(dst, &map_w, kb * BK, x.col + (int)rank * BM, x.e, full, x.once ? stream : keep);
                     }
                 }
             }
@@ -276,15 +318,23 @@ product_tc_kernel(const __grid_constant__ RowMaps map_x, const __grid_constant__
         if (leader) {
             const uint32_t elected = elect_one();
             const uint32_t slices = smem_u32(tiles), bars = smem_u32(&ctl->b), tmem = (uint32_t)uniform((int)tmem_base);
-            uint32_t s = 0, ph = 0, i = 0;
+            uint32_t s = 0, ph = 0, i = 0, slots = 0;
             int at = 0;
             bool ok = true;
             for (int t = t0; ok && t < total; t += dt, ++i) {
                 const int half = uniform(tile_at(t, ctl->first, g, &at).half);
-                ok = __all_sync(0xffffffffu, mbar_wait(&ctl->b.acc_empty[i & 1], ((i >> 1) & 1) ^ 1, g.wait_cycles, abort_flag));
+                const Runs runs(slots, half);
+                {
+                    const uint32_t slot = slots + (uint32_t)lane;  // a lane per slot
+                    if (lane < runs.n0 + runs.n1) ok = mbar_wait(&ctl->b.acc_empty[slot % kSlots], ((slot / kSlots) & 1) ^ 1, g.wait_cycles, abort_flag);
+                    ok = __all_sync(0xffffffffu, ok);
+                }
+                slots += runs.n0 + runs.n1;
                 tc_fence_after();
-                const uint32_t idesc = make_instr_desc_16b(2 * BM, 2 * half, Pack2<TE>::kMmaFormat) | (kDx ? kAMajor : 0u);
-                const uint32_t d = tmem + (i & 1) * ACC_COLS;
+                // N of a run: 32 columns a slot, 16 rows of each block
+                const uint32_t idesc = make_instr_desc_16b(2 * BM, 0, Pack2<TE>::kMmaFormat) | (kDx ? kAMajor : 0u);
+                const uint32_t idesc0 = idesc | ((uint32_t)runs.n0 << 19), idesc1 = idesc | ((uint32_t)runs.n1 << 19);
+                const uint32_t d0 = tmem + runs.slot0 * kSlotCols, d1 = tmem + runs.slot1 * kSlotCols;
                 for (int kb = 0; ok && kb < KS; ++kb) {
                     ok = __all_sync(0xffffffffu, mbar_wait(&ctl->b.full[s], ph, g.wait_cycles, abort_flag));
                     if (!ok) break;
@@ -293,30 +343,36 @@ product_tc_kernel(const __grid_constant__ RowMaps map_x, const __grid_constant__
                     const uint64_t da = kDx ? make_major_desc(sa) : make_smem_desc(sa), db = make_smem_desc(sa + HALF_BYTES);
 #pragma unroll
                     for (int k = 0; k < BK / 16; ++k)
-                        umma_bf16_pair_if(elected, d, da + (kDx ? kMajorStep / 16 : 2u) * k, db + 2 * k, idesc, k != 0 ? 1u : (uint32_t)(kb != 0));
-                    umma_commit_both_if(elected, bars + (uint32_t)offsetof(Barriers<kSlices>, empty) + 8 * s);
+                        umma_bf16_pair_if(elected, d0, da + (kDx ? kMajorStep / 16 : 2u) * k, db + 2 * k, idesc0, k != 0 ? 1u : (uint32_t)(kb != 0));
+                    if (runs.n1 > 0) {
+                        const uint64_t db1 = make_smem_desc(sa + HALF_BYTES + (uint32_t)runs.n0 * 2048);
+#pragma unroll
+                        for (int k = 0; k < BK / 16; ++k)
+                            umma_bf16_pair_if(elected, d1, da + (kDx ? kMajorStep / 16 : 2u) * k, db1 + 2 * k, idesc1, k != 0 ? 1u : (uint32_t)(kb != 0));
+                    }
+                    umma_commit_both_if(elected, bars + (uint32_t)offsetof(ProductBarriers, empty) + 8 * s);
                     if (++s == kSlices) {
                         s = 0;
                         ph ^= 1;
                     }
                 }
                 if (!ok) *abort_flag = 1;
-                else umma_commit_both_if(elected, bars + (uint32_t)offsetof(Barriers<kSlices>, acc_full) + 8 * (i & 1));
+                else umma_commit_both_if(elected, bars + (uint32_t)offsetof(ProductBarriers, acc_full) + 8 * (i % kSlots));
             }
         }
         __syncwarp();
     } else if (warp >= 4) {
         // ------------------------------------------------------------ read-back (both blocks)
-        // Tensor-memory lane = result column, column = row.  Group 0 takes the even sixteens of the rows, group 1 the
-        // odd ones; a warp reads the 32 lanes of its quadrant.
+        // Tensor-memory lane = result column, column = row.  Group 0 takes the first 16 columns of every slot, group 1 the
+        // others; a warp reads the 32 lanes of its quadrant.
         const int q = warp & 3, grp = (warp - 4) >> 2, tg = tid - 128 - grp * 128;
-        const uint32_t stg = smem_u32(ctl->stage[grp]);
         TE* out = static_cast<TE*>(g.out);
-        uint32_t i = 0;
+        uint32_t i = 0, slots = 0, turn = 0;
         int at = 0;
         bool dead = false;
         for (int t = t0; t < total; t += dt, ++i) {
             const Tile x = tile_at(t, ctl->first, g, &at);
+            const Runs runs(slots, x.half);
             const int n0 = x.col + (int)rank * BM;  // this block's first column
             float bv[4] = {};
             if (!kDx && g.bias) {
@@ -327,27 +383,34 @@ product_tc_kernel(const __grid_constant__ RowMaps map_x, const __grid_constant__
                 }
             }
             if (!dead) {
-                const bool ok = mbar_wait(&ctl->b.acc_full[i & 1], (i >> 1) & 1, g.wait_cycles, abort_flag);
+                const bool ok = mbar_wait(&ctl->b.acc_full[i % kSlots], (i / kSlots) & 1, g.wait_cycles, abort_flag);
                 if (!ok) *abort_flag = 1;
                 dead = !all_of_group(ok, 1 + grp);
                 tc_fence_after();
             }
-            const uint32_t acc = tmem_base + (i & 1) * ACC_COLS + (static_cast<uint32_t>(q * 32) << 16);
-            auto fetch = [&](int c, uint32_t* r) {
+            // A turn is 16 columns: 16 rows of one block's share.  Two turns' loads are in flight together.
+            auto fetch = [&](uint32_t slot, uint32_t* r) {
                 if (dead) {
 #pragma unroll
                     for (int k = 0; k < 16; ++k) r[k] = 0x7fffffffu;  // NaN
                     return;
                 }
-                tmem_ld_16x256_x2(acc + c, r);
-                tmem_ld_16x256_x2(acc + c + (16u << 16), r + 8);
+                const uint32_t taddr = tmem_base + (slot % kSlots) * kSlotCols + grp * 16 + (static_cast<uint32_t>(q * 32) << 16);
+                tmem_ld_16x256_x2(taddr, r);
+                tmem_ld_16x256_x2(taddr + (16u << 16), r + 8);
             };
-            auto store = [&](int c, const uint32_t* r) {
-                const int valid = min(16, x.n - c);
+            auto store = [&](int k, const uint32_t* r) {
+                // columns of a run: its rows of block 0, then those of block 1
+                const bool run1 = k >= runs.n0;
+                const int len = (run1 ? runs.n1 : runs.n0) * 16, off = run1 ? runs.n0 * 16 : 0;
+                const int c = (k - (run1 ? runs.n0 : 0)) * kSlotCols + grp * 16;
+                const int r0 = c >= len ? x.half + off + c - len : off + c;  // row of the tile
+                const int valid = min(16, x.n - r0);
                 if (valid <= 0) return;  // (the same for all warps of the group)
                 // transposed through shared memory: the group's four warps put the block's 128 columns of 16 rows
                 // there, and every store instruction writes 256 bytes of two rows
-                asm volatile("bar.sync %0, 128;" ::"r"(1 + grp) : "memory");  // (the rows before have been read)
+                const uint32_t stg = smem_u32(ctl->stage[grp][turn & 1]);
+                ++turn;
 #pragma unroll
                 for (int x8 = 0; x8 < 2; ++x8) {
                     uint32_t m[4];
@@ -359,9 +422,10 @@ product_tc_kernel(const __grid_constant__ RowMaps map_x, const __grid_constant__
                     }
                     stmatrix_x4_trans(stg + (uint32_t)((8 * x8 + (lane & 7)) * STG_ROW + q * 64 + (lane >> 3) * 16), m);
                 }
+                // (before the turn after next is staged here, all threads have met for the next one)
                 asm volatile("bar.sync %0, 128;" ::"r"(1 + grp) : "memory");
                 const int col = (tg & 15) * 8;
-                TE* o = out + (long long)(x.row + c) * g.ldo + n0 + col;
+                TE* o = out + (long long)(x.row + r0) * g.ldo + n0 + col;
 #pragma unroll
                 for (int j = tg >> 4; j < 16; j += 8)
                     if (j < valid && n0 + col < g.M) {
@@ -372,23 +436,22 @@ product_tc_kernel(const __grid_constant__ RowMaps map_x, const __grid_constant__
                         *reinterpret_cast<uint4*>(o + j * g.ldo) = v;
                     }
             };
-            const int cols = 2 * x.half;  // a multiple of 32: each group has as many sixteens
+            const int n_slots = runs.n0 + runs.n1;
 #pragma unroll 1
-            for (int c = grp * 16; c < cols; c += 64) {
+            for (int k = 0; k < n_slots; k += 2) {
                 uint32_t r0[16], r1[16];
-                const bool two = c + 32 < cols;
-                fetch(c, r0);
-                if (two) fetch(c + 32, r1);
+                const bool two = k + 1 < n_slots;
+                fetch(slots + k, r0);
+                if (two) fetch(slots + k + 1, r1);
                 tmem_ld_wait();
-                if (c + 64 >= cols) {
-                    // all of the accumulator is in registers: it goes back to the MMA issuer
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) arrive_relaxed(map_to_cta(smem_u32(&ctl->b.acc_empty[i & 1]), 0));
-                }
-                store(c, r0);
-                if (two) store(c + 32, r1);
+                // this warp's part of the slots is in registers: back to the MMA issuer
+                tc_fence_before();
+                __syncwarp();
+                if (lane < (two ? 2 : 1)) arrive_relaxed(map_to_cta(smem_u32(&ctl->b.acc_empty[(slots + k + lane) % kSlots]), 0));
+                store(k, r0);
+                if (two) store(k + 1, r1);
             }
+            slots += n_slots;
         }
         // rows of nobody
         const int chunks = g.M / 8, end = min(max(g.offsets[g.E], 0), g.rows);
@@ -401,23 +464,22 @@ product_tc_kernel(const __grid_constant__ RowMaps map_x, const __grid_constant__
 // ---------------------------------------------------------------- weight gradients
 namespace wg {
 constexpr int kSlices = 5;
-constexpr int STG_BYTES = 32 * 128;  // a warp's 32 rows of 128 bytes
+constexpr int SLICE_BYTES = 2 * HALF_BYTES;
+constexpr int STG_BYTES = 32 * 128;  // a warp's 32 rows of 128 bytes, twice
+using WeightBarriers = Barriers<kSlices, 2, 2>;
 struct Control {
-    Barriers<kSlices> b;
-    int first[kMaxExperts + 1];
+    WeightBarriers b;
 };
-constexpr int SMEM_BYTES = kSlices * SLICE_BYTES + kBackWarps * STG_BYTES + 1024 + (int)sizeof(Control);
+constexpr int SMEM_BYTES = kSlices * SLICE_BYTES + 2 * kBackWarps * STG_BYTES + 1024 + (int)sizeof(Control);
 static_assert(SMEM_BYTES <= 232448, "227 KiB of shared memory per block");
 
 struct Tile {
     int e, row, n, m, c;  // expert, first row and how many, first row and column of dW[e]
 };
-__device__ __forceinline__ Tile tile_at(int t, const int* first, const TcArgs& g, int CT, int* at) {
-    int e = *at;
-    while (first[e + 1] <= t) ++e;
-    *at = e;
+// Tiles in order of expert, rows, columns of dW: `per` of each expert, `CT` of each row.
+__device__ __forceinline__ Tile tile_at(int t, const TcArgs& g, int per, int CT) {
+    const int e = t / per, r = t - e * per, mt = r / CT;
     const Group rows = group_rows(g.offsets, e, g.rows);
-    const int r = t - first[e], mt = r / CT;
     return Tile{e, rows.begin, rows.end - rows.begin, mt * 2 * BM, (r - mt * CT) * 256};
 }
 }  // namespace wg
@@ -426,11 +488,12 @@ template <typename TE, bool kWideOut>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 weight_tc_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_dw,
                  TcArgs g) {
-    constexpr int kSlices = wg::kSlices;
+    constexpr int kSlices = wg::kSlices, SLICE_BYTES = wg::SLICE_BYTES;
+    using WeightBarriers = wg::WeightBarriers;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* stage = tiles + kSlices * SLICE_BYTES;
-    wg::Control* ctl = reinterpret_cast<wg::Control*>(stage + kBackWarps * wg::STG_BYTES);
+    wg::Control* ctl = reinterpret_cast<wg::Control*>(stage + 2 * kBackWarps * wg::STG_BYTES);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
@@ -438,14 +501,13 @@ weight_tc_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
     set_up(&ctl->b, 2);  // a slice of the expert's own rows: the leader twice; another: a warp of each block
     pdl_wait();
     const int MT = (g.M + 2 * BM - 1) / (2 * BM), CT = (g.len + 255) / 256;
-    count_tiles(ctl->first, g, [&](int) { return MT * CT; });
     __syncthreads();
     tc_fence_before();
     cluster_sync_all();
     tc_fence_after();
     pdl_trigger();
     const uint32_t tmem_base = ctl->b.tmem_base;
-    const int total = ctl->first[g.E];
+    const int per = MT * CT, total = g.E * per;
     const int t0 = blockIdx.x >> 1, dt = gridDim.x >> 1;
     // the last slice of an expert's rows ends inside a step of sixteen: rows of others must not reach the MMA
     auto ragged = [](int n, int kb) { return kb == (n - 1) / BK && (n & 15) != 0; };
@@ -454,10 +516,9 @@ weight_tc_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
         // ------------------------------------------------------------ TMA: x (warp 0) and dy (warp 3)
         if (lane == 0) {
             uint32_t it = 0;
-            int at = 0;
             bool ok = true;
             for (int t = t0; ok && t < total; t += dt) {
-                const wg::Tile x = wg::tile_at(t, ctl->first, g, CT, &at);
+                const wg::Tile x = wg::tile_at(t, g, per, CT);
                 for (int kb = 0; kb * BK < x.n; ++kb, ++it) {
                     const int s = it % kSlices;
                     if (!mbar_wait(&ctl->b.empty[s], ((it / kSlices) & 1) ^ 1, g.wait_cycles, abort_flag)) {
@@ -488,10 +549,9 @@ weight_tc_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
     } else if (warp == 2) {
         // ------------------------------------------------------------ rows of others in a last slice (both blocks)
         uint32_t it = 0, phases = 0;
-        int at = 0;
         bool ok = true;
         for (int t = t0; ok && t < total; t += dt) {
-            const wg::Tile x = wg::tile_at(t, ctl->first, g, CT, &at);
+            const wg::Tile x = wg::tile_at(t, g, per, CT);
             if (x.n == 0) continue;
             const int slices = (x.n + BK - 1) / BK;
             it += slices;
@@ -522,10 +582,9 @@ weight_tc_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
             const uint32_t slices = smem_u32(tiles), bars = smem_u32(&ctl->b), tmem = (uint32_t)uniform((int)tmem_base);
             constexpr uint32_t idesc = make_instr_desc_16b(2 * BM, 256, Pack2<TE>::kMmaFormat) | kAMajor | kBMajor;
             uint32_t s = 0, ph = 0, i = 0;
-            int at = 0;
             bool ok = true;
             for (int t = t0; ok && t < total; t += dt) {
-                const int n = uniform(wg::tile_at(t, ctl->first, g, CT, &at).n);
+                const int n = uniform(wg::tile_at(t, g, per, CT).n);
                 if (n == 0) continue;
                 ok = __all_sync(0xffffffffu, mbar_wait(&ctl->b.acc_empty[i & 1], ((i >> 1) & 1) ^ 1, g.wait_cycles, abort_flag));
                 tc_fence_after();
@@ -540,14 +599,14 @@ weight_tc_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
 #pragma unroll
                     for (int k = 0; k < BK / 16; ++k)
                         if (k < steps) umma_bf16_pair_if(elected, d, da + kMajorStep / 16 * k, db + kMajorStep / 16 * k, idesc, k != 0 ? 1u : (uint32_t)(kb != 0));
-                    umma_commit_both_if(elected, bars + (uint32_t)offsetof(Barriers<kSlices>, empty) + 8 * s);
+                    umma_commit_both_if(elected, bars + (uint32_t)offsetof(WeightBarriers, empty) + 8 * s);
                     if (++s == kSlices) {
                         s = 0;
                         ph ^= 1;
                     }
                 }
                 if (!ok) *abort_flag = 1;
-                else umma_commit_both_if(elected, bars + (uint32_t)offsetof(Barriers<kSlices>, acc_full) + 8 * (i & 1));
+                else umma_commit_both_if(elected, bars + (uint32_t)offsetof(WeightBarriers, acc_full) + 8 * (i & 1));
                 ++i;
             }
         }
@@ -558,12 +617,11 @@ weight_tc_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
         // each at a time: through shared memory, swizzled, and from there by TMA, which leaves out what is past the edges.
         constexpr int kCols = kWideOut ? 32 : 64;
         const int q = warp & 3, grp = (warp - 4) >> 2;
-        const uint32_t stg = smem_u32(stage + (warp - 4) * wg::STG_BYTES), line = stg + lane * 128;
-        uint32_t i = 0;
-        int at = 0;
+        const uint32_t stg = smem_u32(stage + 2 * (warp - 4) * wg::STG_BYTES);
+        uint32_t i = 0, turn = 0;
         bool dead = false;
         for (int t = t0; t < total; t += dt) {
-            const wg::Tile x = wg::tile_at(t, ctl->first, g, CT, &at);
+            const wg::Tile x = wg::tile_at(t, g, per, CT);
             const bool zero = x.n == 0;
             if (!zero && !dead) {
                 const bool ok = mbar_wait(&ctl->b.acc_full[i & 1], (i >> 1) & 1, g.wait_cycles, abort_flag);
@@ -590,8 +648,10 @@ weight_tc_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
                     if (lane == 0) arrive_relaxed(map_to_cta(smem_u32(&ctl->b.acc_empty[i & 1]), 0));
                 }
                 if (m >= g.M || x.c + c >= g.len) continue;  // (the same for the whole warp)
-                if (lane == 0) bulk_store_wait_read();       // the rows before have left shared memory
+                // the rows of the turn before the last have left shared memory
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
                 __syncwarp();
+                const uint32_t half = stg + (turn++ & 1) * wg::STG_BYTES, line = half + lane * 128;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     uint4 v;
@@ -610,7 +670,7 @@ weight_tc_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) tma_store_3d(&map_dw, stg, x.c + c, m, x.e);
+                if (lane == 0) tma_store_3d(&map_dw, half, x.c + c, m, x.e);
             }
             if (!zero) ++i;
         }

@@ -8,6 +8,7 @@
 #include <initializer_list>
 #include <type_traits>
 
+#include "expert_rows.cuh"
 #include "expert_simt.cuh"
 #include "expert_tc.cuh"
 #include "layer_norm.cuh"
@@ -111,27 +112,38 @@ cudaError_t norm_backward(norm::Args a, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------- sort, gather, combine
-template <template <typename, int> class Kernel>
+template <template <typename, int, int> class Kernel>
 int move_rows(const char* call, const sorting::Move& m, int torch_dtype, std::initializer_list<const void*> ptrs, cudaStream_t st) {
     return with_type(call, torch_dtype, [&](auto* null) {
         using T = std::remove_pointer_t<decltype(null)>;
         constexpr int W = 16 / sizeof(T);
-        const int grid = (int)std::min<long long>(std::max(m.T, 1), 148 * 64);
-        if (by_16(sizeof(T), ptrs, {m.ld, m.H})) return finish(call, launch(Kernel<T, W>::get(), dim3(grid), 256, 0, 1, st, m));
-        return finish(call, launch(Kernel<T, 1>::get(), dim3(grid), 256, 0, 1, st, m));
+        const bool wide = by_16(sizeof(T), ptrs, {m.ld, m.H});
+        // four vectors a thread; a token or two where there are few
+        const int vectors = (m.H + (wide ? W : 1) - 1) / (wide ? W : 1), per = m.T >= 4 * sm_count() ? 4 : 1;
+        const int threads = std::min(256, std::max(32, (vectors + 32 * per - 1) / (32 * per) * 32));
+        auto run = [&](auto kt) {
+            constexpr int KT = decltype(kt)::value;
+            return finish(call, wide ? launch(Kernel<T, W, KT>::get(), dim3(m.T), threads, 0, 1, st, m)
+                                     : launch(Kernel<T, 1, KT>::get(), dim3(m.T), threads, 0, 1, st, m));
+        };
+        using std::integral_constant;
+        if (m.K == 1) return run(integral_constant<int, 1>());
+        if (m.K == 2) return run(integral_constant<int, 2>());
+        if (m.K <= 4) return run(integral_constant<int, 4>());
+        return run(integral_constant<int, kMaxTopK>());
     });
 }
-template <typename T, int V>
+template <typename T, int V, int KT>
 struct Gather {
-    static auto get() { return sorting::gather_kernel<T, V>; }
+    static auto get() { return sorting::gather_kernel<T, V, KT>; }
 };
-template <typename T, int V>
+template <typename T, int V, int KT>
 struct Combine {
-    static auto get() { return sorting::combine_kernel<T, V>; }
+    static auto get() { return sorting::combine_kernel<T, V, KT>; }
 };
-template <typename T, int V>
+template <typename T, int V, int KT>
 struct CombineBack {
-    static auto get() { return sorting::combine_back_kernel<T, V>; }
+    static auto get() { return sorting::combine_back_kernel<T, V, KT>; }
 };
 
 const char* bad_places(int T, int K, int H, long long ld) {
@@ -145,12 +157,11 @@ template <int kMode>
 int products_simt(const char* call, const experts::Args& a, int torch_dtype, cudaStream_t st) {
     return with_type(call, torch_dtype, [&](auto* null) {
         using T = std::remove_pointer_t<decltype(null)>;
-        constexpr int W = 16 / sizeof(T);
         const int tile = experts::kTile, cols = kMode == experts::kForward ? a.N : a.K;
         const dim3 grid = kMode == experts::kDw ? dim3((a.N + tile - 1) / tile, (cols + tile - 1) / tile, a.E)
                                                 : dim3(a.rows / tile + a.E + 1, (cols + tile - 1) / tile);
         const bool wide = by_16(sizeof(T), {a.x, a.dy, a.w}, {a.ldx, a.ldy, a.N, a.K});
-        if (wide) return finish(call, launch(experts::product_kernel<T, kMode, W>, grid, 256, 0, 1, st, a));
+        if (wide) return finish(call, launch(experts::product_kernel<T, kMode, 4>, grid, 256, 0, 1, st, a));
         return finish(call, launch(experts::product_kernel<T, kMode, 1>, grid, 256, 0, 1, st, a));
     });
 }
@@ -204,7 +215,7 @@ int products_tc(const char* call, const experts::Args& a, int torch_dtype, cudaS
     if (!ok) return refuse(call, KLEOS_E_CUDA, "cuTensorMapEncodeTiled failed");
     static bool done[64];
     cudaError_t rc = allow_smem(product_tc_kernel<TE, kDx>, done, SMEM_BYTES);
-    const long long tiles = (long long)((g.M + 2 * BM - 1) / (2 * BM)) * (a.rows / 256 + std::min(a.E, a.rows));
+    const long long tiles = (long long)((g.M + 2 * BM - 1) / (2 * BM)) * (a.rows / 256 + std::min(a.E, a.rows));  // at most
     if (rc == cudaSuccess) rc = launch(product_tc_kernel<TE, kDx>, dim3(pair_grid(tiles)), kThreads, SMEM_BYTES, 1, st, rows, w, g);
     return finish(call, rc);
 }
@@ -225,11 +236,39 @@ int weights_tc(const char* call, const experts::Args& a, int torch_dtype, cudaSt
     return finish(call, rc);
 }
 
+// A few rows: the weights are streamed from all multiprocessors.
+template <int kMode>
+int products_few(const char* call, const experts::Args& a, int torch_dtype, cudaStream_t st) {
+    using namespace experts::few;
+    return with_type(call, torch_dtype, [&](auto* null) {
+        using T = std::remove_pointer_t<decltype(null)>;
+        if constexpr (kMode == experts::kForward) {
+            constexpr int W = 16 / sizeof(T);
+            const bool wide = by_16(sizeof(T), {a.x, a.w}, {a.ldx, a.K});
+            // one or two rows: twice the blocks, for which two columns a warp are enough
+            const int columns = a.rows <= 2 ? 16 : 32;
+            const auto kernel = wide ? a.rows <= 2 ? forward_rows_kernel<T, W, 2, 2> : forward_rows_kernel<T, W, 8, 4>
+                                     : a.rows <= 2 ? forward_rows_kernel<T, 1, 2, 2> : forward_rows_kernel<T, 1, 8, 4>;
+            return finish(call, launch(kernel, dim3((a.N + columns - 1) / columns, a.rows), 256, 0, 1, st, a));
+        } else {
+            constexpr int V = 4;
+            if (by_16(sizeof(T), {a.w}, {a.K})) return finish(call, launch(dx_rows_kernel<T, V>, dim3((a.K + 32 * V - 1) / (32 * V), a.rows), 1024, 32 * (32 * V + 1) * sizeof(float), 1, st, a));
+            return finish(call, launch(dx_rows_kernel<T, 1>, dim3((a.K + 31) / 32, a.rows), 1024, 32 * 33 * sizeof(float), 1, st, a));
+        }
+    });
+}
+
 // The tensor cores' kernels load 16-bit elements by TMA, whose rows begin and end on 16-byte boundaries; floats (whose
-// sums are fp32 multiply-adds) and everything else go to the FP32 pipes.
+// sums are fp32 multiply-adds) and everything else go to the FP32 pipes, and so do a few rows.
+constexpr int kFewRows = 32;
 template <int kMode>
 int products(const char* call, const experts::Args& a, int torch_dtype, cudaStream_t st) {
-    if (torch_dtype != 0 && a.rows > 0 && by_16(2, {a.x, a.dy, a.w, a.out}, {a.ldx, a.ldy, a.ldo, a.N, a.K})) {
+    const bool tensor = torch_dtype != 0 && by_16(2, {a.x, a.dy, a.w, a.out}, {a.ldx, a.ldy, a.ldo, a.N, a.K});
+    if constexpr (kMode != experts::kDw) {
+        if (a.rows <= kFewRows && !tensor) return products_few<kMode>(call, a, torch_dtype, st);
+        if (kMode == experts::kForward && a.rows <= 2 && (a.N + 255) / 256 * a.rows <= 32) return products_few<kMode>(call, a, torch_dtype, st);
+    }
+    if (tensor && a.rows > 0) {
         if constexpr (kMode != experts::kDw) {
             return torch_dtype == 2 ? products_tc<__nv_bfloat16, kMode == experts::kDx>(call, a, torch_dtype, st)
                                     : products_tc<__half, kMode == experts::kDx>(call, a, torch_dtype, st);
@@ -305,10 +344,14 @@ int kleos_sort_tokens(const int32_t* topk, int T, int K, int E, int32_t* offsets
     if (!offsets || (T > 0 && (!topk || !row_of))) return refuse(call, KLEOS_E_ARG, "null device pointer");
     if (!whole(4, {topk, offsets, row_of, source})) return refuse(call, KLEOS_E_ARG, kWhole);
     if (!sm_count()) return refuse(call, KLEOS_E_CUDA, "no current CUDA device");
-    const size_t smem = sizeof(int) * sorting::kWarps * E;
-    cudaError_t rc = smem > 32768 ? cudaFuncSetAttribute(sorting::sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
+    // one block up to 4096 places, where meeting the others costs more than they take off it
     const int cluster = (long long)T * K <= 4096 ? 1 : sorting::kCluster;
-    if (rc == cudaSuccess) rc = launch(sorting::sort_kernel, dim3(cluster), sorting::kThreads, smem, cluster, stream_of(stream), topk, T * K, E, offsets, row_of, source);
+    const bool kept = (long long)T * K <= 32LL * sorting::kKeep * sorting::kWarps * cluster;
+    const auto kernel = kept ? sorting::sort_kernel<true> : sorting::sort_kernel<false>;
+    const size_t smem = sizeof(int) * sorting::kWarps * E;
+    static bool allowed[2][64];
+    cudaError_t rc = allow_smem(kernel, allowed[kept], (int)sizeof(int) * sorting::kWarps * kMaxExperts);
+    if (rc == cudaSuccess) rc = launch(kernel, dim3(cluster), sorting::kThreads, smem, cluster, stream_of(stream), topk, T * K, E, offsets, row_of, source);
     return finish(call, rc);
 }
 

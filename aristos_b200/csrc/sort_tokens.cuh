@@ -22,7 +22,10 @@ constexpr int kCluster = 8;
 
 // One cluster sorts: block c takes the c-th share of the places, warp w of it the w-th share of those, 32 at a time in
 // order, so a place's rank is what the blocks, the warps and the turns in front of it counted, and its rank among
-// the lanes.  Counters: hist[w][e].
+// the lanes.  Counters: hist[w][e].  kKept: every warp has at most kKeep turns, whose experts and ranks stay in its
+// registers; otherwise it goes through its share twice.
+constexpr int kKeep = 8;
+template <bool kKept>
 __global__ void __launch_bounds__(kThreads) sort_kernel(const int* topk, int n, int E, int* offsets, int* row_of, int* source) {
     namespace cg = cooperative_groups;
     extern __shared__ int hist[];          // [kWarps][E]
@@ -31,16 +34,16 @@ __global__ void __launch_bounds__(kThreads) sort_kernel(const int* topk, int n, 
     __shared__ int scan[kWarps];
     __shared__ int filled;
     cg::cluster_group cluster = cg::this_cluster();
-    pdl_wait();
-    pdl_trigger();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int blocks = (int)cluster.num_blocks(), block = (int)cluster.block_rank();
     int* count = hist + warp * E;
-    for (int i = tid; i < kWarps * E; i += kThreads) hist[i] = 0;
+    for (int i = lane; i < E; i += 32) count[i] = 0;
     // turns of 32 places, an equal number for every warp
     const long long turns = ((long long)n + 31) / 32, per = (turns + blocks * kWarps - 1) / (blocks * kWarps);
     const long long first = ((long long)block * kWarps + warp) * per, last = min(first + per, turns);
-    __syncthreads();
+    __syncwarp();
+    pdl_wait();
+    pdl_trigger();
     auto expert_at = [&](long long turn) {
         const long long i = turn * 32 + lane;
         const int e = i < n ? topk[i] : -1;
@@ -56,11 +59,21 @@ __global__ void __launch_bounds__(kThreads) sort_kernel(const int* topk, int n, 
         __syncwarp();
         return r;
     };
-    for (long long t = first; t < last; ++t) rank(expert_at(t));
+    int kept_e[kKeep], kept_r[kKeep];
+    if constexpr (kKept) {
+#pragma unroll
+        for (int k = 0; k < kKeep; ++k) kept_e[k] = k < per && first + k < last ? expert_at(first + k) : -1;
+#pragma unroll
+        for (int k = 0; k < kKeep; ++k)
+            if (k < per) kept_r[k] = rank(kept_e[k]);
+    } else {
+        for (long long t = first; t < last; ++t) rank(expert_at(t));
+    }
     __syncthreads();
     // a thread per expert: the warps' counts become the places in front of each warp
     int total = 0;
     if (tid < E) {
+#pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const int c = hist[w * E + tid];
             hist[w * E + tid] = total;
@@ -68,14 +81,17 @@ __global__ void __launch_bounds__(kThreads) sort_kernel(const int* topk, int n, 
         }
         mine[tid] = total;
     }
-    cluster.sync();
-    int before = 0, all = 0;
-    if (tid < E)
-        for (int b = 0; b < blocks; ++b) {
-            const int c = cluster.map_shared_rank(mine, b)[tid];
-            if (b < block) before += c;
-            all += c;
-        }
+    int before = 0, all = total;
+    if (blocks > 1) {
+        cluster.sync();
+        all = 0;
+        if (tid < E)
+            for (int b = 0; b < blocks; ++b) {
+                const int c = cluster.map_shared_rank(mine, b)[tid];
+                if (b < block) before += c;
+                all += c;
+            }
+    }
     // exclusive sums over the experts
     int upto = all;
 #pragma unroll
@@ -85,8 +101,9 @@ __global__ void __launch_bounds__(kThreads) sort_kernel(const int* topk, int n, 
     }
     if (lane == 31) scan[warp] = upto;
     __syncthreads();
-    int front = 0;
-    for (int w = 0; w < warp; ++w) front += scan[w];
+    int front = lane < warp ? scan[lane] : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) front += __shfl_xor_sync(0xffffffffu, front, o);
     upto += front;
     if (tid < E) {
         base[tid] = upto - all + before;
@@ -97,17 +114,27 @@ __global__ void __launch_bounds__(kThreads) sort_kernel(const int* topk, int n, 
     }
     if (tid == E - 1) filled = upto;
     __syncthreads();
-    for (long long t = first; t < last; ++t) {
-        const int e = expert_at(t), r = rank(e);
+    auto place = [&](long long t, int e, int r) {
         const long long i = t * 32 + lane;
-        if (i >= n) continue;
+        if (i >= n) return;
         const int row = e < 0 ? -1 : base[e] + r;
         row_of[i] = row;
         if (source && row >= 0) source[row] = (int)i;
+    };
+    if constexpr (kKept) {
+        // (ranks were counted from the warp's own start; count[] now holds what is in front of the warp)
+#pragma unroll
+        for (int k = 0; k < kKeep; ++k)
+            if (k < per && first + k < last) place(first + k, kept_e[k], kept_r[k] + (kept_e[k] < 0 ? 0 : count[kept_e[k]]));
+    } else {
+        for (long long t = first; t < last; ++t) {
+            const int e = expert_at(t);
+            place(t, e, rank(e));
+        }
     }
     if (source)
         for (long long i = (long long)filled + block * kThreads + tid; i < n; i += (long long)blocks * kThreads) source[i] = -1;
-    cluster.sync();  // (no block leaves while another may still read its counts)
+    if (blocks > 1) cluster.sync();  // (no block leaves while another may still read its counts)
 }
 
 struct Move {
@@ -123,7 +150,6 @@ struct Move {
 // Rows that no place leads to are zeros: the tail, from offsets[E] on.
 template <typename T, int V>
 __device__ __forceinline__ void clear_tail(const Move& m) {
-    if (!m.offsets) return;
     const int filled = min(max(m.offsets[m.E], 0), m.n);
     Vec<T, V> zero;
 #pragma unroll
@@ -132,93 +158,148 @@ __device__ __forceinline__ void clear_tail(const Move& m) {
         for (int j = threadIdx.x * V; j < m.H; j += blockDim.x * V) store_vec<T, V>(static_cast<T*>(m.to) + r * m.H + j, zero);
 }
 
-// A block a token: its row is read once and stored K times.
-template <typename T, int V>
+// A block takes a token, a thread every blockDim-th vector of it, kAhead vectors of each row at a time; KT >= K, so that
+// all their loads are on their way before the first is needed.  What the host chooses so: about four vectors a thread.
+template <int KT>
+constexpr int kAhead = KT >= 4 ? 1 : 4 / KT;
+
+// The rows of a token, -1 where it has none.
+template <int KT>
+__device__ __forceinline__ void rows_of_token(const Move& m, long long t, int (&r)[KT]) {
+#pragma unroll
+    for (int k = 0; k < KT; ++k) {
+        r[k] = k < m.K ? m.row_of[t * m.K + k] : -1;
+        if (r[k] >= m.n) r[k] = -1;
+    }
+}
+
+// The token's row is read once and stored K times.
+template <typename T, int V, int KT>
 __global__ void __launch_bounds__(256) gather_kernel(Move m) {
     pdl_wait();
     pdl_trigger();
+    const int step = blockDim.x * V;
     for (long long t = blockIdx.x; t < m.T; t += gridDim.x) {
         const T* x = static_cast<const T*>(m.from) + t * m.ld;
-        for (int j = threadIdx.x * V; j < m.H; j += blockDim.x * V) {
-            const auto v = load_vec<T, V>(x + j);
-            for (int k = 0; k < m.K; ++k) {
-                const int r = m.row_of[t * m.K + k];
-                if (r >= 0 && r < m.n) store_vec<T, V>(static_cast<T*>(m.to) + (long long)r * m.H + j, v);
-            }
+        int r[KT];
+        rows_of_token<KT>(m, t, r);
+        for (int j0 = threadIdx.x * V; j0 < m.H; j0 += 4 * step) {
+            Vec<T, V> v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (j0 + u * step < m.H) v[u] = load_vec<T, V>(x + j0 + u * step);
+#pragma unroll
+            for (int k = 0; k < KT; ++k)
+                if (r[k] >= 0)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (j0 + u * step < m.H) store_vec<T, V>(static_cast<T*>(m.to) + (long long)r[k] * m.H + j0 + u * step, v[u]);
         }
     }
     clear_tail<T, V>(m);
 }
 
-// A block a token.  Without weights: the gradient of gather.
-template <typename T, int V>
+// Without weights: the gradient of gather.
+template <typename T, int V, int KT>
 __global__ void __launch_bounds__(256) combine_kernel(Move m) {
+    constexpr int U = kAhead<KT>;
     pdl_wait();
     pdl_trigger();
+    const int step = blockDim.x * V;
     for (long long t = blockIdx.x; t < m.T; t += gridDim.x) {
         T* out = static_cast<T*>(m.to) + t * m.ld;
-        for (int j = threadIdx.x * V; j < m.H; j += blockDim.x * V) {
-            float s[V];
+        int r[KT];
+        float w[KT];
+        rows_of_token<KT>(m, t, r);
 #pragma unroll
-            for (int i = 0; i < V; ++i) s[i] = 0.f;
-            for (int k = 0; k < m.K; ++k) {
-                const int r = m.row_of[t * m.K + k];
-                if (r < 0 || r >= m.n) continue;
-                const float w = m.weights ? m.weights[t * m.K + k] : 1.f;
-                const auto v = load_vec<T, V>(static_cast<const T*>(m.from) + (long long)r * m.H + j);
+        for (int k = 0; k < KT; ++k) w[k] = m.weights && r[k] >= 0 ? m.weights[t * m.K + k] : 1.f;
+        for (int j0 = threadIdx.x * V; j0 < m.H; j0 += U * step) {
+            Vec<T, V> v[KT][U];
 #pragma unroll
-                for (int i = 0; i < V; ++i) s[i] = fmaf(w, Elem<T>::to_f(v.v[i]), s[i]);
+            for (int k = 0; k < KT; ++k)
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (r[k] >= 0 && j0 + u * step < m.H) v[k][u] = load_vec<T, V>(static_cast<const T*>(m.from) + (long long)r[k] * m.H + j0 + u * step);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (j0 + u * step >= m.H) continue;
+                float s[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) s[i] = 0.f;
+#pragma unroll
+                for (int k = 0; k < KT; ++k)
+                    if (r[k] >= 0)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) s[i] = fmaf(w[k], Elem<T>::to_f(v[k][u].v[i]), s[i]);
+                Vec<T, V> o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o.v[i] = Elem<T>::from_f(s[i]);
+                store_vec<T, V>(out + j0 + u * step, o);
             }
-            Vec<T, V> o;
-#pragma unroll
-            for (int i = 0; i < V; ++i) o.v[i] = Elem<T>::from_f(s[i]);
-            store_vec<T, V>(out + j, o);
         }
     }
 }
 
-// A block a token: dout[t] is read once for all its K rows.
-template <typename T, int V>
+// dout[t] is read once for all its K rows.
+template <typename T, int V, int KT>
 __global__ void __launch_bounds__(256) combine_back_kernel(Move m) {
-    __shared__ float part[kMaxTopK][8];
+    constexpr int U = kAhead<KT>;
+    __shared__ float part[2][KT][8];
     pdl_wait();
     pdl_trigger();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (long long t = blockIdx.x; t < m.T; t += gridDim.x) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = blockDim.x * V;
+    int turn = 0;
+    for (long long t = blockIdx.x; t < m.T; t += gridDim.x, turn ^= 1) {
         const T* dout = static_cast<const T*>(m.from) + t * m.ld;
-        float dot[kMaxTopK];
+        int r[KT];
+        float w[KT], dot[KT];
+        rows_of_token<KT>(m, t, r);
 #pragma unroll
-        for (int k = 0; k < kMaxTopK; ++k) dot[k] = 0.f;
-        for (int j = threadIdx.x * V; j < m.H; j += 256 * V) {
-            const auto d = load_vec<T, V>(dout + j);
+        for (int k = 0; k < KT; ++k) {
+            w[k] = m.weights && r[k] >= 0 ? m.weights[t * m.K + k] : 1.f;
+            dot[k] = 0.f;
+        }
+        for (int j0 = threadIdx.x * V; j0 < m.H; j0 += U * step) {
+            Vec<T, V> d[U], v[KT][U];
 #pragma unroll
-            for (int k = 0; k < kMaxTopK; ++k) {
-                if (k >= m.K) break;
-                const int r = m.row_of[t * m.K + k];
-                if (r < 0 || r >= m.n) continue;
-                const float w = m.weights ? m.weights[t * m.K + k] : 1.f;
-                const auto v = load_vec<T, V>(static_cast<const T*>(m.other) + (long long)r * m.H + j);
-                Vec<T, V> o;
+            for (int u = 0; u < U; ++u)
+                if (j0 + u * step < m.H) d[u] = load_vec<T, V>(dout + j0 + u * step);
+            if (m.dweights)
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float f = Elem<T>::to_f(d.v[i]);
-                    dot[k] = fmaf(f, Elem<T>::to_f(v.v[i]), dot[k]);
-                    o.v[i] = Elem<T>::from_f(w * f);
+                for (int k = 0; k < KT; ++k)
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (r[k] >= 0 && j0 + u * step < m.H) v[k][u] = load_vec<T, V>(static_cast<const T*>(m.other) + (long long)r[k] * m.H + j0 + u * step);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (j0 + u * step >= m.H) continue;
+                float f[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) f[i] = Elem<T>::to_f(d[u].v[i]);
+#pragma unroll
+                for (int k = 0; k < KT; ++k) {
+                    if (r[k] < 0) continue;
+                    Vec<T, V> o;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o.v[i] = Elem<T>::from_f(w[k] * f[i]);
+                    store_vec<T, V>(static_cast<T*>(m.to) + (long long)r[k] * m.H + j0 + u * step, o);
+                    if (m.dweights)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) dot[k] = fmaf(f[i], Elem<T>::to_f(v[k][u].v[i]), dot[k]);
                 }
-                store_vec<T, V>(static_cast<T*>(m.to) + (long long)r * m.H + j, o);
             }
         }
-        __syncthreads();  // (the sums of the token before have been read)
+        if (!m.dweights) continue;
 #pragma unroll
-        for (int k = 0; k < kMaxTopK; ++k) {
-            if (k >= m.K) break;
-            const float v = warp_sum(dot[k]);
-            if (lane == 0) part[k][warp] = v;
+        for (int k = 0; k < KT; ++k) {
+            dot[k] = warp_sum(dot[k]);
+            if (lane == 0) part[turn][k][warp] = dot[k];
         }
-        __syncthreads();
-        if (threadIdx.x < m.K && m.dweights) {
-            float v = part[threadIdx.x][0];
-            for (int w = 1; w < 8; ++w) v += part[threadIdx.x][w];
+        if (blockDim.x > 32) __syncthreads();  // (a thread still at the sums of the token before has its own half)
+        else __syncwarp();
+        if (threadIdx.x < m.K) {
+            float v = part[turn][threadIdx.x][0];
+            for (int i = 1; i < (int)blockDim.x >> 5; ++i) v += part[turn][threadIdx.x][i];
             m.dweights[t * m.K + threadIdx.x] = v;
         }
     }

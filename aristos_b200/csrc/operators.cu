@@ -8,6 +8,7 @@
 #include <initializer_list>
 #include <type_traits>
 
+#include "expert_f32.cuh"
 #include "expert_rows.cuh"
 #include "expert_simt.cuh"
 #include "expert_tc.cuh"
@@ -236,6 +237,32 @@ int weights_tc(const char* call, const experts::Args& a, int torch_dtype, cudaSt
     return finish(call, rc);
 }
 
+template <int kMode>
+int products_f32(const char* call, const experts::Args& a, cudaStream_t st) {
+    using namespace experts;
+    tcp::TcArgs g{};
+    g.offsets = a.offsets; g.bias = a.bias; g.out = a.out; g.rows = a.rows; g.E = a.E; g.wait_cycles = kWaitCycles;
+    g.M = kMode == kForward ? a.N : a.K;
+    g.len = kMode == kForward ? a.K : a.N;
+    g.ldo = kMode == kDw ? a.K : a.ldo;
+    CUtensorMap m, n;
+    bool ok;
+    long long tiles = (g.M + 2 * tcp::BM - 1) / (2 * tcp::BM);  // at most
+    if constexpr (kMode == kDw) {
+        ok = encode_rows(&m, 0, a.x, a.rows, a.K, a.ldx, f32::BK) && encode_rows(&n, 0, a.dy, a.rows, a.N, a.ldy, f32::BK);
+        tiles *= (long long)a.E * ((a.N + f32::BN - 1) / f32::BN);
+    } else {
+        ok = encode_weights(&m, 0, a.w, a.E, a.N, a.K, kMode == kForward ? tcp::BM : f32::BK) &&
+             encode_rows(&n, 0, kMode == kForward ? a.x : a.dy, a.rows, g.len, kMode == kForward ? a.ldx : a.ldy, f32::kHalf);
+        tiles *= a.rows / f32::BN + std::min(a.E, a.rows);
+    }
+    if (!ok) return refuse(call, KLEOS_E_CUDA, "cuTensorMapEncodeTiled failed");
+    static bool done[64];
+    cudaError_t rc = allow_smem(f32::product_f32_kernel<kMode>, done, f32::SMEM_BYTES);
+    if (rc == cudaSuccess) rc = launch(f32::product_f32_kernel<kMode>, dim3(pair_grid(tiles)), f32::kThreads, f32::SMEM_BYTES, 1, st, m, n, g);
+    return finish(call, rc);
+}
+
 // A few rows: the weights are streamed from all multiprocessors.
 template <int kMode>
 int products_few(const char* call, const experts::Args& a, int torch_dtype, cudaStream_t st) {
@@ -258,27 +285,26 @@ int products_few(const char* call, const experts::Args& a, int torch_dtype, cuda
     });
 }
 
-// The tensor cores' kernels load 16-bit elements by TMA, whose rows begin and end on 16-byte boundaries; floats (whose
-// sums are fp32 multiply-adds) and everything else go to the FP32 pipes, and so do a few rows.
+// The tensor cores' kernels load by TMA, whose rows begin and end on 16-byte boundaries; everything else goes to the FP32
+// pipes, and so do a few rows.
 constexpr int kFewRows = 32;
 template <int kMode>
 int products(const char* call, const experts::Args& a, int torch_dtype, cudaStream_t st) {
-    const bool tensor = torch_dtype != 0 && by_16(2, {a.x, a.dy, a.w, a.out}, {a.ldx, a.ldy, a.ldo, a.N, a.K});
+    const bool tensor = a.rows > 0 && by_16(bytes_of(torch_dtype), {a.x, a.dy, a.w, a.out}, {a.ldx, a.ldy, a.ldo, a.N, a.K});
     if constexpr (kMode != experts::kDw) {
-        if (a.rows <= kFewRows && !tensor) return products_few<kMode>(call, a, torch_dtype, st);
+        if (a.rows <= kFewRows && (!tensor || torch_dtype == 0)) return products_few<kMode>(call, a, torch_dtype, st);
         if (kMode == experts::kForward && a.rows <= 2 && (a.N + 255) / 256 * a.rows <= 32) return products_few<kMode>(call, a, torch_dtype, st);
     }
-    if (tensor && a.rows > 0) {
-        if constexpr (kMode != experts::kDw) {
-            return torch_dtype == 2 ? products_tc<__nv_bfloat16, kMode == experts::kDx>(call, a, torch_dtype, st)
-                                    : products_tc<__half, kMode == experts::kDx>(call, a, torch_dtype, st);
-        } else if (a.wide_out) {
-            return torch_dtype == 2 ? weights_tc<__nv_bfloat16, true>(call, a, torch_dtype, st) : weights_tc<__half, true>(call, a, torch_dtype, st);
-        } else {
-            return torch_dtype == 2 ? weights_tc<__nv_bfloat16, false>(call, a, torch_dtype, st) : weights_tc<__half, false>(call, a, torch_dtype, st);
-        }
+    if (!tensor) return products_simt<kMode>(call, a, torch_dtype, st);
+    if (torch_dtype == 0) return products_f32<kMode>(call, a, st);
+    if constexpr (kMode != experts::kDw) {
+        return torch_dtype == 2 ? products_tc<__nv_bfloat16, kMode == experts::kDx>(call, a, torch_dtype, st)
+                                : products_tc<__half, kMode == experts::kDx>(call, a, torch_dtype, st);
+    } else if (a.wide_out) {
+        return torch_dtype == 2 ? weights_tc<__nv_bfloat16, true>(call, a, torch_dtype, st) : weights_tc<__half, true>(call, a, torch_dtype, st);
+    } else {
+        return torch_dtype == 2 ? weights_tc<__nv_bfloat16, false>(call, a, torch_dtype, st) : weights_tc<__half, false>(call, a, torch_dtype, st);
     }
-    return products_simt<kMode>(call, a, torch_dtype, st);
 }
 
 const char* bad_products(int rows, int E, int N, int K, long long ld_n, long long ld_k) {

@@ -209,3 +209,43 @@ def test_refusals():
     refused(-8, dw, c["dy"], c["x"][:7], c["offsets"], torch.empty_like(c["w"]))
     refused(-8, dw, c["dy"], c["x"], c["offsets"], torch.empty_like(c["w"]).half())
     refused(-8, dw, c["dy"], c["x"], c["offsets"], torch.empty_like(c["w"]), torch.empty(2, 16, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("counts", [[1], [2], [1, 1], [3], [2, 2], [32], [33], [16, 0, 16], [16, 1, 16], [1] * 32, [1] * 33])
+@pytest.mark.parametrize("N,K", [(272, 160), (2304, 200), (8448, 64), (39, 50)])
+def test_as_many_rows_as_another_kernel_takes(dtype, counts, N, K):
+    """Row counts on both sides of where a few rows become many, sizes on both sides of where one or two are streamed."""
+    _verify(_case(counts, N, K, dtype, spare=1))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_most_experts(dtype):
+    counts = [(e * 7919) % 5 if e % 3 else 0 for e in range(1024)]
+    _verify(_case(counts, 72, 40, dtype, spare=2))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_many_tiles_of_every_height(dtype):
+    """More tiles than block pairs, row counts whose last tile ends everywhere in its steps of 16, 32 and 64."""
+    _verify(_case([n for n in range(1, 130, 7)] + [250, 300, 511, 513, 1025], 1056, 328, dtype))
+
+
+def test_rows_past_two_to_the_31_elements():
+    R, K, N = 1100000, 2048, 64
+    g = gen(11)
+    last = 300
+    offsets = torch.tensor([0, R - last, R], dtype=torch.int32, device="cuda")
+    x = torch.zeros(R, K, dtype=torch.bfloat16, device="cuda")
+    dy = torch.zeros(R, N, dtype=torch.bfloat16, device="cuda")
+    x[-last:], dy[-last:] = randn(g, (last, K), x.dtype), randn(g, (last, N), x.dtype)
+    w = randn(g, (2, N, K), x.dtype, K ** -0.5)
+    y, dx, dw = torch.empty_like(dy), torch.empty_like(x), torch.empty_like(w)
+    kleos.expert_products(x, offsets, w, None, y, stream())
+    kleos.expert_products_dx(dy, offsets, w, dx, stream())
+    kleos.expert_products_dw(dy, x, offsets, dw, None, stream())
+    xs, ds, ws = x[-last:].double(), dy[-last:].double(), w[1].double()
+    check(y[-last:], xs @ ws.t(), _bound(K, xs.abs() @ ws.abs().t()), "y")
+    check(dx[-last:], ds @ ws, _bound(N, ds.abs() @ ws.abs()), "dx")
+    check(dw[1], ds.t() @ xs, _bound(last, ds.abs().t() @ xs.abs()), "dw")
+    assert not bool(y[:-last].any()) and not bool(dx[:-last].any()) and not bool(dw[0].any())

@@ -181,3 +181,22 @@ def test_refusals():
     refused(-8, back, x, x, w, m, m, y, w, w)                                                     # no workspace
     refused(-8, back, x, x, w, m, m, y, w, w, torch.empty(100, device="cuda"))                    # too small a one
     refused(-8, back, x, x, w, m.double(), m, y)
+
+
+def test_rows_past_two_to_the_31_elements():
+    R, H = 1100000, 2048
+    g = gen(12)
+    x = torch.ones(R, H, dtype=torch.bfloat16, device="cuda")
+    dy = torch.zeros_like(x)
+    x[-40:], dy[-40:] = randn(g, (40, H), x.dtype), randn(g, (40, H), x.dtype)
+    y, dx = torch.empty_like(x), torch.empty_like(x)
+    mean, rstd = torch.empty(R, device="cuda"), torch.empty(R, device="cuda")
+    w, b = randn(g, (H,), torch.float32, 0.3, 1.0), randn(g, (H,), torch.float32)
+    dw, db = torch.empty(H, device="cuda"), torch.empty(H, device="cuda")
+    ws = torch.empty(kleos.layer_norm_workspace(H), dtype=torch.uint8, device="cuda")
+    kleos.layer_norm(x, w, b, 1e-5, y, mean, rstd, stream())
+    kleos.layer_norm_backward(dy, x, w, mean, rstd, dx, dw, db, ws, stream())
+    got = y[-40:], mean[-40:], rstd[-40:], dx[-40:], dw, db
+    for name, v, ref, bound in zip(NAMES, got, *_reference(x[-40:], w, b, 1e-5, dy[-40:])):
+        check(v, ref, bound, name)
+    assert bool((y[:-40] == b.bfloat16()).all()) and not bool(dx[:-40].any())

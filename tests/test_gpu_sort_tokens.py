@@ -199,3 +199,28 @@ def test_refusals():
     refused(-8, kleos.combine_tokens, rows[:, :63], row_of, w, x[:, :63])
     refused(-8, kleos.combine_tokens_backward, x, rows, row_of, w, off, rows[:5])
     refused(-8, kleos.combine_tokens_backward, x, rows, row_of, w, off, torch.zeros_like(rows), w.t())
+
+
+def test_rows_past_two_to_the_31_elements():
+    T, K, E, H = 550000, 2, 4, 2048
+    topk = torch.zeros(T, K, dtype=torch.int32, device="cuda")
+    topk[:, 1] = 3
+    offsets, row_of, _ = _sort(topk, E)
+    g = gen(8)
+    x = torch.zeros(T, H, dtype=torch.bfloat16, device="cuda")
+    x[-50:] = randn(g, (50, H), x.dtype)
+    rows = torch.empty(T * K, H, dtype=torch.bfloat16, device="cuda")
+    kleos.gather_tokens(x, row_of, offsets, rows, stream())
+    assert torch.equal(rows[-50:], x[-50:]) and not bool(rows[T:-50].any())
+    w = torch.rand(T, K, generator=g, device="cuda")
+    out = torch.empty_like(x)
+    kleos.combine_tokens(rows, row_of, w, out, stream())
+    want = x[-50:].double() * w[-50:].double().sum(1, keepdim=True)
+    check(out[-50:], want, 3 * EPS * want.abs(), "out")
+    dw = torch.empty_like(w)
+    drows = torch.empty_like(rows)
+    kleos.combine_tokens_backward(x, rows, row_of, w, offsets, drows, dw, stream())
+    want = x[-50:].double() * w[-50:, 1:].double()
+    check(drows[-50:], want, 2 * EPS * want.abs(), "drows")
+    squares = x[-50:].double().square().sum(1, keepdim=True).expand(50, 2)
+    check(dw[-50:], squares, (H / 32 + 32) * EPS * squares, "dweights")

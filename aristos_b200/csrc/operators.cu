@@ -119,7 +119,7 @@ int move_rows(const char* call, const sorting::Move& m, int torch_dtype, std::in
         using T = std::remove_pointer_t<decltype(null)>;
         constexpr int W = 16 / sizeof(T);
         const bool wide = by_16(sizeof(T), ptrs, {m.ld, m.H});
-        // four vectors a thread; a token or two where there are few
+        // four vectors a thread, one where there are few tokens
         const int vectors = (m.H + (wide ? W : 1) - 1) / (wide ? W : 1), per = m.T >= 4 * sm_count() ? 4 : 1;
         const int threads = std::min(256, std::max(32, (vectors + 32 * per - 1) / (32 * per) * 32));
         auto run = [&](auto kt) {
@@ -474,9 +474,8 @@ int kleos_expert_products_dw(const void* dy, long long lddy, const void* x, long
     return with_type(call, torch_dtype, [&](auto* null) {
         using T = std::remove_pointer_t<decltype(null)>;
         constexpr int W = 16 / sizeof(T);
-        const dim3 grid((N + 63) / 64, E);
-        if (by_16(sizeof(T), {dy}, {lddy, N})) return finish(call, launch(experts::bias_kernel<T, W>, grid, 256, 0, 1, st, a));
-        return finish(call, launch(experts::bias_kernel<T, 1>, grid, 256, 0, 1, st, a));
+        if (by_16(sizeof(T), {dy}, {lddy, N})) return finish(call, launch(experts::bias_kernel<T, W>, dim3((N + experts::kBiasLanes * W - 1) / (experts::kBiasLanes * W), E), 1024, 0, 1, st, a));
+        return finish(call, launch(experts::bias_kernel<T, 1>, dim3((N + experts::kBiasLanes - 1) / experts::kBiasLanes, E), 1024, 0, 1, st, a));
     });
 }
 

@@ -16,11 +16,17 @@
 //
 // M is always the direction in which the result is contiguous: a read-back lane is a column, and a store instruction
 // writes 128 bytes of a row as it is.  256 columns a pair of blocks by up to 128 rows, which are 32 to 128 of an expert's as
-// its number needs.  Per block, 512 threads: warps 0..7 read back and add up, 8..11 split the M operand into tensor
-// memory (a lane a column), 12 and 13 the N operand into shared memory, 14 issues the MMAs (leader) and owns
-// tensor memory, 15 loads by TMA, 32 steps at a time.  What is contiguous along the sums is loaded and split line by
+// its number needs.  Per block, 576 threads: warps 0..7 read back and add up, 8..11 split the M operand into tensor
+// memory (a lane a column), 12..15 the N operand into shared memory, 16 issues the MMAs (leader) and owns
+// tensor memory, 17 loads by TMA, two slices of 32 steps at a time.  What is contiguous along the sums is loaded and split line by
 // line; what is contiguous across them comes in tiles of 32 x 32 that are read down a column (M operand) or split into
 // N-major parts (N operand).  Rows that are not the expert's are cleared when they are split.
+//
+// What bounds it: the split warps (2048 columns, 256 rows an expert: a step of 64 takes about 2500 cycles, its MMAs
+// 1536 of them; tensor pipe 42 % active), and 4.3 tiles a pair of blocks in five rounds.  4096 rows, 16 experts, N = K =
+// 2048: 252, 251 and 288 us (34.4 GFLOP each: 137, 137 and 119 TFLOP/s; the FP32 pipes 1014, 965 and 734), 1.7e-7 from the
+// 64-bit result (FP32 pipes: 8.1e-7).  A step a barrier instead of a slice and four warps for the N operand instead of two:
+// 287, 289 and 288 before; eight warps for the M operand, whose registers the others then lack: 282, 270 and 332.
 #pragma once
 
 #include <cfloat>
@@ -33,24 +39,25 @@ namespace f32 {
 using namespace tcp;
 
 constexpr int BK = 32, ROW = BK * 2;           // steps of a slice; bytes of a part's row of them
-constexpr int kDrain = 8, kSplitA = 4, kSplitB = 2, kSplit = kSplitA + kSplitB;  // warps
+constexpr int kDrain = 8, kSplitA = 4, kSplitB = 4, kSplit = kSplitA + kSplitB;  // warps
 constexpr int kMmaWarp = kDrain + kSplit, kTmaWarp = kMmaWarp + 1;
-constexpr int kThreads = (kTmaWarp + 1) * 32;  // 128 registers a thread
-constexpr int kStages = 4, kRing = 6;
-constexpr int kStep = 2;   // slices whose h h products share a read-back
+constexpr int kThreads = (kTmaWarp + 1) * 32;  // 112 registers a thread
+constexpr int kStep = 2;   // slices that are loaded, split and multiplied at a time; their h h products share a read-back
 constexpr int kGroup = 2;  // steps whose small products share one
+constexpr int kStages = 2, kRing = 3;  // of a step each
 constexpr int kHalf = 64;  // rows of N per block
 constexpr int BN = 2 * kHalf;
-constexpr int PLANE = kHalf * ROW, STAGE_BYTES = 3 * PLANE;
-constexpr int A_BYTES = BM * BK * 4, SLOT_BYTES = A_BYTES + kHalf * BK * 4;
+constexpr int PLANE = kHalf * ROW, PARTS_BYTES = 3 * PLANE;                        // of a slice
+constexpr int A_BYTES = BM * BK * 4, SLICE_BYTES = A_BYTES + kHalf * BK * 4;  // as loaded
+constexpr int STAGE_BYTES = kStep * PARTS_BYTES, SLOT_BYTES = kStep * SLICE_BYTES;
 constexpr int A_COLS = 3 * BK / 2, A_COL0 = 2 * BN;  // tensor memory: h h sums, small sums, then the M operand's parts
-static_assert(A_COL0 + kStages * A_COLS <= TMEM_COLS, "tensor memory has 512 columns");
+static_assert(A_COL0 + kStages * kStep * A_COLS <= TMEM_COLS, "tensor memory has 512 columns");
 
 struct Control {
     unsigned long long ring_full[kRing];   // TMA bytes of the slot have landed
     unsigned long long ring_empty[kRing];  // the split warps have read the slot
-    unsigned long long full[kStages];      // used on the leader: the slice's parts are in place, split warps of both blocks
-    unsigned long long done[kStages];      // one per block: the MMAs of the slice have completed
+    unsigned long long full[kStages];      // used on the leader: the step's parts are in place, split warps of both blocks
+    unsigned long long done[kStages];      // one per block: the MMAs of the step have completed
     unsigned long long sum_full[2];        // one per block: [0] h h sums of a step, [1] small sums of a group are complete
     unsigned long long sum_empty[2];       // used on the leader: ... and have been read, drain warps of both blocks
     uint32_t tmem_base;
@@ -214,25 +221,28 @@ product_f32_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             bool ok = true;
             for (int t = t0; ok && t < total; t += dt) {
                 const Tile x = tile_at<kMode>(t, ctl->first, g, per, RT, &at);
-                const int slices = x.steps() * kStep, col = x.col + rank * BM;
-                for (int i = 0; i < slices; ++i) {
+                const int steps = x.steps(), col = x.col + rank * BM;
+                for (int i = 0; i < steps; ++i) {
                     if (!(ok = spin(&ctl->ring_empty[slot.at], slot.parity ^ 1, g.wait_cycles, abort_flag))) break;
                     unsigned long long* bar = &ctl->ring_full[slot.at];
                     const uint32_t own = map_to_cta(smem_u32(bar), rank);
-                    uint8_t *a = ring + slot.at * SLOT_BYTES, *b = a + A_BYTES;
-                    const int k = i * BK;
                     mbar_expect_tx(bar, SLOT_BYTES);
-                    if constexpr (kMode == kForward) tma_load_3d_pair(a, &map_a, k, col, x.e, own);
 #pragma unroll
-                    for (int j = 0; j < BM / 32; ++j) {
-                        if constexpr (kMode == kDx) tma_load_3d_pair(a + j * 4096, &map_a, col + 32 * j, k, x.e, own);
-                        if constexpr (kMode == kDw) tma_load_2d(a + j * 4096, &map_a, col + 32 * j, x.k0 + k, bar);
-                    }
-                    if constexpr (kAcrossB) {
-                        tma_load_2d(b, &map_b, x.row + rank * kHalf, x.k0 + k, bar);
-                        tma_load_2d(b + 4096, &map_b, x.row + rank * kHalf + 32, x.k0 + k, bar);
-                    } else {
-                        tma_load_2d(b, &map_b, k, x.row + rank * x.half, bar);
+                    for (int h = 0; h < kStep; ++h) {
+                        uint8_t *a = ring + slot.at * SLOT_BYTES + h * SLICE_BYTES, *b = a + A_BYTES;
+                        const int k = (i * kStep + h) * BK;
+                        if constexpr (kMode == kForward) tma_load_3d_pair(a, &map_a, k, col, x.e, own);
+#pragma unroll
+                        for (int j = 0; j < BM / 32; ++j) {
+                            if constexpr (kMode == kDx) tma_load_3d_pair(a + j * 4096, &map_a, col + 32 * j, k, x.e, own);
+                            if constexpr (kMode == kDw) tma_load_2d(a + j * 4096, &map_a, col + 32 * j, x.k0 + k, bar);
+                        }
+                        if constexpr (kAcrossB) {
+                            tma_load_2d(b, &map_b, x.row + rank * kHalf, x.k0 + k, bar);
+                            tma_load_2d(b + 4096, &map_b, x.row + rank * kHalf + 32, x.k0 + k, bar);
+                        } else {
+                            tma_load_2d(b, &map_b, k, x.row + rank * x.half, bar);
+                        }
                     }
                     slot.next();
                 }
@@ -258,22 +268,19 @@ product_f32_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 const Tile x = tile_at<kMode>(t, ctl->first, g, per, RT, &at);
                 const int steps = uniform(x.steps());
                 const uint32_t idesc = make_instr_desc_bf16(2 * BM, uniform(2 * x.half)) | (kAcrossB ? kBMajor : 0u);
-                auto multiply = [&](int stage, int pa, int pb, uint32_t d, bool more) {
-                    const uint32_t ta = tmem + A_COL0 + stage * A_COLS + pa * (BK / 2);
-                    const uint64_t db = part_desc<kAcrossB>(parts + stage * STAGE_BYTES + pb * PLANE);
+                auto multiply = [&](int slice, int pa, int pb, uint32_t d, bool more) {  // slice: of all stages
+                    const uint32_t ta = tmem + A_COL0 + slice * A_COLS + pa * (BK / 2);
+                    const uint64_t db = part_desc<kAcrossB>(parts + slice * PARTS_BYTES + pb * PLANE);
 #pragma unroll
                     for (int k = 0; k < BK / 16; ++k)
                         umma_ta(elected, d, ta + k * 8, db + (kAcrossB ? kMajorStep / 16 : 2u) * k, idesc, (more || k > 0) ? 1u : 0u);
                 };
                 for (int kd = 0; kd < steps; ++kd) {
-                    ok = wait(&ctl->sum_empty[0], hp ^ 1);
+                    ok = wait(&ctl->sum_empty[0], hp ^ 1) && wait(&ctl->full[s], sp);
+                    if (!ok) break;
                     hp ^= 1;
 #pragma unroll
-                    for (int j = 0; j < kStep; ++j) {
-                        ok = ok && wait(&ctl->full[s + j], sp);
-                        if (ok) multiply(s + j, 0, 0, tmem, j > 0);
-                    }
-                    if (!ok) break;
+                    for (int j = 0; j < kStep; ++j) multiply(s * kStep + j, 0, 0, tmem, j > 0);
                     umma_commit_both_if(elected, bars + (uint32_t)offsetof(Control, sum_full));
                     const bool first = kd % kGroup == 0;
                     if (first) {
@@ -281,14 +288,12 @@ product_f32_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                         lp ^= 1;
                     }
 #pragma unroll
-                    for (int j = 0; j < kStep; ++j) {
+                    for (int j = 0; j < kStep; ++j)
 #pragma unroll
-                        for (int p = 0; p < 5; ++p) multiply(s + j, kPartA[p], kPartB[p], tmem + BN, !first || (j | p) != 0);
-                        umma_commit_both_if(elected, bars + (uint32_t)offsetof(Control, done) + 8 * (s + j));
-                    }
+                        for (int p = 0; p < 5; ++p) multiply(s * kStep + j, kPartA[p], kPartB[p], tmem + BN, !first || (j | p) != 0);
+                    umma_commit_both_if(elected, bars + (uint32_t)offsetof(Control, done) + 8 * s);
                     if (kd + 1 == steps || kd % kGroup == kGroup - 1) umma_commit_both_if(elected, bars + (uint32_t)offsetof(Control, sum_full) + 8);
-                    s += kStep;
-                    if (s == kStages) s = 0, sp ^= 1;
+                    if (++s == kStages) s = 0, sp ^= 1;
                 }
             }
         }
@@ -301,66 +306,72 @@ product_f32_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         bool ok = true;
         for (int t = t0; ok && t < total; t += dt) {
             const Tile x = tile_at<kMode>(t, ctl->first, g, per, RT, &at);
-            const int slices = x.steps() * kStep;
-            for (int i = 0; i < slices; ++i) {
-                // the stage is free once the MMAs of the slice before in it have completed
+            const int steps = x.steps();
+            for (int i = 0; i < steps; ++i) {
+                // the stage is free once the MMAs of the step before in it have completed
                 ok = spin(&ctl->done[stage.at], stage.parity ^ 1, g.wait_cycles, abort_flag) &&
                      spin(&ctl->ring_full[slot.at], slot.parity, g.wait_cycles, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                const uint8_t* src = ring + slot.at * SLOT_BYTES;
-                const int valid = kMode == kDw ? x.len - i * BK : BK;  // steps of the slice that are the expert's rows
-                if (m_side) {
-                    uint32_t h[16], m[16], l[16];
+                tc_fence_after();
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        float v[4];
-                        if constexpr (kAcrossA) {
+                for (int half = 0; half < kStep; ++half) {
+                    const uint8_t* src = ring + slot.at * SLOT_BYTES + half * SLICE_BYTES;
+                    const int valid = kMode == kDw ? x.len - (i * kStep + half) * BK : BK;  // steps of the slice that are the expert's rows
+                    if (m_side) {
+                        uint32_t h[16], m[16], l[16];
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const int k = 4 * c + j;
-                                v[j] = *reinterpret_cast<const float*>(src + q * 4096 + k * 128 + (((lane >> 2) ^ (k & 7)) << 4) + (lane & 3) * 4);
-                                if (kMode == kDw && k >= valid) v[j] = 0.f;
+                        for (int c = 0; c < 8; ++c) {
+                            float v[4];
+                            if constexpr (kAcrossA) {
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const int k = 4 * c + j;
+                                    v[j] = *reinterpret_cast<const float*>(src + q * 4096 + k * 128 + (((lane >> 2) ^ (k & 7)) << 4) + (lane & 3) * 4);
+                                    if (kMode == kDw && k >= valid) v[j] = 0.f;
+                                }
+                            } else {
+                                const float4 f = *reinterpret_cast<const float4*>(src + line * 128 + ((c ^ (line & 7)) << 4));
+                                v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
                             }
-                        } else {
-                            const float4 f = *reinterpret_cast<const float4*>(src + line * 128 + ((c ^ (line & 7)) << 4));
-                            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+                            split4(v, reinterpret_cast<uint2*>(h + 2 * c), reinterpret_cast<uint2*>(m + 2 * c), reinterpret_cast<uint2*>(l + 2 * c));
                         }
-                        split4(v, reinterpret_cast<uint2*>(h + 2 * c), reinterpret_cast<uint2*>(m + 2 * c), reinterpret_cast<uint2*>(l + 2 * c));
+                        const uint32_t ta = tmem_base + A_COL0 + (stage.at * kStep + half) * A_COLS + (static_cast<uint32_t>(q * 32) << 16);
+                        tmem_st_32x16(ta, h);
+                        tmem_st_32x16(ta + BK / 2, m);
+                        tmem_st_32x16(ta + BK, l);
+                    } else {
+                        src += A_BYTES;
+                        uint8_t* dst = stages + stage.at * STAGE_BYTES + half * PARTS_BYTES;
+#pragma unroll
+                        for (int j = 0; j < 16 / kSplitB; ++j) {
+                            uint32_t from, to;
+                            bool in = true;
+                            if constexpr (kAcrossB) {  // four columns of step k
+                                const int k = (tb >> 4) + 2 * kSplitB * j, c = tb & 15;
+                                from = (uint32_t)((c >> 3) * 4096 + k * 128 + (((c & 7) ^ (k & 7)) << 4));
+                                to = (uint32_t)(k * 128 + (((c >> 1) ^ (k & 7)) << 4) + ((c & 1) << 3));
+                                in = k < valid;
+                            } else {  // four steps of row r
+                                const int r = (tb >> 3) + 4 * kSplitB * j, c = tb & 7;
+                                if (r >= x.half) break;
+                                from = (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
+                                to = (uint32_t)(r * ROW + (((c >> 1) ^ ((r >> 1) & 3)) << 4) + ((c & 1) << 3));
+                            }
+                            const float4 f = *reinterpret_cast<const float4*>(src + from);
+                            const float v[4] = {in ? f.x : 0.f, in ? f.y : 0.f, in ? f.z : 0.f, in ? f.w : 0.f};
+                            uint2 h, m, l;
+                            split4(v, &h, &m, &l);
+                            *reinterpret_cast<uint2*>(dst + to) = h;
+                            *reinterpret_cast<uint2*>(dst + to + PLANE) = m;
+                            *reinterpret_cast<uint2*>(dst + to + 2 * PLANE) = l;
+                        }
                     }
-                    tc_fence_after();
-                    const uint32_t ta = tmem_base + A_COL0 + stage.at * A_COLS + (static_cast<uint32_t>(q * 32) << 16);
-                    tmem_st_32x16(ta, h);
-                    tmem_st_32x16(ta + BK / 2, m);
-                    tmem_st_32x16(ta + BK, l);
+                }
+                if (m_side) {
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     tc_fence_before();
                 } else {
-                    src += A_BYTES;
-                    uint8_t* dst = stages + stage.at * STAGE_BYTES;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        uint32_t from, to;
-                        bool in = true;
-                        if constexpr (kAcrossB) {  // four columns of step k
-                            const int k = (tb >> 4) + 4 * j, c = tb & 15;
-                            from = (uint32_t)((c >> 3) * 4096 + k * 128 + (((c & 7) ^ (k & 7)) << 4));
-                            to = (uint32_t)(k * 128 + (((c >> 1) ^ (k & 7)) << 4) + ((c & 1) << 3));
-                            in = k < valid;
-                        } else {  // four steps of row r
-                            const int r = (tb >> 3) + 8 * j, c = tb & 7;
-                            if (r >= x.half) break;
-                            from = (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
-                            to = (uint32_t)(r * ROW + (((c >> 1) ^ ((r >> 1) & 3)) << 4) + ((c & 1) << 3));
-                        }
-                        const float4 f = *reinterpret_cast<const float4*>(src + from);
-                        const float v[4] = {in ? f.x : 0.f, in ? f.y : 0.f, in ? f.z : 0.f, in ? f.w : 0.f};
-                        uint2 h, m, l;
-                        split4(v, &h, &m, &l);
-                        *reinterpret_cast<uint2*>(dst + to) = h;
-                        *reinterpret_cast<uint2*>(dst + to + PLANE) = m;
-                        *reinterpret_cast<uint2*>(dst + to + 2 * PLANE) = l;
-                    }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
                 __syncwarp();

@@ -22,7 +22,7 @@
 // line; what is contiguous across them comes in tiles of 32 x 32 that are read down a column (M operand) or split into
 // N-major parts (N operand).  Rows that are not the expert's are cleared when they are split.
 //
-// What bounds it: the split warps (2048 columns, 256 rows an expert: a step of 64 takes about 2500 cycles, its MMAs
+// What bounds it: the split warps (2048 columns, 256 rows an expert: a step of 64 takes about 2600 cycles, its MMAs
 // 1536 of them; tensor pipe 42 % active), and 4.3 tiles a pair of blocks in five rounds.  4096 rows, 16 experts, N = K =
 // 2048: 252, 251 and 288 us (34.4 GFLOP each: 137, 137 and 119 TFLOP/s; the FP32 pipes 1014, 965 and 734), 1.7e-7 from the
 // 64-bit result (FP32 pipes: 8.1e-7).  A step a barrier instead of a slice and four warps for the N operand instead of two:

@@ -100,8 +100,8 @@ __device__ __forceinline__ float2 row_sum(float a, float b, float2 (*shared)[32]
     return make_float2(a, b);
 }
 
-// Rows on their way to shared memory: tiles of `per` rows of one or two matrices (row i of matrix m of a stage is the
-// stage's row m * per + i), kDepth of them in flight, each filled by bulk copies that one thread issues.
+// Rows on their way to the shared memory of the threads that share a row: one row of one or two matrices a stage, `depth` of
+// them in flight, filled by bulk copies that one thread issues.
 constexpr int kMostDepth = 8;
 template <typename T, int kMatrices>
 struct Ring {
@@ -109,18 +109,16 @@ struct Ring {
     unsigned long long* full;  // [depth]
     const T* from[kMatrices];
     long long ld[kMatrices];
-    int depth, per, H, total;  // total: rows of the matrices
-    // One thread: rows r0 .. r0 + per - 1 to stage s.
-    __device__ __forceinline__ void issue(long long r0, int s) const {
-        if (r0 >= total) return;
-        const int n = (int)min((long long)per, total - r0);
+    int depth, H, total;  // total: rows of the matrices
+    // One thread: row r to stage s.
+    __device__ __forceinline__ void issue(long long r, int s) const {
+        if (r >= total) return;
         const uint32_t bytes = (uint32_t)(H * sizeof(T));
-        tc::mbar_expect_tx(&full[s], kMatrices * n * bytes);
-        for (int m = 0; m < kMatrices; ++m)
-            for (int k = 0; k < n; ++k)
-                tc::bulk_load(rows + (size_t)((s * kMatrices + m) * per + k) * H, from[m] + (r0 + k) * ld[m], bytes, &full[s]);
+        tc::mbar_expect_tx(&full[s], kMatrices * bytes);
+#pragma unroll
+        for (int m = 0; m < kMatrices; ++m) tc::bulk_load(rows + (s * kMatrices + m) * H, from[m] + r * ld[m], bytes, &full[s]);
     }
-    __device__ __forceinline__ const T* row(int s, int m, int k) const { return rows + (s * kMatrices + m) * per * H + k * H; }
+    __device__ __forceinline__ const T* row(int s, int m) const { return rows + (s * kMatrices + m) * H; }
     // False when the copies did not come in about ten seconds: the caller's results are NaN then.
     __device__ __forceinline__ bool wait(int s, uint32_t parity) const {
         if (tc::mbar_try_wait(&full[s], parity)) return true;
@@ -131,12 +129,11 @@ struct Ring {
     }
 };
 template <typename T, int kMatrices>
-__device__ __forceinline__ Ring<T, kMatrices> make_ring(void* smem, unsigned long long* full, const Args& a, int depth, int per, bool first) {
+__device__ __forceinline__ Ring<T, kMatrices> make_ring(void* smem, unsigned long long* full, const Args& a, bool first) {
     Ring<T, kMatrices> r;
     r.rows = static_cast<T*>(smem);
     r.full = full;
-    r.depth = depth;
-    r.per = per;
+    r.depth = a.depth;
     r.H = a.H;
     r.total = a.rows;
     r.from[0] = static_cast<const T*>(a.x);
@@ -146,7 +143,7 @@ __device__ __forceinline__ Ring<T, kMatrices> make_ring(void* smem, unsigned lon
         r.ld[1] = a.lddy;
     }
     if (first) {
-        for (int i = 0; i < depth; ++i) tc::mbar_init(&full[i], 1);
+        for (int i = 0; i < a.depth; ++i) tc::mbar_init(&full[i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
@@ -161,22 +158,34 @@ __device__ __forceinline__ void each_vector(int at, int H, F f) {
         if ((at + i * G) * V < H) f(i, (at + i * G) * V);
 }
 
-// Rows that can be copied in bulk.  G threads a row, N vectors of V elements each; rows of a tile = blockDim / G.  The
-// block meets once a tile: every warp sums the squares around its own mean, and what the warps' means differ by from
-// the row's is added when they meet (the same sum, without a second round).
+// The G threads of a row meet: a warp, or as many as share the named barrier of their group.
+template <int G>
+__device__ __forceinline__ void meet(int group) {
+    if constexpr (G == 32) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(G) : "memory");
+}
+
+// Rows that can be copied in bulk.  G threads have a row, N vectors of V elements each; the block's groups of G threads go
+// through rows of their own, each with a ring and a barrier.  A group meets once a row: every warp sums the squares
+// around its own mean, and what the warps' means differ by from the row's is added when they meet (the same sum,
+// without a second round).
+template <int G>
+constexpr int kForwardGroups = G < 256 ? 256 / G : 1;
+
 template <typename T, int V, int G, int N>
-__global__ void __launch_bounds__(G > 256 ? G : 256, G > 256 ? 1 : 2) forward_kernel(Args a) {
+__global__ void __launch_bounds__(G * kForwardGroups<G>, G > 256 ? 1 : 2) forward_kernel(Args a) {
+    constexpr int P = kForwardGroups<G>, W = G / 32;
+    static_assert(W == 1 || P < 16, "sixteen named barriers");
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ unsigned long long full[kMostDepth];
-    __shared__ float2 shared[2][16];
-    __shared__ float share[16];  // values of a row that a warp holds
-    constexpr int W = G / 32;
-    const int at = threadIdx.x % G, group = threadIdx.x / G, per = blockDim.x / G, H = a.H, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const auto ring = make_ring<T, 1>(smem, full, a, a.depth, per, threadIdx.x == 0);
-    const long long step = (long long)gridDim.x * per, first = (long long)blockIdx.x * per;
+    __shared__ unsigned long long full[P][kMostDepth];
+    __shared__ float2 shared[P][2][W];
+    __shared__ float share[P][W];  // values of a row that a warp holds
+    const int at = threadIdx.x % G, group = threadIdx.x / G, H = a.H, warp = at >> 5, lane = threadIdx.x & 31;
+    const auto ring = make_ring<T, 1>(smem + (size_t)group * a.depth * H * sizeof(T), full[group], a, at == 0);
+    const long long step = (long long)gridDim.x * P, first = blockIdx.x + (long long)group * gridDim.x;
     pdl_wait();
     pdl_trigger();
-    if (threadIdx.x == 0)
+    if (at == 0)
         for (int i = 0; i < a.depth; ++i) ring.issue(first + i * step, i);
     const float inv = 1.f / (float)H;
     F2 w[N][V / 2], b[N][V / 2];
@@ -187,44 +196,40 @@ __global__ void __launch_bounds__(G > 256 ? G : 256, G > 256 ? 1 : 2) forward_ke
         load_params<T, V>(a.bias, j, a.wide, a.param_vec, 0.f, b[i]);
     });
     const float n = warp_sum(mine), inv_n = n > 0.f ? 1.f / n : 0.f;
-    if (lane == 0) share[warp] = n;
+    if (lane == 0) share[group][warp] = n;
     __syncthreads();
-    const float my_share = share[group * W + lane % W];  // of the warp that this lane answers for
-    int stage = 0;
+    const float my_share = share[group][lane % W];  // of the warp that this lane answers for
+    int stage = 0, turn = 0;
     uint32_t parity = 0;
-    long long r = first + group;
-    for (int tile = 0; r - group < a.rows; r += step, ++tile) {
-        const bool came = ring.wait(stage, parity), real = r < a.rows;
+    for (long long r = first; r < a.rows; r += step, turn ^= 1) {
+        const bool came = ring.wait(stage, parity);
         F2 x[N][V / 2], s = both(0.f);
-        if (real)
-            each_vector<V, G, N>(at, H, [&](int i, int j) {
-                to_pairs<T, V>(load_vec<T, V>(ring.row(stage, 0, group) + j), x[i]);
+        each_vector<V, G, N>(at, H, [&](int i, int j) {
+            to_pairs<T, V>(load_vec<T, V>(ring.row(stage, 0) + j), x[i]);
 #pragma unroll
-                for (int k = 0; k < V / 2; ++k) s = add2(s, x[i][k]);
-            });
+            for (int k = 0; k < V / 2; ++k) s = add2(s, x[i][k]);
+        });
         float m = warp_sum(sum2(s)) * inv_n;
         F2 q2 = both(0.f);
         const F2 minus = both(-m);
-        if (real)
-            each_vector<V, G, N>(at, H, [&](int i, int) {
+        each_vector<V, G, N>(at, H, [&](int i, int) {
 #pragma unroll
-                for (int k = 0; k < V / 2; ++k) {
-                    const F2 d = add2(x[i][k], minus);
-                    q2 = fma2(d, d, q2);
-                }
-            });
+            for (int k = 0; k < V / 2; ++k) {
+                const F2 d = add2(x[i][k], minus);
+                q2 = fma2(d, d, q2);
+            }
+        });
         float q = warp_sum(sum2(q2));
-        if (W > 1 && lane == 0) shared[tile & 1][warp] = make_float2(m, q);
-        __syncthreads();  // ... and the tile is in registers
-        if (threadIdx.x == 0) ring.issue(r - group + a.depth * step, stage);
+        if (W > 1 && lane == 0) shared[group][turn][warp] = make_float2(m, q);
+        meet<G>(group);  // ... and the row is in registers
+        if (at == 0) ring.issue(r + a.depth * step, stage);
         if (++stage == a.depth) stage = 0, parity ^= 1;
         if constexpr (W > 1) {
-            const float2 v = shared[tile & 1][group * W + lane % W];
+            const float2 v = shared[group][turn][lane % W];
             m = lanes_sum<W>(v.x * my_share) * inv;
             const float d = v.x - m;
             q = lanes_sum<W>(fmaf(my_share * d, d, v.y));
         }
-        if (!real) continue;
         const float rs = came ? rsqrtf(q * inv + a.eps) : __uint_as_float(0x7fffffffu);
         T* y = static_cast<T*>(a.y) + r * a.ldy;
         const F2 rs2 = both(rs), m2 = both(-m);
@@ -340,6 +345,7 @@ __device__ __forceinline__ void weights_at(const float* p, F2 (&w)[V / 2]) {
 template <typename T, int V, int G, int N>
 __global__ void __launch_bounds__(G * kGroups<G>, 1) backward_kernel(Args a) {
     constexpr int P = kGroups<G>, W = G / 32;
+    static_assert(W == 1 || P < 16, "sixteen named barriers");
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ unsigned long long full[P][kMostDepth];
     __shared__ float shared[P][2][2][W];
@@ -347,7 +353,7 @@ __global__ void __launch_bounds__(G * kGroups<G>, 1) backward_kernel(Args a) {
     // weights as floats, then the groups' rings
     float* weight = reinterpret_cast<float*>(smem);
     unsigned char* rings = smem + (size_t)(H * 4 + 127) / 128 * 128;
-    const auto ring = make_ring<T, 2>(rings + (size_t)group * a.depth * 2 * H * sizeof(T), full[group], a, a.depth, 1, at == 0);
+    const auto ring = make_ring<T, 2>(rings + (size_t)group * a.depth * 2 * H * sizeof(T), full[group], a, at == 0);
     const long long step = (long long)gridDim.x * P, first = blockIdx.x + (long long)group * gridDim.x;
     pdl_wait();
     pdl_trigger();
@@ -370,7 +376,7 @@ __global__ void __launch_bounds__(G * kGroups<G>, 1) backward_kernel(Args a) {
         float m = next_m, rs = next_rs;
         if (r + step < a.rows) next_m = a.mean[r + step], next_rs = a.rstd[r + step];
         if (!ring.wait(stage, parity)) rs = __uint_as_float(0x7fffffffu);
-        const T *px = ring.row(stage, 0, 0), *pdy = ring.row(stage, 1, 0);
+        const T *px = ring.row(stage, 0), *pdy = ring.row(stage, 1);
         const F2 rs2 = both(rs), m2 = both(-m);
         F2 h[N][V / 2], g[N][V / 2], sg2 = both(0.f), sgh2 = both(0.f);
         each_vector<V, G, N>(at, H, [&](int i, int j) {
@@ -393,7 +399,7 @@ __global__ void __launch_bounds__(G * kGroups<G>, 1) backward_kernel(Args a) {
         if constexpr (W > 1) {
             float (*s)[W] = shared[group][turn & 1];
             if ((lane & 15) == 0) s[lane >> 4][warp] = mine;
-            asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(G) : "memory");
+            meet<G>(group);
             sg = sgh = 0.f;
 #pragma unroll
             for (int i = 0; i < W; ++i) {
@@ -401,6 +407,7 @@ __global__ void __launch_bounds__(G * kGroups<G>, 1) backward_kernel(Args a) {
                 sgh += s[1][i];
             }
         } else {
+            meet<G>(group);
             sg = __shfl_sync(0xffffffffu, mine, 0);
             sgh = __shfl_sync(0xffffffffu, mine, 16);
         }

@@ -21,6 +21,8 @@ using namespace ops;
 
 size_t bytes_of(int torch_dtype) { return torch_dtype == 0 ? 4 : 2; }
 bool known_type(int torch_dtype) { return torch_dtype == 0 || torch_dtype == 2 || torch_dtype == 3; }
+constexpr int kMostColumns = 1 << 28;
+constexpr char kNormSizes[] = "rows must be 0 or more, H from 1 to 2^28, and no row longer than its stride";
 constexpr char kTypes[] = "torch_dtype must be 0 (float), 2 (bf16) or 3 (fp16)";
 
 // Whether every pointer (null ones too) is where an element of so many bytes may be.
@@ -53,15 +55,14 @@ cudaError_t norm_forward(norm::Args a, cudaStream_t st) {
     bool done;
     if (by_16(sizeof(T), {a.x, a.y}, {a.ldx, a.ldy, a.H})) {
         done = norm::with_shape<W>(a.H, [&](auto g, auto n) {
-            constexpr int G = decltype(g)::value, kThreads = G > 256 ? G : 256, per = kThreads / G;
+            constexpr int G = decltype(g)::value, P = norm::kForwardGroups<G>, kThreads = G * P;
             const auto kernel = norm::forward_kernel<T, W, G, decltype(n)::value>;
-            const size_t stage = (size_t)per * a.H * sizeof(T);
-            const int tiles = (a.rows + per - 1) / per;
+            const size_t stage = (size_t)P * a.H * sizeof(T);
             static bool allowed[64];
             rc = allow_smem(kernel, allowed, kRingMost);
             a.depth = ring_depth(stage, G > 256 ? 98304 : 49152);
-            const int blocks = tiles <= sms ? tiles : std::min(tiles, std::max(1, resident_blocks(kernel, kThreads, a.depth * stage)));
-            a.depth = std::min(a.depth, (tiles + blocks - 1) / blocks);
+            const int blocks = a.rows <= sms ? a.rows : std::min((a.rows + P - 1) / P, std::max(1, resident_blocks(kernel, kThreads, a.depth * stage)));
+            a.depth = std::min(a.depth, (a.rows + blocks * P - 1) / (blocks * P));
             if (rc == cudaSuccess) rc = launch(kernel, dim3(blocks), kThreads, a.depth * stage, 1, st, a);
         });
     } else {
@@ -149,7 +150,7 @@ struct CombineBack {
 
 const char* bad_places(int T, int K, int H, long long ld) {
     if (T < 0 || K < 1 || K > kMaxTopK || (long long)T * K > 0x7fffff00LL) return "T must be 0 or more, K from 1 to 8, T * K below 2^31";
-    if (H < 1 || ld < H) return "H must be 1 or more, and no row longer than its stride";
+    if (H < 1 || H > kMostColumns || ld < H) return "H must be from 1 to 2^28, and no row longer than its stride";
     return nullptr;
 }
 
@@ -310,6 +311,9 @@ int products(const char* call, const experts::Args& a, int torch_dtype, cudaStre
 const char* bad_products(int rows, int E, int N, int K, long long ld_n, long long ld_k) {
     if (rows < 0 || rows > 0x7fff0000 || E < 1 || E > kMaxExperts) return "rows must be 0 or more, E from 1 to 1024";
     if (N < 1 || K < 1 || N > 1 << 22 || K > 1 << 22) return "N and K must be from 1 to 2^22";
+    // tiles are counted in ints: of rows by columns, and of the weights
+    const long long n = (N + 127) / 128, k = (K + 127) / 128;
+    if ((rows / 32 + (long long)E + 1) * std::max(n, k) > 0x7fffffff || E * n * k > 0x7fffffff) return "too many experts, rows and columns at once";
     if (ld_n < N || ld_k < K) return "no row may be longer than its stride";
     return nullptr;
 }
@@ -321,14 +325,14 @@ using namespace kleos;
 
 extern "C" {
 
-long long kleos_layer_norm_workspace(int H) { return H < 1 ? KLEOS_E_ARG : (long long)norm::kMaxPartials * 2 * H * (long long)sizeof(float); }
+long long kleos_layer_norm_workspace(int H) { return H < 1 || H > kMostColumns ? KLEOS_E_ARG : (long long)norm::kMaxPartials * 2 * H * (long long)sizeof(float); }
 
 int kleos_layer_norm(const void* x, long long ldx, const void* weight, const void* bias, int rows, int H, float eps,
                      int torch_dtype, int param_dtype, void* y, long long ldy, float* mean, float* rstd, void* stream) {
     const char* call = "kleos_layer_norm";
     if (!known_type(torch_dtype)) return refuse(call, KLEOS_E_UNSUPPORTED, kTypes);
     if (param_dtype != 0 && param_dtype != torch_dtype) return refuse(call, KLEOS_E_UNSUPPORTED, "param_dtype must be 0 (float) or the element type");
-    if (rows < 0 || H < 1 || ldx < H || ldy < H) return refuse(call, KLEOS_E_ARG, "rows must be 0 or more, H 1 or more, and no row longer than its stride");
+    if (rows < 0 || H < 1 || H > kMostColumns || ldx < H || ldy < H) return refuse(call, KLEOS_E_ARG, kNormSizes);
     if (!(eps >= 0.f)) return refuse(call, KLEOS_E_ARG, "eps must not be negative");
     if (rows == 0) return KLEOS_OK;
     if (!x || !y) return refuse(call, KLEOS_E_ARG, "null device pointer");
@@ -347,7 +351,7 @@ int kleos_layer_norm_backward(const void* dy, long long lddy, const void* x, lon
     const char* call = "kleos_layer_norm_backward";
     if (!known_type(torch_dtype)) return refuse(call, KLEOS_E_UNSUPPORTED, kTypes);
     if (param_dtype != 0 && param_dtype != torch_dtype) return refuse(call, KLEOS_E_UNSUPPORTED, "param_dtype must be 0 (float) or the element type");
-    if (rows < 0 || H < 1 || ldx < H || lddy < H || lddx < H) return refuse(call, KLEOS_E_ARG, "rows must be 0 or more, H 1 or more, and no row longer than its stride");
+    if (rows < 0 || H < 1 || H > kMostColumns || ldx < H || lddy < H || lddx < H) return refuse(call, KLEOS_E_ARG, kNormSizes);
     if (rows > 0 && (!dy || !x || !mean || !rstd || !dx)) return refuse(call, KLEOS_E_ARG, "null device pointer");
     const bool sums = dweight || dbias;
     if (sums && (!workspace || !aligned(workspace, 16) || workspace_bytes < kleos_layer_norm_workspace(H)))

@@ -34,6 +34,11 @@ DW = [ONE, 32, ONE, 64, ONE, 4, 2, 32, 64, 2, 2, ONE, ONE, None]
     ("kleos_layer_norm", NORM, 5, 0, ARG), ("kleos_layer_norm", NORM, 1, 63, ARG), ("kleos_layer_norm", NORM, 10, 63, ARG),
     ("kleos_layer_norm", NORM, 6, -1e-5, ARG), ("kleos_layer_norm", NORM, 6, float("nan"), ARG), ("kleos_layer_norm", NORM, 0, ONE + 1, ARG),
     ("kleos_layer_norm", NORM, 2, ONE + 1, ARG), ("kleos_layer_norm", NORM, 11, ONE + 2, ARG),
+    ("kleos_layer_norm", _changed(_changed(NORM, 1, 1 << 40), 10, 1 << 40), 5, (1 << 28) + 1, ARG),
+    ("kleos_gather_tokens", _changed(GATHER, 1, 1 << 40), 7, (1 << 28) + 1, ARG),
+    ("kleos_expert_products", PRODUCTS, 7, (1 << 22) + 1, ARG),
+    ("kleos_expert_products", _changed(_changed(PRODUCTS, 5, 0x7fff0000), 11, 1 << 22), 7, 1 << 22, ARG),   # tiles past 2^31
+    ("kleos_expert_products_dw", _changed(_changed(_changed(DW, 1, 1 << 22), 3, 1 << 22), 7, 1 << 22), 8, 1 << 22, ARG),
     ("kleos_layer_norm_backward", BACK, 15, None, ARG), ("kleos_layer_norm_backward", BACK, 16, 296 * 2 * 4 * 64 - 1, ARG),
     ("kleos_layer_norm_backward", BACK, 15, ONE + 8, ARG), ("kleos_layer_norm_backward", BACK, 5, None, ARG),
     ("kleos_layer_norm_backward", BACK, 11, None, ARG), ("kleos_layer_norm_backward", BACK, 12, 32, ARG),

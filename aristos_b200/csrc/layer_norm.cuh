@@ -246,38 +246,60 @@ __global__ void __launch_bounds__(G * kForwardGroups<G>, G > 256 ? 1 : 2) forwar
     }
 }
 
-// Any other row of up to G * N elements, a block a row, loaded one by one while the row before is added up.
+// Any other row, loaded element by element while the row before it is added up.  (16384 rows of 4092 bf16, whose rows begin on
+// 8-byte boundaries: two elements at a time took 158 us forward and 165 back, one at a time 98 and 132.)
 template <typename T, int G, int N>
-__global__ void __launch_bounds__(G) forward_odd_kernel(Args a) {
-    __shared__ float2 shared[2][32];
+struct Row {
+    T v[N];
+    __device__ __forceinline__ void fetch(const void* p, long long at_element, int at, int H) {
+        const T* row = static_cast<const T*>(p) + at_element;
+        each_vector<1, G, N>(at, H, [&](int i, int j) { v[i] = row[j]; });
+    }
+    __device__ __forceinline__ float operator[](int i) const { return Elem<T>::to_f(v[i]); }
+};
+
+template <typename T, int G, int N>
+__global__ void __launch_bounds__(G * kForwardGroups<G>, G > 256 ? 1 : 2) forward_odd_kernel(Args a) {
+    constexpr int P = kForwardGroups<G>, W = G / 32;
+    __shared__ float2 shared[P][2][W];
+    const int at = threadIdx.x % G, group = threadIdx.x / G, H = a.H, warp = at >> 5, lane = threadIdx.x & 31;
+    const long long step = (long long)gridDim.x * P, first = blockIdx.x + (long long)group * gridDim.x;
     pdl_wait();
     pdl_trigger();
-    const int at = threadIdx.x, H = a.H;
     const float inv = 1.f / (float)H;
-    float next[N], x[N];
-    auto fetch = [&](long long r) {
-        const T* row = static_cast<const T*>(a.x) + r * a.ldx;
-        each_vector<1, G, N>(at, H, [&](int i, int j) { next[i] = Elem<T>::to_f(row[j]); });
+    auto sum = [&](float v, int turn) {
+        v = warp_sum(v);
+        if constexpr (W > 1) {
+            if (lane == 0) shared[group][turn][warp].x = v;
+            meet<G>(group);
+            v = lanes_sum<W>(shared[group][turn][lane % W].x);
+        }
+        return v;
     };
-    long long r = blockIdx.x;
-    if (r < a.rows) fetch(r);
-    for (int turn = 0; r < a.rows; r += gridDim.x, turn += 2) {
-        float s = 0.f;
+    float w[N], b[N];
+    each_vector<1, G, N>(at, H, [&](int i, int j) {
+        w[i] = param<T>(a.weight, j, a.wide, 1.f);
+        b[i] = param<T>(a.bias, j, a.wide, 0.f);
+    });
+    Row<T, G, N> next;
+    if (first < a.rows) next.fetch(a.x, first * a.ldx, at, H);
+    for (long long r = first; r < a.rows; r += step) {
+        float x[N], s = 0.f;
         each_vector<1, G, N>(at, H, [&](int i, int) {
             x[i] = next[i];
             s += x[i];
         });
-        if (r + gridDim.x < a.rows) fetch(r + gridDim.x);
-        const float m = row_sum<G>(s, 0.f, shared, turn).x * inv;
+        if (r + step < a.rows) next.fetch(a.x, (r + step) * a.ldx, at, H);
+        const float m = sum(s, 0) * inv;
         s = 0.f;
         each_vector<1, G, N>(at, H, [&](int i, int) {
             const float d = x[i] - m;
             s = fmaf(d, d, s);
         });
-        const float rs = rsqrtf(row_sum<G>(s, 0.f, shared, turn + 1).x * inv + a.eps);
+        const float rs = rsqrtf(sum(s, 1) * inv + a.eps);
         T* y = static_cast<T*>(a.y) + r * a.ldy;
         each_vector<1, G, N>(at, H, [&](int i, int j) {
-            y[j] = Elem<T>::from_f(fmaf((x[i] - m) * rs, param<T>(a.weight, j, a.wide, 1.f), param<T>(a.bias, j, a.wide, 0.f)));
+            y[j] = Elem<T>::from_f(fmaf((x[i] - m) * rs, w[i], b[i]));
         });
         if (at == 0) {
             if (a.mean) a.mean[r] = m;
@@ -332,6 +354,17 @@ __device__ __forceinline__ float warp_sums(float a, float b) {
 template <int G>
 constexpr int kGroups = 512 / G;
 
+// out[j] = sum of the groups' sums[p][j], in their order; all threads of the block call it.
+template <int P>
+__device__ __forceinline__ void add_groups(float* out, const float* sums, int n) {
+    __syncthreads();
+    for (int j = threadIdx.x; j < n; j += blockDim.x) {
+        float v = sums[j];
+#pragma unroll
+        for (int p = 1; p < P; ++p) v += sums[p * n + j];
+        out[j] = v;
+    }
+}
 // V floats of shared memory as pairs.
 template <int V>
 __device__ __forceinline__ void weights_at(const float* p, F2 (&w)[V / 2]) {
@@ -423,71 +456,80 @@ __global__ void __launch_bounds__(G * kGroups<G>, 1) backward_kernel(Args a) {
         if (++stage == a.depth) stage = 0, parity ^= 1;
     }
     if (!a.partial) return;
-    float* out = a.partial + (size_t)blockIdx.x * 2 * H;
-    float* sums = reinterpret_cast<float*>(rings);  // [2 * H]: every row has been read
-    // the groups' sums, added in their order
-    for (int p = 0; p < P; ++p) {
-        __syncthreads();
-        if (group != p) continue;
-        float* to = p < P - 1 ? sums : out;
-        each_vector<V, G, N>(at, H, [&](int i, int j) {
+    // the groups' sums side by side in shared memory, then added in their order
+    float *out = a.partial + (size_t)blockIdx.x * 2 * H, *to = out;
+    float* sums = reinterpret_cast<float*>(rings);  // [P][2 * H]: every row has been read
+    __syncthreads();
+    if (P > 1) to = sums + (size_t)group * 2 * H;
+    each_vector<V, G, N>(at, H, [&](int i, int j) {
 #pragma unroll
-            for (int c = 0; c < V; ++c) {
-                const float2 u = split(dw[i][c / 2]), v = split(db[i][c / 2]);
-                const float f = c & 1 ? u.y : u.x, e = c & 1 ? v.y : v.x;
-                to[j + c] = p ? sums[j + c] + f : f;
-                to[H + j + c] = p ? sums[H + j + c] + e : e;
-            }
-        });
-    }
+        for (int c = 0; c < V; ++c) {
+            const float2 u = split(dw[i][c / 2]), v = split(db[i][c / 2]);
+            to[j + c] = c & 1 ? u.y : u.x;
+            to[H + j + c] = c & 1 ? v.y : v.x;
+        }
+    });
+    if (P > 1) add_groups<P>(out, sums, 2 * H);
 }
 
-// ... of any other row of up to G * N elements
+// ... of any other row
 template <typename T, int G, int N>
-__global__ void __launch_bounds__(G) backward_odd_kernel(Args a) {
-    __shared__ float2 shared[2][32];
+__global__ void __launch_bounds__(G * kGroups<G>, 1) backward_odd_kernel(Args a) {
+    constexpr int P = kGroups<G>, W = G / 32;
+    extern __shared__ float sums[];  // [P][2 * H] where there are several groups
+    __shared__ float2 shared[P][2][W];
+    const int at = threadIdx.x % G, group = threadIdx.x / G, H = a.H, warp = at >> 5, lane = threadIdx.x & 31;
+    const long long step = (long long)gridDim.x * P, first = blockIdx.x + (long long)group * gridDim.x;
     pdl_wait();
     pdl_trigger();
-    const int at = threadIdx.x, H = a.H;
     const float inv = 1.f / (float)H;
-    float w[N], dw[N], db[N], x[N], dy[N], m = 0.f, rs = 0.f;
+    float w[N], dw[N], db[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) dw[i] = db[i] = 0.f;
     each_vector<1, G, N>(at, H, [&](int i, int j) { w[i] = param<T>(a.weight, j, a.wide, 1.f); });
+    Row<T, G, N> x, dy;
+    float m = 0.f, rs = 0.f;
     auto fetch = [&](long long r) {
-        const T *px = static_cast<const T*>(a.x) + r * a.ldx, *pdy = static_cast<const T*>(a.dy) + r * a.lddy;
-        each_vector<1, G, N>(at, H, [&](int i, int j) {
-            x[i] = Elem<T>::to_f(px[j]);
-            dy[i] = Elem<T>::to_f(pdy[j]);
-        });
+        x.fetch(a.x, r * a.ldx, at, H);
+        dy.fetch(a.dy, r * a.lddy, at, H);
         m = a.mean[r];
         rs = a.rstd[r];
     };
-    long long r = blockIdx.x;
-    if (r < a.rows) fetch(r);
-    for (int turn = 0; r < a.rows; r += gridDim.x, ++turn) {
+    if (first < a.rows) fetch(first);
+    int turn = 0;
+    for (long long r = first; r < a.rows; r += step, turn ^= 1) {
         float h[N], g[N], sg = 0.f, sgh = 0.f;
         const float rs_now = rs;
         each_vector<1, G, N>(at, H, [&](int i, int) {
+            const float d = dy[i];
             h[i] = (x[i] - m) * rs;
-            g[i] = dy[i] * w[i];
+            g[i] = d * w[i];
             sg += g[i];
             sgh = fmaf(g[i], h[i], sgh);
-            dw[i] = fmaf(dy[i], h[i], dw[i]);
-            db[i] += dy[i];
+            dw[i] = fmaf(d, h[i], dw[i]);
+            db[i] += d;
         });
-        if (r + gridDim.x < a.rows) fetch(r + gridDim.x);
-        const float2 s = row_sum<G>(sg, sgh, shared, turn);
-        const float c0 = -rs_now * s.x * inv, c1 = -rs_now * s.y * inv;
+        if (r + step < a.rows) fetch(r + step);
+        sg = warp_sum(sg);
+        sgh = warp_sum(sgh);
+        if constexpr (W > 1) {
+            if (lane == 0) shared[group][turn][warp] = make_float2(sg, sgh);
+            meet<G>(group);
+            const float2 v = shared[group][turn][lane % W];
+            sg = lanes_sum<W>(v.x);
+            sgh = lanes_sum<W>(v.y);
+        }
+        const float c0 = -rs_now * sg * inv, c1 = -rs_now * sgh * inv;
         T* dx = static_cast<T*>(a.dx) + r * a.lddx;
         each_vector<1, G, N>(at, H, [&](int i, int j) { dx[j] = Elem<T>::from_f(fmaf(h[i], c1, fmaf(g[i], rs_now, c0))); });
     }
     if (!a.partial) return;
-    float* out = a.partial + (size_t)blockIdx.x * 2 * H;
+    float *out = a.partial + (size_t)blockIdx.x * 2 * H, *to = P > 1 ? sums + (size_t)group * 2 * H : out;
     each_vector<1, G, N>(at, H, [&](int i, int j) {
-        out[j] = dw[i];
-        out[H + j] = db[i];
+        to[j] = dw[i];
+        to[H + j] = db[i];
     });
+    if (P > 1) add_groups<P>(out, sums, 2 * H);
 }
 
 // Rows too long for registers: dx, a block a row; dw and db by column_kernel.
@@ -557,26 +599,35 @@ __global__ void __launch_bounds__(1024) finish_kernel(Args a, int partials) {
     }
 }
 
-// Calls f with threads a row and vectors a thread for H elements in vectors of V: 16 elements a thread where the row is
-// longer than 256, 32 above 8192 elements.  False where a row is too long for registers.
-template <int V, typename F>
+// Calls f with threads a row and vectors a thread for H elements in vectors of V: 16 elements a thread, 8 for short rows, 32
+// for long ones; 24 where that leaves fewer idle and their instructions, not HBM, are the limit: of 16-bit rows (forward,
+// 8192 x 5120 53 us with 16 and 33 with 24, 16384 x 1088 28 and 18; back 72 and 62, but 8192 x 1536 31 and 34; floats the
+// same or slower).  False where a row is too long for registers.
+template <int V, bool kBack, typename F>
 bool with_shape(int H, F f) {
-    constexpr int K = 16 / V;
+    constexpr int K = 8 / V;
     auto shape = [&](auto g, auto n) {
         f(g, n);
         return true;
     };
     using std::integral_constant;
-    if (H <= 256) return shape(integral_constant<int, 32>(), integral_constant<int, K / 2>());
-    if (H <= 512) return shape(integral_constant<int, 32>(), integral_constant<int, K>());
-    if (H <= 1024) return shape(integral_constant<int, 64>(), integral_constant<int, K>());
-    if (H <= 2048) return shape(integral_constant<int, 128>(), integral_constant<int, K>());
-    if (H <= 4096) return shape(integral_constant<int, 256>(), integral_constant<int, K>());
-    if (H <= 8192) return shape(integral_constant<int, 512>(), integral_constant<int, K>());
-    if (H <= 16384) return shape(integral_constant<int, 512>(), integral_constant<int, 2 * K>());
+    if (H <= 256) return shape(integral_constant<int, 32>(), integral_constant<int, K>());
+    if (H <= 512) return shape(integral_constant<int, 32>(), integral_constant<int, 2 * K>());
+    if constexpr (V == 8 && !kBack) {
+        if (H <= 768) return shape(integral_constant<int, 32>(), integral_constant<int, 3>());
+        if (H > 1024 && H <= 1536) return shape(integral_constant<int, 64>(), integral_constant<int, 3>());
+        if (H > 2048 && H <= 128 * 24) return shape(integral_constant<int, 128>(), integral_constant<int, 3>());
+    }
+    if (H <= 1024) return shape(integral_constant<int, 64>(), integral_constant<int, 2 * K>());
+    if (H <= 2048) return shape(integral_constant<int, 128>(), integral_constant<int, 2 * K>());
+    if (H <= 4096) return shape(integral_constant<int, 256>(), integral_constant<int, 2 * K>());
+    if constexpr (V == 8)
+        if (H <= 6144) return shape(integral_constant<int, 256>(), integral_constant<int, 3>());
+    if (H <= 8192) return shape(integral_constant<int, 512>(), integral_constant<int, 2 * K>());
+    if (H <= 16384) return shape(integral_constant<int, 512>(), integral_constant<int, 4 * K>());
     return false;
 }
-// ... for elements one by one
+// ... for rows that are loaded element by element: 8 a thread, 16 above 4096
 template <typename F>
 bool with_odd_shape(int H, F f) {
     auto shape = [&](auto g, auto n) {
@@ -584,9 +635,11 @@ bool with_odd_shape(int H, F f) {
         return true;
     };
     using std::integral_constant;
-    if (H <= 256) return shape(integral_constant<int, 64>(), integral_constant<int, 4>());
-    if (H <= 1024) return shape(integral_constant<int, 256>(), integral_constant<int, 4>());
+    if (H <= 256) return shape(integral_constant<int, 32>(), integral_constant<int, 8>());
+    if (H <= 512) return shape(integral_constant<int, 64>(), integral_constant<int, 8>());
+    if (H <= 1024) return shape(integral_constant<int, 128>(), integral_constant<int, 8>());
     if (H <= 2048) return shape(integral_constant<int, 256>(), integral_constant<int, 8>());
+    if (H <= 4096) return shape(integral_constant<int, 512>(), integral_constant<int, 8>());
     if (H <= 8192) return shape(integral_constant<int, 512>(), integral_constant<int, 16>());
     return false;
 }

@@ -54,7 +54,7 @@ cudaError_t norm_forward(norm::Args a, cudaStream_t st) {
     cudaError_t rc = cudaSuccess;
     bool done;
     if (by_16(sizeof(T), {a.x, a.y}, {a.ldx, a.ldy, a.H})) {
-        done = norm::with_shape<W>(a.H, [&](auto g, auto n) {
+        done = norm::with_shape<W, false>(a.H, [&](auto g, auto n) {
             constexpr int G = decltype(g)::value, P = norm::kForwardGroups<G>, kThreads = G * P;
             const auto kernel = norm::forward_kernel<T, W, G, decltype(n)::value>;
             const size_t stage = (size_t)P * a.H * sizeof(T);
@@ -67,8 +67,10 @@ cudaError_t norm_forward(norm::Args a, cudaStream_t st) {
         });
     } else {
         done = norm::with_odd_shape(a.H, [&](auto g, auto n) {
-            constexpr int G = decltype(g)::value;
-            rc = launch(norm::forward_odd_kernel<T, G, decltype(n)::value>, dim3(std::min(a.rows, sms * (2048 / G))), G, 0, 1, st, a);
+            constexpr int G = decltype(g)::value, P = norm::kForwardGroups<G>, kThreads = G * P;
+            const auto kernel = norm::forward_odd_kernel<T, G, decltype(n)::value>;
+            const int blocks = a.rows <= sms ? a.rows : std::min((a.rows + P - 1) / P, std::max(1, resident_blocks(kernel, kThreads, 0)));
+            rc = launch(kernel, dim3(blocks), kThreads, 0, 1, st, a);
         });
     }
     if (!done) rc = launch(norm::forward_long_kernel<T>, dim3(std::min(a.rows, sms * 2)), 1024, 0, 1, st, a);
@@ -84,10 +86,10 @@ cudaError_t norm_backward(norm::Args a, cudaStream_t st) {
     if (a.rows > 0) {
         bool done;
         if (by_16(sizeof(T), {a.x, a.dy, a.dx}, {a.ldx, a.lddy, a.lddx, a.H})) {
-            done = norm::with_shape<W>(a.H, [&](auto g, auto n) {
+            done = norm::with_shape<W, true>(a.H, [&](auto g, auto n) {
                 constexpr int G = decltype(g)::value, N = decltype(n)::value, P = norm::kGroups<G>;
                 const auto kernel = norm::backward_kernel<T, W, G, N>;
-                const size_t stage = 2 * (size_t)P * a.H * sizeof(T), least = P > 1 && a.partial ? 8 * (size_t)a.H : 0;
+                const size_t stage = 2 * (size_t)P * a.H * sizeof(T), least = P > 1 && a.partial ? 8 * (size_t)a.H * P : 0;
                 partials = std::min(a.rows, std::min(sms, norm::kMaxPartials));
                 const size_t weights = (size_t)(a.H * 4 + 127) / 128 * 128;
                 a.depth = std::min(ring_depth(stage, kRingMost - (int)weights), (a.rows + partials * P - 1) / (partials * P));
@@ -97,9 +99,11 @@ cudaError_t norm_backward(norm::Args a, cudaStream_t st) {
             });
         } else {
             done = norm::with_odd_shape(a.H, [&](auto g, auto n) {
-                constexpr int G = decltype(g)::value;
-                partials = std::min(a.rows, std::min(2 * sms, norm::kMaxPartials));
-                rc = launch(norm::backward_odd_kernel<T, G, decltype(n)::value>, dim3(partials), G, 0, 1, st, a);
+                constexpr int G = decltype(g)::value, P = norm::kGroups<G>, kThreads = G * P;
+                const auto kernel = norm::backward_odd_kernel<T, G, decltype(n)::value>;
+                const size_t smem = P > 1 && a.partial ? 8 * (size_t)a.H * P : 0;
+                partials = a.rows <= sms ? a.rows : std::min({(a.rows + P - 1) / P, norm::kMaxPartials, std::max(1, resident_blocks(kernel, kThreads, smem))});
+                rc = launch(kernel, dim3(partials), kThreads, smem, 1, st, a);
             });
         }
         if (!done) {

@@ -119,18 +119,20 @@ cudaError_t norm_backward(norm::Args a, cudaStream_t st) {
 
 // ---------------------------------------------------------------- sort, gather, combine
 template <template <typename, int, int> class Kernel>
-int move_rows(const char* call, const sorting::Move& m, int torch_dtype, std::initializer_list<const void*> ptrs, cudaStream_t st) {
+int move_rows(const char* call, sorting::Move m, int torch_dtype, std::initializer_list<const void*> ptrs, cudaStream_t st) {
     return with_type(call, torch_dtype, [&](auto* null) {
         using T = std::remove_pointer_t<decltype(null)>;
         constexpr int W = 16 / sizeof(T);
         const bool wide = by_16(sizeof(T), ptrs, {m.ld, m.H});
-        // four vectors a thread, one where there are few tokens
-        const int vectors = (m.H + (wide ? W : 1) - 1) / (wide ? W : 1), per = m.T >= 4 * sm_count() ? 4 : 1;
-        const int threads = std::min(256, std::max(32, (vectors + 32 * per - 1) / (32 * per) * 32));
+        // four vectors a thread, or one where there are few tokens; a token a block, or eight where a warp is enough for one
+        const bool many = m.T >= 4 * sm_count();
+        const int vectors = (m.H + (wide ? W : 1) - 1) / (wide ? W : 1), per = many ? 4 : 1;
+        m.lanes = std::min(256, std::max(32, (vectors + 32 * per - 1) / (32 * per) * 32));
+        const int groups = many && m.lanes == 32 ? 8 : 1;
         auto run = [&](auto kt) {
             constexpr int KT = decltype(kt)::value;
-            return finish(call, wide ? launch(Kernel<T, W, KT>::get(), dim3(m.T), threads, 0, 1, st, m)
-                                     : launch(Kernel<T, 1, KT>::get(), dim3(m.T), threads, 0, 1, st, m));
+            const auto kernel = wide ? Kernel<T, W, KT>::get() : Kernel<T, 1, KT>::get();
+            return finish(call, launch(kernel, dim3((m.T + groups - 1) / groups), groups * m.lanes, 0, 1, st, m));
         };
         using std::integral_constant;
         if (m.K == 1) return run(integral_constant<int, 1>());
@@ -381,10 +383,12 @@ int kleos_sort_tokens(const int32_t* topk, int T, int K, int E, int32_t* offsets
     // one block up to 4096 places, where meeting the others costs more than they take off it
     const int cluster = (long long)T * K <= 4096 ? 1 : sorting::kCluster;
     const bool kept = (long long)T * K <= 32LL * sorting::kKeep * sorting::kWarps * cluster;
-    const auto kernel = kept ? sorting::sort_kernel<true> : sorting::sort_kernel<false>;
+    const bool wide = E > 255;  // the number of bits that an id, E among them, takes: 8, or 11
+    const auto kernel = wide ? kept ? sorting::sort_kernel<true, 11> : sorting::sort_kernel<false, 11>
+                             : kept ? sorting::sort_kernel<true, 8> : sorting::sort_kernel<false, 8>;
     const size_t smem = sizeof(int) * sorting::kWarps * E;
-    static bool allowed[2][64];
-    cudaError_t rc = allow_smem(kernel, allowed[kept], (int)sizeof(int) * sorting::kWarps * kMaxExperts);
+    static bool allowed[4][64];
+    cudaError_t rc = allow_smem(kernel, allowed[2 * wide + kept], (int)sizeof(int) * sorting::kWarps * kMaxExperts);
     if (rc == cudaSuccess) rc = launch(kernel, dim3(cluster), sorting::kThreads, smem, cluster, stream_of(stream), topk, T * K, E, offsets, row_of, source);
     return finish(call, rc);
 }

@@ -22,12 +22,15 @@ constexpr int kCluster = 8;
 
 // One cluster sorts: block c takes the c-th share of the places, warp w of it the w-th share of those, 32 at a time in
 // order, so a place's rank is what the blocks, the warps and the turns in front of it counted, and its rank among
-// the lanes.  Counters: hist[w][e].  kKept: every warp has at most kKeep turns, whose experts and ranks stay in its
-// registers; otherwise it goes through its share twice.
+// the lanes.  Counters: hist[w][e].  Lanes with the same expert find one another by a ballot per bit of it, which takes
+// the same time whatever the experts (kBits: as many as E takes).  match.any takes longer the more of them there are: 32768
+// places spread evenly over 64 experts 9.7 us, now 8.2; by Zipf over 128 6.4 and 7.0; one token 2.7 and 3.1.  kKept: every warp has at
+// most kKeep turns, whose experts and ranks stay in its registers; otherwise it goes through its share twice, kKeep
+// turns' loads at a time.
 constexpr int kKeep = 8;
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-template <bool kKept>
+template <bool kKept, int kBits>
 __global__ void __launch_bounds__(kThreads) sort_kernel(const int* topk, int n, int E, int* offsets, int* row_of, int* source) {
     namespace cg = cooperative_groups;
     extern __shared__ int hist[];          // [kWarps][E]
@@ -53,7 +56,14 @@ __global__ void __launch_bounds__(kThreads) sort_kernel(const int* topk, int n, 
     };
     // the places of expert e in front of this one in the warp's own share
     auto rank = [&](int e) {
-        const unsigned same = __match_any_sync(0xffffffffu, e);
+        unsigned same = 0xffffffffu;
+        const int id = e < 0 ? E : e;
+#pragma unroll
+        for (int b = 0; b < kBits; ++b) {
+            const bool set = (id >> b) & 1;
+            const unsigned with = __ballot_sync(0xffffffffu, set);
+            same &= set ? with : ~with;
+        }
         const int before = __popc(same & ((1u << lane) - 1));
         const int r = e < 0 ? 0 : count[e] + before;
         __syncwarp();
@@ -69,7 +79,13 @@ __global__ void __launch_bounds__(kThreads) sort_kernel(const int* topk, int n, 
         for (int k = 0; k < kKeep; ++k)
             if (k < per) kept_r[k] = rank(kept_e[k]);
     } else {
-        for (long long t = first; t < last; ++t) rank(expert_at(t));
+        for (long long t = first; t < last; t += kKeep) {
+#pragma unroll
+            for (int k = 0; k < kKeep; ++k) kept_e[k] = t + k < last ? expert_at(t + k) : -1;
+#pragma unroll
+            for (int k = 0; k < kKeep; ++k)
+                if (t + k < last) rank(kept_e[k]);
+        }
     }
     __syncthreads();
     // a thread per expert: the warps' counts become the places in front of each warp
@@ -134,9 +150,12 @@ __global__ void __launch_bounds__(kThreads) sort_kernel(const int* topk, int n, 
         for (int k = 0; k < kKeep; ++k)
             if (k < per && first + k < last) place(first + k, kept_e[k], kept_r[k] + (kept_e[k] < 0 ? 0 : count[kept_e[k]]));
     } else {
-        for (long long t = first; t < last; ++t) {
-            const int e = expert_at(t);
-            place(t, e, rank(e));
+        for (long long t = first; t < last; t += kKeep) {
+#pragma unroll
+            for (int k = 0; k < kKeep; ++k) kept_e[k] = t + k < last ? expert_at(t + k) : -1;
+#pragma unroll
+            for (int k = 0; k < kKeep; ++k)
+                if (t + k < last) place(t + k, kept_e[k], rank(kept_e[k]));
         }
     }
     if (source)
@@ -152,6 +171,7 @@ struct Move {
     float* dweights;
     long long ld;  // of the token matrix
     int T, K, E, H, n;  // n = T * K rows
+    int lanes;          // threads of a token: the block, or, where that is larger, a warp
 };
 
 // Rows that no place leads to are zeros: the tail, from offsets[E] on.
@@ -165,13 +185,25 @@ __device__ __forceinline__ void clear_tail(const Move& m) {
         for (int j = threadIdx.x * V; j < m.H; j += blockDim.x * V) store_vec<T, V>(static_cast<T*>(m.to) + r * m.H + j, zero);
 }
 
-// A block takes a token, a thread every blockDim-th vector of it, kAhead vectors of each row at a time; KT >= K, so that
-// all their loads are on their way before the first is needed.  The host chooses as many threads as have four
-// vectors each (as many as have kAhead: 16384 tokens of 2048 bf16, top-2, combine 34 -> 40 us, its gradients 63 -> 73), or one
-// where there are few tokens.
+// m.lanes threads take a token, a thread every m.lanes-th vector of it, kAhead vectors of each row at a time; KT
+// >= K, so that all their loads are on their way before the first is needed.  The host chooses as many threads as
+// have four vectors each (as many as have kAhead: 16384 tokens of 2048 bf16, top-2, combine 34 -> 40 us, its gradients 63 -> 73),
+// or one where there are few tokens, and a token a block; eight where a warp is enough for one (200000 tokens of 64 bf16, a
+// token a block 207 us, which is what the chip takes to start as many; eight 61), not where it is not (8192 tokens of 2048
+// bf16, top-4, combine 29 -> 33).
 template <int KT>
-constexpr int kAhead = KT >= 4 ? 1 : 4 / KT;
+constexpr int kAhead = KT == 8 ? 1 : KT == 4 ? 2 : 4 / KT;
 
+struct Token {
+    long long t;
+    int group, lane;
+    __device__ __forceinline__ explicit Token(const Move& m) {
+        const bool several = (int)blockDim.x != m.lanes;  // (then of a warp each)
+        group = several ? threadIdx.x >> 5 : 0;
+        lane = several ? threadIdx.x & 31 : threadIdx.x;
+        t = several ? (long long)blockIdx.x * (blockDim.x >> 5) + group : blockIdx.x;
+    }
+};
 // The rows of a token, -1 where it has none.
 template <int KT>
 __device__ __forceinline__ void rows_of_token(const Move& m, long long t, int (&r)[KT]) {
@@ -185,28 +217,63 @@ __device__ __forceinline__ void rows_of_token(const Move& m, long long t, int (&
 // The token's row is read once and stored K times.
 template <typename T, int V, int KT>
 __global__ void __launch_bounds__(256) gather_kernel(Move m) {
+    constexpr int U = kAhead<1>;
     pdl_wait();
     pdl_trigger();
-    const int step = blockDim.x * V;
-    for (long long t = blockIdx.x; t < m.T; t += gridDim.x) {
-        const T* x = static_cast<const T*>(m.from) + t * m.ld;
+    const Token token(m);
+    const int step = m.lanes * V;
+    if (token.t < m.T) {
+        const T* x = static_cast<const T*>(m.from) + token.t * m.ld;
         int r[KT];
-        rows_of_token<KT>(m, t, r);
-        for (int j0 = threadIdx.x * V; j0 < m.H; j0 += 4 * step) {
-            Vec<T, V> v[4];
+        rows_of_token<KT>(m, token.t, r);
+        for (int j0 = token.lane * V; j0 < m.H; j0 += U * step) {
+            Vec<T, V> v[U];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < U; ++u)
                 if (j0 + u * step < m.H) v[u] = load_vec<T, V>(x + j0 + u * step);
 #pragma unroll
             for (int k = 0; k < KT; ++k)
                 if (r[k] >= 0)
 #pragma unroll
-                    for (int u = 0; u < 4; ++u)
+                    for (int u = 0; u < U; ++u)
                         if (j0 + u * step < m.H) store_vec<T, V>(static_cast<T*>(m.to) + (long long)r[k] * m.H + j0 + u * step, v[u]);
         }
     }
     clear_tail<T, V>(m);
 }
+
+// V running sums, in pairs where there are two.
+template <int V>
+struct Sums {
+    F2 s[V / 2];
+    __device__ __forceinline__ Sums() {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) s[i] = both(0.f);
+    }
+    template <typename T>
+    __device__ __forceinline__ void add(float w, const Vec<T, V>& v) {
+        F2 p[V / 2];
+        to_pairs<T, V>(v, p);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) s[i] = fma2(both(w), p[i], s[i]);
+    }
+    template <typename T>
+    __device__ __forceinline__ Vec<T, V> rounded() const {
+        return from_pairs<T, V>(s);
+    }
+};
+template <>
+struct Sums<1> {
+    float s = 0.f;
+    template <typename T>
+    __device__ __forceinline__ void add(float w, const Vec<T, 1>& v) {
+        s = fmaf(w, Elem<T>::to_f(v.v[0]), s);
+    }
+    template <typename T>
+    __device__ __forceinline__ Vec<T, 1> rounded() const {
+        return Vec<T, 1>{{Elem<T>::from_f(s)}};
+    }
+};
 
 // Without weights: the gradient of gather.
 template <typename T, int V, int KT>
@@ -214,71 +281,67 @@ __global__ void __launch_bounds__(256) combine_kernel(Move m) {
     constexpr int U = kAhead<KT>;
     pdl_wait();
     pdl_trigger();
-    const int step = blockDim.x * V;
-    for (long long t = blockIdx.x; t < m.T; t += gridDim.x) {
-        T* out = static_cast<T*>(m.to) + t * m.ld;
-        int r[KT];
-        float w[KT];
-        rows_of_token<KT>(m, t, r);
+    const Token token(m);
+    if (token.t >= m.T) return;
+    const int step = m.lanes * V;
+    T* out = static_cast<T*>(m.to) + token.t * m.ld;
+    int r[KT];
+    float w[KT];
+    rows_of_token<KT>(m, token.t, r);
 #pragma unroll
-        for (int k = 0; k < KT; ++k) w[k] = m.weights && r[k] >= 0 ? m.weights[t * m.K + k] : 1.f;
-        for (int j0 = threadIdx.x * V; j0 < m.H; j0 += U * step) {
-            Vec<T, V> v[KT][U];
+    for (int k = 0; k < KT; ++k) w[k] = m.weights && r[k] >= 0 ? m.weights[token.t * m.K + k] : 1.f;
+    for (int j0 = token.lane * V; j0 < m.H; j0 += U * step) {
+        Vec<T, V> v[KT][U];
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (r[k] >= 0 && j0 + u * step < m.H) v[k][u] = load_vec<T, V>(static_cast<const T*>(m.from) + (long long)r[k] * m.H + j0 + u * step);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (j0 + u * step >= m.H) continue;
+            Sums<V> s;
 #pragma unroll
             for (int k = 0; k < KT; ++k)
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (r[k] >= 0 && j0 + u * step < m.H) v[k][u] = load_vec<T, V>(static_cast<const T*>(m.from) + (long long)r[k] * m.H + j0 + u * step);
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (j0 + u * step >= m.H) continue;
-                float s[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) s[i] = 0.f;
-#pragma unroll
-                for (int k = 0; k < KT; ++k)
-                    if (r[k] >= 0)
-#pragma unroll
-                        for (int i = 0; i < V; ++i) s[i] = fmaf(w[k], Elem<T>::to_f(v[k][u].v[i]), s[i]);
-                Vec<T, V> o;
-#pragma unroll
-                for (int i = 0; i < V; ++i) o.v[i] = Elem<T>::from_f(s[i]);
-                store_vec<T, V>(out + j0 + u * step, o);
-            }
+                if (r[k] >= 0) s.template add<T>(w[k], v[k][u]);
+            store_vec<T, V>(out + j0 + u * step, s.template rounded<T>());
         }
     }
 }
 
-// dout[t] is read once for all its K rows.
+// dout[t] is read once for all its K rows.  Vectors past a row's end are its last one, those of no row the first row's: without
+// a condition in front of them all loads are on their way at once (16384 tokens of 2048 bf16, top-2 63 -> 58 us; element by
+// element it is the other way round, 16384 x 2047 108 -> 188, and for combine_kernel, 34.3 -> 35.7).
 template <typename T, int V, int KT>
 __global__ void __launch_bounds__(256) combine_back_kernel(Move m) {
     constexpr int U = kAhead<KT>;
-    __shared__ float part[2][KT][8];
+    __shared__ float part[KT][8];
     pdl_wait();
     pdl_trigger();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = blockDim.x * V;
-    int turn = 0;
-    for (long long t = blockIdx.x; t < m.T; t += gridDim.x, turn ^= 1) {
-        const T* dout = static_cast<const T*>(m.from) + t * m.ld;
-        int r[KT];
-        float w[KT], dot[KT];
-        rows_of_token<KT>(m, t, r);
+    const Token token(m);
+    const int warp = threadIdx.x >> 5, step = m.lanes * V;
+    float dot[KT];
 #pragma unroll
-        for (int k = 0; k < KT; ++k) {
-            w[k] = m.weights && r[k] >= 0 ? m.weights[t * m.K + k] : 1.f;
-            dot[k] = 0.f;
-        }
-        for (int j0 = threadIdx.x * V; j0 < m.H; j0 += U * step) {
+    for (int k = 0; k < KT; ++k) dot[k] = 0.f;
+    if (token.t < m.T) {
+        const T* dout = static_cast<const T*>(m.from) + token.t * m.ld;
+        int r[KT];
+        float w[KT];
+        rows_of_token<KT>(m, token.t, r);
+#pragma unroll
+        for (int k = 0; k < KT; ++k) w[k] = m.weights && r[k] >= 0 ? m.weights[token.t * m.K + k] : 1.f;
+        for (int j0 = token.lane * V; j0 < m.H; j0 += U * step) {
             Vec<T, V> d[U], v[KT][U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (j0 + u * step < m.H) d[u] = load_vec<T, V>(dout + j0 + u * step);
+                if (V > 1 || j0 + u * step < m.H) d[u] = load_vec<T, V>(dout + (V > 1 ? min(j0 + u * step, m.H - V) : j0 + u * step));
             if (m.dweights)
 #pragma unroll
                 for (int k = 0; k < KT; ++k)
 #pragma unroll
                     for (int u = 0; u < U; ++u)
-                        if (r[k] >= 0 && j0 + u * step < m.H) v[k][u] = load_vec<T, V>(static_cast<const T*>(m.other) + (long long)r[k] * m.H + j0 + u * step);
+                        if (V > 1 || (r[k] >= 0 && j0 + u * step < m.H))
+                            v[k][u] = load_vec<T, V>(static_cast<const T*>(m.other) + (long long)max(r[k], 0) * m.H + (V > 1 ? min(j0 + u * step, m.H - V) : j0 + u * step));
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (j0 + u * step >= m.H) continue;
@@ -298,18 +361,19 @@ __global__ void __launch_bounds__(256) combine_back_kernel(Move m) {
                 }
             }
         }
-        if (!m.dweights) continue;
+    }
+    if (m.dweights) {
 #pragma unroll
         for (int k = 0; k < KT; ++k) {
             dot[k] = warp_sum(dot[k]);
-            if (lane == 0) part[turn][k][warp] = dot[k];
+            if ((threadIdx.x & 31) == 0) part[k][warp] = dot[k];
         }
-        if (blockDim.x > 32) __syncthreads();  // (a thread still at the sums of the token before has its own half)
-        else __syncwarp();
-        if (threadIdx.x < m.K) {
-            float v = part[turn][threadIdx.x][0];
-            for (int i = 1; i < (int)blockDim.x >> 5; ++i) v += part[turn][threadIdx.x][i];
-            m.dweights[t * m.K + threadIdx.x] = v;
+        __syncthreads();
+        if (token.t < m.T && token.lane < m.K) {
+            const int first = token.group * (m.lanes >> 5);
+            float v = part[token.lane][first];
+            for (int i = 1; i < m.lanes >> 5; ++i) v += part[token.lane][first + i];
+            m.dweights[token.t * m.K + token.lane] = v;
         }
     }
     clear_tail<T, V>(m);

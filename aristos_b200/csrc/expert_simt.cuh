@@ -1,5 +1,5 @@
-// The experts' products on the FP32 pipes, for floats and for what the tensor-core kernels cannot load (sizes, strides or
-// addresses that are no multiples of 16 bytes).
+// The experts' products on the FP32 pipes, for what the tensor-core kernels cannot load (sizes, strides or addresses that are
+// no multiples of 16 bytes) and for the weight gradients of a few float rows.
 //
 //   kForward  y[r]  = x[r] W[e]^T + b[e]      for the rows r of expert e, offsets[e] <= r < offsets[e + 1]
 //   kDx       dx[r] = dy[r] W[e]
@@ -8,6 +8,8 @@
 // A block computes a 128 x 128 tile of one expert, a thread 8 x 8 of it, over slices of 16 that are loaded into registers
 // while the slice before them is multiplied.  Operands are converted when they are loaded, so products and sums are
 // fp32 multiply-adds whatever the type, two at a time (fma.rn.f32x2: half the instructions, the same rounding).
+// Bound by the FP32 pipes: 4096 float rows of 16 experts, N = K = 2048, 34.4 GFLOP: 1014, 965 and 734 us (34, 36 and 47 TFLOP/s of
+// 74); the few rows of many experts by the stores of dW (128 experts, N = 4424, K = 384, 128 rows: 870 MB in 199 us).
 #pragma once
 
 #include "ops_common.cuh"
@@ -68,12 +70,6 @@ __device__ __forceinline__ int group_of_tile(const int* first, int E, int t) {
 }
 
 constexpr int kTile = 128, kSlice = 16, kPitch = kTile + 4;
-
-__device__ __forceinline__ unsigned long long pack2(float a, float b) {
-    unsigned long long v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-    return v;
-}
 
 // Where line l of step k of a slice lies: eights of lines change places every four steps, so that neither the stores of
 // operands that are contiguous along the steps nor the reads of four lines at once meet a bank conflict.
@@ -171,11 +167,11 @@ __global__ void __launch_bounds__(256, 2) product_kernel(Args a) {
         B.ld = a.ldx;
     }
     const int ty = tid >> 4, tx = tid & 15;  // lines 4 ty.. and 64 + 4 ty.., columns likewise
-    unsigned long long acc[8][4];
+    F2 acc[8][4];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = 0;
+        for (int j = 0; j < 4; ++j) acc[i][j] = both(0.f);
     A.load(0);
     B.load(0);
     A.put(sa[0]);
@@ -198,13 +194,11 @@ __global__ void __launch_bounds__(256, 2) product_kernel(Args a) {
                 v[h] = *reinterpret_cast<const ulonglong2*>(&sb[now][k][place(k, 64 * h + 4 * tx)]);
             }
             const float f[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
-            const unsigned long long g[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
+            const F2 g[4] = {{v[0].x}, {v[0].y}, {v[1].x}, {v[1].y}};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const unsigned long long ff = pack2(f[i], f[i]);
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[i][j]) : "l"(ff), "l"(g[j]));
-            }
+                for (int j = 0; j < 4; ++j) acc[i][j] = fma2(both(f[i]), g[j], acc[i][j]);
         }
         if (more) {
             A.put(sa[now ^ 1]);
@@ -216,17 +210,26 @@ __global__ void __launch_bounds__(256, 2) product_kernel(Args a) {
     for (int i = 0; i < 8; ++i) {
         const int line = (i < 4 ? 0 : 60) + 4 * ty + i;
         if (line >= lines) continue;
+        const size_t row = kMode == kDw ? we + (size_t)(m0 + line) * a.K : (size_t)(m0 + line) * a.ldo;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int c = c0 + (j < 4 ? 0 : 60) + 4 * tx + j;
+        for (int h = 0; h < 2; ++h) {
+            const int c = c0 + 64 * h + 4 * tx;
             if (c >= cols) continue;
-            float2 p;
-            asm("mov.b64 {%0, %1}, %2;" : "=f"(p.x), "=f"(p.y) : "l"(acc[i][j >> 1]));
-            float v = j & 1 ? p.y : p.x;
-            if (kMode == kForward && a.bias && e < a.E) v += Elem<T>::to_f(static_cast<const T*>(a.bias)[(size_t)e * a.N + c]);
-            const size_t at = kMode == kDw ? we + (size_t)(m0 + line) * a.K + c : (size_t)(m0 + line) * a.ldo + c;
-            if (kMode == kDw && a.wide_out) static_cast<float*>(a.out)[at] = v;
-            else static_cast<T*>(a.out)[at] = Elem<T>::from_f(v);
+            const float2 p = split(acc[i][2 * h]), q = split(acc[i][2 * h + 1]);
+            float v[4] = {p.x, p.y, q.x, q.y};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (kMode == kForward && a.bias && e < a.E && c + j < cols) v[j] += Elem<T>::to_f(static_cast<const T*>(a.bias)[(size_t)e * a.N + c + j]);
+            if constexpr (V > 1 && sizeof(T) == 4) {  // whole vectors: the result's rows are such too
+                *reinterpret_cast<float4*>(static_cast<float*>(a.out) + row + c) = make_float4(v[0], v[1], v[2], v[3]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (c + j >= cols) continue;
+                    if (kMode == kDw && a.wide_out) static_cast<float*>(a.out)[row + c + j] = v[j];
+                    else static_cast<T*>(a.out)[row + c + j] = Elem<T>::from_f(v[j]);
+                }
+            }
         }
     }
 }

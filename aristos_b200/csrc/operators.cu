@@ -168,7 +168,7 @@ int products_simt(const char* call, const experts::Args& a, int torch_dtype, cud
         const int tile = experts::kTile, cols = kMode == experts::kForward ? a.N : a.K;
         const dim3 grid = kMode == experts::kDw ? dim3((a.N + tile - 1) / tile, (cols + tile - 1) / tile, a.E)
                                                 : dim3(a.rows / tile + a.E + 1, (cols + tile - 1) / tile);
-        const bool wide = by_16(sizeof(T), {a.x, a.dy, a.w}, {a.ldx, a.ldy, a.N, a.K});
+        const bool wide = by_16(sizeof(T), {a.x, a.dy, a.w, a.out}, {a.ldx, a.ldy, a.ldo, a.N, a.K});
         if (wide) return finish(call, launch(experts::product_kernel<T, kMode, 4>, grid, 256, 0, 1, st, a));
         return finish(call, launch(experts::product_kernel<T, kMode, 1>, grid, 256, 0, 1, st, a));
     });
@@ -303,6 +303,9 @@ int products(const char* call, const experts::Args& a, int torch_dtype, cudaStre
         if (kMode == experts::kForward && a.rows <= 2 && (a.N + 255) / 256 * a.rows <= 32) return products_few<kMode>(call, a, torch_dtype, st);
     }
     if (!tensor) return products_simt<kMode>(call, a, torch_dtype, st);
+    // Weight gradients of few rows an expert are little but stores, and a tile of floats on the tensor cores has a long way
+    // through its roles (128 experts, N = 4424, K = 384: 1 row 199 us on the FP32 pipes and 646, 32 355 and 648, 48 482 and 648).
+    if (kMode == experts::kDw && torch_dtype == 0 && a.rows <= 48LL * a.E) return products_simt<kMode>(call, a, torch_dtype, st);
     if (torch_dtype == 0) return products_f32<kMode>(call, a, st);
     if constexpr (kMode != experts::kDw) {
         return torch_dtype == 2 ? products_tc<__nv_bfloat16, kMode == experts::kDx>(call, a, torch_dtype, st)

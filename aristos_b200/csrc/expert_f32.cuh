@@ -429,12 +429,14 @@ product_f32_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 }
             }
             const int col = x.col + rank * BM + q * 32 + lane, rows = min(x.half, x.n - part * x.half);
-            if (col >= g.M) continue;
-            const float b = kMode == kForward && g.bias ? static_cast<const float*>(g.bias)[(size_t)x.e * g.M + col] : 0.f;
-            float* o = out + (kMode == kDw ? (size_t)x.e * g.len * g.M : 0) + (long long)(x.row + part * x.half) * g.ldo + col;
+            if (col < g.M) {
+                const float b = kMode == kForward && g.bias ? static_cast<const float*>(g.bias)[(size_t)x.e * g.M + col] : 0.f;
+                float* o = out + (kMode == kDw ? (size_t)x.e * g.len * g.M : 0) + (long long)(x.row + part * x.half) * g.ldo + col;
 #pragma unroll
-            for (int j = 0; j < kHalf; ++j)
-                if (j < rows) o[(long long)j * g.ldo] = dead ? __uint_as_float(0x7fffffffu) : acc[j] + b;
+                for (int j = 0; j < kHalf; ++j)
+                    if (j < rows) o[(long long)j * g.ldo] = dead ? __uint_as_float(0x7fffffffu) : acc[j] + b;
+            }
+            __syncwarp();
         }
         if constexpr (kMode != kDw) {
             // rows of nobody

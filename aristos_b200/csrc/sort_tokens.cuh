@@ -32,8 +32,8 @@ constexpr int kCluster = 8;
 // most kKeep turns, whose experts and ranks stay in its registers; otherwise it goes through its share twice, kKeep
 // turns' loads at a time.
 constexpr int kKeep = 8;
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 template <bool kKept, int kBits>
 __global__ void __launch_bounds__(kThreads) sort_kernel(const int* topk, int n, int E, int* offsets, int* row_of, int* source) {
     namespace cg = cooperative_groups;

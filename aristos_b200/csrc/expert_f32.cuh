@@ -6,7 +6,9 @@
 //   place of an fp32 product each, which is what an fp32 multiply-add rounds away.
 //
 // The matrix unit does not round its running sums to nearest, so none stays there for long: the h h sums are read back
-// every 64 steps, the five small products' sums (below 2^-6 of them) every 128, and both are added up in registers.
+// every 128 steps, the five small products' sums (below 2^-6 of them) every 512, and both are added up in registers.  2-norm
+// error of 2048 terms, N(0,1) and all positive: 1.9e-7 and 2.8e-7 (every 64 and 128: 1.7e-7 twice; 256 and 512: 2.9e-7 and
+// 4.8e-7; fp32 multiply-adds 8.1e-7 and 7.0e-7).
 // An infinity or NaN makes the h h sums what fp32 multiply-adds give; the small sums beside it are limited to finite values
 // and leave it as it is.
 //
@@ -22,11 +24,12 @@
 // line; what is contiguous across them comes in tiles of 32 x 32 that are read down a column (M operand) or split into
 // N-major parts (N operand).  Rows that are not the expert's are cleared when they are split.
 //
-// What bounds it: the split warps (2048 columns, 256 rows an expert: a step of 64 takes about 2600 cycles, its MMAs
-// 1536 of them; tensor pipe 42 % active), and 4.3 tiles a pair of blocks in five rounds.  4096 rows, 16 experts, N = K =
-// 2048: 252, 251 and 288 us (34.4 GFLOP each: 137, 137 and 119 TFLOP/s; the FP32 pipes 1014, 965 and 734), 1.7e-7 from the
-// 64-bit result (FP32 pipes: 8.1e-7).  A step a barrier instead of a slice and four warps for the N operand instead of two:
-// 287, 289 and 288 before; eight warps for the M operand, whose registers the others then lack: 282, 270 and 332.
+// What bounds it: the roles' own time, about 1900 to 2200 cycles for a step of 64, for the split of either operand as for
+// the read-back, where its MMAs take 1536 (without them a launch took as long); 2048 columns, 256 rows an expert: 4.3 tiles a
+// pair of blocks in five rounds.  4096 rows, 16 experts, N = K = 2048: 222, 217 and 249 us (34.4 GFLOP each: 155, 158 and 138
+// TFLOP/s; the FP32 pipes 1014, 965 and 734).  Steps, from 287, 289 and 288: a step a barrier instead of a slice, four
+// warps for the N operand instead of two 252, 251, 288; sums read back half and a quarter as often.  Eight warps for the M operand,
+// whose registers the others then lack, 282, 270 and 332 instead of 252, 251 and 288; six for the N operand 219, 221 and 256.
 #pragma once
 
 #include <cfloat>
@@ -42,8 +45,9 @@ constexpr int BK = 32, ROW = BK * 2;           // steps of a slice; bytes of a p
 constexpr int kDrain = 8, kSplitA = 4, kSplitB = 4, kSplit = kSplitA + kSplitB;  // warps
 constexpr int kMmaWarp = kDrain + kSplit, kTmaWarp = kMmaWarp + 1;
 constexpr int kThreads = (kTmaWarp + 1) * 32;  // 112 registers a thread
-constexpr int kStep = 2;   // slices that are loaded, split and multiplied at a time; their h h products share a read-back
-constexpr int kGroup = 2;  // steps whose small products share one
+constexpr int kStep = 2;   // slices that are loaded, split and multiplied at a time
+constexpr int kHigh = 2;   // steps whose h h products share a read-back
+constexpr int kGroup = 8;  // steps whose small products share one
 constexpr int kStages = 2, kRing = 3;  // of a step each
 constexpr int kHalf = 64;  // rows of N per block
 constexpr int BN = 2 * kHalf;
@@ -276,12 +280,15 @@ product_f32_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                         umma_ta(elected, d, ta + k * 8, db + (kAcrossB ? kMajorStep / 16 : 2u) * k, idesc, (more || k > 0) ? 1u : 0u);
                 };
                 for (int kd = 0; kd < steps; ++kd) {
-                    ok = wait(&ctl->sum_empty[0], hp ^ 1) && wait(&ctl->full[s], sp);
-                    if (!ok) break;
-                    hp ^= 1;
+                    const bool fresh = kd % kHigh == 0;
+                    if (fresh) {
+                        if (!(ok = wait(&ctl->sum_empty[0], hp ^ 1))) break;
+                        hp ^= 1;
+                    }
+                    if (!(ok = wait(&ctl->full[s], sp))) break;
 #pragma unroll
-                    for (int j = 0; j < kStep; ++j) multiply(s * kStep + j, 0, 0, tmem, j > 0);
-                    umma_commit_both_if(elected, bars + (uint32_t)offsetof(Control, sum_full));
+                    for (int j = 0; j < kStep; ++j) multiply(s * kStep + j, 0, 0, tmem, !fresh || j > 0);
+                    if (kd + 1 == steps || kd % kHigh == kHigh - 1) umma_commit_both_if(elected, bars + (uint32_t)offsetof(Control, sum_full));
                     const bool first = kd % kGroup == 0;
                     if (first) {
                         if (!(ok = wait(&ctl->sum_empty[1], lp ^ 1))) break;
@@ -421,8 +428,10 @@ product_f32_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 if (lane == 0) mbar_arrive_pair(map_to_cta(smem_u32(&ctl->sum_empty[which]), 0));
             };
             for (int kd = 0; kd < steps; ++kd) {
-                add(0, hp, std::false_type());
-                hp ^= 1;
+                if (kd + 1 == steps || kd % kHigh == kHigh - 1) {
+                    add(0, hp, std::false_type());
+                    hp ^= 1;
+                }
                 if (kd + 1 == steps || kd % kGroup == kGroup - 1) {
                     add(1, lp, std::true_type());
                     lp ^= 1;

@@ -34,13 +34,14 @@ bool whole(size_t bytes, std::initializer_list<const void*> ptrs) {
 constexpr char kWhole[] = "a device pointer is no multiple of its element's size";
 
 // Whether all of it can be moved 16 bytes at a time.
-bool by_16(size_t elem, std::initializer_list<const void*> ptrs, std::initializer_list<long long> elems) {
+bool by(int bytes, size_t elem, std::initializer_list<const void*> ptrs, std::initializer_list<long long> elems) {
     for (const void* p : ptrs)
-        if (!aligned(p, 16)) return false;
+        if (!aligned(p, bytes)) return false;
     for (const long long n : elems)
-        if (n * (long long)elem % 16) return false;
+        if (n * (long long)elem % bytes) return false;
     return true;
 }
+bool by_16(size_t elem, std::initializer_list<const void*> ptrs, std::initializer_list<long long> elems) { return by(16, elem, ptrs, elems); }
 
 // ---------------------------------------------------------------- layer norm
 // Stages of a ring, `bytes` each, for `most` bytes on their way: one at least.
@@ -123,34 +124,43 @@ int move_rows(const char* call, sorting::Move m, int torch_dtype, std::initializ
     return with_type(call, torch_dtype, [&](auto* null) {
         using T = std::remove_pointer_t<decltype(null)>;
         constexpr int W = 16 / sizeof(T);
-        const bool wide = by_16(sizeof(T), ptrs, {m.ld, m.H});
+        const int V = by_16(sizeof(T), ptrs, {m.ld, m.H}) ? W : by(2 * sizeof(T), sizeof(T), ptrs, {m.ld, m.H}) ? 2 : 1;
         // four vectors a thread, or one where there are few tokens; a token a block, or eight where a warp is enough for one
         const bool many = m.T >= 4 * sm_count();
-        const int vectors = (m.H + (wide ? W : 1) - 1) / (wide ? W : 1), per = many ? 4 : 1;
+        const int vectors = (m.H + V - 1) / V, per = many ? 4 : 1;
         m.lanes = std::min(256, std::max(32, (vectors + 32 * per - 1) / (32 * per) * 32));
         const int groups = many && m.lanes == 32 ? 8 : 1;
-        auto run = [&](auto kt) {
-            constexpr int KT = decltype(kt)::value;
-            const auto kernel = wide ? Kernel<T, W, KT>::get() : Kernel<T, 1, KT>::get();
-            return finish(call, launch(kernel, dim3((m.T + groups - 1) / groups), groups * m.lanes, 0, 1, st, m));
+        auto run = [&](auto v, auto kt) {
+            constexpr int kV = decltype(v)::value, KT = decltype(kt)::value, U = Kernel<T, kV, KT>::kAhead;
+            const int parts = U == 0 || many ? 1 : std::min(65535, (vectors + m.lanes * U - 1) / (m.lanes * U));
+            m.span = parts * m.lanes * U * V;
+            return finish(call, launch(Kernel<T, kV, KT>::get(), dim3((m.T + groups - 1) / groups, parts), groups * m.lanes, 0, 1, st, m));
+        };
+        auto with_k = [&](auto kt) {
+            using std::integral_constant;
+            return V == W ? run(integral_constant<int, W>(), kt) : V == 2 ? run(integral_constant<int, 2>(), kt) : run(integral_constant<int, 1>(), kt);
         };
         using std::integral_constant;
-        if (m.K == 1) return run(integral_constant<int, 1>());
-        if (m.K == 2) return run(integral_constant<int, 2>());
-        if (m.K <= 4) return run(integral_constant<int, 4>());
-        return run(integral_constant<int, kMaxTopK>());
+        if (m.K == 1) return with_k(integral_constant<int, 1>());
+        if (m.K == 2) return with_k(integral_constant<int, 2>());
+        if (m.K <= 4) return with_k(integral_constant<int, 4>());
+        return with_k(integral_constant<int, kMaxTopK>());
     });
 }
+// kAhead: vectors of a row that a thread takes at a time; 0: a token's sums take all of a row.
 template <typename T, int V, int KT>
 struct Gather {
+    static constexpr int kAhead = sorting::kAhead<V, 1>;
     static auto get() { return sorting::gather_kernel<T, V, KT>; }
 };
 template <typename T, int V, int KT>
 struct Combine {
+    static constexpr int kAhead = sorting::kAhead<V, KT>;
     static auto get() { return sorting::combine_kernel<T, V, KT>; }
 };
 template <typename T, int V, int KT>
 struct CombineBack {
+    static constexpr int kAhead = 0;
     static auto get() { return sorting::combine_back_kernel<T, V, KT>; }
 };
 

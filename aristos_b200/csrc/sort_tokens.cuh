@@ -175,6 +175,7 @@ struct Move {
     float* dweights;
     long long ld;  // of the token matrix
     int T, K, E, H, n;  // n = T * K rows
+    int span;           // columns that a token's blocks take at a time
     int lanes;          // threads of a token: the block, or, where that is larger, a warp
 };
 
@@ -186,7 +187,7 @@ __device__ __forceinline__ void clear_tail(const Move& m) {
 #pragma unroll
     for (int k = 0; k < V; ++k) zero.v[k] = Elem<T>::from_f(0.f);
     for (long long r = filled + blockIdx.x; r < m.n; r += gridDim.x)
-        for (int j = threadIdx.x * V; j < m.H; j += blockDim.x * V) store_vec<T, V>(static_cast<T*>(m.to) + r * m.H + j, zero);
+        for (int j = (blockIdx.y * blockDim.x + threadIdx.x) * V; j < m.H; j += gridDim.y * blockDim.x * V) store_vec<T, V>(static_cast<T*>(m.to) + r * m.H + j, zero);
 }
 
 // m.lanes threads take a token, a thread every m.lanes-th vector of it, kAhead vectors of each row at a time; KT
@@ -194,9 +195,13 @@ __device__ __forceinline__ void clear_tail(const Move& m) {
 // have four vectors each (as many as have kAhead: 16384 tokens of 2048 bf16, top-2, combine 34 -> 40 us, its gradients 63 -> 73),
 // or one where there are few tokens, and a token a block; eight where a warp is enough for one (200000 tokens of 64 bf16, a
 // token a block 207 us, which is what the chip takes to start as many; eight 61), not where it is not (8192 tokens of 2048
-// bf16, top-4, combine 29 -> 33).
+// bf16, top-4, combine 29 -> 33).  Vectors are 16 bytes, or two elements, or one, as rows and pointers allow (4000 tokens of 1090
+// bf16, top-8, combine one by one 64, in pairs 25 us).  Where there are few tokens the blocks of a column of the grid share one
+// token's row, kAhead vectors a thread each (one token of 7270, top-8: combine in one block 33 us, in 15 2.0).
+template <int V, int KT>
+constexpr int kAhead = KT == 8 ? (V <= 2 ? 2 : 1) : KT == 4 ? (V <= 2 ? 4 : 2) : 4 / KT;
 template <int KT>
-constexpr int kAhead = KT == 8 ? 1 : KT == 4 ? 2 : 4 / KT;
+constexpr int kAhead<2, KT> = KT == 8 ? 2 : 4;
 
 struct Token {
     long long t;
@@ -221,7 +226,7 @@ __device__ __forceinline__ void rows_of_token(const Move& m, long long t, int (&
 // The token's row is read once and stored K times.
 template <typename T, int V, int KT>
 __global__ void __launch_bounds__(256) gather_kernel(Move m) {
-    constexpr int U = kAhead<1>;
+    constexpr int U = kAhead<V, 1>;
     pdl_wait();
     pdl_trigger();
     const Token token(m);
@@ -230,7 +235,7 @@ __global__ void __launch_bounds__(256) gather_kernel(Move m) {
         const T* x = static_cast<const T*>(m.from) + token.t * m.ld;
         int r[KT];
         rows_of_token<KT>(m, token.t, r);
-        for (int j0 = token.lane * V; j0 < m.H; j0 += U * step) {
+        for (int j0 = blockIdx.y * U * step + token.lane * V; j0 < m.H; j0 += m.span) {
             Vec<T, V> v[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -279,10 +284,12 @@ struct Sums<1> {
     }
 };
 
-// Without weights: the gradient of gather.
+// Without weights: the gradient of gather.  Vectors of one or two elements are loaded without a condition, at row 0
+// and the row's last vector where there is none (4000 tokens of 1087, top-8 64 -> 34 us); the bounds on registers are what wide
+// rows took before a token could have several blocks (16384 tokens of 64, top-4: 7.9 us, without them 10.8).
 template <typename T, int V, int KT>
-__global__ void __launch_bounds__(256) combine_kernel(Move m) {
-    constexpr int U = kAhead<KT>;
+__global__ void __launch_bounds__(256, V <= 2 ? (KT >= 4 ? 3 : 5) : KT >= 4 ? 3 : KT == 2 ? 5 : 6) combine_kernel(Move m) {
+    constexpr int U = kAhead<V, KT>;
     pdl_wait();
     pdl_trigger();
     const Token token(m);
@@ -294,13 +301,17 @@ __global__ void __launch_bounds__(256) combine_kernel(Move m) {
     rows_of_token<KT>(m, token.t, r);
 #pragma unroll
     for (int k = 0; k < KT; ++k) w[k] = m.weights && r[k] >= 0 ? m.weights[token.t * m.K + k] : 1.f;
-    for (int j0 = token.lane * V; j0 < m.H; j0 += U * step) {
+#pragma unroll 1
+    for (int j0 = blockIdx.y * U * step + token.lane * V; j0 < m.H; j0 += m.span) {
         Vec<T, V> v[KT][U];
 #pragma unroll
         for (int k = 0; k < KT; ++k)
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (r[k] >= 0 && j0 + u * step < m.H) v[k][u] = load_vec<T, V>(static_cast<const T*>(m.from) + (long long)r[k] * m.H + j0 + u * step);
+                if constexpr (V <= 2)
+                    v[k][u] = load_vec<T, V>(static_cast<const T*>(m.from) + (long long)max(r[k], 0) * m.H + min(j0 + u * step, m.H - V));
+                else if (r[k] >= 0 && j0 + u * step < m.H)
+                    v[k][u] = load_vec<T, V>(static_cast<const T*>(m.from) + (long long)r[k] * m.H + j0 + u * step);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (j0 + u * step >= m.H) continue;
@@ -318,7 +329,7 @@ __global__ void __launch_bounds__(256) combine_kernel(Move m) {
 // element it is the other way round, 16384 x 2047 108 -> 188, and for combine_kernel, 34.3 -> 35.7).
 template <typename T, int V, int KT>
 __global__ void __launch_bounds__(256) combine_back_kernel(Move m) {
-    constexpr int U = kAhead<KT>;
+    constexpr int U = kAhead<V, KT>;
     __shared__ float part[KT][8];
     pdl_wait();
     pdl_trigger();

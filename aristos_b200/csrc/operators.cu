@@ -499,8 +499,12 @@ int kleos_expert_products_dw(const void* dy, long long lddy, const void* x, long
     return with_type(call, torch_dtype, [&](auto* null) {
         using T = std::remove_pointer_t<decltype(null)>;
         constexpr int W = 16 / sizeof(T);
-        if (by_16(sizeof(T), {dy}, {lddy, N})) return finish(call, launch(experts::bias_kernel<T, W>, dim3((N + experts::kBiasLanes * W - 1) / (experts::kBiasLanes * W), E), 1024, 0, 1, st, a));
-        return finish(call, launch(experts::bias_kernel<T, 1>, dim3((N + experts::kBiasLanes - 1) / experts::kBiasLanes, E), 1024, 0, 1, st, a));
+        const bool wide = by_16(sizeof(T), {dy}, {lddy, N});
+        const int columns = experts::kBiasLanes * (wide ? W : 1), tiles = (N + columns - 1) / columns;
+        // two blocks a multiprocessor; blocks that share an expert's rows have 128 of them each
+        const int parts = (int)std::max(1LL, std::min({8LL, 2LL * sm_count() / ((long long)tiles * E), (long long)rows / E / 128}));
+        const auto kernel = wide ? experts::bias_kernel<T, W> : experts::bias_kernel<T, 1>;
+        return finish(call, launch(kernel, dim3(tiles * parts, E), 1024, 0, parts, st, a));
     });
 }
 

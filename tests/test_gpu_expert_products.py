@@ -249,3 +249,15 @@ def test_rows_past_two_to_the_31_elements():
     check(dx[-last:], ds @ ws, _bound(N, ds.abs() @ ws.abs()), "dx")
     check(dw[1], ds.t() @ xs, _bound(last, ds.abs().t() @ xs.abs()), "dw")
     assert not bool(y[:-last].any()) and not bool(dx[:-last].any()) and not bool(dw[0].any())
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("counts,N", [([2500], 136), ([2500], 37), ([1300, 0, 71], 264), ([129], 2048), ([1025], 8)])
+def test_bias_gradient_of_many_rows(counts, N, dtype):
+    c = _case(counts, N, 16, dtype, spare=3)
+    for grad in (c["dt"], torch.float32):
+        _, db = _dw(c, grad)
+        for e, n in enumerate(counts):
+            dy = c["dy"][c["at"][e]:c["at"][e + 1]].double()
+            check(db[e], dy.sum(0), _bound(n, dy.abs().sum(0)), f"dbias of expert {e}")
+        assert torch.equal(_dw(c, grad)[1], db)

@@ -224,3 +224,11 @@ def test_rows_past_two_to_the_31_elements():
     check(drows[-50:], want, 2 * EPS * want.abs(), "drows")
     squares = x[-50:].double().square().sum(1, keepdim=True).expand(50, 2)
     check(dw[-50:], squares, (H / 32 + 32) * EPS * squares, "dweights")
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("T,K,E,H", [(1, 8, 12, 8190), (3, 8, 9, 7271), (2, 3, 4, 4098), (40, 1, 4, 2050), (2400, 3, 8, 66), (1300, 8, 16, 322)])
+def test_pairs_of_elements_and_several_blocks_a_token(T, K, E, H, dtype):
+    for pad in ((0, 0), (2, 0), (1, 0)):
+        test_gather_and_its_gradient(T, K, E, H, "dropped", dtype, pad)
+        test_combine_and_its_gradients(T, K, E, H, "dropped", dtype, pad)

@@ -61,6 +61,7 @@ struct TcArgs {
     int rows, E;
     int M;            // columns of the result (kernels of products), rows of dW[e] (weight gradients)
     int len;          // length of the sums (products), columns of dW[e]
+    int units;        // products: units of 32 rows that a tile has at most, nine
     bool wide_out;    // dW as floats
     long long wait_cycles;
 };
@@ -191,8 +192,9 @@ __device__ __forceinline__ int split_cost(int units, int s) {  // units of 32 ro
     auto cost = [](int u) { return u > 8 ? 672 : u > 7 ? 512 : 32 * u + 256; };
     return more * cost(low + 1) + (s - more) * cost(low);
 }
-__device__ __forceinline__ int row_splits(int n) {
+__device__ __forceinline__ int row_splits(int n, int most) {
     const int units = (n + 31) >> 5, a = (units + 8) / 9, b = (units + 7) >> 3;
+    if (most < 9) return (units + most - 1) / most;
     return a == b || split_cost(units, a) <= split_cost(units, b) ? a : b;
 }
 
@@ -220,7 +222,7 @@ __device__ __forceinline__ Tile tile_at(int t, const int* first, const TcArgs& g
     while (first[e + 1] <= t) ++e;
     *at = e;
     const Group rows = group_rows(g.offsets, e, g.rows);
-    const int n = rows.end - rows.begin, splits = row_splits(n), r = t - first[e];
+    const int n = rows.end - rows.begin, splits = row_splits(n, g.units), r = t - first[e];
     Tile x;
     x.e = e;
     const int mt = r / splits, j = r - mt * splits;
@@ -272,7 +274,7 @@ product_tc_kernel(const __grid_constant__ RowMaps map_x, const __grid_constant__
     set_up(&ctl->b, 1);
     pdl_wait();
     const int MT = (g.M + 2 * BM - 1) / (2 * BM);
-    count_tiles(ctl->first, g, [&](int n) { return row_splits(n) * MT; });
+    count_tiles(ctl->first, g, [&](int n) { return row_splits(n, g.units) * MT; });
     __syncthreads();
     tc_fence_before();
     cluster_sync_all();

@@ -11,6 +11,7 @@
 #include "expert_f32.cuh"
 #include "expert_rows.cuh"
 #include "expert_simt.cuh"
+#include "expert_split.cuh"
 #include "expert_tc.cuh"
 #include "layer_norm.cuh"
 #include "sort_tokens.cuh"
@@ -214,10 +215,59 @@ bool encode_weights(CUtensorMap* map, int torch_dtype, const void* base, int E, 
     return encode(map, torch_dtype, base, 3, sizes, strides, lines);
 }
 
+constexpr int kLeastSteps = 4;  // of 64 elements that a part of a split sum has
 constexpr long long kWaitCycles = 20000000000LL;  // about ten seconds: nothing but a copy or an MMA is waited for
 
 // Pairs of blocks for so many tiles at most.
 int pair_grid(long long tiles) { return 2 * (int)std::max<long long>(1, std::min<long long>(sm_count() / 2, tiles)); }
+
+// Clusters of a kernel that the device holds at once.
+template <typename... P>
+int resident_clusters(void (*kernel)(P...), int cluster, int threads, size_t smem) {
+    cudaLaunchConfig_t lc{};
+    lc.gridDim = dim3((unsigned)cluster);
+    lc.blockDim = dim3((unsigned)threads);
+    lc.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)cluster;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    lc.attrs = &at;
+    lc.numAttrs = 1;
+    int n = 0;
+    return cudaOccupancyMaxActiveClusters(&n, kernel, &lc) == cudaSuccess ? n : 0;
+}
+
+// Whether the call's tiles, `tiles` at most, are so few that a cluster of kParts pairs of blocks can take each and run at once;
+// the call is launched then and its result is in *code.
+template <typename TE, bool kDx, int kParts>
+bool products_split(const char* call, const experts::Args& a, const experts::tcp::TcArgs& g, long long tiles, int torch_dtype, cudaStream_t st, int* code) {
+    using namespace experts;
+    if ((g.len + tcp::BK - 1) / tcp::BK < kLeastSteps * kParts) return false;
+    const auto kernel = tcs::split_tc_kernel<TE, kDx, kParts>;
+    static bool done[64];
+    static int known[64];
+    int dev = -1, most = 0;
+    cudaError_t rc = cudaGetDevice(&dev);
+    if (rc == cudaSuccess) rc = allow_smem(kernel, done, tcs::SMEM_BYTES);
+    if (rc == cudaSuccess && dev < 64) most = known[dev];
+    if (rc == cudaSuccess && !most) {
+        most = resident_clusters(kernel, 2 * kParts, tcp::kThreads, tcs::SMEM_BYTES);
+        if (dev < 64) known[dev] = most;
+    }
+    if (rc == cudaSuccess && tiles > most) return false;
+    tcs::HalfMaps rows;
+    CUtensorMap w;
+    bool ok = rc == cudaSuccess && encode_weights(&w, torch_dtype, a.w, a.E, a.N, a.K, kDx ? 64 : 128);
+    for (int i = 0; i < 2; ++i) ok = ok && encode_rows(&rows.box[i], torch_dtype, kDx ? a.dy : a.x, a.rows, g.len, kDx ? a.ldy : a.ldx, 16 << i);
+    if (rc == cudaSuccess && !ok) {
+        *code = refuse(call, KLEOS_E_CUDA, "cuTensorMapEncodeTiled failed");
+        return true;
+    }
+    if (rc == cudaSuccess) rc = launch(kernel, dim3(2 * kParts * (int)tiles), tcp::kThreads, tcs::SMEM_BYTES, 2 * kParts, st, rows, w, g);
+    *code = finish(call, rc);
+    return true;
+}
 
 template <typename TE, bool kDx>
 int products_tc(const char* call, const experts::Args& a, int torch_dtype, cudaStream_t st) {
@@ -226,6 +276,11 @@ int products_tc(const char* call, const experts::Args& a, int torch_dtype, cudaS
     g.offsets = a.offsets; g.bias = a.bias; g.out = a.out; g.ldo = a.ldo; g.rows = a.rows; g.E = a.E; g.wait_cycles = kWaitCycles;
     g.M = kDx ? a.K : a.N;
     g.len = kDx ? a.N : a.K;
+    const long long pairs = (g.M + 2 * BM - 1) / (2 * BM), at_most = pairs * (a.rows / experts::tcs::kRows + std::min(a.E, a.rows));
+    int code;
+    if (products_split<TE, kDx, 4>(call, a, g, at_most, torch_dtype, st, &code) || products_split<TE, kDx, 2>(call, a, g, at_most, torch_dtype, st, &code)) return code;
+    // tiles of fewer rows where there would be fewer tiles than pairs of blocks (one expert's 1000 rows, N = K = 1024: 12.3 -> 9.4 us)
+    g.units = (int)std::min(9LL, std::max(2LL, (pairs * (a.rows / 32 + std::min(a.E, a.rows)) * 2 + sm_count() - 1) / sm_count()));
     RowMaps rows;
     CUtensorMap w;
     bool ok = encode_weights(&w, torch_dtype, a.w, a.E, a.N, a.K, kDx ? 64 : 128);
@@ -233,7 +288,7 @@ int products_tc(const char* call, const experts::Args& a, int torch_dtype, cudaS
     if (!ok) return refuse(call, KLEOS_E_CUDA, "cuTensorMapEncodeTiled failed");
     static bool done[64];
     cudaError_t rc = allow_smem(product_tc_kernel<TE, kDx>, done, SMEM_BYTES);
-    const long long tiles = (long long)((g.M + 2 * BM - 1) / (2 * BM)) * (a.rows / 256 + std::min(a.E, a.rows));  // at most
+    const long long tiles = pairs * (a.rows / (g.units < 9 ? 32 * g.units : 256) + std::min(a.E, a.rows));  // at most
     if (rc == cudaSuccess) rc = launch(product_tc_kernel<TE, kDx>, dim3(pair_grid(tiles)), kThreads, SMEM_BYTES, 1, st, rows, w, g);
     return finish(call, rc);
 }
@@ -310,7 +365,10 @@ int products(const char* call, const experts::Args& a, int torch_dtype, cudaStre
     const bool tensor = a.rows > 0 && by_16(bytes_of(torch_dtype), {a.x, a.dy, a.w, a.out}, {a.ldx, a.ldy, a.ldo, a.N, a.K});
     if constexpr (kMode != experts::kDw) {
         if (a.rows <= kFewRows && (!tensor || torch_dtype == 0)) return products_few<kMode>(call, a, torch_dtype, st);
-        if (kMode == experts::kForward && a.rows <= 2 && (a.N + 255) / 256 * a.rows <= 32) return products_few<kMode>(call, a, torch_dtype, st);
+        // (64 experts, N = K = 2048, a row: 5.6 us and 8.9 on the tensor cores; 2 rows of 8 experts, N = K = 4096: 23.9 and 16.5;
+        // 1 row, N = 256, K = 8192: 13.8 and 11.7)
+        if (kMode == experts::kForward && a.rows <= 2 && a.K <= 4096 && (long long)((a.N + 255) / 256) * a.rows * a.K <= 65536)
+            return products_few<kMode>(call, a, torch_dtype, st);
     }
     if (!tensor) return products_simt<kMode>(call, a, torch_dtype, st);
     // Weight gradients of few rows an expert are little but stores, and a tile of floats on the tensor cores has a long way

@@ -261,3 +261,41 @@ def test_bias_gradient_of_many_rows(counts, N, dtype):
             dy = c["dy"][c["at"][e]:c["at"][e + 1]].double()
             check(db[e], dy.sum(0), _bound(n, dy.abs().sum(0)), f"dbias of expert {e}")
         assert torch.equal(_dw(c, grad)[1], db)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("counts,N,K", [([1], 264, 2056), ([3], 1088, 4104), ([70, 0, 1], 520, 1032), ([64, 65], 256, 4096), ([2, 0, 33, 0], 4096, 264),
+                                        ([538], 728, 1544), ([31, 1, 96], 8, 2048), ([17], 1024, 1024), ([150, 150], 512, 512)])
+def test_few_tiles_with_long_sums(counts, N, K, dtype):
+    for pads in ((0, 0), (8, 16)):
+        c = _case(counts, N, K, dtype, spare=3, pads=pads)
+        _verify(c)
+        y, dx = _forward(c), _dx(c)
+        for _ in range(3):
+            assert torch.equal(_forward(c), y) and torch.equal(_dx(c), dx)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("N,K", [(520, 1032), (264, 2056)])
+def test_infinite_values_stay_with_their_expert_in_split_sums(dtype, N, K):
+    test_infinite_values_stay_with_their_expert(dtype, N, K)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_split_sums_with_offsets_that_lie(dtype):
+    c = _case([60, 40], 256, 2048, dtype)
+    c["offsets"] = torch.tensor([-5, 70, 400], dtype=torch.int32, device="cuda")
+    y = _forward(c)
+    x, w = c["x"].double(), c["w"].double()
+    for e, r in ((0, slice(0, 70)), (1, slice(70, 100))):
+        b = c["bias"][e].double()
+        check(y[r], x[r] @ w[e].t() + b, _bound(2048, x[r].abs() @ w[e].abs().t() + b.abs()), "y")
+    c["offsets"] = torch.tensor([0, 90, 30], dtype=torch.int32, device="cuda")
+    _forward(c), _dx(c)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("counts,N,K", [([1000], 1024, 136), ([300, 0, 900], 512, 192), ([2000], 520, 264), ([64] * 20, 256, 128)])
+def test_tiles_of_fewer_rows(counts, N, K, dtype):
+    _verify(_case(counts, N, K, dtype, spare=2))

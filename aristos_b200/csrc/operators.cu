@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <initializer_list>
 #include <type_traits>
 
@@ -346,13 +347,18 @@ int products_few(const char* call, const experts::Args& a, int torch_dtype, cuda
             const bool wide = by_16(sizeof(T), {a.x, a.w}, {a.ldx, a.K});
             // one or two rows: twice the blocks, for which two columns a warp are enough
             const int columns = a.rows <= 2 ? 16 : 32;
-            const auto kernel = wide ? a.rows <= 2 ? forward_rows_kernel<T, W, 2, 2> : forward_rows_kernel<T, W, 8, 4>
-                                     : a.rows <= 2 ? forward_rows_kernel<T, 1, 2, 2> : forward_rows_kernel<T, 1, 8, 4>;
+            auto of = [&](auto v) {
+                constexpr int V = decltype(v)::value;
+                return a.rows <= 2 ? forward_rows_kernel<T, V, 2, 2> : a.rows <= 2 * a.E ? forward_rows_kernel<T, V, 2, 4> : forward_rows_kernel<T, V, 4, 4>;
+            };
+            const auto kernel = wide ? of(std::integral_constant<int, W>()) : of(std::integral_constant<int, 1>());
             return finish(call, launch(kernel, dim3((a.N + columns - 1) / columns, a.rows), 256, 0, 1, st, a));
         } else {
-            constexpr int V = 4;
-            if (by_16(sizeof(T), {a.w}, {a.K})) return finish(call, launch(dx_rows_kernel<T, V>, dim3((a.K + 32 * V - 1) / (32 * V), a.rows), 1024, 32 * (32 * V + 1) * sizeof(float), 1, st, a));
-            return finish(call, launch(dx_rows_kernel<T, 1>, dim3((a.K + 31) / 32, a.rows), 1024, 32 * 33 * sizeof(float), 1, st, a));
+            const int V = by_16(sizeof(T), {a.w}, {a.K}) ? 4 : 1, tiles = (a.K + 32 * V - 1) / (32 * V);
+            // a cluster shares the weights' rows, 512 a block in turn, where the blocks would leave multiprocessors idle
+            const int parts = std::max(1, std::min({8, (a.N + 32 * kDxWarps - 1) / (32 * kDxWarps), (int)(sm_count() / ((long long)tiles * std::max(std::min(a.rows, a.E), a.rows / 4)))}));
+            const auto kernel = V == 4 ? dx_rows_kernel<T, 4> : dx_rows_kernel<T, 1>;
+            return finish(call, launch(kernel, dim3(tiles * parts, a.rows), 32 * kDxWarps, kDxWarps * (32 * V + 1) * sizeof(float), parts, st, a));
         }
     });
 }
@@ -360,11 +366,26 @@ int products_few(const char* call, const experts::Args& a, int torch_dtype, cuda
 // The tensor cores' kernels load by TMA, whose rows begin and end on 16-byte boundaries; everything else goes to the FP32
 // pipes, and so do a few rows.
 constexpr int kFewRows = 32;
+
+// Whether float products are sooner done by streaming the weights once for every four rows, at 6.2 TB/s (c chunks of rows, every
+// second expert's last one shorter), than by tiles of 128 rows, a microsecond for every 64 of the sums in as many rounds as
+// there are tiles for a pair of blocks.  33 and 64 rows, N = K = 2048, forward: one expert 24 and 42 us (tiles 37 and 37), 16 experts
+// 55 and 76 (67 and 68); 64 experts, N = K = 1024 24 and 36 (40 and 56); one expert, N = 512, K = 8192 32 and 34 (123 and 124), its
+// dx 43 and 80 (16 and 16).
+bool few_floats(const experts::Args& a, int M, int len) {
+    if (a.rows > 256) return false;
+    const double c = a.rows / 4.0 + std::min(a.rows, a.E) / 2.0, pairs = std::max(1, sm_count() / 2);
+    const double tiles = (double)((M + 255) / 256) * (a.rows / 128 + std::min(a.rows, a.E));
+    return 4 + c * a.N * a.K * 4 / 6.2e6 < 7 + std::ceil(tiles / pairs) * len / 64.0;
+}
+
 template <int kMode>
 int products(const char* call, const experts::Args& a, int torch_dtype, cudaStream_t st) {
     const bool tensor = a.rows > 0 && by_16(bytes_of(torch_dtype), {a.x, a.dy, a.w, a.out}, {a.ldx, a.ldy, a.ldo, a.N, a.K});
     if constexpr (kMode != experts::kDw) {
-        if (a.rows <= kFewRows && (!tensor || torch_dtype == 0)) return products_few<kMode>(call, a, torch_dtype, st);
+        const bool forward = kMode == experts::kForward;
+        if (!tensor ? a.rows <= kFewRows : torch_dtype == 0 && few_floats(a, forward ? a.N : a.K, forward ? a.K : a.N))
+            return products_few<kMode>(call, a, torch_dtype, st);
         // (64 experts, N = K = 2048, a row: 5.6 us and 8.9 on the tensor cores; 2 rows of 8 experts, N = K = 4096: 23.9 and 16.5;
         // 1 row, N = 256, K = 8192: 13.8 and 11.7)
         if (kMode == experts::kForward && a.rows <= 2 && a.K <= 4096 && (long long)((a.N + 255) / 256) * a.rows * a.K <= 65536)

@@ -321,7 +321,7 @@ def layer_norm(x, weight, bias, eps, y, mean=None, rstd=None, stream=None) -> No
     ldy = _rows(call, "y", y, R, H, dt, dev)
     pt = _param_type(call, dt, weight, bias)
     _launch(call, dev, x.data_ptr(), ldx, _maybe(call, "weight", weight, (H,), pt, dev), _maybe(call, "bias", bias, (H,), pt, dev), R, H, eps,
-            _codes.get(dt, -1), _codes[pt], y.data_ptr(), ldy, _maybe(call, "mean", mean, (R,), torch.float32, dev),
+            _codes.get(dt, -1), _codes.get(pt, -1), y.data_ptr(), ldy, _maybe(call, "mean", mean, (R,), torch.float32, dev),
             _maybe(call, "rstd", rstd, (R,), torch.float32, dev), stream)
 
 
@@ -336,7 +336,7 @@ def layer_norm_backward(dy, x, weight, mean, rstd, dx, dweight=None, dbias=None,
         space, room = _whole(call, "workspace", workspace, workspace.shape, workspace.dtype, dev), workspace.nbytes
     _launch(call, dev, dy.data_ptr(), lddy, x.data_ptr(), ldx, _maybe(call, "weight", weight, (H,), pt, dev),
             _whole(call, "mean", mean, (R,), torch.float32, dev), _whole(call, "rstd", rstd, (R,), torch.float32, dev), R, H,
-            _codes.get(dt, -1), _codes[pt], dx.data_ptr(), lddx, _maybe(call, "dweight", dweight, (H,), pt, dev),
+            _codes.get(dt, -1), _codes.get(pt, -1), dx.data_ptr(), lddx, _maybe(call, "dweight", dweight, (H,), pt, dev),
             _maybe(call, "dbias", dbias, (H,), pt, dev), space, room, stream)
 
 

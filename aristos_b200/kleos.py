@@ -293,7 +293,7 @@ def _launch(call, dev, *args) -> None:
 
 def layer_norm_workspace(H: int) -> int:
     """Bytes of workspace that layer_norm_backward needs for dweight and dbias."""
-    n = load_library().kleos_layer_norm_workspace(H)
+    n = load_library().kleos_layer_norm_workspace(H) if H <= _MOST_ROWS else _ARG
     if n < 0:
         _check(n, "kleos_layer_norm_workspace")
     return n
@@ -342,14 +342,14 @@ def layer_norm_backward(dy, x, weight, mean, rstd, dx, dweight=None, dbias=None,
 
 def _offsets(call, offsets, dev):
     """Number of experts and address."""
-    if offsets.dim() != 1 or offsets.shape[0] < 2:
+    if offsets.dim() != 1 or not 2 <= offsets.shape[0] <= _MOST_ROWS:
         _refuse(call, "offsets must have an entry per expert and one more")
     return offsets.shape[0] - 1, _whole(call, "offsets", offsets, offsets.shape, _torch.int32, dev)
 
 
 def _places(call, row_of, T, dev):
     """Experts of a token and address."""
-    if row_of.dim() != 2 or row_of.shape[0] != T:
+    if row_of.dim() != 2 or row_of.shape[0] != T or row_of.shape[1] > _MOST_ROWS:
         _refuse(call, "row_of must have a row per token and a column per expert of it")
     return row_of.shape[1], _whole(call, "row_of", row_of, row_of.shape, _torch.int32, dev)
 
@@ -360,6 +360,8 @@ def sort_tokens(topk, num_experts, offsets, row_of, source=None, stream=None) ->
     if topk.dim() != 2 or not topk.is_cuda:
         _refuse(call, "topk must be a matrix on the GPU")
     (T, K), i32, dev = topk.shape, torch.int32, topk.get_device()
+    if max(T, K, num_experts) > 0x7fffffff:  # (the entry point refuses what else is too large)
+        _refuse(call, "too many tokens, places or experts")
     _launch(call, dev, _whole(call, "topk", topk, (T, K), i32, dev), T, K, num_experts,
             _whole(call, "offsets", offsets, (num_experts + 1,), i32, dev), _whole(call, "row_of", row_of, (T, K), i32, dev),
             _maybe(call, "source", source, (T * K,), i32, dev), stream)

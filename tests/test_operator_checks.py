@@ -65,3 +65,28 @@ def test_norm_of_a_type_with_parameters_of_the_same(launched, dtype, params):
     b = Stand((64,), dtype) if params != "weight" else None
     _refused(UNSUPPORTED, kleos.layer_norm, x, w, b, 1e-5, y)
     _refused(UNSUPPORTED, kleos.layer_norm_backward, x, x, w, m, m, y, w, b, Stand((1 << 20,), torch.uint8))
+
+
+PAST = 2 ** 32  # a C int takes the sizes below from PAST + 4 for 4
+
+
+def test_sizes_that_a_c_int_does_not_hold(launched):
+    i32, f32 = torch.int32, torch.float32
+    offsets = Stand((9,), i32)
+    for T, K in ((PAST + 4, 2), (4, PAST + 2), (2 ** 31, 1)):
+        _refused(ARG, kleos.sort_tokens, Stand((T, K), i32), 8, offsets, Stand((T, K), i32))
+    x, many = Stand((4, 64), f32), Stand((PAST + 9,), i32)
+    topk, row_of, w = Stand((4, 2), i32), Stand((4, 2), i32), Stand((PAST + 8, 16, 64), f32)
+    rows, y = Stand((8, 64), f32), Stand((4, 16), f32)
+    _refused(ARG, kleos.sort_tokens, topk, PAST + 8, many, row_of)
+    _refused(ARG, kleos.gather_tokens, x, row_of, many, rows)
+    _refused(ARG, kleos.combine_tokens_backward, x, rows, row_of, None, many, rows)
+    _refused(ARG, kleos.expert_products, x, many, w, None, y)
+    _refused(ARG, kleos.expert_products_dx, y, many, w, x)
+    _refused(ARG, kleos.expert_products_dw, y, x, many, w)
+    wide, all_rows = Stand((4, PAST + 2), i32), Stand((4 * (PAST + 2), 64), f32)
+    _refused(ARG, kleos.gather_tokens, x, wide, offsets, all_rows)
+    _refused(ARG, kleos.combine_tokens, all_rows, wide, None, x)
+    _refused(ARG, kleos.combine_tokens_backward, x, all_rows, wide, None, offsets, all_rows)
+    _refused(ARG, kleos.layer_norm_workspace, PAST + 64)
+    assert not launched

@@ -24,7 +24,8 @@ using namespace ops;
 size_t bytes_of(int torch_dtype) { return torch_dtype == 0 ? 4 : 2; }
 bool known_type(int torch_dtype) { return torch_dtype == 0 || torch_dtype == 2 || torch_dtype == 3; }
 constexpr int kMostColumns = 1 << 28;
-constexpr char kNormSizes[] = "rows must be 0 or more, H from 1 to 2^28, and no row longer than its stride";
+constexpr int kMostRows = 0x7fff0000;  // launches count rows in ints, and round them up to whole blocks
+constexpr char kNormSizes[] = "rows must be from 0 to 2^31 - 2^16, H from 1 to 2^28, and no row longer than its stride";
 constexpr char kTypes[] = "torch_dtype must be 0 (float), 2 (bf16) or 3 (fp16)";
 
 // Whether every pointer (null ones too) is where an element of so many bytes may be.
@@ -407,7 +408,7 @@ int products(const char* call, const experts::Args& a, int torch_dtype, cudaStre
 }
 
 const char* bad_products(int rows, int E, int N, int K, long long ld_n, long long ld_k) {
-    if (rows < 0 || rows > 0x7fff0000 || E < 1 || E > kMaxExperts) return "rows must be 0 or more, E from 1 to 1024";
+    if (rows < 0 || rows > kMostRows || E < 1 || E > kMaxExperts) return "rows must be from 0 to 2^31 - 2^16, E from 1 to 1024";
     if (N < 1 || K < 1 || N > 1 << 22 || K > 1 << 22) return "N and K must be from 1 to 2^22";
     // tiles are counted in ints: of rows by columns, and of the weights
     const long long n = (N + 127) / 128, k = (K + 127) / 128;
@@ -430,7 +431,7 @@ int kleos_layer_norm(const void* x, long long ldx, const void* weight, const voi
     const char* call = "kleos_layer_norm";
     if (!known_type(torch_dtype)) return refuse(call, KLEOS_E_UNSUPPORTED, kTypes);
     if (param_dtype != 0 && param_dtype != torch_dtype) return refuse(call, KLEOS_E_UNSUPPORTED, "param_dtype must be 0 (float) or the element type");
-    if (rows < 0 || H < 1 || H > kMostColumns || ldx < H || ldy < H) return refuse(call, KLEOS_E_ARG, kNormSizes);
+    if (rows < 0 || rows > kMostRows || H < 1 || H > kMostColumns || ldx < H || ldy < H) return refuse(call, KLEOS_E_ARG, kNormSizes);
     if (!(eps >= 0.f)) return refuse(call, KLEOS_E_ARG, "eps must not be negative");
     if (rows == 0) return KLEOS_OK;
     if (!x || !y) return refuse(call, KLEOS_E_ARG, "null device pointer");
@@ -449,7 +450,7 @@ int kleos_layer_norm_backward(const void* dy, long long lddy, const void* x, lon
     const char* call = "kleos_layer_norm_backward";
     if (!known_type(torch_dtype)) return refuse(call, KLEOS_E_UNSUPPORTED, kTypes);
     if (param_dtype != 0 && param_dtype != torch_dtype) return refuse(call, KLEOS_E_UNSUPPORTED, "param_dtype must be 0 (float) or the element type");
-    if (rows < 0 || H < 1 || H > kMostColumns || ldx < H || lddy < H || lddx < H) return refuse(call, KLEOS_E_ARG, kNormSizes);
+    if (rows < 0 || rows > kMostRows || H < 1 || H > kMostColumns || ldx < H || lddy < H || lddx < H) return refuse(call, KLEOS_E_ARG, kNormSizes);
     if (rows > 0 && (!dy || !x || !mean || !rstd || !dx)) return refuse(call, KLEOS_E_ARG, "null device pointer");
     const bool sums = dweight || dbias;
     if (sums && (!workspace || !aligned(workspace, 16) || workspace_bytes < kleos_layer_norm_workspace(H)))

@@ -274,7 +274,7 @@ int kleos_placement_model(const char* config_json_path, uint32_t* moe_stages, ui
  * lengths are multiples of 16 bytes the kernels move 16 bytes at a time; others are taken too, more slowly. */
 
 /* y = (x - mean) * rstd * weight + bias of every row, rstd = 1 / sqrt(var + eps), var the mean square of
- * x - mean.  x [rows, H] and y of torch_dtype; weight [H] and bias [H] of param_dtype, 0 (float) or
+ * x - mean.  x [rows, H] and y of torch_dtype, rows up to 2^31 - 2^16; weight [H] and bias [H] of param_dtype, 0 (float) or
  * torch_dtype, NULL for ones and zeros.  mean [rows] and rstd [rows] are floats for the backward pass and
  * may be NULL. */
 int kleos_layer_norm(const void* x, long long ldx, const void* weight, const void* bias, int rows, int H, float eps,
@@ -316,7 +316,7 @@ int kleos_combine_tokens_backward(const void* dout, long long ldd, const void* r
 
 /* y[r] = x[r] W[e]^T + bias[e] for the rows r of expert e, offsets[e] <= r < offsets[e + 1]; zeros for rows from
  * offsets[E] on.  x [rows, K], W [E, N, K], bias [E, N] or NULL, y [rows, N].  offsets is ascending from 0; what it says
- * beyond `rows` is not read.  E from 1 to 1024. */
+ * beyond `rows` is not read.  E from 1 to 1024, rows up to 2^31 - 2^16. */
 int kleos_expert_products(const void* x, long long ldx, const int32_t* offsets, const void* w, const void* bias, int rows,
                           int E, int N, int K, int torch_dtype, void* y, long long ldy, void* stream);
 

@@ -31,6 +31,7 @@ struct Args {
     float *mean, *rstd, *partial;
     long long ldx, lddy, ldy, lddx;
     int rows, H, depth;  // depth: stages of the ring
+    long long wait_cycles;  // for a row's copies
     bool wide;       // parameters are floats, whatever the element type
     bool param_vec;  // ... and can be loaded as vectors
     float eps;
@@ -125,12 +126,13 @@ struct Ring {
         for (int m = 0; m < kMatrices; ++m) tc::bulk_load(rows + (s * kMatrices + m) * H, from[m] + r * ld[m], bytes, &full[s]);
     }
     __device__ __forceinline__ const T* row(int s, int m) const { return rows + (s * kMatrices + m) * H; }
-    // False when the copies did not come in about ten seconds: the caller's results are NaN then.
-    __device__ __forceinline__ bool wait(int s, uint32_t parity) const {
+    // False when the copies did not come in so many cycles.  The thread then gives up: what it owes becomes NaN, it waits for
+    // no row after this one (its group's rows would each take as long again) and issues no copies.
+    __device__ __forceinline__ bool wait(int s, uint32_t parity, long long cycles) const {
         if (tc::mbar_try_wait(&full[s], parity)) return true;
         const long long t0 = clock64();
         while (!tc::mbar_try_wait(&full[s], parity))
-            if (clock64() - t0 > 20000000000LL) return false;
+            if (clock64() - t0 > cycles) return false;
         return true;
     }
 };
@@ -207,9 +209,10 @@ __global__ void __launch_bounds__(G * kForwardGroups<G>, G > 256 ? 1 : 2) forwar
     const float my_share = share[group][lane % W];  // of the warp that this lane answers for
     int stage = 0, turn = 0;
     uint32_t parity = 0;
+    bool dead = false;
     for (long long r = first; r < a.rows; r += step, turn ^= 1) {
-        const bool came = ring.wait(stage, parity);
-        F2 x[N][V / 2], s = both(0.f);
+        if (!dead) dead = !ring.wait(stage, parity, a.wait_cycles);
+        F2 x[N][V / 2], s = both(dead ? __uint_as_float(0x7fffffffu) : 0.f);  // (mean and deviation of the whole row with it)
         each_vector<V, G, N>(at, H, [&](int i, int j) {
             to_pairs<T, V>(load_vec<T, V>(ring.row(stage, 0) + j), x[i]);
 #pragma unroll
@@ -228,7 +231,7 @@ __global__ void __launch_bounds__(G * kForwardGroups<G>, G > 256 ? 1 : 2) forwar
         float q = warp_sum(sum2(q2));
         if (W > 1 && lane == 0) shared[group][turn][warp] = make_float2(m, q);
         meet<G>(group);  // ... and the row is in registers
-        if (at == 0) ring.issue(r + a.depth * step, stage);
+        if (at == 0 && !dead) ring.issue(r + a.depth * step, stage);
         if (++stage == a.depth) stage = 0, parity ^= 1;
         if constexpr (W > 1) {
             const float2 v = shared[group][turn][lane % W];
@@ -236,7 +239,7 @@ __global__ void __launch_bounds__(G * kForwardGroups<G>, G > 256 ? 1 : 2) forwar
             const float d = v.x - m;
             q = lanes_sum<W>(fmaf(my_share * d, d, v.y));
         }
-        const float rs = came ? rsqrtf(q * inv + a.eps) : __uint_as_float(0x7fffffffu);
+        const float rs = rsqrtf(q * inv + a.eps);
         T* y = static_cast<T*>(a.y) + r * a.ldy;
         const F2 rs2 = both(rs), m2 = both(-m);
         each_vector<V, G, N>(at, H, [&](int i, int j) {
@@ -250,6 +253,7 @@ __global__ void __launch_bounds__(G * kForwardGroups<G>, G > 256 ? 1 : 2) forwar
             if (a.rstd) a.rstd[r] = rs;
         }
     }
+    if (dead) tc::settle_after_abort();
 }
 
 // Any other row, loaded element by element while the row before it is added up.  (16384 rows of 4092 bf16, whose rows begin on
@@ -411,10 +415,12 @@ __global__ void __launch_bounds__(G * kGroups<G>, 1) backward_kernel(Args a) {
     int stage = 0;
     uint32_t parity = 0;
     long long turn = 0;
+    bool dead = false;
     for (long long r = first; r < a.rows; r += step, ++turn) {
         float m = next_m, rs = next_rs;
         if (r + step < a.rows) next_m = a.mean[r + step], next_rs = a.rstd[r + step];
-        if (!ring.wait(stage, parity)) rs = __uint_as_float(0x7fffffffu);
+        if (!dead) dead = !ring.wait(stage, parity, a.wait_cycles);
+        if (dead) rs = __uint_as_float(0x7fffffffu);  // (dx of the whole row and this thread's dw with it; db below)
         const T *px = ring.row(stage, 0), *pdy = ring.row(stage, 1);
         const F2 rs2 = both(rs), m2 = both(-m);
         F2 h[N][V / 2], g[N][V / 2], sg2 = both(0.f), sgh2 = both(0.f);
@@ -450,7 +456,7 @@ __global__ void __launch_bounds__(G * kGroups<G>, 1) backward_kernel(Args a) {
             sg = __shfl_sync(0xffffffffu, mine, 0);
             sgh = __shfl_sync(0xffffffffu, mine, 16);
         }
-        if (at == 0) ring.issue(r + a.depth * step, stage);  // (the group has met: the row is in registers)
+        if (at == 0 && !dead) ring.issue(r + a.depth * step, stage);  // (the group has met: the row is in registers)
         const F2 c0 = both(-rs * sg * inv), c1 = both(-rs * sgh * inv);
         T* dx = static_cast<T*>(a.dx) + r * a.lddx;
         each_vector<V, G, N>(at, H, [&](int i, int j) {
@@ -460,6 +466,13 @@ __global__ void __launch_bounds__(G * kGroups<G>, 1) backward_kernel(Args a) {
             store_vec<T, V>(dx + j, from_pairs<T, V>(o));
         });
         if (++stage == a.depth) stage = 0, parity ^= 1;
+    }
+    if (dead) {
+        tc::settle_after_abort();
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int k = 0; k < V / 2; ++k) db[i][k] = both(__uint_as_float(0x7fffffffu));
     }
     if (!a.partial) return;
     // the groups' sums side by side in shared memory, then added in their order

@@ -46,6 +46,8 @@ bool by(int bytes, size_t elem, std::initializer_list<const void*> ptrs, std::in
 }
 bool by_16(size_t elem, std::initializer_list<const void*> ptrs, std::initializer_list<long long> elems) { return by(16, elem, ptrs, elems); }
 
+constexpr long long kWaitCycles = 20000000000LL;  // about ten seconds: nothing but a copy or an MMA is waited for
+
 // ---------------------------------------------------------------- layer norm
 // Stages of a ring, `bytes` each, for `most` bytes on their way: one at least.
 constexpr int kRingMost = 224 * 1024;
@@ -218,7 +220,6 @@ bool encode_weights(CUtensorMap* map, int torch_dtype, const void* base, int E, 
 }
 
 constexpr int kLeastSteps = 4;  // of 64 elements that a part of a split sum has
-constexpr long long kWaitCycles = 20000000000LL;  // about ten seconds: nothing but a copy or an MMA is waited for
 
 // Pairs of blocks for so many tiles at most.
 int pair_grid(long long tiles) { return 2 * (int)std::max<long long>(1, std::min<long long>(sm_count() / 2, tiles)); }
@@ -439,7 +440,7 @@ int kleos_layer_norm(const void* x, long long ldx, const void* weight, const voi
     if (!sm_count()) return refuse(call, KLEOS_E_CUDA, "no current CUDA device");
     norm::Args a{};
     a.x = x; a.weight = weight; a.bias = bias; a.y = y; a.mean = mean; a.rstd = rstd;
-    a.ldx = ldx; a.ldy = ldy; a.rows = rows; a.H = H; a.wide = param_dtype == 0; a.eps = eps;
+    a.ldx = ldx; a.ldy = ldy; a.rows = rows; a.H = H; a.wide = param_dtype == 0; a.eps = eps; a.wait_cycles = kWaitCycles;
     a.param_vec = whole(16, {weight, bias});
     return with_type(call, torch_dtype, [&](auto* null) { return finish(call, norm_forward<std::remove_pointer_t<decltype(null)>>(a, stream_of(stream))); });
 }
@@ -461,7 +462,7 @@ int kleos_layer_norm_backward(const void* dy, long long lddy, const void* x, lon
     a.x = x; a.dy = dy; a.weight = weight; a.dx = dx; a.dweight = dweight; a.dbias = dbias;
     a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
     a.partial = sums ? static_cast<float*>(workspace) : nullptr;
-    a.ldx = ldx; a.lddy = lddy; a.lddx = lddx; a.rows = rows; a.H = H; a.wide = param_dtype == 0;
+    a.ldx = ldx; a.lddy = lddy; a.lddx = lddx; a.rows = rows; a.H = H; a.wide = param_dtype == 0; a.wait_cycles = kWaitCycles;
     a.param_vec = whole(16, {weight});
     return with_type(call, torch_dtype, [&](auto* null) { return finish(call, norm_backward<std::remove_pointer_t<decltype(null)>>(a, stream_of(stream))); });
 }

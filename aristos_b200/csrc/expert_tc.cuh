@@ -13,8 +13,8 @@
 // are multiplied, and in the last of those a warp of each block clears the rows that are not its own before the MMA
 // reads them (a factor of zero would not do: the other expert's row may be infinite).
 // Sums are fp32 in tensor memory: sixteen slots of 32 columns of which a tile of products takes as many as its rows need,
-// two accumulators of 256 columns for the weight gradients, so that the read-back of a tile runs beside the next one's main
-// loop.  No load is multicast; every wait is bounded, and a block that gives up stores NaN for what it owes.
+// two accumulators of 256 columns for the weight gradients (see kRead for those in floats), so that the read-back of a tile runs
+// beside the next one's main loop.  No load is multicast; every wait is bounded, and a block that gives up stores NaN for what it owes.
 //
 // What bounds them, measured alone: few rows an expert the weight stream (256 rows of 64 experts, N = K = 2048: 82 us for
 // 529 MB = 6.5 TB/s); 256 rows an expert HBM, and the tensor pipe at the clock the power limit leaves (16384 rows: 127 us forward,
@@ -476,6 +476,13 @@ namespace wg {
 constexpr int kSlices = 5;
 constexpr int SLICE_BYTES = 2 * HALF_BYTES;
 constexpr int STG_BYTES = 32 * 128;  // a warp's 32 rows of 128 bytes, twice
+// The matrix unit cuts its running sums off instead of rounding them: about 2^-27 of the sum of magnitudes a term, of one sign.  16-bit
+// results' own rounding covers that (16384 rows 1.1e-4, where rounding to fp16 takes up to 4.9e-4); that of floats does not: their sums
+// are read back every kRead slices, 256 rows, and added up in registers (128 a thread; 60 bytes of them spill).  2-norm error of 16384
+// rows, N(0,1) and of one sign: bf16 2.7e-7 and 4.0e-7, fp16 3.7e-7 and 1.2e-6 (all of the sum in the unit 1.9e-5 both, 8.3e-5 and
+// 1.1e-4).  One expert of 16384 rows, N = K = 2048: 112 us instead of 96; 8192 rows of 8, N = 14336, K = 4096 876 instead of 815;
+// 16384 of 64, N = K = 2048 232 instead of 227.  Tiles of 128 columns, whose sums are 64 registers, 198, 1186 and 249.
+constexpr int kRead = 4;
 using WeightBarriers = Barriers<kSlices, 2, 2>;
 struct Control {
     WeightBarriers b;
@@ -595,29 +602,33 @@ weight_tc_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
             bool ok = true;
             for (int t = t0; ok && t < total; t += dt) {
                 const int n = uniform(wg::tile_at(t, g, per, CT).n);
-                if (n == 0) continue;
-                ok = __all_sync(0xffffffffu, mbar_wait(&ctl->b.acc_empty[i & 1], ((i >> 1) & 1) ^ 1, g.wait_cycles, abort_flag));
-                tc_fence_after();
-                const uint32_t d = tmem + (i & 1) * ACC_COLS;
-                for (int kb = 0; ok && kb * BK < n; ++kb) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&ctl->b.full[s], ph, g.wait_cycles, abort_flag));
-                    if (!ok) break;
+                // (a sum is all of an expert's rows, or, of floats, the part that is read back at once)
+                for (int k0 = 0; ok && k0 * BK < n; k0 += wg::kRead) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&ctl->b.acc_empty[i & 1], ((i >> 1) & 1) ^ 1, g.wait_cycles, abort_flag));
                     tc_fence_after();
-                    const uint32_t sa = slices + s * SLICE_BYTES;
-                    const uint64_t da = make_major_desc(sa), db = make_major_desc(sa + HALF_BYTES);
-                    const int steps = min(BK / 16, (n - kb * BK + 15) >> 4);
+                    const uint32_t d = tmem + (i & 1) * ACC_COLS;
+                    const int end = kWideOut ? min(n, (k0 + wg::kRead) * BK) : n;
+                    for (int kb = k0; ok && kb * BK < end; ++kb) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(&ctl->b.full[s], ph, g.wait_cycles, abort_flag));
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t sa = slices + s * SLICE_BYTES;
+                        const uint64_t da = make_major_desc(sa), db = make_major_desc(sa + HALF_BYTES);
+                        const int steps = min(BK / 16, (end - kb * BK + 15) >> 4);
 #pragma unroll
-                    for (int k = 0; k < BK / 16; ++k)
-                        if (k < steps) umma_bf16_pair_if(elected, d, da + kMajorStep / 16 * k, db + kMajorStep / 16 * k, idesc, k != 0 ? 1u : (uint32_t)(kb != 0));
-                    umma_commit_both_if(elected, bars + (uint32_t)offsetof(WeightBarriers, empty) + 8 * s);
-                    if (++s == kSlices) {
-                        s = 0;
-                        ph ^= 1;
+                        for (int k = 0; k < BK / 16; ++k)
+                            if (k < steps) umma_bf16_pair_if(elected, d, da + kMajorStep / 16 * k, db + kMajorStep / 16 * k, idesc, k != 0 ? 1u : (uint32_t)(kb != k0));
+                        umma_commit_both_if(elected, bars + (uint32_t)offsetof(WeightBarriers, empty) + 8 * s);
+                        if (++s == kSlices) {
+                            s = 0;
+                            ph ^= 1;
+                        }
                     }
+                    if (!ok) *abort_flag = 1;
+                    else umma_commit_both_if(elected, bars + (uint32_t)offsetof(WeightBarriers, acc_full) + 8 * (i & 1));
+                    ++i;
+                    if (!kWideOut) break;
                 }
-                if (!ok) *abort_flag = 1;
-                else umma_commit_both_if(elected, bars + (uint32_t)offsetof(WeightBarriers, acc_full) + 8 * (i & 1));
-                ++i;
             }
         }
         __syncwarp();
@@ -625,39 +636,31 @@ weight_tc_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
         // ------------------------------------------------------------ read-back (both blocks)
         // Tensor-memory lane = row of dW[e], column = its column.  A warp takes the 32 rows of its quadrant, 128 bytes of
         // each at a time: through shared memory, swizzled, and from there by TMA, which leaves out what is past the edges.
-        constexpr int kCols = kWideOut ? 32 : 64;
+        constexpr int kCols = kWideOut ? 32 : 64, kMine = 128;  // columns of a turn, of a group
         const int q = warp & 3, grp = (warp - 4) >> 2;
         const uint32_t stg = smem_u32(stage + 2 * (warp - 4) * wg::STG_BYTES);
         uint32_t i = 0, turn = 0;
         bool dead = false;
         for (int t = t0; t < total; t += dt) {
             const wg::Tile x = wg::tile_at(t, g, per, CT);
-            const bool zero = x.n == 0;
-            if (!zero && !dead) {
+            const int m = x.m + (int)rank * BM + q * 32;
+            auto await = [&] {  // the next accumulator
+                if (dead) return;
                 const bool ok = mbar_wait(&ctl->b.acc_full[i & 1], (i >> 1) & 1, g.wait_cycles, abort_flag);
                 if (!ok) *abort_flag = 1;
                 dead = !__all_sync(0xffffffffu, ok);
                 tc_fence_after();
-            }
-            const uint32_t acc = tmem_base + (i & 1) * ACC_COLS + (static_cast<uint32_t>(q * 32) << 16);
-            const int m = x.m + (int)rank * BM + q * 32;
-#pragma unroll 1
-            for (int c = grp * 128; c < grp * 128 + 128; c += kCols) {
-                uint32_t r[kCols];
-                if (zero || dead) {
-#pragma unroll
-                    for (int k = 0; k < kCols; ++k) r[k] = dead ? 0x7fffffffu : 0u;
-                } else {
-                    tmem_ld_32x32(acc + c, r);
-                    if constexpr (!kWideOut) tmem_ld_32x32(acc + c + 32, r + 32);
-                    tmem_ld_wait();
-                }
-                if (c + kCols == grp * 128 + 128 && !zero) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) arrive_relaxed(map_to_cta(smem_u32(&ctl->b.acc_empty[i & 1]), 0));
-                }
-                if (m >= g.M || x.c + c >= g.len) continue;  // (the same for the whole warp)
+            };
+            auto acc = [&] { return tmem_base + (i & 1) * ACC_COLS + (static_cast<uint32_t>(q * 32) << 16) + grp * kMine; };
+            auto give_back = [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_relaxed(map_to_cta(smem_u32(&ctl->b.acc_empty[i & 1]), 0));
+                ++i;
+            };
+            auto store = [&](int c, const uint32_t* r) {  // columns grp * kMine + c ..
+                const int col = x.c + grp * kMine + c;
+                if (m >= g.M || col >= g.len) return;  // (the same for the whole warp)
                 // the rows of the turn before the last have left shared memory
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
                 __syncwarp();
@@ -680,9 +683,50 @@ weight_tc_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) tma_store_3d(&map_dw, half, x.c + c, m, x.e);
+                if (lane == 0) tma_store_3d(&map_dw, half, col, m, x.e);
+            };
+            if constexpr (kWideOut) {
+                uint32_t sum[kMine] = {};
+                for (int left = x.n; left > 0; left -= wg::kRead * BK) {
+                    await();
+                    if (!dead) {
+#pragma unroll
+                        for (int c = 0; c < kMine; c += 16) {
+                            uint32_t r[16];
+                            tmem_ld_32x16(acc() + c, r);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) sum[c + k] = __float_as_uint(__uint_as_float(sum[c + k]) + __uint_as_float(r[k]));
+                        }
+                    }
+                    give_back();
+                }
+                if (x.n > 0 && dead) {
+#pragma unroll
+                    for (int k = 0; k < kMine; ++k) sum[k] = 0x7fffffffu;  // NaN
+                }
+#pragma unroll
+                for (int c = 0; c < kMine; c += kCols) store(c, sum + c);
+            } else {
+                if (x.n > 0) await();
+#pragma unroll 1
+                for (int c = 0; c < kMine; c += kCols) {
+                    uint32_t r[kCols];
+                    if (x.n == 0 || dead) {
+#pragma unroll
+                        for (int k = 0; k < kCols; ++k) r[k] = x.n == 0 ? 0u : 0x7fffffffu;
+                    } else {
+                        tmem_ld_32x32(acc() + c, r);
+                        tmem_ld_32x32(acc() + c + 32, r + 32);
+                        tmem_ld_wait();
+                    }
+                    if (c + kCols == kMine && x.n > 0) {
+                        // (store() is behind: the accumulator is in registers)
+                        give_back();
+                    }
+                    store(c, r);
+                }
             }
-            if (!zero) ++i;
         }
         if (lane == 0) bulk_store_wait_all();
     }

@@ -62,7 +62,6 @@ struct TcArgs {
     int M;            // columns of the result (kernels of products), rows of dW[e] (weight gradients)
     int len;          // length of the sums (products), columns of dW[e]
     int units;        // products: units of 32 rows that a tile has at most, nine
-    bool wide_out;    // dW as floats
     long long wait_cycles;
 };
 

@@ -361,6 +361,8 @@ __device__ __forceinline__ float warp_sums(float a, float b) {
 // over the group, a barrier, addresses) is as many instructions as 16 elements.  A thread's columns are the same
 // in every row, so their sums stay in its registers; the weights, which would take as many again, are in shared
 // memory.  The groups of G threads go through rows of their own, each with a ring and a barrier, and add up at the end.
+// Above 8192 elements a row those sums are 64 registers a thread and about 440 bytes spill: 16384 x 16384 bf16 471 us = 3.4 TB/s, floats
+// 769 = 4.2.
 template <int G>
 constexpr int kGroups = 512 / G;
 

@@ -366,7 +366,7 @@ int products_few(const char* call, const experts::Args& a, int torch_dtype, cuda
 }
 
 // The tensor cores' kernels load by TMA, whose rows begin and end on 16-byte boundaries; everything else goes to the FP32
-// pipes, and so do a few rows.
+// pipes: up to so many rows with the weights streamed, more in tiles.
 constexpr int kFewRows = 32;
 
 // Whether float products are sooner done by streaming the weights once for every four rows, at 6.2 TB/s (c chunks of rows, every
@@ -395,7 +395,8 @@ int products(const char* call, const experts::Args& a, int torch_dtype, cudaStre
     }
     if (!tensor) return products_simt<kMode>(call, a, torch_dtype, st);
     // Weight gradients of few rows an expert are little but stores, and a tile of floats on the tensor cores has a long way
-    // through its roles (128 experts, N = 4424, K = 384: 1 row 199 us on the FP32 pipes and 646, 32 355 and 648, 48 482 and 648).
+    // through its roles (128 experts, N = 4424, K = 384: 1 row 199 us on the FP32 pipes and 646, 32 355 and 648, 48 482 and 648;
+    // the host knows the average only: 4096 rows on four of the 128 experts 371).
     if (kMode == experts::kDw && torch_dtype == 0 && a.rows <= 48LL * a.E) return products_simt<kMode>(call, a, torch_dtype, st);
     if (torch_dtype == 0) return products_f32<kMode>(call, a, st);
     if constexpr (kMode != experts::kDw) {
@@ -582,7 +583,8 @@ int kleos_expert_products_dw(const void* dy, long long lddy, const void* x, long
         constexpr int W = 16 / sizeof(T);
         const bool wide = by_16(sizeof(T), {dy}, {lddy, N});
         const int columns = experts::kBiasLanes * (wide ? W : 1), tiles = (N + columns - 1) / columns;
-        // two blocks a multiprocessor; blocks that share an expert's rows have 128 of them each
+        // two blocks a multiprocessor; blocks that share an expert's rows have 128 of them each (on average, which is what the host
+        // knows: N = 2048, bf16, 16384 rows of 64 experts 24 us, by Zipf 56, all of one expert 170)
         const int parts = (int)std::max(1LL, std::min({8LL, 2LL * sm_count() / ((long long)tiles * E), (long long)rows / E / 128}));
         const auto kernel = wide ? experts::bias_kernel<T, W> : experts::bias_kernel<T, 1>;
         return finish(call, launch(kernel, dim3(tiles * parts, E), 1024, 0, parts, st, a));

@@ -286,7 +286,8 @@ struct Sums<1> {
 
 // Without weights: the gradient of gather.  Vectors of one or two elements are loaded without a condition, at row 0
 // and the row's last vector where there is none (4000 tokens of 1087, top-8 64 -> 34 us); the bounds on registers are what wide
-// rows took before a token could have several blocks (16384 tokens of 64, top-4: 7.9 us, without them 10.8).
+// rows took before a token could have several blocks (16384 tokens of 64, top-4: 7.9 us, without them 10.8); eight rows of 16-byte
+// vectors spill 4 to 40 bytes under theirs.
 template <typename T, int V, int KT>
 __global__ void __launch_bounds__(256, V <= 2 ? (KT >= 4 ? 3 : 5) : KT >= 4 ? 3 : KT == 2 ? 5 : 6) combine_kernel(Move m) {
     constexpr int U = kAhead<V, KT>;

@@ -326,7 +326,7 @@ int kleos_expert_products(const void* x, long long ldx, const int32_t* offsets, 
  *
  * The sums of 16-bit products that become 16-bit results stay on the matrix unit, which cuts them off instead of rounding
  * them: up to about 2^-27 of the sum of the terms' magnitudes for every term, half a unit of fp16 after 2^16 terms of one
- * sign, of bf16 after 2^19.  dW in floats is read back every 256 rows instead and is within 1.3e-6 of the
+ * sign, of bf16 after 2^19.  dW in floats is read back every 256 rows instead and is within 1.4e-6 of the
  * 2-norm (measured up to 262144 rows). */
 int kleos_expert_products_dx(const void* dy, long long lddy, const int32_t* offsets, const void* w, int rows, int E, int N,
                              int K, int torch_dtype, void* dx, long long lddx, void* stream);

@@ -186,12 +186,15 @@ def _run_own(s):
         kleos.moe_tokens(s["x"], s["gate"], s["gate_bias"], s["w1"], s["b1"], s["w2"], s["b2"], case["act"], s["out"], s["topk"],
                          s["weights"], s["workspace"], stream)
         return {k: s[k] for k in ("out", "topk", "weights")}
-    kleos.adapter_products(s["x"], s["offsets"], s["adapter"], s["a"], s["b"], s["scale"], s["base"], s["y"], s["u"], stream)
+    # in 32 bits the plain form adds in place, into what the projection gave: so do the calls
+    y = s["base"] if case["dtype"] == "fp32" else s["y"]
+    kleos.adapter_products(s["x"], s["offsets"], s["adapter"], s["a"], s["b"], s["scale"], s["base"], y, s["u"], stream)
     if not case["train"]:
-        return dict(y=s["y"], u=s["u"])
-    kleos.adapter_products_backward(s["dy"], s["x"], s["u"], s["offsets"], s["adapter"], s["a"], s["b"], s["scale"], s["dbase"], s["dx"],
+        return dict(y=y, u=s["u"])
+    dx = s["dbase"] if case["dtype"] == "fp32" else s["dx"]
+    kleos.adapter_products_backward(s["dy"], s["x"], s["u"], s["offsets"], s["adapter"], s["a"], s["b"], s["scale"], s["dbase"], dx,
                                     s["da"], s["db"], s["workspace"], stream)
-    return {k: s[k] for k in ("y", "u", "dx", "da", "db")}
+    return dict(y=y, u=s["u"], dx=dx, da=s["da"], db=s["db"])
 
 
 def _run_plain(s):

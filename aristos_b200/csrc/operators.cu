@@ -21,32 +21,8 @@ namespace kleos {
 namespace {
 using namespace ops;
 
-size_t bytes_of(int torch_dtype) { return torch_dtype == 0 ? 4 : 2; }
-bool known_type(int torch_dtype) { return torch_dtype == 0 || torch_dtype == 2 || torch_dtype == 3; }
 constexpr int kMostColumns = 1 << 28;
-constexpr int kMostRows = 0x7fff0000;  // launches count rows in ints, and round them up to whole blocks
 constexpr char kNormSizes[] = "rows must be from 0 to 2^31 - 2^16, H from 1 to 2^28, and no row longer than its stride";
-constexpr char kTypes[] = "torch_dtype must be 0 (float), 2 (bf16) or 3 (fp16)";
-
-// Whether every pointer (null ones too) is where an element of so many bytes may be.
-bool whole(size_t bytes, std::initializer_list<const void*> ptrs) {
-    for (const void* p : ptrs)
-        if (!aligned(p, bytes)) return false;
-    return true;
-}
-constexpr char kWhole[] = "a device pointer is no multiple of its element's size";
-
-// Whether all of it can be moved 16 bytes at a time.
-bool by(int bytes, size_t elem, std::initializer_list<const void*> ptrs, std::initializer_list<long long> elems) {
-    for (const void* p : ptrs)
-        if (!aligned(p, bytes)) return false;
-    for (const long long n : elems)
-        if (n * (long long)elem % bytes) return false;
-    return true;
-}
-bool by_16(size_t elem, std::initializer_list<const void*> ptrs, std::initializer_list<long long> elems) { return by(16, elem, ptrs, elems); }
-
-constexpr long long kWaitCycles = 20000000000LL;  // about ten seconds: nothing but a copy or an MMA is waited for
 
 // ---------------------------------------------------------------- layer norm
 // Stages of a ring, `bytes` each, for `most` bytes on their way: one at least.

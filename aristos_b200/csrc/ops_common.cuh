@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cstdio>
+#include <initializer_list>
 
 #include "common.cuh"
 
@@ -115,7 +116,31 @@ inline int refuse(const char* call, int code, const char* what) {
     return code;
 }
 
+inline size_t bytes_of(int torch_dtype) { return torch_dtype == 0 ? 4 : 2; }
+inline bool known_type(int torch_dtype) { return torch_dtype == 0 || torch_dtype == 2 || torch_dtype == 3; }
+constexpr int kMostRows = 0x7fff0000;  // launches count rows in ints, and round them up to whole blocks
+constexpr char kTypes[] = "torch_dtype must be 0 (float), 2 (bf16) or 3 (fp16)";
+constexpr char kWhole[] = "a device pointer is no multiple of its element's size";
+constexpr long long kWaitCycles = 20000000000LL;  // about ten seconds: nothing but a copy or an MMA is waited for
+
 inline bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// Whether every pointer (null ones too) is where an element of so many bytes may be.
+inline bool whole(size_t bytes, std::initializer_list<const void*> ptrs) {
+    for (const void* p : ptrs)
+        if (!aligned(p, bytes)) return false;
+    return true;
+}
+
+// Whether all of it can be moved 16 bytes at a time.
+inline bool by(int bytes, size_t elem, std::initializer_list<const void*> ptrs, std::initializer_list<long long> elems) {
+    for (const void* p : ptrs)
+        if (!aligned(p, bytes)) return false;
+    for (const long long n : elems)
+        if (n * (long long)elem % bytes) return false;
+    return true;
+}
+inline bool by_16(size_t elem, std::initializer_list<const void*> ptrs, std::initializer_list<long long> elems) { return by(16, elem, ptrs, elems); }
 
 inline cudaStream_t stream_of(void* stream) { return stream ? static_cast<cudaStream_t>(stream) : cudaStreamPerThread; }
 
@@ -185,7 +210,7 @@ int with_type(const char* call, int torch_dtype, F f) {
         case 0: return f(static_cast<float*>(nullptr));
         case 2: return f(static_cast<__nv_bfloat16*>(nullptr));
         case 3: return f(static_cast<__half*>(nullptr));
-        default: return refuse(call, KLEOS_E_UNSUPPORTED, "torch_dtype must be 0 (float), 2 (bf16) or 3 (fp16)");
+        default: return refuse(call, KLEOS_E_UNSUPPORTED, kTypes);
     }
 }
 

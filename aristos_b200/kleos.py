@@ -30,7 +30,8 @@ EXPORTS = (
     "kleos_phase_times", "kleos_flow_timeline", "kleos_debug_flow_stamps", "kleos_debug_flow_stalls", "kleos_debug_tile_order", "kleos_launch_count", "kleos_debug_gemm_stats", "kleos_debug_suppress_return_flag", "kleos_gate_stats", "kleos_plan_placement", "kleos_placement_model", "kleos_route_static",
     "kleos_layer_norm", "kleos_layer_norm_workspace", "kleos_layer_norm_backward", "kleos_sort_tokens", "kleos_gather_tokens",
     "kleos_combine_tokens", "kleos_combine_tokens_backward", "kleos_expert_products", "kleos_expert_products_dx",
-    "kleos_expert_products_dw", "kleos_finalize", "kleos_error_string",
+    "kleos_expert_products_dw", "kleos_activation", "kleos_activation_backward", "kleos_moe_tokens_workspace", "kleos_moe_tokens",
+    "kleos_adapter_products", "kleos_adapter_products_workspace", "kleos_adapter_products_backward", "kleos_finalize", "kleos_error_string",
 )
 
 PHASE_NAMES = ("route", "slots", "dispatch", "plan", "gemm1", "gemm2", "combine", "total")
@@ -61,6 +62,10 @@ _OPERATOR_ARGS = {
     "kleos_sort_tokens": "piiipppp", "kleos_gather_tokens": "plppiiiiipp", "kleos_combine_tokens": "pppiiiiplp",
     "kleos_combine_tokens_backward": "plppppiiiiippp", "kleos_expert_products": "plpppiiiiiplp",
     "kleos_expert_products_dx": "plppiiiiiplp", "kleos_expert_products_dw": "plplpiiiiiippp",
+    "kleos_activation": "plliiiiplp", "kleos_activation_backward": "plplliiiiplp",
+    "kleos_moe_tokens_workspace": "iii", "kleos_moe_tokens": "plppppppiiiiiiiiplppplp",
+    "kleos_adapter_products": "plppppppliiiiiiiplpp", "kleos_adapter_products_workspace": "ii",
+    "kleos_adapter_products_backward": "plplpppppppliiiiiiiiplppplp",
 }
 
 _lib = None
@@ -87,7 +92,8 @@ def load_library() -> ctypes.CDLL:
         lib.kleos_gate_stats.argtypes = [ctypes.c_void_p] * 3
         lib.kleos_phase_times.argtypes = [ctypes.POINTER(ctypes.c_float), ctypes.c_int]
         lib.kleos_get_unique_id.argtypes = [ctypes.c_void_p]
-        lib.kleos_layer_norm_workspace.restype = ctypes.c_longlong
+        for name in ("kleos_layer_norm_workspace", "kleos_moe_tokens_workspace", "kleos_adapter_products_workspace"):
+            getattr(lib, name).restype = ctypes.c_longlong
         for name, args in _OPERATOR_ARGS.items():
             getattr(lib, name).argtypes = [_C[c] for c in args]
         _lib = lib
@@ -435,6 +441,126 @@ def expert_products_dw(dy, x, offsets, dw, dbias=None, stream=None) -> None:
     gt = torch.float32 if dw.dtype is torch.float32 else dt
     _launch(call, dev, dy.data_ptr(), lddy, x.data_ptr(), ldx, off, R, E, N, K, _codes.get(dt, -1), _codes.get(gt, -1),
             _whole(call, "dw", dw, (E, N, K), gt, dev), _maybe(call, "dbias", dbias, (E, N), gt, dev), stream)
+
+
+ACTIVATIONS = {"relu": 0, "gelu": 1, "silu": 2}
+
+
+def _activation_code(call, act) -> int:
+    code = ACTIVATIONS.get(act)
+    return _refuse(call, f"act must be one of {', '.join(ACTIVATIONS)}") if code is None else code
+
+
+def _gated(call, name, wide, I) -> int:
+    """Whether the first product has a second half that the activated one is multiplied with."""
+    if wide not in (I, 2 * I):
+        _refuse(call, f"{name} must have {I} columns, or gated {2 * I}")
+    return int(wide != I)
+
+
+def activation(z, act, h, stream=None) -> None:
+    """h = f(z), or f(z[:, :I]) * z[:, I:] where z has twice the columns of h; act is "relu", "gelu" (erf form) or "silu"."""
+    call = "kleos_activation"
+    _torch or _bind()
+    (R, I), ldh, dt, dev = _first(call, "h", h)
+    gated = _gated(call, "z", z.shape[1] if z.dim() == 2 else _refuse(call, "z must be a matrix"), I)
+    ldz = _rows(call, "z", z, R, I << gated, dt, dev)
+    _launch(call, dev, z.data_ptr(), ldz, R, I, _activation_code(call, act), gated, _codes.get(dt, -1), h.data_ptr(), ldh, stream)
+
+
+def activation_backward(dh, z, act, dz, stream=None) -> None:
+    """Gradient of activation: dz from dh and z."""
+    call = "kleos_activation_backward"
+    _torch or _bind()
+    (R, I), lddh, dt, dev = _first(call, "dh", dh)
+    gated = _gated(call, "z", z.shape[1] if z.dim() == 2 else _refuse(call, "z must be a matrix"), I)
+    ldz, lddz = _rows(call, "z", z, R, I << gated, dt, dev), _rows(call, "dz", dz, R, I << gated, dt, dev)
+    _launch(call, dev, dh.data_ptr(), lddh, z.data_ptr(), ldz, R, I, _activation_code(call, act), gated, _codes.get(dt, -1), dz.data_ptr(), lddz, stream)
+
+
+def moe_tokens_workspace(tokens: int, inner: int, top_k: int) -> int:
+    """Bytes of workspace that moe_tokens needs."""
+    n = load_library().kleos_moe_tokens_workspace(tokens, inner, top_k) if max(tokens, inner, top_k) <= _MOST_ROWS else _ARG
+    if n < 0:
+        _check(n, "kleos_moe_tokens_workspace")
+    return n
+
+
+def moe_tokens(x, gate, gate_bias, w1, b1, w2, b2, act, out, topk, weights, workspace, stream=None) -> None:
+    """A whole MoE layer for up to 128 tokens: the router (gate [E, H], gate_bias [E] floats or None), the experts that it chose
+    (w1 [E, I, H], gated [E, 2 I, H], w2 [E, H, I], biases or None) and the weighted sum of their results.
+
+    topk and weights [T, K] are written; without a gate they are read, as the caller's own router chose.  workspace has
+    moe_tokens_workspace(T, I, K) bytes."""
+    call, torch = "kleos_moe_tokens", _torch or _bind()
+    (T, H), ldx, dt, dev = _first(call, "x", x)
+    if w1.dim() != 3 or w2.dim() != 3 or topk.dim() != 2:
+        _refuse(call, "w1 and w2 must have three dimensions, topk two")
+    E, _, I = w2.shape
+    K = topk.shape[1]
+    gated = _gated(call, "w1", w1.shape[1], I)
+    if max(T, E, I, K) > _MOST_ROWS:
+        _refuse(call, "too many experts, columns or places")
+    ldo = _rows(call, "out", out, T, H, dt, dev)
+    space = _whole(call, "workspace", workspace, workspace.shape, workspace.dtype, dev)
+    _launch(call, dev, x.data_ptr(), ldx, _maybe(call, "gate", gate, (E, H), dt, dev), _maybe(call, "gate_bias", gate_bias, (E,), torch.float32, dev),
+            _whole(call, "w1", w1, (E, I << gated, H), dt, dev), _maybe(call, "b1", b1, (E, I << gated), dt, dev),
+            _whole(call, "w2", w2, (E, H, I), dt, dev), _maybe(call, "b2", b2, (E, H), dt, dev), T, H, I, E, K, _activation_code(call, act), gated,
+            _codes.get(dt, -1), out.data_ptr(), ldo, _whole(call, "topk", topk, (T, K), torch.int32, dev),
+            _whole(call, "weights", weights, (T, K), torch.float32, dev), space, workspace.nbytes, stream)
+
+
+def _adapters(call, offsets, adapter, a, b, scale, K, N, dt, dev):
+    """Requests, adapters and rank, and the addresses that both passes take."""
+    if adapter.dim() != 1 or a.dim() != 3:
+        _refuse(call, "adapter must be a vector and a [adapters, rank, K]")
+    R, (L, r, _) = adapter.shape[0], a.shape
+    if max(R, L, r) > _MOST_ROWS or R < 1:
+        _refuse(call, "there must be a request, and not more requests, adapters or ranks than an int holds")
+    return (R, L, r), (_whole(call, "offsets", offsets, (R + 1,), _torch.int32, dev), _whole(call, "adapter", adapter, (R,), _torch.int32, dev),
+                       _whole(call, "a", a, (L, r, K), dt, dev), _whole(call, "b", b, (L, N, r), dt, dev),
+                       _maybe(call, "scale", scale, (L,), _torch.float32, dev))
+
+
+def adapter_products(x, offsets, adapter, a, b, scale, base, y, u=None, stream=None) -> None:
+    """y = base + scale[l] u b[l]^T, u = x a[l]^T, for the rows of every request (offsets [R + 1]) and its adapter l (adapter [R],
+    -1 without one).  a [L, r, K], b [L, N, r]; scale may be None; base may be y itself or None; u [rows, r] floats, for the
+    backward pass, may be None."""
+    call, torch = "kleos_adapter_products", _torch or _bind()
+    (rows, K), ldx, dt, dev = _first(call, "x", x)
+    N = y.shape[1] if y.dim() == 2 else _refuse(call, "y must be a matrix")
+    ldy = _rows(call, "y", y, rows, N, dt, dev)
+    ldb = ldy if base is None else _rows(call, "base", base, rows, N, dt, dev)
+    (R, L, r), at = _adapters(call, offsets, adapter, a, b, scale, K, N, dt, dev)
+    _launch(call, dev, x.data_ptr(), ldx, *at, None if base is None else base.data_ptr(), ldb, rows, R, L, r, N, K, _codes.get(dt, -1), y.data_ptr(),
+            ldy, _maybe(call, "u", u, (rows, r), torch.float32, dev), stream)
+
+
+def adapter_products_workspace(rows: int, rank: int) -> int:
+    """Bytes of workspace that adapter_products_backward needs for da."""
+    n = load_library().kleos_adapter_products_workspace(rows, rank) if max(rows, rank) <= _MOST_ROWS else _ARG
+    if n < 0:
+        _check(n, "kleos_adapter_products_workspace")
+    return n
+
+
+def adapter_products_backward(dy, x, u, offsets, adapter, a, b, scale, dbase, dx, da=None, db=None, workspace=None, stream=None) -> None:
+    """Gradients of adapter_products: dx = dbase + scale[l] dy b[l] a[l] (dbase may be dx itself or None), da and db [as a and b, in
+    the element type or floats], summed over each adapter's rows.  da needs a workspace of adapter_products_workspace(rows, r) bytes."""
+    call, torch = "kleos_adapter_products_backward", _torch or _bind()
+    (rows, N), lddy, dt, dev = _first(call, "dy", dy)
+    K = x.shape[1] if x.dim() == 2 else _refuse(call, "x must be a matrix")
+    ldx, lddx = _rows(call, "x", x, rows, K, dt, dev), _rows(call, "dx", dx, rows, K, dt, dev)
+    ldb = lddx if dbase is None else _rows(call, "dbase", dbase, rows, K, dt, dev)
+    (R, L, r), at = _adapters(call, offsets, adapter, a, b, scale, K, N, dt, dev)
+    one = da if da is not None else db
+    gt = torch.float32 if one is not None and one.dtype is torch.float32 else dt
+    space, room = None, 0
+    if workspace is not None:
+        space, room = _whole(call, "workspace", workspace, workspace.shape, workspace.dtype, dev), workspace.nbytes
+    _launch(call, dev, dy.data_ptr(), lddy, x.data_ptr(), ldx, _whole(call, "u", u, (rows, r), torch.float32, dev), *at,
+            None if dbase is None else dbase.data_ptr(), ldb, rows, R, L, r, N, K, _codes.get(dt, -1), _codes.get(gt, -1), dx.data_ptr(), lddx,
+            _maybe(call, "da", da, (L, r, K), gt, dev), _maybe(call, "db", db, (L, N, r), gt, dev), space, room, stream)
 
 
 FLOW_MILESTONES = ("start", "planned", "first_tile", "last_gemm1_tile", "last_tile", "dispatched",

@@ -333,6 +333,55 @@ int kleos_expert_products_dx(const void* dy, long long lddy, const int32_t* offs
 int kleos_expert_products_dw(const void* dy, long long lddy, const void* x, long long ldx, const int32_t* offsets, int rows,
                              int E, int N, int K, int torch_dtype, int grad_dtype, void* dw, void* dbias, void* stream);
 
+/* The activation between an expert's two products: h = f(z), or gated h = f(z[:, :I]) * z[:, I:], with f of hidden_act
+ * 0 (ReLU), 1 (GELU, erf form) or 2 (SiLU, z / (1 + e^-z)).  z [rows, I], gated [rows, 2 I] (an expert's W1 has the rows of the
+ * activated half first), h [rows, I].  Elements are computed in 32 bits. */
+int kleos_activation(const void* z, long long ldz, long long rows, int I, int hidden_act, int gated, int torch_dtype, void* h,
+                     long long ldh, void* stream);
+
+/* Gradient of kleos_activation: dz from dh and z.  ReLU's slope at 0 is 0. */
+int kleos_activation_backward(const void* dh, long long lddh, const void* z, long long ldz, long long rows, int I, int hidden_act,
+                              int gated, int torch_dtype, void* dz, long long lddz, void* stream);
+
+/* A whole MoE layer for the few tokens of a decode step.
+ *   l = x gate^T + gate_bias;  the K largest l of a token (ties: the lower expert), their softmax as weights;
+ *   out = sum over k of weights[t, k] (W2[e] h + b2[e]),  h as kleos_activation makes it of W1[e] x + b1[e],  e = topk[t, k]
+ * x [T, H] and out [T, H] with row strides, gate [E, H], gate_bias [E] floats or NULL, W1 [E, I, H] (gated [E, 2 I, H]) and W2 [E, H, I]
+ * as the products above take them, b1 and b2 or NULL; T from 0 to 128, K from 1 to 8.
+ * topk [T, K] and weights [T, K] are written; with gate NULL they are what the caller's own router chose and are read: an id outside
+ * 0 .. E - 1 is a place without an expert, and an expert may be named twice.  Logits are 64-bit sums of the elements.  An expert
+ * whose logit is minus infinity (a gate_bias that takes it out of service) is never chosen: its place has topk -1 and weight 0, and a
+ * token without any expert has zeros.  NaN counts as the largest logit and makes its token's weights and results NaN.
+ * The workspace (16-byte aligned, kleos_moe_tokens_workspace(T, I, K) bytes, contents of no matter) belongs to the call while it runs:
+ * calls that may overlap have one each. */
+long long kleos_moe_tokens_workspace(int T, int I, int K);
+int kleos_moe_tokens(const void* x, long long ldx, const void* gate, const float* gate_bias, const void* w1, const void* b1,
+                     const void* w2, const void* b2, int T, int H, int I, int E, int K, int hidden_act, int gated, int torch_dtype,
+                     void* out, long long ldo, int32_t* topk, float* weights, void* workspace, long long workspace_bytes, void* stream);
+
+/* Low-rank adapters of many requests beside a projection that they share: for the rows of request i, offsets[i] <= row <
+ * offsets[i + 1], with l = adapter[i]
+ *   u = x A[l]^T,   y = base + scale[l] u B[l]^T
+ * x [rows, K], base and y [rows, N], A [L, r, K], B [L, N, r], scale [L] floats or NULL for ones, u [rows, r] floats for the backward
+ * pass, or NULL.  base (what the shared projection gave) may be y itself, or NULL for zeros.  offsets [R + 1] is ascending; rows before the
+ * first request or behind the last, and those of requests whose adapter is outside 0 .. L - 1, have y = base and u = 0.
+ * R from 1 to 65536, L from 1 to 65535, r from 1 to 128. */
+int kleos_adapter_products(const void* x, long long ldx, const int32_t* offsets, const int32_t* adapter, const void* a, const void* b,
+                           const float* scale, const void* base, long long ldb, int rows, int R, int L, int r, int N, int K,
+                           int torch_dtype, void* y, long long ldy, float* u, void* stream);
+
+/* Gradients of kleos_adapter_products, from dy, x and the u of the forward pass:
+ *   v = scale[l] dy B[l],   dx = dbase + v A[l],   dA[l] = sum of v^T x,   dB[l] = scale[l] sum of dy^T u
+ * dbase (the shared projection's dx) may be dx itself, or NULL for zeros.  dA [L, r, K] and dB [L, N, r] of grad_dtype, 0 (float) or
+ * torch_dtype, zeros for an adapter without rows, may be NULL.  dA needs a 16-byte aligned workspace of
+ * kleos_adapter_products_workspace(rows, r) bytes, whose contents do not matter. */
+long long kleos_adapter_products_workspace(int rows, int r);
+int kleos_adapter_products_backward(const void* dy, long long lddy, const void* x, long long ldx, const float* u, const int32_t* offsets,
+                                    const int32_t* adapter, const void* a, const void* b, const float* scale, const void* dbase,
+                                    long long ldb, int rows, int R, int L, int r, int N, int K, int torch_dtype, int grad_dtype,
+                                    void* dx, long long lddx, void* da, void* db, void* workspace, long long workspace_bytes,
+                                    void* stream);
+
 /* Test hook for the failure path: while on, the expert FFN does not raise its "results
  * returned" flags, so the combine's bounded wait runs out, the forward records
  * {KLEOS_E_DEVICE, KLEOS_AT_COMBINE_WAIT} and returns with the context intact.  Nothing is

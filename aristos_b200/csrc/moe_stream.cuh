@@ -1,0 +1,444 @@
+// The experts of a few tokens (moe_tokens.cuh) where rows begin on 16-byte boundaries: the chosen experts' weights are streamed once.
+//
+//   stream_kernel<kUp>    h of every place, the second factor of a gated expert in the same pass
+//   stream_kernel<kDown>  out, all experts' shares of a column added up by the block that owns it
+//
+// One block a multiprocessor owns a share of the columns of EVERY expert, so the work is even however the tokens were sent, each sum is
+// finished where it began, and nothing is joined between blocks.  Its eight warps are teams that take the experts in turn; each warp of
+// a team goes through its own 128 or 256 bytes of the weights' rows, and of the rows they are multiplied with, by 16-byte copies to
+// shared memory that are kDepth - 1 steps ahead, across experts (copies of whole rows by the bulk engine took 90 cycles each of the
+// warp that issued them: 1480 us instead of 383 for 128 tokens).  A step is multiplied on the tensor cores (warp_mma.cuh), weights on the
+// instruction's 16 rows, up to 32 rows of an expert on its columns; floats by 32-bit multiply-adds, which up to 16 rows an expert are
+// fewer than the splitting that the tensor cores would want.  A team's partial sums meet in shared memory once an expert and tile.
+//
+// h goes from one kernel to the other rounded to the element type, as in the library's other layer.
+//
+// The second kernel's first weights are on their way before the first kernel has ended (common.cuh: which experts those are was
+// written by the kernel before both).
+#pragma once
+
+#include <cuda.h>
+
+#include "moe_tokens.cuh"
+#include "tc_common.cuh"
+#include "warp_mma.cuh"
+
+namespace kleos {
+namespace tokens {
+
+constexpr int kUp = 0, kUpGated = 1, kDown = 2;
+constexpr int kStreamWarps = 8, kStreamThreads = 32 * kStreamWarps;
+constexpr int kDepth = 3;                            // steps of a warp in shared memory
+constexpr int kMostSmem = 214 * 1024;
+constexpr int kMostRowsAtOnce = 32, kTileColumns = 16;
+constexpr int kTeam2 = 16, kTeam4 = 8;               // experts from which teams are of two warps, of four
+constexpr int kLine = 128;                           // bytes of a row that a warp takes at a time
+
+// How a launch cuts the work up; the same for all its blocks.
+struct Cut {
+    int share;   // columns of a block
+    int tile;    // columns of those at a time
+    int rows;    // rows of an expert at a time
+    int slot;    // bytes of a warp's step
+    int past;    // bytes behind the last slot that are read for rows that it does not have, whose products nobody takes
+};
+// Rows of a slot: 16 of the weights (32 of a gated expert, or of more columns), then those that they are multiplied with.
+__host__ __device__ constexpr int padded_rows(int rows) { return (rows + 7) / 8 * 8; }
+// Floats that the warps need beside their slots: two buffers to meet in, and (kDown) a tile's results by team.
+__host__ __device__ constexpr int meet_floats(int sets, int rows) { return kStreamWarps * 16 * sets * padded_rows(rows); }
+
+// Places by expert, within an expert in their own order; those without an expert are left out.
+struct Groups {
+    short of[kMostPlaces], token[kMostPlaces];  // the places in order, and whose they are
+    float weight[kMostPlaces];                  // kDown
+    short expert[kMaxExperts];                  // those that have a place, ascending
+    short begin[kMaxExperts + 1];               // where their places begin
+    int n;
+};
+struct Counts {
+    short of[kMaxExperts];
+};
+
+// All threads of the block call it; one warp goes through the places, 32 at a time.  `counts` is only used where there are more than 32.
+__device__ __forceinline__ void group_places(const Args& a, Groups& g, Counts& counts) {
+    const int lane = threadIdx.x & 31, n = a.T * a.K;
+    if (n > 32) {
+        for (int e = threadIdx.x; e < a.E; e += blockDim.x) counts.of[e] = 0;
+        __syncthreads();
+    }
+    auto expert_of = [&](int i) {
+        const int e = i < n ? __ldcg(a.topk + i) : -1;
+        return e >= 0 && e < a.E ? e : -1;
+    };
+    auto put = [&](int to, int i) {
+        g.of[to] = (short)i;
+        g.token[to] = (short)(i / a.K);
+    };
+    const unsigned below_me = (1u << lane) - 1;
+    if (threadIdx.x < 32 && n <= 32) {
+        const int e = expert_of(lane);
+        const unsigned same = __match_any_sync(0xffffffffu, e), firsts = __ballot_sync(0xffffffffu, e >= 0 && (same & below_me) == 0);
+        int rank = __popc(same & below_me), used = 0;
+        for (unsigned m = firsts; m; m &= m - 1) {  // experts before this one
+            const int from = __ffs(m) - 1, other = __shfl_sync(0xffffffffu, e, from), places = __popc(__shfl_sync(0xffffffffu, same, from));
+            if (other < e) rank += places, ++used;
+        }
+        if (e >= 0) {
+            put(rank, lane);
+            if ((same & below_me) == 0) g.expert[used] = (short)e, g.begin[used] = (short)rank;
+        }
+        const int places = __popc(__ballot_sync(0xffffffffu, e >= 0));
+        if (lane == 0) g.n = __popc(firsts), g.begin[__popc(firsts)] = (short)places;
+    } else if (threadIdx.x < 32) {
+        constexpr int kSteps = kMostPlaces / 32;
+        short at[kSteps], expert[kSteps];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) expert[s] = s * 32 < n ? (short)expert_of(s * 32 + lane) : (short)-1;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            if (s * 32 >= n) break;
+            const unsigned same = __match_any_sync(0xffffffffu, expert[s]);
+            const int below = __popc(same & below_me);
+            if (expert[s] >= 0) at[s] = (short)(counts.of[expert[s]] + below);
+            __syncwarp();
+            if (expert[s] >= 0 && below == 0) counts.of[expert[s]] += (short)__popc(same);
+            __syncwarp();
+        }
+        int begin = 0, used = 0;
+        for (int e0 = 0; e0 < a.E; e0 += 32) {
+            const int e = e0 + lane, c = e < a.E ? counts.of[e] : 0;
+            int up = c;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const int v = __shfl_up_sync(0xffffffffu, up, o);
+                if (lane >= o) up += v;
+            }
+            const unsigned any = __ballot_sync(0xffffffffu, c > 0);
+            if (e < a.E) counts.of[e] = (short)(begin + up - c);
+            if (c > 0) {
+                const int u = used + __popc(any & below_me);
+                g.expert[u] = (short)e;
+                g.begin[u] = (short)(begin + up - c);
+            }
+            begin += __shfl_sync(0xffffffffu, up, 31);
+            used += __popc(any);
+        }
+        if (lane == 0) g.n = used, g.begin[used] = (short)begin;
+        __syncwarp();
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            if (s * 32 >= n) break;
+            if (expert[s] >= 0) put(counts.of[expert[s]] + at[s], s * 32 + lane);
+        }
+    }
+    __syncthreads();
+}
+
+// With experts enough for every team to have several, a warp goes through more of a sum before it meets others (128 tokens of 63 experts:
+// teams of eight 383 us, of four 355, of two 346; 37 tokens of 22: 186, 163, 158).
+__host__ __device__ __forceinline__ int team_size(int experts) { return experts >= kTeam2 ? 2 : experts >= kTeam4 ? 4 : 8; }
+
+__device__ __forceinline__ void copy_16(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void zero_16(uint32_t to) { asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory"); }
+
+// Where a warp's copies are in a launch's work: columns c0 .. c0 + w - 1 of expert e (number u of those that have a place), its places
+// p0 .. p0 + n - 1, step along the sum.
+struct At {
+    int c0, w, u, e, p0, n, end, step;
+};
+
+// kLines: lines of a row in a warp's step.  kSets: sets of 16 rows of the weights (of a gated expert one a half).
+template <typename T, int kKind, int kMode, int kLines, int kSets>
+__global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
+    constexpr bool kGated = kMode == kUpGated, kIsDown = kMode == kDown, kMma = sizeof(T) == 2;
+    static_assert(!kGated || kSets == 2, "a set for each half");
+    constexpr int kHalves = kGated ? 2 : 1;              // row sets of W1
+    constexpr int kNTiles = kMostRowsAtOnce / 8;
+    constexpr int kFloatRows = kSets == 2 ? 8 : 16;      // floats: rows at a time
+    constexpr int kRowBytes = kLines * kLine;            // of a slot's row
+    extern __shared__ __align__(128) char ring[];
+    __shared__ Groups g;
+
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, t = lane & 3;
+    const int cols = kIsDown ? a.H : a.I, row_bytes = (kIsDown ? a.I : a.H) * (int)sizeof(T);
+    const int first = blockIdx.x * c.share, last = min(cols, first + c.share);
+    const int padded = padded_rows(c.rows);
+    char* mine = ring + warp * kDepth * c.slot;
+    float* const behind = reinterpret_cast<float*>(ring + kStreamWarps * kDepth * c.slot + c.past);
+
+    // the down kernel waits for the kernel before it only where it needs h: the choice of experts was there before that began
+    if (!kIsDown) pdl_wait();
+    group_places(a, g, *reinterpret_cast<Counts*>(ring));
+    if (kIsDown)
+        for (int i = threadIdx.x; i < g.begin[g.n]; i += kStreamThreads) g.weight[i] = __ldcg(a.weights + g.of[i]);
+    __syncthreads();
+    if (!kIsDown) pdl_trigger();
+
+    // Warps that share a sum, and teams of so many that take every other expert.
+    const int size = team_size(g.n), teams = kStreamWarps / size, team = warp / size, part = warp % size;
+    const int stride = size * kRowBytes, steps = (row_bytes + stride - 1) / stride;
+    float* const results = behind + 2 * meet_floats(kSets, c.rows);
+    float* const sums = results + team * a.T * c.tile;
+    auto team_sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(32 * size) : "memory"); };
+
+    // Copies: 8 lanes a line, 16 bytes each.  In odd rows the halves of a line change places: eight rows of 64 bytes are read without two of
+    // them on one bank.
+    const int line = lane >> 3, sub = lane & 7, my_byte = part * kRowBytes + sub * 16;
+    const size_t next_set = (size_t)(kGated ? a.I : kTileColumns) * row_bytes;
+    const uint32_t to_lane = tc::smem_u32(mine) + line * kRowBytes + ((sub ^ (line & 1) * 4) * 16);
+    const char* const w_all = static_cast<const char*>(kIsDown ? a.w2 : a.w1);
+    const char* const x_all = static_cast<const char*>(kIsDown ? a.h : a.x);
+    const size_t x_row = (kIsDown ? a.ldh : a.ldx) * sizeof(T);
+    const short* const x_of = kIsDown ? g.of : g.token;
+    const char *weights = nullptr, *row0 = nullptr;  // of this lane's first rows, at the step where the copies are
+    const size_t next_rows = (size_t)4 * row_bytes;
+    int byte = 0;                                    // of the row, there
+    At ahead{};
+    auto enter = [&] {
+        ahead.e = g.expert[ahead.u];
+        ahead.p0 = g.begin[ahead.u];
+        ahead.end = g.begin[ahead.u + 1];
+    };
+    auto find = [&] {
+        ahead.n = min(c.rows, ahead.end - ahead.p0);
+        const size_t row = kIsDown ? (size_t)ahead.e * a.H + ahead.c0 : (size_t)ahead.e * kHalves * a.I + ahead.c0;
+        weights = w_all + (row + line) * row_bytes + my_byte;
+        if (line < ahead.n) row0 = x_all + x_of[ahead.p0 + line] * x_row + my_byte;
+        byte = my_byte;
+    };
+    auto begin = [&] {
+        ahead.u = team;
+        ahead.c0 = team < g.n ? first : last;
+        ahead.w = min(c.tile, last - first);
+        ahead.step = 0;
+        if (team < g.n) enter(), find();
+    };
+    auto go_on = [&] {
+        weights += stride;
+        row0 += stride;
+        byte += stride;
+        if (++ahead.step < steps) return;
+        ahead.step = 0;
+        ahead.p0 += c.rows;
+        if (ahead.p0 >= ahead.end) {
+            ahead.u += teams;
+            if (ahead.u >= g.n) {
+                ahead.u = team;
+                ahead.c0 += c.tile;
+                ahead.w = min(c.tile, last - ahead.c0);
+            }
+            enter();
+        }
+        find();
+    };
+    // (a row may end inside a step: there the copies are of zeros.  A line ends in one too, or is whole: 128 bytes are eight lanes' 16.)
+    auto copy = [&](int slot, bool take_weights, bool take_rows) {
+        const uint32_t to = to_lane + slot * c.slot;
+#pragma unroll
+        for (int l = 0; l < kLines; ++l) {
+            const bool there = byte + l * kLine < row_bytes;
+            if (take_weights) {
+                const char* p = weights + l * kLine;
+#pragma unroll
+                for (int m = 0; m < kSets; ++m) {
+                    const int rows = (kGated ? ahead.w : ahead.w - m * kTileColumns) - line;
+                    const char* q = p + (m ? next_set : 0);
+#pragma unroll
+                    for (int i = 0; i < kTileColumns / 4; ++i, q += next_rows) {
+                        const uint32_t at = to + (m * kTileColumns + 4 * i) * kRowBytes + l * kLine;
+                        if (there && 4 * i < rows) copy_16(at, q);
+                    }
+                }
+            }
+            if (take_rows) {
+                const uint32_t to_row = to + kSets * kTileColumns * kRowBytes + l * kLine;
+                if (there && line < ahead.n) copy_16(to_row, row0 + l * kLine);
+                if (ahead.n > 4)
+                    for (int r = line + 4; r < ahead.n; r += 4) {
+                        const char* q = x_all + x_of[ahead.p0 + r] * x_row + byte + l * kLine;
+                        if (!there) break;
+                        copy_16(to_row + (r - line) * kRowBytes, q);
+                    }
+            }
+            if (!there) {  // zeros for all the slot's rows: what is multiplied with zeros has to be a number
+                if (take_weights)
+                    for (int r = 0; r < kSets * kTileColumns; r += 4) zero_16(to + r * kRowBytes + l * kLine);
+                if (take_rows) {
+                    const uint32_t to_row = to + kSets * kTileColumns * kRowBytes + l * kLine;
+                    for (int r = line; r < ahead.n; r += 4) zero_16(to_row + (r - line) * kRowBytes);
+                }
+            }
+        }
+    };
+    auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+
+    begin();
+    if constexpr (kIsDown) {
+        for (int i = 0; i < kDepth - 1 && ahead.c0 < last; ++i) {
+            copy(i, true, false);
+            go_on();
+        }
+        pdl_wait();  // (who reads what is in out, or wrote what h is made of, is done)
+        pdl_trigger();
+        begin();
+    }
+    for (int i = 0; i < kDepth - 1; ++i) {
+        if (ahead.c0 < last) {
+            copy(i, !kIsDown, true);
+            go_on();
+        }
+        commit();
+    }
+
+    int slot = 0, turn = 0;
+    const int lane_in_team = part * 32 + lane;
+    const char* in_lane = mine + quad * kRowBytes;
+    const int chunk[2] = {(t ^ (quad & 1) * 4) * 16, ((4 + t) ^ (quad & 1) * 4) * 16};  // this lane's 16 bytes of either half of a line
+    auto next_slot = [&] {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
+        __syncwarp();
+        if (ahead.c0 < last) {  // into the slot that the step before has left
+            copy(slot == 0 ? kDepth - 1 : slot - 1, true, true);
+            go_on();
+        }
+        commit();
+        const char* in = in_lane + slot * c.slot;
+        if (++slot == kDepth) slot = 0;
+        return in;
+    };
+    for (int c0 = first; c0 < last; c0 += c.tile) {
+        const int w = min(c.tile, last - c0);
+        if (kIsDown)
+            for (int i = lane_in_team; i < a.T * w; i += 32 * size) sums[i] = 0.f;
+        for (int u = team; u < g.n; u += teams) {
+            const int e = g.expert[u], end = g.begin[u + 1];
+            for (int p0 = g.begin[u]; p0 < end; p0 += c.rows) {
+                const int n = min(c.rows, end - p0);
+                // what a finished sum becomes: of a gated expert, z and what it is multiplied with
+                auto finish_up = [&](int column, int row, float z, float z2) {
+                    const T* b1 = static_cast<const T*>(a.b1) + (size_t)e * kHalves * a.I + c0 + column;
+                    if (a.b1) z += Elem<T>::to_f(*b1);
+                    float h = act::value<kKind, kMma>(z);
+                    if constexpr (kGated) h *= a.b1 ? z2 + Elem<T>::to_f(b1[a.I]) : z2;
+                    T* out = static_cast<T*>(a.h) + (size_t)g.of[p0 + row] * a.ldh + c0 + column;
+                    *out = Elem<T>::from_f(h);
+                };
+                // two buffers in turn, so that a team meets once a sum
+                float* meet = behind + (turn ? meet_floats(kSets, c.rows) : 0) + team * size * 16 * kSets * padded;
+                turn ^= 1;
+                if constexpr (kMma) {
+                    const int tiles = (n + 7) / 8;
+                    float s[kSets][kNTiles][4];
+#pragma unroll
+                    for (int m = 0; m < kSets; ++m)
+#pragma unroll
+                        for (int j = 0; j < kNTiles; ++j)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[m][j][i] = 0.f;
+                    for (int step = 0; step < steps; ++step) {
+                        const char* in = next_slot();
+#pragma unroll
+                        for (int b = 0; b < 2 * kLines; ++b) {
+                            const char* at_block = in + b / 2 * kLine + chunk[b & 1];
+                            wm::Rows16<T> q[kSets];
+#pragma unroll
+                            for (int m = 0; m < kSets; ++m)
+                                q[m].set(*reinterpret_cast<const uint4*>(at_block + 16 * m * kRowBytes), *reinterpret_cast<const uint4*>(at_block + (16 * m + 8) * kRowBytes));
+                            at_block += kSets * kTileColumns * kRowBytes;
+#pragma unroll
+                            for (int j = 0; j < kNTiles; ++j) {
+                                if (j >= tiles) break;
+                                wm::Rows8<T> x;
+                                x.set(*reinterpret_cast<const uint4*>(at_block + j * 8 * kRowBytes));
+#pragma unroll
+                                for (int m = 0; m < kSets; ++m) wm::multiply<T>(s[m][j], q[m], x);
+                            }
+                        }
+                        __syncwarp();
+                    }
+#pragma unroll
+                    for (int m = 0; m < kSets; ++m)
+#pragma unroll
+                        for (int j = 0; j < kNTiles; ++j) {
+                            if (j >= tiles) break;
+                            float* to = meet + ((part * kSets + m) * 16 + quad) * padded + j * 8 + t * 2;
+                            *reinterpret_cast<float2*>(to) = make_float2(s[m][j][0], s[m][j][1]);
+                            *reinterpret_cast<float2*>(to + 8 * padded) = make_float2(s[m][j][2], s[m][j][3]);
+                        }
+                } else {
+                    // floats: a lane multiplies its 16 bytes of two rows of each set with the same bytes of every row
+                    F2 s[2 * kSets][kFloatRows];
+#pragma unroll
+                    for (int m = 0; m < 2 * kSets; ++m)
+#pragma unroll
+                        for (int j = 0; j < kFloatRows; ++j) s[m][j] = both(0.f);
+                    for (int step = 0; step < steps; ++step) {
+                        const char* in = next_slot();
+#pragma unroll
+                        for (int b = 0; b < 2 * kLines; ++b) {
+                            F2 q[2 * kSets][2];
+#pragma unroll
+                            for (int m = 0; m < 2 * kSets; ++m)
+                                to_pairs<float, 4>(load_vec<float, 4>(reinterpret_cast<const float*>(in + 8 * m * kRowBytes + b / 2 * kLine + chunk[b & 1])), q[m]);
+                            const char* x0 = in - quad * kRowBytes + kSets * kTileColumns * kRowBytes + b / 2 * kLine;
+#pragma unroll
+                            for (int j = 0; j < kFloatRows; ++j) {
+                                if (j >= n) break;
+                                F2 x[2];
+                                to_pairs<float, 4>(load_vec<float, 4>(reinterpret_cast<const float*>(x0 + j * kRowBytes + ((((b & 1) * 4 + t) ^ (j & 1) * 4) * 16))), x);
+#pragma unroll
+                                for (int m = 0; m < 2 * kSets; ++m) s[m][j] = fma2(q[m][1], x[1], fma2(q[m][0], x[0], s[m][j]));
+                            }
+                        }
+                        __syncwarp();
+                    }
+#pragma unroll
+                    for (int j = 0; j < kFloatRows; ++j) {
+                        if (j >= n) break;
+#pragma unroll
+                        for (int m = 0; m < 2 * kSets; ++m) {
+                            float v = sum2(s[m][j]);
+                            v += __shfl_xor_sync(0xffffffffu, v, 1);
+                            v += __shfl_xor_sync(0xffffffffu, v, 2);
+                            if (t == 0) meet[(part * 16 * kSets + 8 * m + quad) * padded + j] = v;
+                        }
+                    }
+                }
+                team_sync();
+                auto sum_of = [&](int column, int row) {
+                    const float* from = meet + column * padded + row;
+                    float v = *from;
+                    for (int k = 1; k < size; ++k) v += *(from += 16 * kSets * padded);
+                    return v;
+                };
+                for (int i = lane_in_team; i < w * n; i += 32 * size) {
+                    const int row = i / w, column = i - row * w;
+                    if constexpr (!kIsDown) {
+                        finish_up(column, row, sum_of(column, row), kGated ? sum_of(kTileColumns + column, row) : 0.f);
+                    } else {  // one thread a column and token: a choice may name an expert twice
+                        const int token = g.token[p0 + row];
+                        if (row > 0 && g.token[p0 + row - 1] == token) continue;
+                        const float b2 = a.b2 ? Elem<T>::to_f(static_cast<const T*>(a.b2)[(size_t)e * a.H + c0 + column]) : 0.f;
+                        float v = sums[token * w + column];
+                        for (int r = row; r < n && g.token[p0 + r] == token; ++r) v += g.weight[p0 + r] * (sum_of(column, r) + b2);
+                        sums[token * w + column] = v;
+                    }
+                }
+            }
+        }
+        if constexpr (kIsDown) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < a.T * w; i += kStreamThreads) {
+                float v = results[i];
+                for (int k = 1; k < teams; ++k) v += results[k * a.T * c.tile + i];
+                static_cast<T*>(a.out)[i / w * a.ldo + c0 + i % w] = Elem<T>::from_f(v);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+}  // namespace tokens
+}  // namespace kleos

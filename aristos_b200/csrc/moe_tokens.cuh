@@ -7,7 +7,7 @@
 // Three launches: gate_kernel chooses, up_kernel makes h, down_kernel makes out.  A call reads the chosen experts' weights
 // once and little else: bound by HBM, and by latency for one token.
 //
-// The logits are sums in 64 bits: which expert is chosen does not hang on the order of a sum.  An expert whose logit is
+// The logits are sums of 46 bits: which expert is chosen does not hang on the order of a sum.  An expert whose logit is
 // minus infinity is never chosen: the place keeps -1 and a weight of 0, and a token all of whose experts are out gives zeros.
 #pragma once
 
@@ -35,20 +35,30 @@ struct Args {
 };
 
 // ---------------------------------------------------------------- the router
-constexpr int kGateBlocks = 8, kGateWarps = 8, kGateTokens = 8;
+constexpr int kGateBlocks = 8, kGateWarps = 8, kGateTokens = 2;
 
-// Whether logit (a, i) comes before (b, j): the larger one, NaN before all, ties to the lower expert.
-__device__ __forceinline__ bool before(double a, int i, double b, int j) {
-    const bool na = a != a, nb = b != b;
-    if (na != nb) return na;
-    if (!na && a != b) return a > b;
-    return i < j;
-}
+// A sum that keeps what its additions round off (two floats at once): the total is exact to about 2^-46.  The multiprocessor's 64-bit
+// additions and conversions would take ten times as long (128 tokens, 64 experts: 41 us).
+struct Kept {
+    F2 s, rest;
+    __device__ __forceinline__ Kept() : s(both(0.f)), rest(both(0.f)) {}
+    static __device__ __forceinline__ F2 minus(F2 a, F2 b) { return fma2(b, both(-1.f), a); }
+    __device__ __forceinline__ void add(F2 p) {
+        const F2 to = add2(s, p), b = minus(to, s);
+        rest = add2(rest, add2(minus(s, minus(to, b)), minus(p, b)));
+        s = to;
+    }
+    __device__ __forceinline__ double total() const {
+        const float2 a = split(s), b = split(rest);
+        return ((double)a.x + (double)a.y) + ((double)b.x + (double)b.y);
+    }
+};
 
 // A cluster takes up to kGateTokens tokens: its warps share the experts, its blocks the tokens that are then chosen for.
 template <typename T, int V>
 __global__ void __launch_bounds__(32 * kGateWarps) gate_kernel(Args a) {
     namespace cg = cooperative_groups;
+    constexpr int P = V > 1 ? V / 2 : 1, U = 8;  // vectors of a row on their way
     cg::cluster_group cluster = cg::this_cluster();
     __shared__ double logits[kMaxExperts];
     const int block = (int)cluster.block_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -57,53 +67,71 @@ __global__ void __launch_bounds__(32 * kGateWarps) gate_kernel(Args a) {
     pdl_wait();
     pdl_trigger();
     const T* x = static_cast<const T*>(a.x) + t0 * a.ldx;
+    auto pairs_of = [](const Vec<T, V>& v, F2 (&p)[P]) {
+        if constexpr (V > 1) to_pairs<T, V>(v, p);
+        else p[0] = pair(Elem<T>::to_f(v.v[0]), 0.f);
+    };
     for (int e = block * kGateWarps + warp; e < a.E; e += kGateBlocks * kGateWarps) {
         const T* w = static_cast<const T*>(a.gate) + (size_t)e * a.H;
-        double s[kGateTokens];
+        Kept s[kGateTokens];
+        for (int k0 = lane * V; k0 < a.H; k0 += 32 * V * U) {
+            Vec<T, V> wv[U];
 #pragma unroll
-        for (int t = 0; t < kGateTokens; ++t) s[t] = 0.0;
-#pragma unroll 4
-        for (int k = lane * V; k < a.H; k += 32 * V) {
-            const Vec<T, V> wv = load_vec<T, V>(w + k);
+            for (int i = 0; i < U; ++i) wv[i] = load_vec<T, V>(w + min(k0 + i * 32 * V, a.H - V));
 #pragma unroll
             for (int t = 0; t < kGateTokens; ++t) {
                 if (t >= n) break;
-                const Vec<T, V> xv = load_vec<T, V>(x + t * a.ldx + k);
+                Vec<T, V> xv[U];
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    // (16-bit factors have an exact product in 32 bits)
-                    if constexpr (sizeof(T) == 2) s[t] += (double)(Elem<T>::to_f(wv.v[j]) * Elem<T>::to_f(xv.v[j]));
-                    else s[t] = fma((double)wv.v[j], (double)xv.v[j], s[t]);
+                for (int i = 0; i < U; ++i) xv[i] = load_vec<T, V>(x + t * a.ldx + min(k0 + i * 32 * V, a.H - V));
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    if (k0 + i * 32 * V >= a.H) break;
+                    F2 p[P], q[P];
+                    pairs_of(wv[i], p);
+                    pairs_of(xv[i], q);
+#pragma unroll
+                    for (int j = 0; j < P; ++j) {
+                        const F2 r = mul2(p[j], q[j]);  // (of 16-bit factors: exact)
+                        s[t].add(r);
+                        if constexpr (sizeof(T) == 4) s[t].rest = add2(s[t].rest, fma2(p[j], q[j], mul2(r, both(-1.f))));
+                    }
                 }
             }
         }
 #pragma unroll
         for (int t = 0; t < kGateTokens; ++t) {
             if (t >= n) break;
+            double v = s[t].total();
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) s[t] += __shfl_xor_sync(0xffffffffu, s[t], o);
-            if (lane == 0) *cluster.map_shared_rank(&logits[e], t) = a.gate_bias ? s[t] + (double)a.gate_bias[e] : s[t];
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if (lane == 0) *cluster.map_shared_rank(&logits[e], t) = a.gate_bias ? v + (double)a.gate_bias[e] : v;
         }
     }
     cluster.sync();
     if (block >= n || warp != 0) return;
     const int t = t0 + block;
+    // a logit as a number that grows with it, NaN above all; 0: minus infinity, or chosen already
+    auto key_of = [](double v) {
+        const unsigned long long b = __double_as_longlong(v == 0.0 ? 0.0 : v);
+        return v != v ? ~0ull : v == -INFINITY ? 0ull : (b >> 63) ? ~b : b | 1ull << 63;
+    };
     double mine = 0.0, top = 0.0;  // lane k: the k-th logit
     int id = -1;
     for (int k = 0; k < a.K; ++k) {
-        double best = -INFINITY;
-        int at = a.E;
-        for (int e = lane; e < a.E; e += 32)
-            if (before(logits[e], e, best, at)) best = logits[e], at = e;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const double other = __shfl_xor_sync(0xffffffffu, best, o);
-            const int place = __shfl_xor_sync(0xffffffffu, at, o);
-            if (before(other, place, best, at)) best = other, at = place;
+        unsigned long long best = 0;
+        int at = kMaxExperts;
+        for (int e = lane; e < a.E; e += 32) {
+            const unsigned long long key = key_of(logits[e]);
+            if (key > best) best = key, at = e;
         }
-        if (at >= a.E || best == -INFINITY) break;  // only experts that are out are left
-        if (k == 0) top = best;
-        if (lane == k) mine = best, id = at;
+        const unsigned high = __reduce_max_sync(0xffffffffu, (unsigned)(best >> 32));
+        const unsigned low = __reduce_max_sync(0xffffffffu, (unsigned)(best >> 32) == high ? (unsigned)best : 0u);
+        if (high == 0 && low == 0) break;  // only experts that are out are left
+        at = __reduce_min_sync(0xffffffffu, (unsigned)(best >> 32) == high && (unsigned)best == low ? at : kMaxExperts);
+        const double v = logits[at];
+        if (k == 0) top = v;
+        if (lane == k) mine = v, id = at;
         __syncwarp();
         if (lane == 0) logits[at] = -INFINITY;
         __syncwarp();

@@ -9,6 +9,7 @@
 
 #include "activation.cuh"
 #include "adapters.cuh"
+#include "moe_stream.cuh"
 #include "moe_tokens.cuh"
 
 namespace kleos {
@@ -68,6 +69,63 @@ const char* bad_activation(long long rows, int I, int gated, long long ldz, long
 // ---------------------------------------------------------------- layer for a few tokens
 long long moe_workspace(int T, int I, int K) { return (long long)T * K * 4 * ((I + 7) / 8 * 8); }
 
+// Shared memory of a launch that takes `rows` of an expert at a time, and where what is in it lies.
+template <typename T, int kMode, int kLines, int kSets>
+int moe_smem(const tokens::Args& a, tokens::Cut& c, int rows) {
+    using namespace tokens;
+    c.rows = rows;
+    c.slot = (kSets * kTileColumns + rows) * kLines * kLine;
+    c.past = (padded_rows(rows) - rows) * kLines * kLine;
+    const int teams = kStreamWarps / team_size(std::min(a.E, a.T * a.K));  // at most
+    return kStreamWarps * kDepth * c.slot + c.past + 4 * (2 * meet_floats(kSets, rows) + (kMode == kDown ? teams * a.T * c.tile : 0));
+}
+
+// False where not even `least` rows of an expert fit at a time.
+template <typename T, int kKind, int kMode, int kLines, int kSets>
+bool moe_stream_of(const tokens::Args& a, tokens::Cut c, int least, cudaStream_t st, cudaError_t* rc) {
+    using namespace tokens;
+    int rows = c.rows, smem;
+    least = std::min(least, rows);
+    while ((smem = moe_smem<T, kMode, kLines, kSets>(a, c, rows)) > kMostSmem) {
+        if (rows <= least) return false;
+        rows = std::max(least, (rows - 1) / 8 * 8);
+    }
+    const int cols = kMode == kDown ? a.H : a.I;
+    const auto kernel = stream_kernel<T, kKind, kMode, kLines, kSets>;
+    static bool allowed[64];
+    *rc = allow_smem(kernel, allowed, kMostSmem);
+    if (*rc == cudaSuccess) *rc = launch(kernel, dim3((cols + c.share - 1) / c.share), kStreamThreads, smem, 1, st, a, c);
+    return true;
+}
+
+template <typename T, int kKind, int kMode>
+cudaError_t moe_stream(const tokens::Args& a, cudaStream_t st) {
+    using namespace tokens;
+    const int sms = sm_count(), cols = kMode == kDown ? a.H : a.I;
+    cudaError_t rc = cudaErrorInvalidConfiguration;
+    Cut c{};
+    c.share = (cols + sms - 1) / sms;
+    // rows of an expert at a time: as many as it has on average and some
+    c.rows = std::min(a.T, a.T * a.K > 12 * a.E ? kMostRowsAtOnce : kMostRowsAtOnce / 2);
+    // two sets of 16 columns where that takes fewer tiles (a gated expert's are its halves)
+    const bool two = kMode != kUpGated && sizeof(T) == 2 && (c.share + 31) / 32 < (c.share + 15) / 16;
+    auto cut = [&](int most) {
+        const int tiles = (c.share + most - 1) / most;
+        c.tile = (c.share + tiles - 1) / tiles;
+    };
+    cut(two ? 2 * kTileColumns : kTileColumns);
+    if constexpr (sizeof(T) == 4) c.rows = std::min(c.rows, kMode == kUpGated ? 8 : 16);
+    if constexpr (kMode == kUpGated) {
+        if (moe_stream_of<T, kKind, kMode, 1, 2>(a, c, 8, st, &rc)) return rc;
+    } else {
+        if constexpr (sizeof(T) == 2)
+            if (two && moe_stream_of<T, kKind, kMode, 1, 2>(a, c, 8, st, &rc)) return rc;
+        cut(kTileColumns);
+        if (moe_stream_of<T, kKind, kMode, 2, 1>(a, c, 8, st, &rc) || moe_stream_of<T, kKind, kMode, 1, 1>(a, c, 8, st, &rc)) return rc;
+    }
+    return rc;
+}
+
 template <typename T>
 cudaError_t moe_layer(tokens::Args a, int kind, bool gated, bool route, cudaStream_t st) {
     using namespace tokens;
@@ -75,11 +133,16 @@ cudaError_t moe_layer(tokens::Args a, int kind, bool gated, bool route, cudaStre
     const int sms = sm_count();
     cudaError_t rc = cudaSuccess;
     if (route) {
-        // a token a cluster where there are clusters for all of them
-        const int clusters = std::max(1, sms / kGateBlocks);
-        a.group = std::min(kGateTokens, (a.T + clusters - 1) / clusters);
+        a.group = a.T <= 2 * sms / kGateBlocks ? 1 : kGateTokens;  // (a token's two blocks a multiprocessor)
         const auto kernel = by_16(sizeof(T), {a.x, a.gate}, {a.ldx, a.H}) ? gate_kernel<T, W> : gate_kernel<T, 1>;
         rc = launch(kernel, dim3((a.T + a.group - 1) / a.group * kGateBlocks), 32 * kGateWarps, 0, kGateBlocks, st, a);
+    }
+    if (rc == cudaSuccess && by_16(sizeof(T), {a.x, a.w1, a.w2, a.h}, {a.ldx, a.H, a.I})) {
+        rc = act::with_kind(kind, [&](auto k) {
+            constexpr int kKind = decltype(k)::value;
+            return gated ? moe_stream<T, kKind, kUpGated>(a, st) : moe_stream<T, kKind, kUp>(a, st);
+        });
+        return rc == cudaSuccess ? moe_stream<T, 0, kDown>(a, st) : rc;
     }
     if (rc == cudaSuccess) rc = act::with_kind(kind, [&](auto k) {
         constexpr int kKind = decltype(k)::value;

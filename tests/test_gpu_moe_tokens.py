@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from aristos_b200 import kleos
-from tests.operator_util import DT, EPS, check, gen, randn, stream, wide
+from tests.operator_util import DT, EPS, HALF_UNIT, LEAST, check, gen, randn, stream, wide
 from tests.test_gpu_activation import reference
 
 pytestmark = pytest.mark.gpu
@@ -58,7 +58,7 @@ class Layer:
             if self.gated:
                 u, du = z[:, I:], dz[:, I:]
                 h, dh = f * u, df * (u.abs() + du) + f.abs() * du + EPS * (f * u).abs()
-            dh = dh + (2.0 ** -16 if fast else 0.0) * h.abs()
+            dh = dh + (HALF_UNIT[self.x.dtype] * (h.abs() + dh) + LEAST[self.x.dtype] if fast else 0.0)
             y, dy = h @ w2.t(), dh @ w2.abs().t() + (I + 1) * EPS * (h.abs() @ w2.abs().t())
             if self.b2 is not None:
                 y = y + self.b2[e].double()

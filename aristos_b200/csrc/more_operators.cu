@@ -9,6 +9,7 @@
 
 #include "activation.cuh"
 #include "adapters.cuh"
+#include "adapters_mma.cuh"
 #include "moe_stream.cuh"
 #include "moe_tokens.cuh"
 
@@ -166,10 +167,42 @@ const char* bad_adapters(int rows, int R, int L, int r, int N, int K) {
     return nullptr;
 }
 
+// f with the smallest of the ranks that kernels are made for as a constant.
+template <typename F>
+cudaError_t with_rank(int r, F f) {
+    using std::integral_constant;
+    if (r <= 16) return f(integral_constant<int, 16>());
+    if (r <= 32) return f(integral_constant<int, 32>());
+    if (r <= 64) return f(integral_constant<int, 64>());
+    return f(integral_constant<int, 128>());
+}
+
+template <typename T, bool kBack, int RT, int TR>
+cudaError_t adapter_rows_mma(const adapters::Args& a, cudaStream_t st) {
+    using namespace adapters;
+    const long long tiles = a.rows / TR + a.R + 2;  // at most
+    // blocks of a cluster: while every warp has 128 bytes of a row to sum, and until two blocks a multiprocessor are there
+    int cluster = 1;
+    while (cluster < 8 && tiles * cluster < 2LL * sm_count() && a.len * 2 > cluster * Shape<RT, TR>::KS * 128) cluster *= 2;
+    if (tiles * cluster > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    const auto kernel = rows_mma_kernel<T, kBack, RT, TR>;
+    static bool allowed[64];
+    cudaError_t rc = allow_smem(kernel, allowed, Shape<RT, TR>::kBytes);
+    if (rc == cudaSuccess) rc = launch(kernel, dim3((unsigned)(tiles * cluster)), 256, Shape<RT, TR>::kBytes, cluster, st, a);
+    return rc;
+}
+
 template <typename T, bool kBack>
 cudaError_t adapter_rows(const adapters::Args& a, cudaStream_t st) {
     using namespace adapters;
     constexpr int W = 16 / sizeof(T);
+    if constexpr (sizeof(T) == 2) {
+        if (a.r % 8 == 0 && by_16(2, {a.in, a.p, a.q, a.base, a.out}, {a.ldi, a.ldb, a.ldo, a.len, a.cols}))
+            return with_rank(a.r, [&](auto rt) {
+                // requests of few rows: tiles of as many as the tensor cores take
+                return a.rows < 24LL * a.R ? adapter_rows_mma<T, kBack, decltype(rt)::value, 16>(a, st) : adapter_rows_mma<T, kBack, decltype(rt)::value, 64>(a, st);
+            });
+    }
     const long long tiles = a.rows / kRowsSimt + a.R + 2;  // at most
     int cluster = 8;
     while (cluster > 1 && tiles * cluster > 8LL * sm_count()) cluster /= 2;
@@ -181,6 +214,21 @@ cudaError_t adapter_rows(const adapters::Args& a, cudaStream_t st) {
 
 template <typename T, bool kDb>
 cudaError_t adapter_grads(const adapters::Grads& a, cudaStream_t st) {
+    using namespace adapters;
+    if constexpr (sizeof(T) == 2) {
+        if (a.r % 8 == 0 && by_16(2, {a.in}, {a.ldi, a.cols}))
+            return with_rank(std::min(a.r, 64), [&](auto rt) {
+                constexpr int RT = decltype(rt)::value, kBytes = GradShape<T, RT>::kBytes;
+                const auto kernel = grads_mma_kernel<T, kDb, RT>;
+                const long long strips = (a.cols + kGradColumns - 1) / kGradColumns, groups = strips * a.L * ((a.r + RT - 1) / RT);
+                int cluster = 1;
+                while (cluster < 8 && groups * cluster < 4LL * sm_count() && a.rows > cluster * kGradRows * 2LL) cluster *= 2;
+                static bool allowed[64];
+                cudaError_t rc = allow_smem(kernel, allowed, kBytes);
+                if (rc == cudaSuccess) rc = launch(kernel, dim3((unsigned)(strips * cluster), a.L, (a.r + RT - 1) / RT), 256, kBytes, cluster, st, a);
+                return rc;
+            });
+    }
     return launch(adapters::grads_kernel<T, kDb>, dim3((a.cols + 31) / 32, a.L, (a.r + 15) / 16), 256, 0, 1, st, a);
 }
 

@@ -49,7 +49,7 @@ __device__ __forceinline__ Group request_rows(const int* offsets, int R, int i, 
     return g;
 }
 
-// The `index`-th tile of so many rows; false when there are fewer.  All threads of the block (256) call it.
+// The `index`-th tile of so many rows; false when there are fewer.  All threads of the block (256 at most) call it.
 template <int kRows>
 __device__ __forceinline__ bool find_tile(const Args& a, int index, Tile* tile) {
     __shared__ Tile found;
@@ -57,7 +57,7 @@ __device__ __forceinline__ bool find_tile(const Args& a, int index, Tile* tile) 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) found.begin = -1;
     int before = 0;
-    for (int i0 = -1; i0 <= a.R; i0 += 256) {
+    for (int i0 = -1; i0 <= a.R; i0 += blockDim.x) {
         const int i = i0 + (int)threadIdx.x;
         Group g{0, 0};
         if (i <= a.R) g = request_rows(a.offsets, a.R, i, a.rows);
@@ -71,7 +71,7 @@ __device__ __forceinline__ bool find_tile(const Args& a, int index, Tile* tile) 
         if (lane == 31) sums[warp] = up;
         __syncthreads();
         int first = before + up - n;
-        for (int w = 0; w < 8; ++w) {
+        for (int w = 0; w < (int)blockDim.x / 32; ++w) {
             first += w < warp ? sums[w] : 0;
             before += sums[w];
         }
@@ -88,15 +88,27 @@ __device__ __forceinline__ bool find_tile(const Args& a, int index, Tile* tile) 
     return found.begin >= 0;
 }
 
-// out = base (zeros without one) for the columns [c0, c1) of a tile's rows.
-template <typename T>
+// out = base (zeros without one) for the columns [c0, c1) of a tile's rows, V elements at once.
+template <typename T, int V>
 __device__ __forceinline__ void copy_base(const Args& a, const Tile& t, int c0, int c1) {
     const T* base = static_cast<const T*>(a.base);
     T* out = static_cast<T*>(a.out);
     if (base == out) return;
-    for (int row = t.begin; row < t.end; ++row)
-        for (int c = c0 + (int)threadIdx.x; c < c1; c += blockDim.x)
-            out[row * a.ldo + c] = base ? base[row * a.ldb + c] : Elem<T>::from_f(0.f);
+    constexpr int U = 8;  // of a thread on their way
+    const int across = (c1 - c0 + V - 1) / V, n = (t.end - t.begin) * across;
+    for (int i0 = threadIdx.x; i0 < n; i0 += U * blockDim.x) {
+        Vec<T, V> v[U] = {};
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int i = i0 + k * (int)blockDim.x;
+            if (base && i < n) v[k] = load_vec<T, V>(base + (long long)(t.begin + i / across) * a.ldb + c0 + i % across * V);
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int i = i0 + k * (int)blockDim.x;
+            if (i < n) store_vec<T, V>(out + (long long)(t.begin + i / across) * a.ldo + c0 + i % across * V, v[k]);
+        }
+    }
 }
 
 // ---------------------------------------------------------------- rows, any element type and alignment
@@ -116,7 +128,7 @@ __global__ void __launch_bounds__(256) rows_kernel(Args a) {
     if (!find_tile<M>(a, blockIdx.x / blocks, &t)) return;  // (all blocks of the cluster)
     const int n = t.end - t.begin, share = (a.cols + blocks - 1) / blocks, c0 = min(a.cols, block * share), c1 = min(a.cols, c0 + share);
     if (t.adapter < 0) {
-        copy_base<T>(a, t, c0, c1);
+        copy_base<T, 1>(a, t, c0, c1);
         if (a.u && block == 0)
             for (int i = threadIdx.x; i < n * a.r; i += 256) a.u[(long long)t.begin * a.r + i] = 0.f;
         return;

@@ -58,7 +58,8 @@ __global__ void __launch_bounds__(256, RT == 64 && TR == 64 ? 1 : 2) rows_mma_ke
     constexpr int MT = S::MT, RG = S::RG, KS = S::KS, NT = S::NT;
     constexpr int kQ = RT == 16 ? 2 : 4;   // n-tiles of a vector of P, backward
     constexpr bool kShrink = std::is_same<T, __half>::value;
-    extern __shared__ __align__(16) float part[];       // [KS][TR][pitch]
+    extern __shared__ __align__(128) char memory[];
+    float* const part = reinterpret_cast<float*>(memory);  // [KS][TR][pitch]
     __shared__ __align__(16) T ub[TR][RT + 8];
     __shared__ float grow[TR];                          // what a row's second product is multiplied with
     cg::cluster_group cluster = cg::this_cluster();
@@ -71,8 +72,8 @@ __global__ void __launch_bounds__(256, RT == 64 && TR == 64 ? 1 : 2) rows_mma_ke
     if (!find_tile<TR>(a, blockIdx.x / blocks, &tile)) return;  // (all blocks of the cluster)
     const int n = tile.end - tile.begin;
     if (tile.adapter < 0) {
-        const int share = (a.cols + blocks - 1) / blocks, c0 = min(a.cols, block * share);
-        copy_base<T>(a, tile, c0, min(a.cols, c0 + share));
+        const int share = ((a.cols + blocks - 1) / blocks + 7) / 8 * 8, c0 = min(a.cols, block * share);
+        copy_base<T, 8>(a, tile, c0, min(a.cols, c0 + share));
         if (a.u && block == 0)
             for (int i = threadIdx.x; i < n * a.r; i += 256) a.u[(long long)tile.begin * a.r + i] = 0.f;
         return;
@@ -316,29 +317,286 @@ __global__ void __launch_bounds__(256, RT == 64 && TR == 64 ? 1 : 2) rows_mma_ke
     }
 }
 
+// ---------------------------------------------------------------- many rows
+// The same for tiles enough to fill the GPU: a block of four warps takes 64 rows alone.  What it multiplies comes through a ring of kStages
+// steps of 64 elements in shared memory, 16-byte copies that run ahead from the first product into the second, and reaches the tensor cores by
+// ldmatrix (transposed where the summed direction is not the contiguous one).  Rows of 128, 64 or 32 bytes with their 16-byte pieces
+// exchanged, so that eight of them meet no bank twice.
+constexpr int kPipeRows = 64, kPipeStep = 64, kPipeThreads = 128, kStages = 4;
+
+template <int kRowBytes>
+__device__ __forceinline__ int piece_at(int row, int piece) {
+    if constexpr (kRowBytes == 128) return row * 128 + (piece ^ (row & 7)) * 16;
+    if constexpr (kRowBytes == 64) return row * 64 + (piece ^ (row >> 1 & 3)) * 16;
+    return row * 32 + (piece ^ (row >> 2 & 1)) * 16;
+}
+__device__ __forceinline__ void copy_16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void copy_or_zero(uint32_t to, const void* from, bool there) {  // (nothing is read where it is not there)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+template <bool kTrans>
+__device__ __forceinline__ void load_blocks(uint32_t (&f)[4], uint32_t at) {  // four 8 x 8 blocks, a row's address a lane
+    if constexpr (kTrans)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3]) : "r"(at) : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3]) : "r"(at) : "memory");
+}
+
+template <int RT>
+struct PipeShape {
+    static constexpr int kRowTile = kPipeRows * kPipeStep * 2, kOther = RT * kPipeStep * 2, kStage = kRowTile + kOther;
+    static constexpr int kSumPitch = RT + 4, kFactorPitch = RT + 8;
+    static constexpr int kFactors = kStages * kStage, kSums = kFactors + kPipeRows * kFactorPitch * 2;
+    static constexpr int kBytes = kSums + kPipeRows * kSumPitch * 4;
+};
+
+template <typename T, bool kBack, int RT>
+__global__ void __launch_bounds__(kPipeThreads, RT == 64 ? 2 : 3) rows_pipe_kernel(Args a) {
+    using S = PipeShape<RT>;
+    constexpr int MT = RT == 64 ? 2 : 1, RG = 4 / MT;        // of 16 rows: a warp's, and groups of warps
+    constexpr int NT1 = RT / 8 / MT, NT2 = 8 / MT, KB = RT / 16;
+    constexpr bool kShrink = std::is_same<T, __half>::value;
+    extern __shared__ __align__(128) char memory[];
+    __shared__ float grow[kPipeRows];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, t = lane & 3, rg = warp % RG, half = warp / RG;
+    pdl_wait();
+    pdl_trigger();
+    Tile tile;
+    if (!find_tile<kPipeRows>(a, blockIdx.x, &tile)) return;
+    const int n = tile.end - tile.begin;
+    if (tile.adapter < 0) {
+        copy_base<T, 8>(a, tile, 0, a.cols);
+        if (a.u)
+            for (int i = threadIdx.x; i < n * a.r; i += kPipeThreads) a.u[(long long)tile.begin * a.r + i] = 0.f;
+        return;
+    }
+    const float scale = a.scale ? a.scale[tile.adapter] : 1.f;
+    const T* P = static_cast<const T*>(a.p) + (size_t)tile.adapter * a.r * a.len;
+    const T* Q = static_cast<const T*>(a.q) + (size_t)tile.adapter * a.r * a.cols;
+    const T* in = static_cast<const T*>(a.in) + (long long)tile.begin * a.ldi;
+    const T* base = a.base ? static_cast<const T*>(a.base) + (long long)tile.begin * a.ldb : nullptr;
+    T* out = static_cast<T*>(a.out) + (long long)tile.begin * a.ldo;
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(memory));
+    const int steps1 = (a.len + kPipeStep - 1) / kPipeStep, steps = steps1 + (a.cols + kPipeStep - 1) / kPipeStep;
+
+    // A thread's copies: a piece of 16 bytes of every so many rows, at addresses that only move on from step to step.
+    struct Lane {
+        const T* from;    // of the first of its rows
+        long long rows;   // elements from one of its rows to the next
+        uint32_t to;      // in the stage
+        int first;        // row
+    };
+    const int row16 = threadIdx.x / 8, piece = threadIdx.x % 8;  // 16 rows of 128 bytes at a time
+    constexpr int kTallPieces = RT / 8, kTallRows = kPipeThreads / kTallPieces;
+    const int tall_row = threadIdx.x / kTallPieces, tall_piece = threadIdx.x % kTallPieces;
+    auto lane_of = [&](const T* m, long long ld) { return Lane{m + row16 * ld + piece * 8, 16 * ld, (uint32_t)piece_at<128>(row16, piece), row16}; };
+    // rows: of a tile, or [RT] rows of 64 elements of a matrix [r][width].  What is not there is zeros; rows that are not are left out
+    // where nobody takes their sums (kZeros false).
+    auto copy_rows = [&](uint32_t to, Lane& l, int rows, int width, int k0, auto count, auto zeros) {
+        constexpr int kCount = decltype(count)::value;
+        const bool whole = k0 + kPipeStep <= width;
+        const T* from = l.from;
+#pragma unroll
+        for (int i = 0; i < kCount; ++i, from += l.rows) {
+            const bool there = l.first + 16 * i < rows;
+            if (whole && there) copy_16(to + l.to + i * 16 * 128, from);
+            else if (decltype(zeros)::value || there) {
+                const bool in_row = there && k0 + piece * 8 < width;
+                copy_or_zero(to + l.to + i * 16 * 128, in_row ? from : static_cast<const T*>(a.p), in_row);
+            }
+        }
+        l.from += kPipeStep;
+    };
+    // 64 rows of a matrix [width][r]
+    auto tall_of = [&](const T* m) { return Lane{m + (long long)tall_row * a.r + tall_piece * 8, (long long)kTallRows * a.r, (uint32_t)piece_at<RT * 2>(tall_row, tall_piece), tall_row}; };
+    auto copy_tall = [&](uint32_t to, Lane& l, int width, int k0) {
+        const T* from = l.from;
+#pragma unroll
+        for (int i = 0; i < kPipeStep / kTallRows; ++i, from += l.rows) {
+            const bool there = tall_piece * 8 < a.r && k0 + l.first + i * kTallRows < width;
+            copy_or_zero(to + l.to + i * kTallRows * RT * 2, there ? from : static_cast<const T*>(a.p), there);
+        }
+        l.from += (long long)kPipeStep * a.r;
+    };
+    using std::integral_constant;
+    Lane rows_at = lane_of(in, a.ldi), other = kBack ? tall_of(P) : lane_of(P, a.len);
+    uint32_t fill = ring, take = ring;  // stages that are copied to and read next
+    int copied = 0;
+    auto copy = [&] {
+        if (copied < steps) {
+            if (copied == steps1) {
+                if (base) rows_at = lane_of(base, a.ldb);
+                other = kBack ? lane_of(Q, a.cols) : tall_of(Q);
+            }
+            const bool second = copied >= steps1;
+            const int width = second ? a.cols : a.len, k0 = (copied - (second ? steps1 : 0)) * kPipeStep;
+            if (!second || base) copy_rows(fill, rows_at, n, width, k0, integral_constant<int, kPipeRows / 16>(), std::false_type());
+            if (kBack != second) copy_tall(fill + S::kRowTile, other, width, k0);
+            else copy_rows(fill + S::kRowTile, other, a.r, width, k0, integral_constant<int, RT / 16>(), std::true_type());
+            ++copied;
+            fill = fill == ring + (kStages - 1) * S::kStage ? ring : fill + S::kStage;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto next = [&] {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        __syncthreads();
+        copy();
+        const uint32_t from = take;
+        take = take == ring + (kStages - 1) * S::kStage ? ring : take + S::kStage;
+        return from;
+    };
+    for (int i = 0; i < kStages - 1; ++i) copy();
+
+    // ------------------------------------------------ first product
+    const int low = lane & 7, mid = lane >> 3 & 1, high = lane >> 4;  // which row of which 8 x 8 block this lane's address is of
+    float d[MT][NT1][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < NT1; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[m][j][i] = 0.f;
+    for (int step = 0; step < steps1; ++step) {
+        const uint32_t from = next();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            uint32_t f[MT][4];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) load_blocks<false>(f[m], from + piece_at<128>((rg * MT + m) * 16 + low + mid * 8, 2 * k + high));
+#pragma unroll
+            for (int j = 0; j < NT1; j += 2) {
+                uint32_t b[4];
+                const int j0 = half * NT1 + j;
+                if constexpr (kBack) load_blocks<true>(b, from + S::kRowTile + piece_at<RT * 2>(16 * k + low + mid * 8, j0 + high));
+                else load_blocks<false>(b, from + S::kRowTile + piece_at<128>(j0 * 8 + low + high * 8, 2 * k + mid));
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    wm::mma16<T>(d[m][j], f[m][0], f[m][1], f[m][2], f[m][3], b[0], b[1]);
+                    wm::mma16<T>(d[m][j + 1], f[m][0], f[m][1], f[m][2], f[m][3], b[2], b[3]);
+                }
+            }
+        }
+    }
+    float* sums = reinterpret_cast<float*>(memory + S::kSums);
+    T* factors = reinterpret_cast<T*>(memory + S::kFactors);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < NT1; ++j) {
+            float* to = sums + ((rg * MT + m) * 16 + quad) * S::kSumPitch + (half * NT1 + j) * 8 + t * 2;
+            const float by = kBack ? scale : 1.f;
+            *reinterpret_cast<float2*>(to) = make_float2(d[m][j][0] * by, d[m][j][1] * by);
+            *reinterpret_cast<float2*>(to + 8 * S::kSumPitch) = make_float2(d[m][j][2] * by, d[m][j][3] * by);
+        }
+    __syncthreads();
+    // a warp takes a row: u, and what of it the second product takes
+    for (int row = warp; row < kPipeRows; row += kPipeThreads / 32) {
+        constexpr int V = RT >= 32 ? RT / 32 : 1;
+        float v[V], most = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int j = i * 32 + lane;
+            v[i] = j < RT && row < n ? sums[row * S::kSumPitch + j] : 0.f;
+            if (a.u && row < n && j < a.r) a.u[(long long)(tile.begin + row) * a.r + j] = v[i];
+            most = fmaxf(most, fabsf(v[i]));
+        }
+        float shrink = 1.f;
+        if constexpr (kShrink) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            shrink = shrink_of(most);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i * 32 + lane < RT) factors[row * S::kFactorPitch + i * 32 + lane] = Elem<T>::from_f(v[i] * shrink);
+        if (lane == 0) grow[row] = (kBack ? 1.f : scale) / shrink;
+    }
+    __syncthreads();
+
+    // ------------------------------------------------ second product
+    uint32_t f[MT][KB][4];
+    float up[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int row = (rg * MT + m) * 16;
+        up[m][0] = grow[row + quad], up[m][1] = grow[row + 8 + quad];
+#pragma unroll
+        for (int k = 0; k < KB; ++k)
+            load_blocks<false>(f[m][k], ring + S::kFactors + ((row + low + mid * 8) * S::kFactorPitch + k * 16 + high * 8) * 2);
+    }
+    for (int step = steps1; step < steps; ++step) {
+        const uint32_t from = next();
+        const int c0 = (step - steps1) * kPipeStep;
+        float s[MT][NT2][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < NT2; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[m][j][i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KB; ++k)
+#pragma unroll
+            for (int j = 0; j < NT2; j += 2) {
+                uint32_t b[4];
+                const int j0 = half * NT2 + j;
+                if constexpr (kBack) load_blocks<true>(b, from + S::kRowTile + piece_at<128>(16 * k + low + mid * 8, j0 + high));
+                else load_blocks<false>(b, from + S::kRowTile + piece_at<RT * 2>(j0 * 8 + low + high * 8, 2 * k + mid));
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    wm::mma16<T>(s[m][j], f[m][k][0], f[m][k][1], f[m][k][2], f[m][k][3], b[0], b[1]);
+                    wm::mma16<T>(s[m][j + 1], f[m][k][0], f[m][k][1], f[m][k][2], f[m][k][3], b[2], b[3]);
+                }
+            }
+        // onto base, in its place in the ring, whence the warp stores its rows 16 bytes at a time
+        char* tile_at = memory + (from - ring);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < NT2; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t* at = reinterpret_cast<uint32_t*>(tile_at + piece_at<128>((rg * MT + m) * 16 + h * 8 + quad, half * NT2 + j) + t * 4);
+                    const float2 b = base ? Pack2<T>::to_f2(*reinterpret_cast<const typename Pack2<T>::type*>(at)) : make_float2(0.f, 0.f);
+                    *at = pack<T>(fmaf(up[m][h], s[m][j][2 * h], b.x), fmaf(up[m][h], s[m][j][2 * h + 1], b.y));
+                }
+        __syncwarp();
+#pragma unroll
+        for (int i = lane; i < 16 * MT * NT2; i += 32) {
+            const int row = rg * MT * 16 + i / NT2, piece = half * NT2 + i % NT2;
+            if (row < n && c0 + piece * 8 < a.cols)
+                *reinterpret_cast<uint4*>(out + row * a.ldo + c0 + piece * 8) = *reinterpret_cast<const uint4*>(tile_at + piece_at<128>(row, piece));
+        }
+    }
+}
+
 // ---------------------------------------------------------------- gradients of the adapters
-constexpr int kGradRows = 64, kGradColumns = 256;
+constexpr int kGradRows = 32, kGradColumns = 256, kGradStages = 4;
 
 template <typename T, int RT>
 struct GradShape {
     static constexpr int kPitch = RT + 8;                          // elements of a row of c
-    static constexpr int kSums = RT * (kGradColumns + 4) * 4;
-    static constexpr int kBytes = kSums > 2 * kGradRows * kPitch * 2 ? kSums : 2 * kGradRows * kPitch * 2;
+    static constexpr int kRowPitch = kGradColumns * 2 + 16;        // bytes of a row of the other factor
+    static constexpr int kStage = kGradRows * kRowPitch, kFactors = kGradStages * kStage;
+    static constexpr int kSums = RT * (kGradColumns + 1) * 4, kRing = kFactors + 2 * kGradRows * kPitch * 2;
+    static constexpr int kBytes = kSums > kRing ? kSums : kRing;
 };
 
-// RT: columns of c (u or v) from blockIdx.z * RT on.  The cluster's blocks take 64 rows of a request in turn.
+// RT: columns of c (u or v) from blockIdx.z * RT on.  The cluster's blocks take kGradRows rows of a request in turn; those of the other factor come
+// through a ring in shared memory.
 template <typename T, bool kDb, int RT>
-__global__ void __launch_bounds__(256, RT == 64 ? 1 : 2) grads_mma_kernel(Grads a) {
+__global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads a) {
     namespace cg = cooperative_groups;
     using S = GradShape<T, RT>;
     constexpr int MT = RT / 16;
     constexpr bool kShrink = std::is_same<T, __half>::value;
-    extern __shared__ __align__(16) char memory[];
+    extern __shared__ __align__(128) char memory[];
     __shared__ float largest[kWarps];
     cg::cluster_group cluster = cg::this_cluster();
     const int blocks = (int)cluster.num_blocks(), block = (int)cluster.block_rank();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, t = lane & 3;
-    const int l = blockIdx.y, j0 = blockIdx.z * RT, c0 = (int)(blockIdx.x / blocks) * kGradColumns, mine = c0 + warp * 32 + t * 8;
+    const int l = blockIdx.y, j0 = blockIdx.z * RT, c0 = (int)(blockIdx.x / blocks) * kGradColumns;
     pdl_wait();
     pdl_trigger();
     float s[MT][4][4];
@@ -348,113 +606,162 @@ __global__ void __launch_bounds__(256, RT == 64 ? 1 : 2) grads_mma_kernel(Grads 
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[m][j][i] = 0.f;
-    T* c = reinterpret_cast<T*>(memory);
+    T* c = reinterpret_cast<T*>(memory + S::kFactors);
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(memory));
+
+    // This block's share of the adapter's rows, kGradRows of a request at a time.
+    struct {
+        int i0, row, end, count;
+        unsigned of;
+    } walk{-32, 0, 0, 0, 0};
+    auto advance = [&](int* row0) {  // rows of the next step, 0 at the end; uniform over the block
+        for (;;) {
+            while (walk.row < walk.end) {
+                const int row = walk.row, n = min(kGradRows, walk.end - row);
+                walk.row += kGradRows;
+                if (walk.count++ % blocks != block) continue;
+                *row0 = row;
+                return n;
+            }
+            while (!walk.of) {
+                walk.i0 += 32;
+                if (walk.i0 >= a.R) {
+                    walk.i0 = a.R;  // (stays at the end)
+                    return 0;
+                }
+                const int i = walk.i0 + lane;
+                walk.of = __ballot_sync(0xffffffffu, i < a.R && a.adapter[i] == l);
+            }
+            const Group g = group_rows(a.offsets, walk.i0 + __ffs(walk.of) - 1, a.rows);
+            walk.of &= walk.of - 1;
+            walk.row = g.begin;
+            walk.end = g.end;
+        }
+    };
+    const T* in = static_cast<const T*>(a.in);
+    auto copy = [&](int stage, int row0, int n) {
+#pragma unroll
+        for (int i = threadIdx.x; i < kGradRows * (kGradColumns / 8); i += 256) {
+            const int row = i / (kGradColumns / 8), col = i % (kGradColumns / 8) * 8;
+            const bool there = row < n && c0 + col < a.cols;  // (rows of others are zeros here, not multiplied by zero)
+            copy_or_zero(ring + stage * S::kStage + row * S::kRowPitch + col * 2, there ? in + (row0 + row) * a.ldi + c0 + col : in, there);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    constexpr int kMine = kGradRows * RT / 256 / 2;  // pairs of c of a thread
+    auto fetch = [&](int row0, int n, float2 (&v)[kMine]) {
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) {
+            const int at = (k * 256 + (int)threadIdx.x) * 2, row = at / RT, j = at % RT;
+            v[k] = row < n && j0 + j < a.r ? *reinterpret_cast<const float2*>(a.c + (long long)(row0 + row) * a.r + j0 + j) : make_float2(0.f, 0.f);
+        }
+    };
+
+    // this step and those that are on their way: begin and number of their rows
+    int row[kGradStages] = {}, n[kGradStages];
+#pragma unroll
+    for (int i = 0; i < kGradStages - 1; ++i) {
+        n[i] = advance(&row[i]);
+        copy(i, row[i], n[i]);
+    }
+    float2 v[kMine];
+    fetch(row[0], n[0], v);
     float shrink = 1.f;  // what the values of c are multiplied with (a power of two; the sums then have it too)
     bool any = false;    // whether one of them was not zero
-    int turn = 0, count = 0;
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    for (int i0 = 0; i0 < a.R; i0 += 32) {
-        const int i = i0 + lane;
-        unsigned of = __ballot_sync(0xffffffffu, i < a.R && a.adapter[i] == l);
-        for (; of; of &= of - 1) {
-            const Group g = group_rows(a.offsets, i0 + __ffs(of) - 1, a.rows);
-            for (int row0 = g.begin; row0 < g.end; row0 += kGradRows) {
-                if (count++ % blocks != block) continue;
-                const int n = min(kGradRows, g.end - row0);
-                // this step's rows of the other factor are on their way while c is made
-                const T* in = static_cast<const T*>(a.in) + (long long)(row0 + quad) * a.ldi + mine;
-                auto load = [&](int k, uint4 (&x)[2]) {
+    for (int step = 0; n[0] > 0; ++step) {
+        float most = 0.f;
+        if constexpr (kShrink) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        x[h] = mine < a.cols && k * 16 + h * 8 + quad < n ? *reinterpret_cast<const uint4*>(in + (long long)(k * 16 + h * 8) * a.ldi) : zero;
-                };
-                uint4 x[kGradRows / 16][2];
+            for (int k = 0; k < kMine; ++k) most = fmaxf(most, fmaxf(fabsf(v[k].x), fabsf(v[k].y)));
 #pragma unroll
-                for (int k = 0; k < kGradRows / 16; ++k) load(k, x[k]);
-                constexpr int kMine = kGradRows * RT / 256 / 2;  // pairs of c of a thread
-                float2 v[kMine];
-                float most = 0.f;
+            for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            if (lane == 0) largest[warp] = most;
+            __syncthreads();
 #pragma unroll
-                for (int k = 0; k < kMine; ++k) {
-                    const int at = (k * 256 + (int)threadIdx.x) * 2, row = at / RT, j = at % RT;
-                    v[k] = row < n && j0 + j < a.r ? *reinterpret_cast<const float2*>(a.c + (long long)(row0 + row) * a.r + j0 + j) : make_float2(0.f, 0.f);
-                    most = fmaxf(most, fmaxf(fabsf(v[k].x), fabsf(v[k].y)));
-                }
-                if constexpr (kShrink) {
+            for (int w = 0; w < kWarps; ++w) most = fmaxf(most, largest[w]);
+            const float want = shrink_of(most);
+            if (most > 0.f && (!any || want < shrink)) {  // (the first, or larger ones than before)
+                any = true;
+                const float by = want / shrink;
 #pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                    if (lane == 0) largest[warp] = most;
-                    __syncthreads();
+                for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int w = 0; w < kWarps; ++w) most = fmaxf(most, largest[w]);
-                    const float want = shrink_of(most);
-                    if (most > 0.f && (!any || want < shrink)) {  // (the first, or larger ones than before)
-                        any = true;
-                        const float by = want / shrink;
+                    for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int m = 0; m < MT; ++m)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                                for (int q = 0; q < 4; ++q) s[m][j][q] *= by;
-                        shrink = want;
-                    }
-                }
-                T* to = c + turn * kGradRows * S::kPitch;
-                turn ^= 1;
-#pragma unroll
-                for (int k = 0; k < kMine; ++k) {
-                    const int at = (k * 256 + (int)threadIdx.x) * 2;
-                    *reinterpret_cast<uint32_t*>(to + at / RT * S::kPitch + at % RT) = pack<T>(v[k].x * shrink, v[k].y * shrink);
-                }
-                __syncthreads();  // (two buffers in turn)
-#pragma unroll
-                for (int k = 0; k < kGradRows / 16; ++k) {
-                    if (k * 16 >= n) break;
-                    const uint32_t w[2][4] = {{x[k][0].x, x[k][0].y, x[k][0].z, x[k][0].w}, {x[k][1].x, x[k][1].y, x[k][1].z, x[k][1].w}};
-                    uint32_t b[4][2];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) b[j][0] = transposed(w[0][j]), b[j][1] = transposed(w[1][j]);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        uint32_t f[4];
-                        // four 8 x 8 blocks of c: rows (k) lane % 8 (+ 8 for lanes 16 on), columns (m) + 8 for every second eight lanes
-                        const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to + (k * 16 + (lane & 7) + (lane >> 4) * 8) * S::kPitch + m * 16 + (lane >> 3 & 1) * 8));
-                        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                                     : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3]) : "r"(at) : "memory");
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) wm::mma16<T>(s[m][j], f[0], f[1], f[2], f[3], b[j][0], b[j][1]);
-                    }
-                }
+                        for (int q = 0; q < 4; ++q) s[m][j][q] *= by;
+                shrink = want;
             }
         }
+        T* to = c + (step & 1) * kGradRows * S::kPitch;  // (two buffers in turn: one meeting a step)
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) {
+            const int at = (k * 256 + (int)threadIdx.x) * 2;
+            *reinterpret_cast<uint32_t*>(to + at / RT * S::kPitch + at % RT) = pack<T>(v[k].x * shrink, v[k].y * shrink);
+        }
+        asm volatile("cp.async.wait_group %0;" ::"n"(kGradStages - 2) : "memory");
+        __syncthreads();
+        n[kGradStages - 1] = advance(&row[kGradStages - 1]);
+        copy((step + kGradStages - 1) % kGradStages, row[kGradStages - 1], n[kGradStages - 1]);
+        fetch(row[1], n[1], v);
+        const uint32_t from = ring + step % kGradStages * S::kStage;
+        const uint32_t factors = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+        // 8 x 8 blocks: of c rows lane % 8 (+ 8 for lanes 16 on) and columns + 8 for every second eight lanes; of the other the other way round
+        const int low = lane & 7, mid = lane >> 3 & 1, high = lane >> 4;
+#pragma unroll
+        for (int k = 0; k < kGradRows / 16; ++k) {
+            if (k * 16 >= n[0]) break;
+            uint32_t b[2][4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) load_blocks<true>(b[j], from + (k * 16 + low + mid * 8) * S::kRowPitch + (warp * 32 + j * 16 + high * 8) * 2);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                uint32_t f[4];
+                load_blocks<true>(f, factors + ((k * 16 + low + high * 8) * S::kPitch + m * 16 + mid * 8) * 2);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) wm::mma16<T>(s[m][j], f[0], f[1], f[2], f[3], b[j / 2][j % 2 * 2], b[j / 2][j % 2 * 2 + 1]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kGradStages - 1; ++i) row[i] = row[i + 1], n[i] = n[i + 1];
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     // the cluster's sums meet; the blocks share what is then to be stored
-    float* sums = reinterpret_cast<float*>(memory);  // [RT][columns + 4]
-    constexpr int kPitch = kGradColumns + 4;
+    float* sums = reinterpret_cast<float*>(memory);  // [RT][columns + 1]
+    constexpr int kPitch = kGradColumns + 1;
     const float scale = a.scale ? a.scale[l] : 1.f, grow = scale / shrink;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            float* to = sums + (m * 16 + h * 8 + quad) * kPitch + warp * 32 + t * 8;
+            float* to = sums + (m * 16 + h * 8 + quad) * kPitch + warp * 32 + t * 2;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) to[2 * j] = s[m][j][2 * h] * grow, to[2 * j + 1] = s[m][j][2 * h + 1] * grow;
+            for (int j = 0; j < 4; ++j) to[8 * j] = s[m][j][2 * h] * grow, to[8 * j + 1] = s[m][j][2 * h + 1] * grow;
         }
     if (blocks > 1) cluster.sync();
     else __syncthreads();
-    const int width = min(RT, a.r - j0), columns = min(kGradColumns, a.cols - c0);
-    for (int i = block * 256 + threadIdx.x; i < width * columns; i += blocks * 256) {
-        const int j = kDb ? i % width : i / columns, col = kDb ? i / width : i % columns;
-        float* at = sums + j * kPitch + col;
+    // (neighbours in a row of the sums are read together from the other blocks; dB's results change places in this block's own memory)
+    const int width = min(RT, a.r - j0), share = kGradColumns / blocks, first = block * share, columns = min(share, a.cols - c0 - first);
+    T* const out = static_cast<T*>(a.out);
+    float* const wide_out = static_cast<float*>(a.out);
+    auto store = [&](int j, int col, float v) {
+        const size_t to = kDb ? ((size_t)l * a.cols + c0 + first + col) * a.r + j0 + j : ((size_t)l * a.r + j0 + j) * a.cols + c0 + first + col;
+        if (a.wide_out) wide_out[to] = v;
+        else out[to] = Elem<T>::from_f(v);
+    };
+    for (int i = threadIdx.x; i < width * share; i += 256) {
+        const int j = i / share, col = i % share;
+        float* at = sums + j * kPitch + first + col;
         float v = 0.f;
         if (blocks == 1) v = *at;
         else
             for (int k = 0; k < blocks; ++k) v += *cluster.map_shared_rank(at, k);
-        const size_t to = kDb ? ((size_t)l * a.cols + c0 + col) * a.r + j0 + j : ((size_t)l * a.r + j0 + j) * a.cols + c0 + col;
-        if (a.wide_out) static_cast<float*>(a.out)[to] = v;
-        else static_cast<T*>(a.out)[to] = Elem<T>::from_f(v);
+        if (kDb) *at = v;  // (nobody else reads this block's share of its own sums but itself)
+        else if (col < columns) store(j, col, v);
+    }
+    if constexpr (kDb) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < width * columns; i += 256) store(i % width, i / width, sums[i % width * kPitch + first + i / width]);
     }
     if (blocks > 1) cluster.sync();
 }

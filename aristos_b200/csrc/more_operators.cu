@@ -199,8 +199,18 @@ cudaError_t adapter_rows(const adapters::Args& a, cudaStream_t st) {
     if constexpr (sizeof(T) == 2) {
         if (a.r % 8 == 0 && by_16(2, {a.in, a.p, a.q, a.base, a.out}, {a.ldi, a.ldb, a.ldo, a.len, a.cols}))
             return with_rank(a.r, [&](auto rt) {
+                constexpr int RT = decltype(rt)::value;
                 // requests of few rows: tiles of as many as the tensor cores take
-                return a.rows < 24LL * a.R ? adapter_rows_mma<T, kBack, decltype(rt)::value, 16>(a, st) : adapter_rows_mma<T, kBack, decltype(rt)::value, 64>(a, st);
+                if (a.rows < 24LL * a.R) return adapter_rows_mma<T, kBack, RT, 16>(a, st);
+                if constexpr (RT <= 64)
+                    if (a.rows / kPipeRows + a.R / 2 >= sm_count()) {
+                        const auto kernel = rows_pipe_kernel<T, kBack, RT>;
+                        static bool allowed[64];
+                        cudaError_t rc = allow_smem(kernel, allowed, PipeShape<RT>::kBytes);
+                        if (rc == cudaSuccess) rc = launch(kernel, dim3((unsigned)(a.rows / kPipeRows + a.R + 2)), kPipeThreads, PipeShape<RT>::kBytes, 1, st, a);
+                        return rc;
+                    }
+                return adapter_rows_mma<T, kBack, RT, 64>(a, st);
             });
     }
     const long long tiles = a.rows / kRowsSimt + a.R + 2;  // at most

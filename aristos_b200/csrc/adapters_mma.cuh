@@ -318,11 +318,11 @@ __global__ void __launch_bounds__(256, RT == 64 && TR == 64 ? 1 : 2) rows_mma_ke
 }
 
 // ---------------------------------------------------------------- many rows
-// The same for tiles enough to fill the GPU: a block of four warps takes 64 rows alone.  What it multiplies comes through a ring of kStages
+// The same for tiles enough to fill the GPU: a block takes 64 rows alone.  What it multiplies comes through a ring of kStages
 // steps of 64 elements in shared memory, 16-byte copies that run ahead from the first product into the second, and reaches the tensor cores by
 // ldmatrix (transposed where the summed direction is not the contiguous one).  Rows of 128, 64 or 32 bytes with their 16-byte pieces
 // exchanged, so that eight of them meet no bank twice.
-constexpr int kPipeRows = 64, kPipeStep = 64, kPipeThreads = 128, kStages = 4;
+constexpr int kPipeRows = 64, kPipeStep = 64, kPipeThreads = 256, kStages = 4;
 
 template <int kRowBytes>
 __device__ __forceinline__ int piece_at(int row, int piece) {
@@ -351,14 +351,16 @@ struct PipeShape {
 };
 
 template <typename T, bool kBack, int RT>
-__global__ void __launch_bounds__(kPipeThreads, RT == 64 ? 2 : 3) rows_pipe_kernel(Args a) {
+__global__ void __launch_bounds__(kPipeThreads, 2) rows_pipe_kernel(Args a) {
     using S = PipeShape<RT>;
     constexpr int MT = RT == 64 ? 2 : 1, RG = 4 / MT;        // of 16 rows: a warp's, and groups of warps
-    constexpr int NT1 = RT / 8 / MT, NT2 = 8 / MT, KB = RT / 16;
+    constexpr int NT1 = RT / 8 / MT, KB = RT / 16;           // first product: the ranks of a warp by eight; two warps share the elements of a step
+    constexpr int CG = kWarps / RG, NT2 = 8 / CG;            // second: the warps of a group share the columns
     constexpr bool kShrink = std::is_same<T, __half>::value;
     extern __shared__ __align__(128) char memory[];
     __shared__ float grow[kPipeRows];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, t = lane & 3, rg = warp % RG, half = warp / RG;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, t = lane & 3, rg = warp % RG, group = warp / RG;
+    const int half = group % MT, kpart = group / MT;
     pdl_wait();
     pdl_trigger();
     Tile tile;
@@ -386,23 +388,24 @@ __global__ void __launch_bounds__(kPipeThreads, RT == 64 ? 2 : 3) rows_pipe_kern
         uint32_t to;      // in the stage
         int first;        // row
     };
-    const int row16 = threadIdx.x / 8, piece = threadIdx.x % 8;  // 16 rows of 128 bytes at a time
+    constexpr int kRows = kPipeThreads / 8;                      // of 128 bytes at a time
+    const int row8 = threadIdx.x / 8, piece = threadIdx.x % 8;
     constexpr int kTallPieces = RT / 8, kTallRows = kPipeThreads / kTallPieces;
     const int tall_row = threadIdx.x / kTallPieces, tall_piece = threadIdx.x % kTallPieces;
-    auto lane_of = [&](const T* m, long long ld) { return Lane{m + row16 * ld + piece * 8, 16 * ld, (uint32_t)piece_at<128>(row16, piece), row16}; };
+    auto lane_of = [&](const T* m, long long ld) { return Lane{m + row8 * ld + piece * 8, kRows * ld, (uint32_t)piece_at<128>(row8, piece), row8}; };
     // rows: of a tile, or [RT] rows of 64 elements of a matrix [r][width].  What is not there is zeros; rows that are not are left out
     // where nobody takes their sums (kZeros false).
-    auto copy_rows = [&](uint32_t to, Lane& l, int rows, int width, int k0, auto count, auto zeros) {
-        constexpr int kCount = decltype(count)::value;
+    auto copy_rows = [&](uint32_t to, Lane& l, int rows, int width, int k0, auto all, auto zeros) {
+        constexpr int kAll = decltype(all)::value;
         const bool whole = k0 + kPipeStep <= width;
         const T* from = l.from;
 #pragma unroll
-        for (int i = 0; i < kCount; ++i, from += l.rows) {
-            const bool there = l.first + 16 * i < rows;
-            if (whole && there) copy_16(to + l.to + i * 16 * 128, from);
-            else if (decltype(zeros)::value || there) {
+        for (int i = 0; i < kAll; i += kRows, from += l.rows) {
+            const bool there = l.first + i < rows;
+            if (whole && there) copy_16(to + l.to + i * 128, from);
+            else if (there || (decltype(zeros)::value && l.first + i < kAll)) {
                 const bool in_row = there && k0 + piece * 8 < width;
-                copy_or_zero(to + l.to + i * 16 * 128, in_row ? from : static_cast<const T*>(a.p), in_row);
+                copy_or_zero(to + l.to + i * 128, in_row ? from : static_cast<const T*>(a.p), in_row);
             }
         }
         l.from += kPipeStep;
@@ -412,9 +415,9 @@ __global__ void __launch_bounds__(kPipeThreads, RT == 64 ? 2 : 3) rows_pipe_kern
     auto copy_tall = [&](uint32_t to, Lane& l, int width, int k0) {
         const T* from = l.from;
 #pragma unroll
-        for (int i = 0; i < kPipeStep / kTallRows; ++i, from += l.rows) {
-            const bool there = tall_piece * 8 < a.r && k0 + l.first + i * kTallRows < width;
-            copy_or_zero(to + l.to + i * kTallRows * RT * 2, there ? from : static_cast<const T*>(a.p), there);
+        for (int i = 0; i < kPipeStep; i += kTallRows, from += l.rows) {
+            const bool there = tall_piece * 8 < a.r && k0 + l.first + i < width;
+            if (l.first + i < kPipeStep) copy_or_zero(to + l.to + i * RT * 2, there ? from : static_cast<const T*>(a.p), there);
         }
         l.from += (long long)kPipeStep * a.r;
     };
@@ -430,9 +433,9 @@ __global__ void __launch_bounds__(kPipeThreads, RT == 64 ? 2 : 3) rows_pipe_kern
             }
             const bool second = copied >= steps1;
             const int width = second ? a.cols : a.len, k0 = (copied - (second ? steps1 : 0)) * kPipeStep;
-            if (!second || base) copy_rows(fill, rows_at, n, width, k0, integral_constant<int, kPipeRows / 16>(), std::false_type());
+            if (!second || base) copy_rows(fill, rows_at, n, width, k0, integral_constant<int, kPipeRows>(), std::false_type());
             if (kBack != second) copy_tall(fill + S::kRowTile, other, width, k0);
-            else copy_rows(fill + S::kRowTile, other, a.r, width, k0, integral_constant<int, RT / 16>(), std::true_type());
+            else copy_rows(fill + S::kRowTile, other, a.r, width, k0, integral_constant<int, RT>(), std::true_type());
             ++copied;
             fill = fill == ring + (kStages - 1) * S::kStage ? ring : fill + S::kStage;
         }
@@ -460,7 +463,8 @@ __global__ void __launch_bounds__(kPipeThreads, RT == 64 ? 2 : 3) rows_pipe_kern
     for (int step = 0; step < steps1; ++step) {
         const uint32_t from = next();
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int i = 0; i < 2; ++i) {
+            const int k = 2 * kpart + i;
             uint32_t f[MT][4];
 #pragma unroll
             for (int m = 0; m < MT; ++m) load_blocks<false>(f[m], from + piece_at<128>((rg * MT + m) * 16 + low + mid * 8, 2 * k + high));
@@ -480,16 +484,20 @@ __global__ void __launch_bounds__(kPipeThreads, RT == 64 ? 2 : 3) rows_pipe_kern
     }
     float* sums = reinterpret_cast<float*>(memory + S::kSums);
     T* factors = reinterpret_cast<T*>(memory + S::kFactors);
+    for (int part = 0; part < 2; ++part) {  // one half of the sums, and the other onto it
+        if (kpart == part)
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int j = 0; j < NT1; ++j) {
-            float* to = sums + ((rg * MT + m) * 16 + quad) * S::kSumPitch + (half * NT1 + j) * 8 + t * 2;
-            const float by = kBack ? scale : 1.f;
-            *reinterpret_cast<float2*>(to) = make_float2(d[m][j][0] * by, d[m][j][1] * by);
-            *reinterpret_cast<float2*>(to + 8 * S::kSumPitch) = make_float2(d[m][j][2] * by, d[m][j][3] * by);
-        }
-    __syncthreads();
+                for (int j = 0; j < NT1; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float2* to = reinterpret_cast<float2*>(sums + ((rg * MT + m) * 16 + h * 8 + quad) * S::kSumPitch + (half * NT1 + j) * 8 + t * 2);
+                        const float2 before = part ? *to : make_float2(0.f, 0.f);
+                        *to = make_float2(before.x + d[m][j][2 * h], before.y + d[m][j][2 * h + 1]);
+                    }
+        __syncthreads();
+    }
     // a warp takes a row: u, and what of it the second product takes
     for (int row = warp; row < kPipeRows; row += kPipeThreads / 32) {
         constexpr int V = RT >= 32 ? RT / 32 : 1;
@@ -497,7 +505,7 @@ __global__ void __launch_bounds__(kPipeThreads, RT == 64 ? 2 : 3) rows_pipe_kern
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int j = i * 32 + lane;
-            v[i] = j < RT && row < n ? sums[row * S::kSumPitch + j] : 0.f;
+            v[i] = j < RT && row < n ? sums[row * S::kSumPitch + j] * (kBack ? scale : 1.f) : 0.f;
             if (a.u && row < n && j < a.r) a.u[(long long)(tile.begin + row) * a.r + j] = v[i];
             most = fmaxf(most, fabsf(v[i]));
         }
@@ -540,7 +548,7 @@ __global__ void __launch_bounds__(kPipeThreads, RT == 64 ? 2 : 3) rows_pipe_kern
 #pragma unroll
             for (int j = 0; j < NT2; j += 2) {
                 uint32_t b[4];
-                const int j0 = half * NT2 + j;
+                const int j0 = group * NT2 + j;
                 if constexpr (kBack) load_blocks<true>(b, from + S::kRowTile + piece_at<128>(16 * k + low + mid * 8, j0 + high));
                 else load_blocks<false>(b, from + S::kRowTile + piece_at<RT * 2>(j0 * 8 + low + high * 8, 2 * k + mid));
 #pragma unroll
@@ -557,14 +565,14 @@ __global__ void __launch_bounds__(kPipeThreads, RT == 64 ? 2 : 3) rows_pipe_kern
             for (int j = 0; j < NT2; ++j)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    uint32_t* at = reinterpret_cast<uint32_t*>(tile_at + piece_at<128>((rg * MT + m) * 16 + h * 8 + quad, half * NT2 + j) + t * 4);
+                    uint32_t* at = reinterpret_cast<uint32_t*>(tile_at + piece_at<128>((rg * MT + m) * 16 + h * 8 + quad, group * NT2 + j) + t * 4);
                     const float2 b = base ? Pack2<T>::to_f2(*reinterpret_cast<const typename Pack2<T>::type*>(at)) : make_float2(0.f, 0.f);
                     *at = pack<T>(fmaf(up[m][h], s[m][j][2 * h], b.x), fmaf(up[m][h], s[m][j][2 * h + 1], b.y));
                 }
         __syncwarp();
 #pragma unroll
         for (int i = lane; i < 16 * MT * NT2; i += 32) {
-            const int row = rg * MT * 16 + i / NT2, piece = half * NT2 + i % NT2;
+            const int row = rg * MT * 16 + i / NT2, piece = group * NT2 + i % NT2;
             if (row < n && c0 + piece * 8 < a.cols)
                 *reinterpret_cast<uint4*>(out + row * a.ldo + c0 + piece * 8) = *reinterpret_cast<const uint4*>(tile_at + piece_at<128>(row, piece));
         }
@@ -638,22 +646,31 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads a) {
             walk.end = g.end;
         }
     };
-    const T* in = static_cast<const T*>(a.in);
-    auto copy = [&](int stage, int row0, int n) {
+    // a thread's copies: 16 bytes of every eighth row
+    const int my_row = threadIdx.x / 32, my_col = threadIdx.x % 32 * 8;
+    const bool my_column = c0 + my_col < a.cols;
+    const T* const in = static_cast<const T*>(a.in) + my_row * a.ldi + c0 + my_col;
+    const uint32_t ring_end = ring + kGradStages * S::kStage;
+    uint32_t fill = ring + my_row * S::kRowPitch + my_col * 2, take = ring;
+    auto copy = [&](int row0, int n) {
+        const T* from = in + row0 * a.ldi;
 #pragma unroll
-        for (int i = threadIdx.x; i < kGradRows * (kGradColumns / 8); i += 256) {
-            const int row = i / (kGradColumns / 8), col = i % (kGradColumns / 8) * 8;
-            const bool there = row < n && c0 + col < a.cols;  // (rows of others are zeros here, not multiplied by zero)
-            copy_or_zero(ring + stage * S::kStage + row * S::kRowPitch + col * 2, there ? in + (row0 + row) * a.ldi + c0 + col : in, there);
+        for (int i = 0; i < kGradRows; i += 8, from += 8 * a.ldi) {
+            const bool there = my_column && my_row + i < n;  // (rows of others are zeros here, not multiplied by zero)
+            copy_or_zero(fill + i * S::kRowPitch, there ? from : static_cast<const T*>(a.in), there);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
+        fill += S::kStage;
+        if (fill >= ring_end) fill -= kGradStages * S::kStage;
     };
     constexpr int kMine = kGradRows * RT / 256 / 2;  // pairs of c of a thread
+    const bool my_factor = j0 + (int)threadIdx.x * 2 % RT < a.r;
+    const float* const factor = a.c + (long long)((int)threadIdx.x * 2 / RT) * a.r + j0 + (int)threadIdx.x * 2 % RT;
     auto fetch = [&](int row0, int n, float2 (&v)[kMine]) {
 #pragma unroll
         for (int k = 0; k < kMine; ++k) {
-            const int at = (k * 256 + (int)threadIdx.x) * 2, row = at / RT, j = at % RT;
-            v[k] = row < n && j0 + j < a.r ? *reinterpret_cast<const float2*>(a.c + (long long)(row0 + row) * a.r + j0 + j) : make_float2(0.f, 0.f);
+            const int row = k * (512 / RT) + (int)threadIdx.x * 2 / RT;
+            v[k] = row < n && my_factor ? *reinterpret_cast<const float2*>(factor + (long long)(row0 + k * (512 / RT)) * a.r) : make_float2(0.f, 0.f);
         }
     };
 
@@ -662,7 +679,7 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads a) {
 #pragma unroll
     for (int i = 0; i < kGradStages - 1; ++i) {
         n[i] = advance(&row[i]);
-        copy(i, row[i], n[i]);
+        copy(row[i], n[i]);
     }
     float2 v[kMine];
     fetch(row[0], n[0], v);
@@ -701,9 +718,10 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads a) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kGradStages - 2) : "memory");
         __syncthreads();
         n[kGradStages - 1] = advance(&row[kGradStages - 1]);
-        copy((step + kGradStages - 1) % kGradStages, row[kGradStages - 1], n[kGradStages - 1]);
+        copy(row[kGradStages - 1], n[kGradStages - 1]);
         fetch(row[1], n[1], v);
-        const uint32_t from = ring + step % kGradStages * S::kStage;
+        const uint32_t from = take;
+        take = take + S::kStage == ring_end ? ring : take + S::kStage;
         const uint32_t factors = static_cast<uint32_t>(__cvta_generic_to_shared(to));
         // 8 x 8 blocks: of c rows lane % 8 (+ 8 for lanes 16 on) and columns + 8 for every second eight lanes; of the other the other way round
         const int low = lane & 7, mid = lane >> 3 & 1, high = lane >> 4;

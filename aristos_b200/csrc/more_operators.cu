@@ -232,7 +232,7 @@ cudaError_t adapter_grads(const adapters::Grads& a, cudaStream_t st) {
                 const auto kernel = grads_mma_kernel<T, kDb, RT>;
                 const long long strips = (a.cols + kGradColumns - 1) / kGradColumns, groups = strips * a.L * ((a.r + RT - 1) / RT);
                 int cluster = 1;
-                while (cluster < 8 && groups * cluster < 4LL * sm_count() && a.rows > cluster * kGradRows * 2LL) cluster *= 2;
+                while (cluster < 8 && 2 * groups * cluster <= 2LL * sm_count() && a.rows > cluster * kGradRows * 4LL) cluster *= 2;
                 static bool allowed[64];
                 cudaError_t rc = allow_smem(kernel, allowed, kBytes);
                 if (rc == cudaSuccess) rc = launch(kernel, dim3((unsigned)(strips * cluster), a.L, (a.r + RT - 1) / RT), 256, kBytes, cluster, st, a);

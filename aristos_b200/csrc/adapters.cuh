@@ -112,16 +112,42 @@ __device__ __forceinline__ void copy_base(const Args& a, const Tile& t, int c0, 
 }
 
 // ---------------------------------------------------------------- rows, any element type and alignment
+// Sums of N values over a warp, N / 32 of them a lane: half of the values go to the other lane at every step, N - 1 exchanges instead of 5 N.
+// Lane l ends with those from index sum of (l >> 4 - k & 1) N / 2^(k + 1) on.
+template <int N>
+__device__ __forceinline__ void warp_sums(float (&v)[N]) {
+    const int lane = threadIdx.x & 31;
+    int n = N / 2;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1, n /= 2) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            if (i >= n) break;
+            const float keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+    }
+}
+template <int N>
+__device__ __forceinline__ int warp_sums_index() {
+    const int lane = threadIdx.x & 31;
+    return (lane >> 4 & 1) * (N / 2) + (lane >> 3 & 1) * (N / 4) + (lane >> 2 & 1) * (N / 8) + (lane >> 1 & 1) * (N / 16) + (lane & 1) * (N / 32);
+}
+
 constexpr int kRowsSimt = 8;
 
-// V elements of `in` (and of p, forward) at once.
+// FP32 multiply-adds: two groups of four warps have four rows each; a group's warps (times the cluster's blocks) take the sums' elements in turn,
+// a lane for 8 or 16 columns of u at once.  V elements of `in` (and of p, forward) at once.
 template <typename T, int V, bool kBack>
-__global__ void __launch_bounds__(256) rows_kernel(Args a) {
+__global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
-    constexpr int M = kRowsSimt, J = 2;
+    constexpr int M = kRowsSimt, MW = 4, J = V > 1 ? 8 : 16, KS = 4;
+    __shared__ float part[KS][M][kMostRank + 1];
     __shared__ float u[M][kMostRank];
     const int blocks = (int)cluster.num_blocks(), block = (int)cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int rg = warp & 1, ks = warp >> 1;
     pdl_wait();
     pdl_trigger();
     Tile t;
@@ -136,20 +162,18 @@ __global__ void __launch_bounds__(256) rows_kernel(Args a) {
     const float scale = a.scale ? a.scale[t.adapter] : 1.f;
     const T* p = static_cast<const T*>(a.p) + (size_t)t.adapter * a.r * a.len;
     const T* q = static_cast<const T*>(a.q) + (size_t)t.adapter * a.r * a.cols;
-    const T* in[M];
+    const T* in[MW];  // rows past the last are the last; nobody takes their sums
 #pragma unroll
-    for (int m = 0; m < M; ++m) in[m] = static_cast<const T*>(a.in) + (long long)(t.begin + min(m, n - 1)) * a.ldi;
-    cluster.sync();  // (every block of the cluster is there to be written to)
-    // the cluster's warps share the columns of u, two at a time
-    for (int j0 = (block * 8 + warp) * J; j0 < a.r; j0 += blocks * 8 * J) {
-        float s[M][J];
+    for (int m = 0; m < MW; ++m) in[m] = static_cast<const T*>(a.in) + (long long)(t.begin + min(rg * MW + m, n - 1)) * a.ldi;
+    for (int j0 = 0; j0 < a.r; j0 += J) {
+        float s[MW * J];
 #pragma unroll
-        for (int m = 0; m < M; ++m)
+        for (int i = 0; i < MW * J; ++i) s[i] = 0.f;
+#pragma unroll 1
+        for (int k = ((block * KS + ks) * 32 + lane) * V; k < a.len; k += blocks * KS * 32 * V) {
+            Vec<T, V> w[J], x[MW];
 #pragma unroll
-            for (int j = 0; j < J; ++j) s[m][j] = 0.f;
-#pragma unroll 2
-        for (int k = lane * V; k < a.len; k += 32 * V) {
-            Vec<T, V> w[J], x[M];
+            for (int m = 0; m < MW; ++m) x[m] = load_vec<T, V>(in[m] + k);
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 const int jj = min(j0 + j, a.r - 1);
@@ -161,43 +185,57 @@ __global__ void __launch_bounds__(256) rows_kernel(Args a) {
                 }
             }
 #pragma unroll
-            for (int m = 0; m < M; ++m) x[m] = load_vec<T, V>(in[m] + k);
-#pragma unroll
-            for (int m = 0; m < M; ++m)
+            for (int m = 0; m < MW; ++m)
 #pragma unroll
                 for (int j = 0; j < J; ++j)
 #pragma unroll
-                    for (int v = 0; v < V; ++v) s[m][j] = fmaf(Elem<T>::to_f(x[m].v[v]), Elem<T>::to_f(w[j].v[v]), s[m][j]);
+                    for (int v = 0; v < V; ++v) s[m * J + j] = fmaf(Elem<T>::to_f(x[m].v[v]), Elem<T>::to_f(w[j].v[v]), s[m * J + j]);
         }
+        warp_sums<MW * J>(s);
+        const int first = warp_sums_index<MW * J>();
 #pragma unroll
-        for (int m = 0; m < M; ++m)
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const float v = warp_sum(s[m][j]) * (kBack ? scale : 1.f);
-                if (j0 + j >= a.r) continue;
-                if (lane < blocks) *cluster.map_shared_rank(&u[m][j0 + j], lane) = v;
-                if (lane == 0 && a.u && m < n) a.u[(long long)(t.begin + m) * a.r + j0 + j] = v;
-            }
+        for (int i = 0; i < MW * J / 32; ++i)
+            if (j0 + (first + i) % J < a.r) part[ks][rg * MW + (first + i) / J][j0 + (first + i) % J] = s[i];
     }
-    cluster.sync();
+    __syncthreads();
+    for (int i = threadIdx.x; i < n * a.r; i += 256) {
+        const int m = i / a.r, j = i % a.r;
+        float v = part[0][m][j];
+#pragma unroll
+        for (int k = 1; k < KS; ++k) v += part[k][m][j];
+        part[0][m][j] = kBack ? v * scale : v;
+    }
+    if (blocks > 1) cluster.sync();
+    else __syncthreads();
+    for (int i = threadIdx.x; i < n * a.r; i += 256) {
+        const int m = i / a.r, j = i % a.r;
+        float v = 0.f;
+        if (blocks == 1) v = part[0][m][j];
+        else
+            for (int k = 0; k < blocks; ++k) v += *cluster.map_shared_rank(&part[0][m][j], k);
+        u[m][j] = v;
+        if (a.u && block == 0) a.u[(long long)t.begin * a.r + i] = v;
+    }
+    if (blocks > 1) cluster.sync();  // (no block leaves while its sums may still be read)
+    else __syncthreads();
     const T* base = static_cast<const T*>(a.base);
     T* out = static_cast<T*>(a.out);
     for (int c = c0 + (int)threadIdx.x; c < c1; c += 256) {
-        float s[M];
+        float s[M], before[M];
 #pragma unroll
-        for (int m = 0; m < M; ++m) s[m] = 0.f;
-#pragma unroll 4
+        for (int m = 0; m < M; ++m) {
+            s[m] = 0.f;
+            before[m] = base && m < n ? Elem<T>::to_f(base[(long long)(t.begin + m) * a.ldb + c]) : 0.f;
+        }
+#pragma unroll 8
         for (int j = 0; j < a.r; ++j) {
             const float w = Elem<T>::to_f(kBack ? q[(size_t)j * a.cols + c] : q[(size_t)c * a.r + j]);
 #pragma unroll
             for (int m = 0; m < M; ++m) s[m] = fmaf(u[m][j], w, s[m]);
         }
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
-            if (m >= n) break;
-            const float before = base ? Elem<T>::to_f(base[(long long)(t.begin + m) * a.ldb + c]) : 0.f;
-            out[(long long)(t.begin + m) * a.ldo + c] = Elem<T>::from_f(fmaf(kBack ? 1.f : scale, s[m], before));
-        }
+        for (int m = 0; m < M; ++m)
+            if (m < n) out[(long long)(t.begin + m) * a.ldo + c] = Elem<T>::from_f(fmaf(kBack ? 1.f : scale, s[m], before[m]));
     }
 }
 
@@ -213,42 +251,81 @@ struct Grads {
     bool wide_out;       // results are floats
 };
 
-// dA (kDb false) or dB: a block takes 32 columns of one adapter, eight groups of warps its rows in turn.
+// dA (kDb false) or dB: a cluster takes 32 columns and 16 ranks of one adapter; its blocks take 64 rows of a request in turn, whose factors
+// are in shared memory, and a warp every eighth of those.
 template <typename T, bool kDb>
 __global__ void __launch_bounds__(256) grads_kernel(Grads a) {
-    constexpr int J = 16;
+    namespace cg = cooperative_groups;
+    constexpr int J = 16, kRows = 64, kMine = kRows / 8;
+    cg::cluster_group cluster = cg::this_cluster();
+    __shared__ __align__(16) float c[2][kRows][J];
     __shared__ float part[8][J][33];
+    __shared__ float sums[J][33];
+    const int blocks = (int)cluster.num_blocks(), block = (int)cluster.block_rank();
     pdl_wait();
     pdl_trigger();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = blockIdx.y, j0 = blockIdx.z * J, n = min(J, a.r - j0);
-    const int c = blockIdx.x * 32 + lane;
+    const int first = blockIdx.x / blocks * 32, col = first + lane;
+    const bool there = col < a.cols;
+    const T* in = static_cast<const T*>(a.in) + (there ? col : 0);
     float s[J];
 #pragma unroll
     for (int j = 0; j < J; ++j) s[j] = 0.f;
-    for (int i = 0; i < a.R; ++i) {
-        if (a.adapter[i] != l) continue;
-        const Group g = group_rows(a.offsets, i, a.rows);
-        for (int row = g.begin + warp; row < g.end; row += 8) {
-            const float x = c < a.cols ? Elem<T>::to_f(static_cast<const T*>(a.in)[row * a.ldi + c]) : 0.f;
-            const float* f = a.c + (long long)row * a.r + j0;
+    int count = 0, turn = 0;
+    for (int i0 = 0; i0 < a.R; i0 += 32) {
+        const int i = i0 + lane;
+        unsigned of = __ballot_sync(0xffffffffu, i < a.R && a.adapter[i] == l);
+        for (; of; of &= of - 1) {
+            const Group g = group_rows(a.offsets, i0 + __ffs(of) - 1, a.rows);
+            for (int row0 = g.begin; row0 < g.end; row0 += kRows) {
+                if (count++ % blocks != block) continue;
+                const int rows = min(kRows, g.end - row0);
+                float x[kMine];
 #pragma unroll
-            for (int j = 0; j < J; ++j) s[j] = fmaf(f[min(j, n - 1)], x, s[j]);
+                for (int k = 0; k < kMine; ++k) x[k] = there && warp + 8 * k < rows ? Elem<T>::to_f(in[(long long)(row0 + warp + 8 * k) * a.ldi]) : 0.f;
+                turn ^= 1;  // (two buffers in turn: one meeting a step)
+                for (int k = threadIdx.x; k < kRows * J; k += 256) {
+                    const int row = k / J, j = k % J;
+                    c[turn][row][j] = row < rows && j < n ? a.c[(long long)(row0 + row) * a.r + j0 + j] : 0.f;
+                }
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < kMine; ++k) {
+                    if (warp + 8 * k >= rows) break;
+#pragma unroll
+                    for (int j = 0; j < J; j += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(&c[turn][warp + 8 * k][j]);
+                        s[j] = fmaf(f.x, x[k], s[j]);
+                        s[j + 1] = fmaf(f.y, x[k], s[j + 1]);
+                        s[j + 2] = fmaf(f.z, x[k], s[j + 2]);
+                        s[j + 3] = fmaf(f.w, x[k], s[j + 3]);
+                    }
+                }
+            }
         }
     }
 #pragma unroll
     for (int j = 0; j < J; ++j) part[warp][j][lane] = s[j];
     __syncthreads();
     const float scale = a.scale ? a.scale[l] : 1.f;
-    for (int i = threadIdx.x; i < n * 32; i += 256) {
-        const int j = kDb ? i % n : i / 32, cc = kDb ? i / n : i % 32, col = blockIdx.x * 32 + cc;
-        if (col >= a.cols) continue;
+    for (int i = threadIdx.x; i < J * 32; i += 256) {
         float v = 0.f;
-        for (int w = 0; w < 8; ++w) v += part[w][j][cc];
-        v *= scale;
-        const size_t at = kDb ? ((size_t)l * a.cols + col) * a.r + j0 + j : ((size_t)l * a.r + j0 + j) * a.cols + col;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) v += part[w][i / 32][i % 32];
+        sums[i / 32][i % 32] = v * scale;
+    }
+    if (blocks > 1) cluster.sync();
+    else __syncthreads();
+    for (int i = block * 256 + threadIdx.x; i < n * 32; i += blocks * 256) {
+        const int j = kDb ? i % n : i / 32, cc = kDb ? i / n : i % 32;
+        if (first + cc >= a.cols) continue;
+        float v = 0.f;
+        for (int k = 0; k < blocks; ++k) v += *cluster.map_shared_rank(&sums[j][cc], k);
+        const size_t at = kDb ? ((size_t)l * a.cols + first + cc) * a.r + j0 + j : ((size_t)l * a.r + j0 + j) * a.cols + first + cc;
         if (a.wide_out) static_cast<float*>(a.out)[at] = v;
         else static_cast<T*>(a.out)[at] = Elem<T>::from_f(v);
     }
+    if (blocks > 1) cluster.sync();
 }
 
 }  // namespace adapters

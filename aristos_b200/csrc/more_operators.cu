@@ -214,8 +214,8 @@ cudaError_t adapter_rows(const adapters::Args& a, cudaStream_t st) {
             });
     }
     const long long tiles = a.rows / kRowsSimt + a.R + 2;  // at most
-    int cluster = 8;
-    while (cluster > 1 && tiles * cluster > 8LL * sm_count()) cluster /= 2;
+    int cluster = 1;
+    while (cluster < 8 && 2 * tiles * cluster <= 4LL * sm_count() && a.len > cluster * 256) cluster *= 2;
     if (tiles * cluster > 0x7fffffff) return cudaErrorInvalidConfiguration;
     const bool wide = by_16(sizeof(T), {a.in, kBack ? nullptr : a.p}, {a.ldi, a.len});
     const auto kernel = wide ? rows_kernel<T, kBack ? 4 : W, kBack> : rows_kernel<T, 1, kBack>;
@@ -239,7 +239,10 @@ cudaError_t adapter_grads(const adapters::Grads& a, cudaStream_t st) {
                 return rc;
             });
     }
-    return launch(adapters::grads_kernel<T, kDb>, dim3((a.cols + 31) / 32, a.L, (a.r + 15) / 16), 256, 0, 1, st, a);
+    const long long strips = (a.cols + 31) / 32, groups = strips * a.L * ((a.r + 15) / 16);
+    int cluster = 1;
+    while (cluster < 8 && 2 * groups * cluster <= 6LL * sm_count() && a.rows > cluster * 256) cluster *= 2;
+    return launch(grads_kernel<T, kDb>, dim3((unsigned)(strips * cluster), a.L, (a.r + 15) / 16), 256, 0, cluster, st, a);
 }
 
 }  // namespace

@@ -4,7 +4,8 @@
 //   stream_kernel<kDown>  out, all experts' shares of a column added up by the block that owns it
 //
 // One block a multiprocessor owns a share of the columns of EVERY expert, so the work is even however the tokens were sent, each sum is
-// finished where it began, and nothing is joined between blocks.  Its eight warps are teams that take the experts in turn; each warp of
+// finished where it began, and nothing is joined between blocks (where that would be too few columns at once, two to eight blocks share
+// columns and deal the experts among them: 23 tokens of 98 experts, I = 256, floats 291 -> SPREAD us).  Its eight warps are teams that take the experts in turn; each warp of
 // a team goes through its own 128 or 256 bytes of the weights' rows, and of the rows they are multiplied with, by 16-byte copies to
 // shared memory that are kDepth - 1 steps ahead, across experts (copies of whole rows by the bulk engine took 90 cycles each of the
 // warp that issued them: 1480 us instead of 383 for 128 tokens).  A step is multiplied on the tensor cores (warp_mma.cuh), weights on the
@@ -36,6 +37,7 @@ constexpr int kLine = 128;                           // bytes of a row that a wa
 
 // How a launch cuts the work up; the same for all its blocks.
 struct Cut {
+    int spread;  // blocks that share the same columns, each with every so-manyth expert (kDown: a cluster, whose results are added up)
     int share;   // columns of a block
     int tile;    // columns of those at a time
     int rows;    // rows of an expert at a time
@@ -141,6 +143,9 @@ __host__ __device__ __forceinline__ int team_size(int experts) { return experts 
 __device__ __forceinline__ void copy_16(uint32_t to, const void* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
+__device__ __forceinline__ void copy_4(uint32_t to, const void* from, bool there) {  // (zeros, and nothing is read, where it is not there)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
+}
 __device__ __forceinline__ void zero_16(uint32_t to) { asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory"); }
 
 // Where a warp's copies are in a launch's work: columns c0 .. c0 + w - 1 of expert e (number u of those that have a place), its places
@@ -149,8 +154,9 @@ struct At {
     int c0, w, u, e, p0, n, end, step;
 };
 
-// kLines: lines of a row in a warp's step.  kSets: sets of 16 rows of the weights (of a gated expert one a half).
-template <typename T, int kKind, int kMode, int kLines, int kSets>
+// kLines: lines of a row in a warp's step.  kSets: sets of 16 rows of the weights (of a gated expert one a half).  kUnit: bytes that all rows
+// may be copied in: 16 or 4, by the asynchronous copies, or 2.
+template <typename T, int kKind, int kMode, int kLines, int kSets, int kUnit>
 __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
     constexpr bool kGated = kMode == kUpGated, kIsDown = kMode == kDown, kMma = sizeof(T) == 2;
     static_assert(!kGated || kSets == 2, "a set for each half");
@@ -163,7 +169,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, t = lane & 3;
     const int cols = kIsDown ? a.H : a.I, row_bytes = (kIsDown ? a.I : a.H) * (int)sizeof(T);
-    const int first = blockIdx.x * c.share, last = min(cols, first + c.share);
+    const int rank = blockIdx.x % c.spread, first = blockIdx.x / c.spread * c.share, last = min(cols, first + c.share);
     const int padded = padded_rows(c.rows);
     char* mine = ring + warp * kDepth * c.slot;
     float* const behind = reinterpret_cast<float*>(ring + kStreamWarps * kDepth * c.slot + c.past);
@@ -177,7 +183,8 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
     if (!kIsDown) pdl_trigger();
 
     // Warps that share a sum, and teams of so many that take every other expert.
-    const int size = team_size(g.n), teams = kStreamWarps / size, team = warp / size, part = warp % size;
+    const int size = team_size(g.n / c.spread), teams = kStreamWarps / size, team = warp / size, part = warp % size;
+    const int u_first = team * c.spread + rank, u_next = teams * c.spread;
     const int stride = size * kRowBytes, steps = (row_bytes + stride - 1) / stride;
     float* const results = behind + 2 * meet_floats(kSets, c.rows);
     float* const sums = results + team * a.T * c.tile;
@@ -185,7 +192,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
 
     // Copies: 8 lanes a line, 16 bytes each.  In odd rows the halves of a line change places: eight rows of 64 bytes are read without two of
     // them on one bank.
-    const int line = lane >> 3, sub = lane & 7, my_byte = part * kRowBytes + sub * 16;
+    const int line = kUnit == 16 ? lane >> 3 : 0, sub = lane & 7, my_byte = part * kRowBytes + (kUnit == 16 ? sub * 16 : lane * kUnit);
     const size_t next_set = (size_t)(kGated ? a.I : kTileColumns) * row_bytes;
     const uint32_t to_lane = tc::smem_u32(mine) + line * kRowBytes + ((sub ^ (line & 1) * 4) * 16);
     const char* const w_all = static_cast<const char*>(kIsDown ? a.w2 : a.w1);
@@ -209,11 +216,11 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
         byte = my_byte;
     };
     auto begin = [&] {
-        ahead.u = team;
-        ahead.c0 = team < g.n ? first : last;
+        ahead.u = u_first;
+        ahead.c0 = u_first < g.n ? first : last;
         ahead.w = min(c.tile, last - first);
         ahead.step = 0;
-        if (team < g.n) enter(), find();
+        if (u_first < g.n) enter(), find();
     };
     auto go_on = [&] {
         weights += stride;
@@ -223,9 +230,9 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
         ahead.step = 0;
         ahead.p0 += c.rows;
         if (ahead.p0 >= ahead.end) {
-            ahead.u += teams;
+            ahead.u += u_next;
             if (ahead.u >= g.n) {
-                ahead.u = team;
+                ahead.u = u_first;
                 ahead.c0 += c.tile;
                 ahead.w = min(c.tile, last - ahead.c0);
             }
@@ -233,8 +240,44 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
         }
         find();
     };
+    // Rows that do not begin on 16 bytes: a line at a time, each lane 4 bytes of it, or 2 and 2 by way of a register, sixteen lines on their way.
+    const uint32_t mine_at = tc::smem_u32(mine);
+    auto place_of = [&](int row, int byte) { return mine_at + row * kRowBytes + (byte ^ (row & 1) * 64); };
+    auto copy_units = [&](int slot, bool take_weights, bool take_rows) {
+        const uint32_t at = slot * c.slot;
+#pragma unroll 1
+        for (int l = 0; l < kLines; ++l) {
+            const int here = byte + l * kLine;  // this lane's byte of a row
+            auto lines = [&](int row0, int rows, auto from_of) {
+#pragma unroll 1
+                for (int r0 = 0; r0 < rows; r0 += 16) {
+                    if constexpr (kUnit == 4) {
+                        const bool there = here < row_bytes;
+                        for (int r = r0; r < min(rows, r0 + 16); ++r) copy_4(at + l * kLine + place_of(row0 + r, lane * 4), there ? from_of(r) + l * kLine : w_all, there);
+                    } else {
+                        uint16_t v[16][2];
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+                                v[r][k] = r0 + r < rows && here + k * 64 < row_bytes ? *reinterpret_cast<const uint16_t*>(from_of(r0 + r) + l * kLine + k * 64) : (uint16_t)0;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+                                if (r0 + r < rows) asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + l * kLine + place_of(row0 + r0 + r, lane * 2 + k * 64)), "h"(v[r][k]) : "memory");
+                    }
+                }
+            };
+            if (take_weights)
+                for (int m = 0; m < kSets; ++m)
+                    lines(m * kTileColumns, min(kTileColumns, kGated ? ahead.w : ahead.w - m * kTileColumns), [&](int r) { return weights + (m ? next_set : 0) + (size_t)r * row_bytes; });
+            if (take_rows) lines(kSets * kTileColumns, ahead.n, [&](int r) { return x_all + x_of[ahead.p0 + r] * x_row + byte; });
+        }
+    };
     // (a row may end inside a step: there the copies are of zeros.  A line ends in one too, or is whole: 128 bytes are eight lanes' 16.)
     auto copy = [&](int slot, bool take_weights, bool take_rows) {
+        if constexpr (kUnit < 16) return copy_units(slot, take_weights, take_rows);
         const uint32_t to = to_lane + slot * c.slot;
 #pragma unroll
         for (int l = 0; l < kLines; ++l) {
@@ -312,7 +355,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
         const int w = min(c.tile, last - c0);
         if (kIsDown)
             for (int i = lane_in_team; i < a.T * w; i += 32 * size) sums[i] = 0.f;
-        for (int u = team; u < g.n; u += teams) {
+        for (int u = u_first; u < g.n; u += u_next) {
             const int e = g.expert[u], end = g.begin[u + 1];
             for (int p0 = g.begin[u]; p0 < end; p0 += c.rows) {
                 const int n = min(c.rows, end - p0);
@@ -429,13 +472,26 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
             }
         }
         if constexpr (kIsDown) {
+            namespace cg = cooperative_groups;
+            cg::cluster_group cluster = cg::this_cluster();
             __syncthreads();
             for (int i = threadIdx.x; i < a.T * w; i += kStreamThreads) {
                 float v = results[i];
                 for (int k = 1; k < teams; ++k) v += results[k * a.T * c.tile + i];
+                if (c.spread > 1) results[i] = v;
+                else static_cast<T*>(a.out)[i / w * a.ldo + c0 + i % w] = Elem<T>::from_f(v);
+            }
+            if (c.spread == 1) {
+                __syncthreads();
+                continue;
+            }
+            cluster.sync();
+            for (int i = rank * kStreamThreads + threadIdx.x; i < a.T * w; i += c.spread * kStreamThreads) {
+                float v = 0.f;
+                for (int k = 0; k < c.spread; ++k) v += *cluster.map_shared_rank(results + i, k);
                 static_cast<T*>(a.out)[i / w * a.ldo + c0 + i % w] = Elem<T>::from_f(v);
             }
-            __syncthreads();
+            cluster.sync();
         }
     }
 }

@@ -4,7 +4,7 @@
 //   l = x Wg^T + bias;  e_1 .. e_K the K largest l (ties: the lower expert);  w_k = exp(l_k) / (exp(l_1) + .. + exp(l_K))
 //   out = sum over k of w_k (W2[e_k] h_k + b2[e_k]),   h_k = f(z) or, gated, f(z) z',   z (and z') = W1[e_k] x + b1[e_k]
 //
-// Three launches: gate_kernel chooses, up_kernel makes h, down_kernel makes out.  A call reads the chosen experts' weights
+// Three launches: gate_kernel chooses, stream_kernel (moe_stream.cuh) makes h and then out.  A call reads the chosen experts' weights
 // once and little else: bound by HBM, and by latency for one token.
 //
 // The logits are sums of 46 bits: which expert is chosen does not hang on the order of a sum.  An expert whose logit is
@@ -142,162 +142,6 @@ __global__ void __launch_bounds__(32 * kGateWarps) gate_kernel(Args a) {
     if (lane < a.K) {
         a.topk[t * a.K + lane] = id;
         a.weights[t * a.K + lane] = id < 0 ? 0.f : (float)(p / sum);
-    }
-}
-
-// ---------------------------------------------------------------- places by expert
-// Places (t * K + k) in the order of their experts, within an expert in their own; those without an expert are left out.
-struct Places {
-    int of[kMostPlaces];        // the places in order
-    int expert[kMostPlaces];    // topk, then the expert of every place in order
-    int n;
-};
-
-// All threads of the block call it; `topk` may be what the kernel before wrote.
-__device__ __forceinline__ void order_places(const Args& a, Places& p) {
-    const int n = a.T * a.K;
-    if (threadIdx.x == 0) p.n = 0;
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-        const int e = __ldcg(a.topk + i);
-        p.expert[i] = e >= 0 && e < a.E ? e : kMaxExperts;
-    }
-    __syncthreads();
-    constexpr int kMine = (kMostPlaces + 255) / 256;  // of a block of 256 threads or more
-    int rank[kMine], own[kMine];
-#pragma unroll
-    for (int m = 0; m < kMine; ++m) {
-        const int i = threadIdx.x + m * blockDim.x;
-        rank[m] = -1;
-        own[m] = 0;
-        if (i >= n || p.expert[i] == kMaxExperts) continue;
-        own[m] = p.expert[i];
-        int r = 0;
-        for (int j = 0; j < n; ++j) r += p.expert[j] < own[m] || (p.expert[j] == own[m] && j < i);
-        rank[m] = r;
-        atomicAdd(&p.n, 1);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int m = 0; m < kMine; ++m)
-        if (rank[m] >= 0) {
-            p.of[rank[m]] = threadIdx.x + m * blockDim.x;
-            p.expert[rank[m]] = own[m];
-        }
-    __syncthreads();
-}
-
-// ---------------------------------------------------------------- any element type and alignment
-// Sums of C columns by kRows rows, lanes along the sum; columns and rows past the last are the last.
-template <typename TX, typename T, int V, int kRows, int C>
-__device__ __forceinline__ void dot_rows(const T* const (&w)[C], const TX* const (&x)[kRows], int len, float (&s)[kRows][C]) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int r = 0; r < kRows; ++r)
-#pragma unroll
-        for (int c = 0; c < C; ++c) s[r][c] = 0.f;
-#pragma unroll 4
-    for (int k = lane * V; k < len; k += 32 * V) {
-        Vec<T, V> wv[C];
-        Vec<TX, V> xv[kRows];
-#pragma unroll
-        for (int c = 0; c < C; ++c) wv[c] = load_vec<T, V>(w[c] + k);
-#pragma unroll
-        for (int r = 0; r < kRows; ++r) xv[r] = load_vec<TX, V>(x[r] + k);
-#pragma unroll
-        for (int r = 0; r < kRows; ++r)
-#pragma unroll
-            for (int c = 0; c < C; ++c)
-#pragma unroll
-                for (int j = 0; j < V; ++j) s[r][c] = fmaf(Elem<TX>::to_f(xv[r].v[j]), Elem<T>::to_f(wv[c].v[j]), s[r][c]);
-    }
-#pragma unroll
-    for (int r = 0; r < kRows; ++r)
-#pragma unroll
-        for (int c = 0; c < C; ++c) s[r][c] = warp_sum(s[r][c]);
-}
-
-constexpr int kRows = 4;  // of an expert that are taken at a time
-
-// h of every place, in floats: a warp takes a column (and the one that it is multiplied with) of one expert.
-template <typename T, int V, int kKind, bool kGated>
-__global__ void __launch_bounds__(256) up_kernel(Args a) {
-    __shared__ int list[kMostPlaces];
-    __shared__ int counts[8];
-    pdl_wait();
-    pdl_trigger();
-    const int e = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = a.T * a.K;
-    int rows = 0;
-    for (int i0 = 0; i0 < n; i0 += 256) {
-        const int i = i0 + (int)threadIdx.x;
-        const bool is = i < n && a.topk[i] == e;
-        const unsigned m = __ballot_sync(0xffffffffu, is);
-        if (lane == 0) counts[warp] = __popc(m);
-        __syncthreads();
-        int at = rows;
-        for (int v = 0; v < 8; ++v) {
-            at += v < warp ? counts[v] : 0;
-            rows += counts[v];
-        }
-        if (is) list[at + __popc(m & ((1u << lane) - 1))] = i;
-        __syncthreads();
-    }
-    const int up = kGated ? 2 * a.I : a.I;
-    for (int i = blockIdx.x * 8 + warp; i < a.I; i += gridDim.x * 8) {
-        constexpr int C = kGated ? 2 : 1;
-        const T* w[C];
-        float bias[C];
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const size_t row = (size_t)e * up + c * a.I + i;
-            w[c] = static_cast<const T*>(a.w1) + row * a.H;
-            bias[c] = a.b1 ? Elem<T>::to_f(static_cast<const T*>(a.b1)[row]) : 0.f;
-        }
-        for (int r0 = 0; r0 < rows; r0 += kRows) {
-            const T* x[kRows];
-            float s[kRows][C];
-#pragma unroll
-            for (int r = 0; r < kRows; ++r) x[r] = static_cast<const T*>(a.x) + list[min(r0 + r, rows - 1)] / a.K * a.ldx;
-            dot_rows<T, T, V, kRows, C>(w, x, a.H, s);
-#pragma unroll
-            for (int r = 0; r < kRows; ++r) {
-                if (r0 + r >= rows || lane != 0) continue;
-                float f = act::value<kKind, false>(s[r][0] + bias[0]);
-                if constexpr (kGated) f *= s[r][C - 1] + bias[C - 1];
-                static_cast<float*>(a.h)[list[r0 + r] * a.ldh + i] = f;
-            }
-        }
-    }
-}
-
-// out: a warp takes a column of all experts and keeps every token's sum, experts in their order.
-template <typename T, int V>
-__global__ void __launch_bounds__(256) down_kernel(Args a) {
-    __shared__ Places p;
-    __shared__ float sums[8][kMostTokens];
-    pdl_wait();
-    pdl_trigger();
-    order_places(a, p);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int n = blockIdx.x * 8 + warp; n < a.H; n += gridDim.x * 8) {
-        for (int t = lane; t < a.T; t += 32) sums[warp][t] = 0.f;
-        __syncwarp();
-        int end;
-        for (int i = 0; i < p.n; i = end) {
-            const int e = p.expert[i];
-            for (end = i + 1; end < p.n && end < i + kRows && p.expert[end] == e; ++end) {}
-            const T* const w[1] = {static_cast<const T*>(a.w2) + ((size_t)e * a.H + n) * a.I};
-            const float bias = a.b2 ? Elem<T>::to_f(static_cast<const T*>(a.b2)[(size_t)e * a.H + n]) : 0.f;
-            const float* h[kRows];
-            float s[kRows][1];
-#pragma unroll
-            for (int r = 0; r < kRows; ++r) h[r] = static_cast<const float*>(a.h) + p.of[min(i + r, end - 1)] * a.ldh;
-            dot_rows<float, T, V, kRows, 1>(w, h, a.I, s);
-            if (lane == 0)
-                for (int r = 0; r < end - i; ++r) sums[warp][p.of[i + r] / a.K] += a.weights[p.of[i + r]] * (s[r][0] + bias);
-        }
-        __syncwarp();
-        for (int t = lane; t < a.T; t += 32) static_cast<T*>(a.out)[t * a.ldo + n] = Elem<T>::from_f(sums[warp][t]);
-        __syncwarp();
     }
 }
 

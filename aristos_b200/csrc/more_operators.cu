@@ -82,7 +82,7 @@ int moe_smem(const tokens::Args& a, tokens::Cut& c, int rows) {
 }
 
 // False where not even `least` rows of an expert fit at a time.
-template <typename T, int kKind, int kMode, int kLines, int kSets>
+template <typename T, int kKind, int kMode, int kLines, int kSets, int kUnit>
 bool moe_stream_of(const tokens::Args& a, tokens::Cut c, int least, cudaStream_t st, cudaError_t* rc) {
     using namespace tokens;
     int rows = c.rows, smem;
@@ -92,20 +92,32 @@ bool moe_stream_of(const tokens::Args& a, tokens::Cut c, int least, cudaStream_t
         rows = std::max(least, (rows - 1) / 8 * 8);
     }
     const int cols = kMode == kDown ? a.H : a.I;
-    const auto kernel = stream_kernel<T, kKind, kMode, kLines, kSets>;
+    const auto kernel = stream_kernel<T, kKind, kMode, kLines, kSets, kUnit>;
     static bool allowed[64];
     *rc = allow_smem(kernel, allowed, kMostSmem);
-    if (*rc == cudaSuccess) *rc = launch(kernel, dim3((cols + c.share - 1) / c.share), kStreamThreads, smem, 1, st, a, c);
+    if (*rc == cudaSuccess) *rc = launch(kernel, dim3((cols + c.share - 1) / c.share * c.spread), kStreamThreads, smem, kMode == kDown ? c.spread : 1, st, a, c);
     return true;
 }
 
-template <typename T, int kKind, int kMode>
+template <typename T, int kKind, int kMode, int kUnit>
 cudaError_t moe_stream(const tokens::Args& a, cudaStream_t st) {
     using namespace tokens;
     const int sms = sm_count(), cols = kMode == kDown ? a.H : a.I;
     cudaError_t rc = cudaErrorInvalidConfiguration;
     Cut c{};
-    c.share = (cols + sms - 1) / sms;
+    // Blocks that share columns: a step costs as much as some six rows of weights, and experts are dealt unevenly by about half a one.
+    // (Clusters of four and more leave some multiprocessors of a group out.)
+    const double used = a.E * (1 - std::pow(1 - std::min(1.0, (double)a.K / a.E), a.T));
+    double best = 0;
+    for (int spread = 1; spread <= 8 && spread <= std::min(a.E, a.T * a.K); spread *= 2) {
+        const int over = (kMode == kDown && spread > 2 ? sms * 7 / 8 : sms) / spread;
+        if (over < 1) break;
+        const int share = (cols + over - 1) / over, most = kMode == kUpGated || sizeof(T) == 4 ? kTileColumns : 2 * kTileColumns;
+        const int tiles = (share + most - 1) / most, tile = (share + tiles - 1) / tiles, halves = kMode == kUpGated ? 2 : 1;
+        const double even = a.T == 1 ? used / (spread * std::ceil(used / spread)) : used / (used + 0.5 * (spread - 1)), filled = (double)cols / ((cols + share - 1) / share) / share;
+        const double good = even * filled * over * spread / sms * (halves * tile) / (halves * tile + 6.0);
+        if (good > best * 1.02) best = good, c.spread = spread, c.share = share;
+    }
     // rows of an expert at a time: as many as it has on average and some
     c.rows = std::min(a.T, a.T * a.K > 12 * a.E ? kMostRowsAtOnce : kMostRowsAtOnce / 2);
     // two sets of 16 columns where that takes fewer tiles (a gated expert's are its halves)
@@ -117,12 +129,12 @@ cudaError_t moe_stream(const tokens::Args& a, cudaStream_t st) {
     cut(two ? 2 * kTileColumns : kTileColumns);
     if constexpr (sizeof(T) == 4) c.rows = std::min(c.rows, kMode == kUpGated ? 8 : 16);
     if constexpr (kMode == kUpGated) {
-        if (moe_stream_of<T, kKind, kMode, 1, 2>(a, c, 8, st, &rc)) return rc;
+        if (moe_stream_of<T, kKind, kMode, 1, 2, kUnit>(a, c, 8, st, &rc)) return rc;
     } else {
         if constexpr (sizeof(T) == 2)
-            if (two && moe_stream_of<T, kKind, kMode, 1, 2>(a, c, 8, st, &rc)) return rc;
+            if (two && moe_stream_of<T, kKind, kMode, 1, 2, kUnit>(a, c, 8, st, &rc)) return rc;
         cut(kTileColumns);
-        if (moe_stream_of<T, kKind, kMode, 2, 1>(a, c, 8, st, &rc) || moe_stream_of<T, kKind, kMode, 1, 1>(a, c, 8, st, &rc)) return rc;
+        if (moe_stream_of<T, kKind, kMode, 2, 1, kUnit>(a, c, 8, st, &rc) || moe_stream_of<T, kKind, kMode, 1, 1, kUnit>(a, c, 8, st, &rc)) return rc;
     }
     return rc;
 }
@@ -138,25 +150,24 @@ cudaError_t moe_layer(tokens::Args a, int kind, bool gated, bool route, cudaStre
         const auto kernel = by_16(sizeof(T), {a.x, a.gate}, {a.ldx, a.H}) ? gate_kernel<T, W> : gate_kernel<T, 1>;
         rc = launch(kernel, dim3((a.T + a.group - 1) / a.group * kGateBlocks), 32 * kGateWarps, 0, kGateBlocks, st, a);
     }
-    if (rc == cudaSuccess && by_16(sizeof(T), {a.x, a.w1, a.w2, a.h}, {a.ldx, a.H, a.I})) {
-        rc = act::with_kind(kind, [&](auto k) {
-            constexpr int kKind = decltype(k)::value;
-            return gated ? moe_stream<T, kKind, kUpGated>(a, st) : moe_stream<T, kKind, kUp>(a, st);
+    if (rc != cudaSuccess) return rc;
+    auto with_unit = [&](int bytes, auto f) {
+        using std::integral_constant;
+        if constexpr (sizeof(T) == 2)
+            if (bytes < 4) return f(integral_constant<int, 2>());
+        return bytes < 16 ? f(integral_constant<int, 4>()) : f(integral_constant<int, 16>());
+    };
+    auto unit_of = [](const void* x, const void* w, std::initializer_list<long long> elems) {
+        return by(16, sizeof(T), {x, w}, elems) ? 16 : by(4, sizeof(T), {x, w}, elems) ? 4 : 2;
+    };
+    rc = act::with_kind(kind, [&](auto k) {
+        return with_unit(unit_of(a.x, a.w1, {a.ldx, a.H}), [&](auto u) {
+            constexpr int kKind = decltype(k)::value, kUnit = decltype(u)::value;
+            return gated ? moe_stream<T, kKind, kUpGated, kUnit>(a, st) : moe_stream<T, kKind, kUp, kUnit>(a, st);
         });
-        return rc == cudaSuccess ? moe_stream<T, 0, kDown>(a, st) : rc;
-    }
-    if (rc == cudaSuccess) rc = act::with_kind(kind, [&](auto k) {
-        constexpr int kKind = decltype(k)::value;
-        const bool wide = by_16(sizeof(T), {a.x, a.w1}, {a.ldx, a.H});
-        const auto kernel = gated ? wide ? up_kernel<T, W, kKind, true> : up_kernel<T, 1, kKind, true>
-                                  : wide ? up_kernel<T, W, kKind, false> : up_kernel<T, 1, kKind, false>;
-        return launch(kernel, dim3((a.I + 7) / 8, a.E), 256, 0, 1, st, a);
     });
-    if (rc == cudaSuccess) {
-        const bool wide = by_16(sizeof(T), {a.w2, a.h}, {a.I, a.ldh});
-        rc = launch(wide ? down_kernel<T, W> : down_kernel<T, 1>, dim3((a.H + 7) / 8), 256, 0, 1, st, a);
-    }
-    return rc;
+    if (rc != cudaSuccess) return rc;
+    return with_unit(unit_of(a.h, a.w2, {a.ldh, a.I}), [&](auto u) { return moe_stream<T, 0, kDown, decltype(u)::value>(a, st); });
 }
 
 // ---------------------------------------------------------------- adapters

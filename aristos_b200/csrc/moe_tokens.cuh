@@ -35,7 +35,7 @@ struct Args {
 };
 
 // ---------------------------------------------------------------- the router
-constexpr int kGateBlocks = 8, kGateWarps = 8, kGateTokens = 2;
+constexpr int kGateBlocks = 8, kGateWarps = 8, kGateTokens = 4;
 
 // A sum that keeps what its additions round off (two floats at once): the total is exact to about 2^-46.  The multiprocessor's 64-bit
 // additions and conversions would take ten times as long (128 tokens, 64 experts: 41 us).
@@ -54,49 +54,77 @@ struct Kept {
     }
 };
 
-// A cluster takes up to kGateTokens tokens: its warps share the experts, its blocks the tokens that are then chosen for.
+// A cluster takes up to kGateTokens tokens: its warps share the experts, its blocks the tokens that are then chosen for.  Rows on 16-byte
+// boundaries (V above 1) come a kilobyte at a time through shared memory, three steps of it.
+constexpr int kGateChunk = 1024, kGateStages = 3;
+
 template <typename T, int V>
 __global__ void __launch_bounds__(32 * kGateWarps) gate_kernel(Args a) {
     namespace cg = cooperative_groups;
-    constexpr int P = V > 1 ? V / 2 : 1, U = 8;  // vectors of a row on their way
+    constexpr int P = V > 1 ? V / 2 : 1, kRows = kGateWarps + kGateTokens;
     cg::cluster_group cluster = cg::this_cluster();
     __shared__ double logits[kMaxExperts];
+    __shared__ __align__(16) char stage[V > 1 ? kGateStages : 1][V > 1 ? kRows : 1][V > 1 ? kGateChunk : 16];  // a row of every warp's expert, then the tokens
     const int block = (int)cluster.block_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int t0 = (int)(blockIdx.x / kGateBlocks) * a.group, n = min(a.group, a.T - t0);
     cluster.sync();  // (every block of the cluster is there to be written to)
     pdl_wait();
     pdl_trigger();
     const T* x = static_cast<const T*>(a.x) + t0 * a.ldx;
-    auto pairs_of = [](const Vec<T, V>& v, F2 (&p)[P]) {
-        if constexpr (V > 1) to_pairs<T, V>(v, p);
-        else p[0] = pair(Elem<T>::to_f(v.v[0]), 0.f);
+    auto add = [](Kept& s, F2 p, F2 q) {
+        const F2 r = mul2(p, q);  // (of 16-bit factors: exact)
+        s.add(r);
+        if constexpr (sizeof(T) == 4) s.rest = add2(s.rest, fma2(p, q, mul2(r, both(-1.f))));
     };
-    for (int e = block * kGateWarps + warp; e < a.E; e += kGateBlocks * kGateWarps) {
-        const T* w = static_cast<const T*>(a.gate) + (size_t)e * a.H;
+    for (int e0 = block * kGateWarps; e0 < a.E; e0 += kGateBlocks * kGateWarps) {
+        const int e = e0 + warp;
+        const T* w = static_cast<const T*>(a.gate) + (size_t)min(e, a.E - 1) * a.H;
         Kept s[kGateTokens];
-        for (int k0 = lane * V; k0 < a.H; k0 += 32 * V * U) {
-            Vec<T, V> wv[U];
+        if constexpr (V > 1) {
+            const int row_bytes = a.H * (int)sizeof(T), steps = (row_bytes + kGateChunk - 1) / kGateChunk;
+            auto copy = [&](int step) {
+                if (step < steps)
 #pragma unroll
-            for (int i = 0; i < U; ++i) wv[i] = load_vec<T, V>(w + min(k0 + i * 32 * V, a.H - V));
+                    for (int i = threadIdx.x; i < kRows * (kGateChunk / 16); i += 32 * kGateWarps) {
+                        const int row = i / (kGateChunk / 16), piece = i % (kGateChunk / 16) * 16, at = step * kGateChunk + piece;
+                        if (row >= kGateWarps + n) break;
+                        const char* from = row < kGateWarps ? reinterpret_cast<const char*>(static_cast<const T*>(a.gate) + (size_t)min(e0 + row, a.E - 1) * a.H)
+                                                            : reinterpret_cast<const char*>(x + (row - kGateWarps) * a.ldx);
+                        const bool there = at < row_bytes;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(&stage[step % kGateStages][row][piece])),
+                                     "l"(there ? from + at : from), "r"(there ? 16 : 0) : "memory");
+                    }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            for (int i = 0; i < kGateStages - 1; ++i) copy(i);
+            for (int step = 0; step < steps; ++step) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kGateStages - 2) : "memory");
+                __syncthreads();
+                copy(step + kGateStages - 1);
+                const auto& rows = stage[step % kGateStages];
 #pragma unroll
-            for (int t = 0; t < kGateTokens; ++t) {
-                if (t >= n) break;
-                Vec<T, V> xv[U];
+                for (int i = 0; i < kGateChunk / 512; ++i) {
+                    const int at = i * 512 + lane * 16;
+                    F2 p[P];
+                    to_pairs<T, V>(load_vec<T, V>(reinterpret_cast<const T*>(&rows[warp][at])), p);
 #pragma unroll
-                for (int i = 0; i < U; ++i) xv[i] = load_vec<T, V>(x + t * a.ldx + min(k0 + i * 32 * V, a.H - V));
+                    for (int t = 0; t < kGateTokens; ++t) {
+                        if (t >= n) break;
+                        F2 q[P];
+                        to_pairs<T, V>(load_vec<T, V>(reinterpret_cast<const T*>(&rows[kGateWarps + t][at])), q);
 #pragma unroll
-                for (int i = 0; i < U; ++i) {
-                    if (k0 + i * 32 * V >= a.H) break;
-                    F2 p[P], q[P];
-                    pairs_of(wv[i], p);
-                    pairs_of(xv[i], q);
-#pragma unroll
-                    for (int j = 0; j < P; ++j) {
-                        const F2 r = mul2(p[j], q[j]);  // (of 16-bit factors: exact)
-                        s[t].add(r);
-                        if constexpr (sizeof(T) == 4) s[t].rest = add2(s[t].rest, fma2(p[j], q[j], mul2(r, both(-1.f))));
+                        for (int j = 0; j < P; ++j) add(s[t], p[j], q[j]);
                     }
                 }
+            }
+            __syncthreads();  // (the next experts' rows come into the same places)
+        } else {
+#pragma unroll 4
+            for (int k = lane; k < a.H; k += 32) {
+                const F2 p = pair(Elem<T>::to_f(w[k]), 0.f);
+#pragma unroll
+                for (int t = 0; t < kGateTokens; ++t)
+                    if (t < n) add(s[t], p, pair(Elem<T>::to_f(x[t * a.ldx + k]), 0.f));
             }
         }
 #pragma unroll
@@ -105,7 +133,7 @@ __global__ void __launch_bounds__(32 * kGateWarps) gate_kernel(Args a) {
             double v = s[t].total();
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            if (lane == 0) *cluster.map_shared_rank(&logits[e], t) = a.gate_bias ? v + (double)a.gate_bias[e] : v;
+            if (lane == 0 && e < a.E) *cluster.map_shared_rank(&logits[e], t) = a.gate_bias ? v + (double)a.gate_bias[e] : v;
         }
     }
     cluster.sync();

@@ -146,7 +146,7 @@ cudaError_t moe_layer(tokens::Args a, int kind, bool gated, bool route, cudaStre
     const int sms = sm_count();
     cudaError_t rc = cudaSuccess;
     if (route) {
-        a.group = a.T <= 2 * sms / kGateBlocks ? 1 : kGateTokens;  // (a token's two blocks a multiprocessor)
+        a.group = std::min(kGateTokens, (a.T * kGateBlocks + 2 * sms - 1) / (2 * sms));  // clusters that run at once: two blocks a multiprocessor
         const auto kernel = by_16(sizeof(T), {a.x, a.gate}, {a.ldx, a.H}) ? gate_kernel<T, W> : gate_kernel<T, 1>;
         rc = launch(kernel, dim3((a.T + a.group - 1) / a.group * kGateBlocks), 32 * kGateWarps, 0, kGateBlocks, st, a);
     }

@@ -63,36 +63,49 @@ auto with_kind(int kind, F f) {
     return f(std::integral_constant<int, 2>());
 }
 
-// A block takes blockDim.x vectors of columns of blockDim.y rows at a time.
+// A block takes blockDim.x vectors of columns of blockDim.y rows at a time; a thread has so many rows on their way that it is 16 bytes of each
+// matrix or more.
 template <typename T, int V, int kKind, bool kGated, bool kBack>
 __global__ void __launch_bounds__(256) activation_kernel(Args a) {
     constexpr bool kFast = sizeof(T) == 2;
+    constexpr int U = V * sizeof(T) >= 16 ? 1 : V * sizeof(T) >= 8 ? 2 : 4;
     pdl_wait();
     pdl_trigger();
     const int i = (blockIdx.x * blockDim.x + threadIdx.x) * V;
     if (i >= a.I) return;
     const T* z = static_cast<const T*>(a.z) + i;
     T* out = static_cast<T*>(a.out) + i;
-    for (long long r = (long long)blockIdx.y * blockDim.y + threadIdx.y; r < a.rows; r += (long long)gridDim.y * blockDim.y) {
-        const Vec<T, V> g = load_vec<T, V>(z + r * a.ldz);
-        Vec<T, V> u{}, d{}, first, second;
-        if constexpr (kGated) u = load_vec<T, V>(z + r * a.ldz + a.I);
-        if constexpr (kBack) d = load_vec<T, V>(static_cast<const T*>(a.dh) + r * a.ldh + i);
+    const long long step = (long long)gridDim.y * blockDim.y;
+    for (long long r0 = (long long)blockIdx.y * blockDim.y + threadIdx.y; r0 < a.rows; r0 += U * step) {
+        Vec<T, V> g[U], u[U], d[U];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float x = Elem<T>::to_f(g.v[j]);
-            if constexpr (!kBack) {
-                const float f = value<kKind, kFast>(x);
-                first.v[j] = Elem<T>::from_f(kGated ? f * Elem<T>::to_f(u.v[j]) : f);
-            } else {
-                const float2 f = both_of<kKind, kFast>(x);
-                const float dh = Elem<T>::to_f(d.v[j]);
-                first.v[j] = Elem<T>::from_f(kGated ? dh * Elem<T>::to_f(u.v[j]) * f.y : dh * f.y);
-                if constexpr (kGated) second.v[j] = Elem<T>::from_f(dh * f.x);
-            }
+        for (int k = 0; k < U; ++k) {  // (rows past the last are the last)
+            const long long r = min(r0 + k * step, a.rows - 1);
+            g[k] = load_vec<T, V>(z + r * a.ldz);
+            if constexpr (kGated) u[k] = load_vec<T, V>(z + r * a.ldz + a.I);
+            if constexpr (kBack) d[k] = load_vec<T, V>(static_cast<const T*>(a.dh) + r * a.ldh + i);
         }
-        store_vec<T, V>(out + r * a.ldo, first);
-        if constexpr (kGated && kBack) store_vec<T, V>(out + r * a.ldo + a.I, second);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const long long r = r0 + k * step;
+            if (r >= a.rows) break;
+            Vec<T, V> first, second;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float x = Elem<T>::to_f(g[k].v[j]);
+                if constexpr (!kBack) {
+                    const float f = value<kKind, kFast>(x);
+                    first.v[j] = Elem<T>::from_f(kGated ? f * Elem<T>::to_f(u[k].v[j]) : f);
+                } else {
+                    const float2 f = both_of<kKind, kFast>(x);
+                    const float dh = Elem<T>::to_f(d[k].v[j]);
+                    first.v[j] = Elem<T>::from_f(kGated ? dh * Elem<T>::to_f(u[k].v[j]) * f.y : dh * f.y);
+                    if constexpr (kGated) second.v[j] = Elem<T>::from_f(dh * f.x);
+                }
+            }
+            store_vec<T, V>(out + r * a.ldo, first);
+            if constexpr (kGated && kBack) store_vec<T, V>(out + r * a.ldo + a.I, second);
+        }
     }
 }
 

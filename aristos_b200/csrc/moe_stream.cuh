@@ -30,7 +30,7 @@ namespace tokens {
 constexpr int kUp = 0, kUpGated = 1, kDown = 2;
 constexpr int kStreamWarps = 8, kStreamThreads = 32 * kStreamWarps;
 constexpr int kDepth = 3;                            // steps of a warp in shared memory
-constexpr int kMostSmem = 214 * 1024;
+constexpr int kMostSmem = 226 * 1024;
 constexpr int kMostRowsAtOnce = 32, kTileColumns = 16;
 constexpr int kTeam2 = 16, kTeam4 = 8;               // experts from which teams are of two warps, of four
 constexpr int kLine = 128;                           // bytes of a row that a warp takes at a time
@@ -46,24 +46,34 @@ struct Cut {
 };
 // Rows of a slot: 16 of the weights (32 of a gated expert, or of more columns), then those that they are multiplied with.
 __host__ __device__ constexpr int padded_rows(int rows) { return (rows + 7) / 8 * 8; }
+__host__ __device__ constexpr int even_rows(int rows) { return (rows + 1) / 2 * 2; }
 // Floats that the warps need beside their slots: two buffers to meet in, and (kDown) a tile's results by team.
-__host__ __device__ constexpr int meet_floats(int sets, int rows) { return kStreamWarps * 16 * sets * padded_rows(rows); }
+__host__ __device__ constexpr int meet_floats(int sets, int rows) { return kStreamWarps * 16 * sets * even_rows(rows); }
 
 // Places by expert, within an expert in their own order; those without an expert are left out.
 struct Groups {
-    short of[kMostPlaces], token[kMostPlaces];  // the places in order, and whose they are
-    float weight[kMostPlaces];                  // kDown
-    short expert[kMaxExperts];                  // those that have a place, ascending
-    short begin[kMaxExperts + 1];               // where their places begin
-    int n;
+    float* weight;         // of the places in order (kDown)
+    short *of, *token;     // the places in order, and whose they are
+    short *expert;         // those that have a place, ascending
+    short *begin;          // where their places begin
+    int n;                 // experts
 };
+// Shared memory for them, as little as the call needs: where it is little, the down kernel's blocks are there before the up kernel's have ended.
+__host__ __device__ __forceinline__ int groups_bytes(int places, int experts) { return (places * 8 + (experts < places ? experts : places) * 4 + 2 + 127) / 128 * 128; }
 struct Counts {
     short of[kMaxExperts];
 };
 
 // All threads of the block call it; one warp goes through the places, 32 at a time.  `counts` is only used where there are more than 32.
-__device__ __forceinline__ void group_places(const Args& a, Groups& g, Counts& counts) {
+__device__ __forceinline__ Groups group_places(const Args& a, char* memory, Counts& counts) {
+    __shared__ int experts;
     const int lane = threadIdx.x & 31, n = a.T * a.K;
+    Groups g;
+    g.weight = reinterpret_cast<float*>(memory);
+    g.of = reinterpret_cast<short*>(g.weight + n);
+    g.token = g.of + n;
+    g.expert = g.token + n;
+    g.begin = g.expert + min(a.E, n);
     if (n > 32) {
         for (int e = threadIdx.x; e < a.E; e += blockDim.x) counts.of[e] = 0;
         __syncthreads();
@@ -90,7 +100,7 @@ __device__ __forceinline__ void group_places(const Args& a, Groups& g, Counts& c
             if ((same & below_me) == 0) g.expert[used] = (short)e, g.begin[used] = (short)rank;
         }
         const int places = __popc(__ballot_sync(0xffffffffu, e >= 0));
-        if (lane == 0) g.n = __popc(firsts), g.begin[__popc(firsts)] = (short)places;
+        if (lane == 0) experts = __popc(firsts), g.begin[__popc(firsts)] = (short)places;
     } else if (threadIdx.x < 32) {
         constexpr int kSteps = kMostPlaces / 32;
         short at[kSteps], expert[kSteps];
@@ -125,7 +135,7 @@ __device__ __forceinline__ void group_places(const Args& a, Groups& g, Counts& c
             begin += __shfl_sync(0xffffffffu, up, 31);
             used += __popc(any);
         }
-        if (lane == 0) g.n = used, g.begin[used] = (short)begin;
+        if (lane == 0) experts = used, g.begin[used] = (short)begin;
         __syncwarp();
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
@@ -134,6 +144,8 @@ __device__ __forceinline__ void group_places(const Args& a, Groups& g, Counts& c
         }
     }
     __syncthreads();
+    g.n = experts;
+    return g;
 }
 
 // With experts enough for every team to have several, a warp goes through more of a sum before it meets others (128 tokens of 63 experts:
@@ -164,19 +176,19 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
     constexpr int kNTiles = kMostRowsAtOnce / 8;
     constexpr int kFloatRows = kSets == 2 ? 8 : 16;      // floats: rows at a time
     constexpr int kRowBytes = kLines * kLine;            // of a slot's row
-    extern __shared__ __align__(128) char ring[];
-    __shared__ Groups g;
+    extern __shared__ __align__(128) char memory[];
+    char* const ring = memory + groups_bytes(a.T * a.K, a.E);
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, t = lane & 3;
     const int cols = kIsDown ? a.H : a.I, row_bytes = (kIsDown ? a.I : a.H) * (int)sizeof(T);
     const int rank = blockIdx.x % c.spread, first = blockIdx.x / c.spread * c.share, last = min(cols, first + c.share);
-    const int padded = padded_rows(c.rows);
+    const int pitch = even_rows(c.rows);  // of the sums that meet
     char* mine = ring + warp * kDepth * c.slot;
     float* const behind = reinterpret_cast<float*>(ring + kStreamWarps * kDepth * c.slot + c.past);
 
     // the down kernel waits for the kernel before it only where it needs h: the choice of experts was there before that began
     if (!kIsDown) pdl_wait();
-    group_places(a, g, *reinterpret_cast<Counts*>(ring));
+    const Groups g = group_places(a, memory, *reinterpret_cast<Counts*>(ring));
     if (kIsDown)
         for (int i = threadIdx.x; i < g.begin[g.n]; i += kStreamThreads) g.weight[i] = __ldcg(a.weights + g.of[i]);
     __syncthreads();
@@ -369,7 +381,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
                     *out = Elem<T>::from_f(h);
                 };
                 // two buffers in turn, so that a team meets once a sum
-                float* meet = behind + (turn ? meet_floats(kSets, c.rows) : 0) + team * size * 16 * kSets * padded;
+                float* meet = behind + (turn ? meet_floats(kSets, c.rows) : 0) + team * size * 16 * kSets * pitch;
                 turn ^= 1;
                 if constexpr (kMma) {
                     const int tiles = (n + 7) / 8;
@@ -406,9 +418,10 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
 #pragma unroll
                         for (int j = 0; j < kNTiles; ++j) {
                             if (j >= tiles) break;
-                            float* to = meet + ((part * kSets + m) * 16 + quad) * padded + j * 8 + t * 2;
+                            if (j * 8 + t * 2 >= pitch) break;
+                            float* to = meet + ((part * kSets + m) * 16 + quad) * pitch + j * 8 + t * 2;
                             *reinterpret_cast<float2*>(to) = make_float2(s[m][j][0], s[m][j][1]);
-                            *reinterpret_cast<float2*>(to + 8 * padded) = make_float2(s[m][j][2], s[m][j][3]);
+                            *reinterpret_cast<float2*>(to + 8 * pitch) = make_float2(s[m][j][2], s[m][j][3]);
                         }
                 } else {
                     // floats: a lane multiplies its 16 bytes of two rows of each set with the same bytes of every row
@@ -445,15 +458,15 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
                             float v = sum2(s[m][j]);
                             v += __shfl_xor_sync(0xffffffffu, v, 1);
                             v += __shfl_xor_sync(0xffffffffu, v, 2);
-                            if (t == 0) meet[(part * 16 * kSets + 8 * m + quad) * padded + j] = v;
+                            if (t == 0) meet[(part * 16 * kSets + 8 * m + quad) * pitch + j] = v;
                         }
                     }
                 }
                 team_sync();
                 auto sum_of = [&](int column, int row) {
-                    const float* from = meet + column * padded + row;
+                    const float* from = meet + column * pitch + row;
                     float v = *from;
-                    for (int k = 1; k < size; ++k) v += *(from += 16 * kSets * padded);
+                    for (int k = 1; k < size; ++k) v += *(from += 16 * kSets * pitch);
                     return v;
                 };
                 for (int i = lane_in_team; i < w * n; i += 32 * size) {

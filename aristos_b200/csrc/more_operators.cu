@@ -78,7 +78,7 @@ int moe_smem(const tokens::Args& a, tokens::Cut& c, int rows) {
     c.slot = (kSets * kTileColumns + rows) * kLines * kLine;
     c.past = (padded_rows(rows) - rows) * kLines * kLine;
     const int teams = kStreamWarps / team_size(std::min(a.E, a.T * a.K));  // at most
-    return kStreamWarps * kDepth * c.slot + c.past + 4 * (2 * meet_floats(kSets, rows) + (kMode == kDown ? teams * a.T * c.tile : 0));
+    return groups_bytes(a.T * a.K, a.E) + kStreamWarps * kDepth * c.slot + c.past + 4 * (2 * meet_floats(kSets, rows) + (kMode == kDown ? teams * a.T * c.tile : 0));
 }
 
 // False where not even `least` rows of an expert fit at a time.
@@ -214,7 +214,7 @@ cudaError_t adapter_rows(const adapters::Args& a, cudaStream_t st) {
                 // requests of few rows: tiles of as many as the tensor cores take
                 if (a.rows < 24LL * a.R) return adapter_rows_mma<T, kBack, RT, 16>(a, st);
                 if constexpr (RT <= 64)
-                    if (a.rows / kPipeRows + a.R / 2 >= sm_count()) {
+                    if (a.rows / kPipeRows + a.R / 2 >= sm_count() ) {
                         const auto kernel = rows_pipe_kernel<T, kBack, RT>;
                         static bool allowed[64];
                         cudaError_t rc = allow_smem(kernel, allowed, PipeShape<RT>::kBytes);

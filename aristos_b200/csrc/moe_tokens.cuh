@@ -55,16 +55,19 @@ struct Kept {
 };
 
 // A cluster takes up to kGateTokens tokens: its warps share the experts, its blocks the tokens that are then chosen for.  Rows on 16-byte
-// boundaries (V above 1) come a kilobyte at a time through shared memory, three steps of it.
-constexpr int kGateChunk = 1024, kGateStages = 3;
+// boundaries (V above 1) come a kilobyte at a time through shared memory, kGateStages steps of it.
+constexpr int kGateChunk = 1024, kGateStages = 5, kGateRows = kGateWarps + kGateTokens;
+constexpr int kGateSmem = kGateStages * kGateRows * kGateChunk;  // (where V is above 1)
 
 template <typename T, int V>
 __global__ void __launch_bounds__(32 * kGateWarps) gate_kernel(Args a) {
     namespace cg = cooperative_groups;
-    constexpr int P = V > 1 ? V / 2 : 1, kRows = kGateWarps + kGateTokens;
+    constexpr int P = V > 1 ? V / 2 : 1;
+    typedef char Stage[kGateRows][kGateChunk];  // a row of every warp's expert, then the tokens
     cg::cluster_group cluster = cg::this_cluster();
     __shared__ double logits[kMaxExperts];
-    __shared__ __align__(16) char stage[V > 1 ? kGateStages : 1][V > 1 ? kRows : 1][V > 1 ? kGateChunk : 16];  // a row of every warp's expert, then the tokens
+    extern __shared__ __align__(128) char memory[];
+    Stage* const stage = reinterpret_cast<Stage*>(memory);
     const int block = (int)cluster.block_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int t0 = (int)(blockIdx.x / kGateBlocks) * a.group, n = min(a.group, a.T - t0);
     cluster.sync();  // (every block of the cluster is there to be written to)
@@ -85,7 +88,7 @@ __global__ void __launch_bounds__(32 * kGateWarps) gate_kernel(Args a) {
             auto copy = [&](int step) {
                 if (step < steps)
 #pragma unroll
-                    for (int i = threadIdx.x; i < kRows * (kGateChunk / 16); i += 32 * kGateWarps) {
+                    for (int i = threadIdx.x; i < kGateRows * (kGateChunk / 16); i += 32 * kGateWarps) {
                         const int row = i / (kGateChunk / 16), piece = i % (kGateChunk / 16) * 16, at = step * kGateChunk + piece;
                         if (row >= kGateWarps + n) break;
                         const char* from = row < kGateWarps ? reinterpret_cast<const char*>(static_cast<const T*>(a.gate) + (size_t)min(e0 + row, a.E - 1) * a.H)

@@ -147,8 +147,11 @@ cudaError_t moe_layer(tokens::Args a, int kind, bool gated, bool route, cudaStre
     cudaError_t rc = cudaSuccess;
     if (route) {
         a.group = std::min(kGateTokens, (a.T * kGateBlocks + 2 * sms - 1) / (2 * sms));  // clusters that run at once: two blocks a multiprocessor
-        const auto kernel = by_16(sizeof(T), {a.x, a.gate}, {a.ldx, a.H}) ? gate_kernel<T, W> : gate_kernel<T, 1>;
-        rc = launch(kernel, dim3((a.T + a.group - 1) / a.group * kGateBlocks), 32 * kGateWarps, 0, kGateBlocks, st, a);
+        const bool wide = by_16(sizeof(T), {a.x, a.gate}, {a.ldx, a.H});
+        const auto kernel = wide ? gate_kernel<T, W> : gate_kernel<T, 1>;
+        static bool allowed[64];
+        if (wide) rc = allow_smem(gate_kernel<T, W>, allowed, kGateSmem);
+        if (rc == cudaSuccess) rc = launch(kernel, dim3((a.T + a.group - 1) / a.group * kGateBlocks), 32 * kGateWarps, wide ? kGateSmem : 0, kGateBlocks, st, a);
     }
     if (rc != cudaSuccess) return rc;
     auto with_unit = [&](int bytes, auto f) {

@@ -584,15 +584,16 @@ constexpr int kGradRows = 32, kGradColumns = 256, kGradStages = 4;
 
 template <typename T, int RT>
 struct GradShape {
-    static constexpr int kPitch = RT + 8;                          // elements of a row of c
+    static constexpr int kPitch = RT + 8;                          // elements of a row of c as a factor
     static constexpr int kRowPitch = kGradColumns * 2 + 16;        // bytes of a row of the other factor
-    static constexpr int kStage = kGradRows * kRowPitch, kFactors = kGradStages * kStage;
+    static constexpr int kRows = kGradRows * kRowPitch, kStage = kRows + kGradRows * RT * 4;
+    static constexpr int kFactors = kGradStages * kStage;
     static constexpr int kSums = RT * (kGradColumns + 1) * 4, kRing = kFactors + 2 * kGradRows * kPitch * 2;
     static constexpr int kBytes = kSums > kRing ? kSums : kRing;
 };
 
-// RT: columns of c (u or v) from blockIdx.z * RT on.  The cluster's blocks take kGradRows rows of a request in turn; those of the other factor come
-// through a ring in shared memory.
+// RT: columns of c (u or v) from blockIdx.z * RT on.  The cluster's blocks take kGradRows rows of a request in turn; both factors come through a
+// ring in shared memory, c a step before it is needed, when it is rounded to a factor of the products.
 template <typename T, bool kDb, int RT>
 __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads a) {
     namespace cg = cooperative_groups;
@@ -652,6 +653,13 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads a) {
     const T* const in = static_cast<const T*>(a.in) + my_row * a.ldi + c0 + my_col;
     const uint32_t ring_end = ring + kGradStages * S::kStage;
     uint32_t fill = ring + my_row * S::kRowPitch + my_col * 2, take = ring;
+    // 8 bytes of c, of every so-manyth row (a rank that is a multiple of 8 begins on 8 bytes, not on 16)
+    constexpr int kMine = kGradRows * RT / 256 / 2, kEvery = 512 / RT;
+    const int c_row = (int)threadIdx.x * 2 / RT, c_col = (int)threadIdx.x * 2 % RT;
+    const bool c_column = j0 + c_col < a.r;
+    const float* const c_in = a.c + (long long)c_row * a.r + j0 + c_col;
+    const int c_at = (c_row * RT + c_col) * 4;
+    uint32_t fill_c = ring + S::kRows + c_at;
     auto copy = [&](int row0, int n) {
         const T* from = in + row0 * a.ldi;
 #pragma unroll
@@ -659,39 +667,32 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads a) {
             const bool there = my_column && my_row + i < n;  // (rows of others are zeros here, not multiplied by zero)
             copy_or_zero(fill + i * S::kRowPitch, there ? from : static_cast<const T*>(a.in), there);
         }
+        const float* c_from = c_in + (long long)row0 * a.r;
+#pragma unroll
+        for (int k = 0; k < kMine; ++k, c_from += (long long)kEvery * a.r) {
+            const bool there = c_column && c_row + k * kEvery < n;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(fill_c + k * kEvery * RT * 4), "l"(there ? c_from : a.c), "r"(there ? 8 : 0) : "memory");
+        }
         asm volatile("cp.async.commit_group;" ::: "memory");
         fill += S::kStage;
-        if (fill >= ring_end) fill -= kGradStages * S::kStage;
+        fill_c += S::kStage;
+        if (fill >= ring_end) fill -= kGradStages * S::kStage, fill_c -= kGradStages * S::kStage;
     };
-    constexpr int kMine = kGradRows * RT / 256 / 2;  // pairs of c of a thread
-    const bool my_factor = j0 + (int)threadIdx.x * 2 % RT < a.r;
-    const float* const factor = a.c + (long long)((int)threadIdx.x * 2 / RT) * a.r + j0 + (int)threadIdx.x * 2 % RT;
-    auto fetch = [&](int row0, int n, float2 (&v)[kMine]) {
-#pragma unroll
-        for (int k = 0; k < kMine; ++k) {
-            const int row = k * (512 / RT) + (int)threadIdx.x * 2 / RT;
-            v[k] = row < n && my_factor ? *reinterpret_cast<const float2*>(factor + (long long)(row0 + k * (512 / RT)) * a.r) : make_float2(0.f, 0.f);
-        }
-    };
-
-    // this step and those that are on their way: begin and number of their rows
-    int row[kGradStages] = {}, n[kGradStages];
-#pragma unroll
-    for (int i = 0; i < kGradStages - 1; ++i) {
-        n[i] = advance(&row[i]);
-        copy(row[i], n[i]);
-    }
-    float2 v[kMine];
-    fetch(row[0], n[0], v);
     float shrink = 1.f;  // what the values of c are multiplied with (a power of two; the sums then have it too)
     bool any = false;    // whether one of them was not zero
-    for (int step = 0; n[0] > 0; ++step) {
+    // the factors of a step whose copies are there, into one of two buffers
+    auto round = [&](const char* stage, int which) {
+        float2 v[kMine];
         float most = 0.f;
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) {
+            v[k] = *reinterpret_cast<const float2*>(stage + S::kRows + c_at + k * kEvery * RT * 4);
+            most = fmaxf(most, fmaxf(fabsf(v[k].x), fabsf(v[k].y)));
+        }
         if constexpr (kShrink) {
 #pragma unroll
-            for (int k = 0; k < kMine; ++k) most = fmaxf(most, fmaxf(fabsf(v[k].x), fabsf(v[k].y)));
-#pragma unroll
             for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            __syncthreads();  // (all are through with the step before)
             if (lane == 0) largest[warp] = most;
             __syncthreads();
 #pragma unroll
@@ -709,22 +710,32 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads a) {
                 shrink = want;
             }
         }
-        T* to = c + (step & 1) * kGradRows * S::kPitch;  // (two buffers in turn: one meeting a step)
+        T* to = c + which * kGradRows * S::kPitch + c_row * S::kPitch + c_col;
 #pragma unroll
-        for (int k = 0; k < kMine; ++k) {
-            const int at = (k * 256 + (int)threadIdx.x) * 2;
-            *reinterpret_cast<uint32_t*>(to + at / RT * S::kPitch + at % RT) = pack<T>(v[k].x * shrink, v[k].y * shrink);
-        }
-        asm volatile("cp.async.wait_group %0;" ::"n"(kGradStages - 2) : "memory");
+        for (int k = 0; k < kMine; ++k) *reinterpret_cast<uint32_t*>(to + k * kEvery * S::kPitch) = pack<T>(v[k].x * shrink, v[k].y * shrink);
+    };
+
+    // rows of this step and of those that are on their way
+    int n[kGradStages];
+    auto one_more = [&](int i) {
+        int row0 = 0;
+        n[i] = advance(&row0);
+        copy(row0, n[i]);
+    };
+#pragma unroll
+    for (int i = 0; i < kGradStages - 1; ++i) one_more(i);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kGradStages - 2) : "memory");
+    // (a thread reads the values of c that it copied itself)
+    if (n[0] > 0) round(memory, 0);
+    const int low = lane & 7, mid = lane >> 3 & 1, high = lane >> 4;
+    for (int step = 0; n[0] > 0; ++step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kGradStages - 3) : "memory");
         __syncthreads();
-        n[kGradStages - 1] = advance(&row[kGradStages - 1]);
-        copy(row[kGradStages - 1], n[kGradStages - 1]);
-        fetch(row[1], n[1], v);
+        one_more(kGradStages - 1);
         const uint32_t from = take;
         take = take + S::kStage == ring_end ? ring : take + S::kStage;
-        const uint32_t factors = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+        const uint32_t factors = static_cast<uint32_t>(__cvta_generic_to_shared(c + (step & 1) * kGradRows * S::kPitch));
         // 8 x 8 blocks: of c rows lane % 8 (+ 8 for lanes 16 on) and columns + 8 for every second eight lanes; of the other the other way round
-        const int low = lane & 7, mid = lane >> 3 & 1, high = lane >> 4;
 #pragma unroll
         for (int k = 0; k < kGradRows / 16; ++k) {
             if (k * 16 >= n[0]) break;
@@ -740,7 +751,8 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads a) {
             }
         }
 #pragma unroll
-        for (int i = 0; i < kGradStages - 1; ++i) row[i] = row[i + 1], n[i] = n[i + 1];
+        for (int i = 0; i < kGradStages - 1; ++i) n[i] = n[i + 1];
+        if (n[0] > 0) round(memory + (take - ring), step + 1 & 1);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();

@@ -1,5 +1,5 @@
-// The adapters' products (adapters.cuh) where 16-bit rows begin on 16-byte boundaries and the rank is a multiple of 8: on the tensor
-// cores, straight from memory (warp_mma.cuh).
+// The adapters' products (adapters.cuh) where 16-bit rows begin on 16-byte boundaries and the rank is a multiple of 8 (up to 16, of 4; for the
+// gradients, of 2): on the tensor cores, straight from memory (warp_mma.cuh).
 //
 //   rows_mma_kernel   u and y, or v and dx: a cluster of blocks takes up to TR rows of a request
 //   grads_mma_kernel  dA or dB: a cluster takes 256 columns of one adapter and goes through the rows of its requests
@@ -653,7 +653,7 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads a) {
     const T* const in = static_cast<const T*>(a.in) + my_row * a.ldi + c0 + my_col;
     const uint32_t ring_end = ring + kGradStages * S::kStage;
     uint32_t fill = ring + my_row * S::kRowPitch + my_col * 2, take = ring;
-    // 8 bytes of c, of every so-manyth row (a rank that is a multiple of 8 begins on 8 bytes, not on 16)
+    // 8 bytes of c, of every so-manyth row
     constexpr int kMine = kGradRows * RT / 256 / 2, kEvery = 512 / RT;
     const int c_row = (int)threadIdx.x * 2 / RT, c_col = (int)threadIdx.x * 2 % RT;
     const bool c_column = j0 + c_col < a.r;

@@ -211,13 +211,14 @@ cudaError_t adapter_rows(const adapters::Args& a, cudaStream_t st) {
     using namespace adapters;
     constexpr int W = 16 / sizeof(T);
     if constexpr (sizeof(T) == 2) {
-        if (a.r % 8 == 0 && by_16(2, {a.in, a.p, a.q, a.base, a.out}, {a.ldi, a.ldb, a.ldo, a.len, a.cols}))
+        // (ranks up to 16 are read 8 bytes at a time)
+        if ((a.r % 8 == 0 || (a.r % 4 == 0 && a.r < 16)) && by_16(2, {a.in, a.p, a.q, a.base, a.out}, {a.ldi, a.ldb, a.ldo, a.len, a.cols}))
             return with_rank(a.r, [&](auto rt) {
                 constexpr int RT = decltype(rt)::value;
                 // requests of few rows: tiles of as many as the tensor cores take
                 if (a.rows < 24LL * a.R) return adapter_rows_mma<T, kBack, RT, 16>(a, st);
                 if constexpr (RT <= 64)
-                    if (a.rows / kPipeRows + a.R / 2 >= sm_count() ) {
+                    if (a.r % 8 == 0 && a.rows / kPipeRows + a.R / 2 >= sm_count()) {  // (its copies are of 16 bytes)
                         const auto kernel = rows_pipe_kernel<T, kBack, RT>;
                         static bool allowed[64];
                         cudaError_t rc = allow_smem(kernel, allowed, PipeShape<RT>::kBytes);
@@ -240,7 +241,7 @@ template <typename T, bool kDb>
 cudaError_t adapter_grads(const adapters::Grads& a, cudaStream_t st) {
     using namespace adapters;
     if constexpr (sizeof(T) == 2) {
-        if (a.r % 8 == 0 && by_16(2, {a.in}, {a.ldi, a.cols}))
+        if (a.r % 2 == 0 && by_16(2, {a.in}, {a.ldi, a.cols}) && aligned(a.c, 8))
             return with_rank(std::min(a.r, 64), [&](auto rt) {
                 constexpr int RT = decltype(rt)::value, kBytes = GradShape<T, RT>::kBytes;
                 const auto kernel = grads_mma_kernel<T, kDb, RT>;

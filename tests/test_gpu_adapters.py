@@ -96,14 +96,15 @@ def _uneven(rows, R, seed):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
-@pytest.mark.parametrize("r", [1, 4, 8, 12, 16, 24, 32, 48, 64, 128])
+@pytest.mark.parametrize("r", [1, 2, 4, 6, 8, 12, 16, 20, 24, 32, 48, 64, 66, 128])
 def test_ranks(r, dtype):
     Case([5, 70, 0, 17, 1], [1, 0, 2, -1, 1], 3, r, 264, 328, dtype, first=2, spare=3).all().verify()
 
 
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("rows,R,r,N,K", [(1, 1, 16, 2048, 2048), (1, 1, 8, 8, 8), (64, 64, 16, 512, 256), (500, 7, 32, 264, 1096), (1500, 300, 16, 136, 520),
-                                          (4096, 3, 16, 512, 640), (300, 2, 64, 2048, 264), (33, 33, 16, 40, 2888), (129, 2, 16, 1032, 24)])
+                                          (4096, 3, 16, 512, 640), (300, 2, 64, 2048, 264), (33, 33, 16, 40, 2888), (129, 2, 16, 1032, 24),
+                                          (20000, 5, 64, 136, 72), (20000, 5, 32, 72, 136), (12000, 30, 16, 8, 200), (20000, 3, 12, 136, 72), (700, 2, 4, 264, 136)])
 def test_shapes(rows, R, r, N, K, dtype):
     lengths, which = _uneven(rows, R, rows) if R != rows else ([1] * R, [i % 5 - 1 for i in range(R)])
     Case(lengths, which if rows > 1 else [0], 4, r, N, K, dtype, spare=5).all().verify()

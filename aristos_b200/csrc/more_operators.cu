@@ -112,7 +112,7 @@ cudaError_t moe_stream(const tokens::Args& a, cudaStream_t st) {
     for (int spread = 1; spread <= 8 && spread <= std::min(a.E, a.T * a.K); spread *= 2) {
         const int over = (kMode == kDown && spread > 2 ? sms * 7 / 8 : sms) / spread;
         if (over < 1) break;
-        const int share = (cols + over - 1) / over, most = kMode == kUpGated || sizeof(T) == 4 ? kTileColumns : 2 * kTileColumns;
+        const int share = (cols + over - 1) / over, most = kMode == kUpGated || (sizeof(T) == 4 && a.T > 8) ? kTileColumns : 2 * kTileColumns;
         const int tiles = (share + most - 1) / most, tile = (share + tiles - 1) / tiles, halves = kMode == kUpGated ? 2 : 1;
         const double even = a.T == 1 ? used / (spread * std::ceil(used / spread)) : used / (used + 0.5 * (spread - 1)), filled = (double)cols / ((cols + share - 1) / share) / share;
         const double good = even * filled * over * spread / sms * (halves * tile) / (halves * tile + 6.0);
@@ -120,19 +120,18 @@ cudaError_t moe_stream(const tokens::Args& a, cudaStream_t st) {
     }
     // rows of an expert at a time: as many as it has on average and some
     c.rows = std::min(a.T, a.T * a.K > 12 * a.E ? kMostRowsAtOnce : kMostRowsAtOnce / 2);
+    if (sizeof(T) == 4) c.rows = std::min(c.rows, kMode == kUpGated ? 8 : 16);  // (registers)
     // two sets of 16 columns where that takes fewer tiles (a gated expert's are its halves)
-    const bool two = kMode != kUpGated && sizeof(T) == 2 && (c.share + 31) / 32 < (c.share + 15) / 16;
+    const bool two = kMode != kUpGated && (sizeof(T) == 2 || c.rows <= 8) && (c.share + 31) / 32 < (c.share + 15) / 16;
     auto cut = [&](int most) {
         const int tiles = (c.share + most - 1) / most;
         c.tile = (c.share + tiles - 1) / tiles;
     };
     cut(two ? 2 * kTileColumns : kTileColumns);
-    if constexpr (sizeof(T) == 4) c.rows = std::min(c.rows, kMode == kUpGated ? 8 : 16);
     if constexpr (kMode == kUpGated) {
         if (moe_stream_of<T, kKind, kMode, 1, 2, kUnit>(a, c, 8, st, &rc)) return rc;
     } else {
-        if constexpr (sizeof(T) == 2)
-            if (two && moe_stream_of<T, kKind, kMode, 1, 2, kUnit>(a, c, 8, st, &rc)) return rc;
+        if (two && moe_stream_of<T, kKind, kMode, 1, 2, kUnit>(a, c, 8, st, &rc)) return rc;
         cut(kTileColumns);
         if (moe_stream_of<T, kKind, kMode, 2, 1, kUnit>(a, c, 8, st, &rc) || moe_stream_of<T, kKind, kMode, 1, 1, kUnit>(a, c, 8, st, &rc)) return rc;
     }

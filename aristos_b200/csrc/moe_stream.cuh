@@ -7,7 +7,7 @@
 // finished where it began, and nothing is joined between blocks (where that would be too few columns at once, two to eight blocks share
 // columns and deal the experts among them: 23 tokens of 98 experts, I = 256, floats 291 -> SPREAD us).  Its eight warps are teams that take the experts in turn; each warp of
 // a team goes through its own 128 or 256 bytes of the weights' rows, and of the rows they are multiplied with, by 16-byte copies to
-// shared memory that are kDepth - 1 steps ahead, across experts (copies of whole rows by the bulk engine took 90 cycles each of the
+// shared memory that are two or three steps ahead, across experts (copies of whole rows by the bulk engine took 90 cycles each of the
 // warp that issued them: 1480 us instead of 383 for 128 tokens).  A step is multiplied on the tensor cores (warp_mma.cuh), weights on the
 // instruction's 16 rows, up to 32 rows of an expert on its columns; floats by 32-bit multiply-adds, which up to 16 rows an expert are
 // fewer than the splitting that the tensor cores would want.  A team's partial sums meet in shared memory once an expert and tile.
@@ -29,7 +29,6 @@ namespace tokens {
 
 constexpr int kUp = 0, kUpGated = 1, kDown = 2;
 constexpr int kStreamWarps = 8, kStreamThreads = 32 * kStreamWarps;
-constexpr int kDepth = 3;                            // steps of a warp in shared memory
 constexpr int kMostSmem = 226 * 1024;
 constexpr int kMostRowsAtOnce = 32, kTileColumns = 16;
 constexpr int kTeam2 = 16, kTeam4 = 8;               // experts from which teams are of two warps, of four
@@ -167,8 +166,8 @@ struct At {
 };
 
 // kLines: lines of a row in a warp's step.  kSets: sets of 16 rows of the weights (of a gated expert one a half).  kUnit: bytes that all rows
-// may be copied in: 16 or 4, by the asynchronous copies, or 2.
-template <typename T, int kKind, int kMode, int kLines, int kSets, int kUnit>
+// may be copied in: 16 or 4, by the asynchronous copies, or 2.  kDepth: steps of a warp in shared memory.
+template <typename T, int kMode, int kLines, int kSets, int kUnit, int kDepth>
 __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
     constexpr bool kGated = kMode == kUpGated, kIsDown = kMode == kDown, kMma = sizeof(T) == 2;
     static_assert(!kGated || kSets == 2, "a set for each half");
@@ -375,7 +374,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
                 auto finish_up = [&](int column, int row, float z, float z2) {
                     const T* b1 = static_cast<const T*>(a.b1) + (size_t)e * kHalves * a.I + c0 + column;
                     if (a.b1) z += Elem<T>::to_f(*b1);
-                    float h = act::value<kKind, kMma>(z);
+                    float h = a.act == 0 ? act::value<0, kMma>(z) : a.act == 1 ? act::value<1, kMma>(z) : act::value<2, kMma>(z);
                     if constexpr (kGated) h *= a.b1 ? z2 + Elem<T>::to_f(b1[a.I]) : z2;
                     T* out = static_cast<T*>(a.h) + (size_t)g.of[p0 + row] * a.ldh + c0 + column;
                     *out = Elem<T>::from_f(h);

@@ -31,6 +31,7 @@ struct Args {
     void* h;         // [T * K] rows of ldh
     long long ldx, ldo, ldh;
     int T, H, I, E, K;
+    int act;
     int group;  // tokens of a cluster of gate_kernel
 };
 

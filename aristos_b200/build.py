@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libkleos_b200.so")
 DRIVER = os.path.join(HERE, "kleos_driver")
-SOURCES = ["kleos_api.cu", "operators.cu", "more_operators.cu"]
+SOURCES = ["kleos_api.cu", "operators.cu", "more_operators.cu", "moe_tokens.cu"]
 
 
 def _newest_source_mtime() -> float:

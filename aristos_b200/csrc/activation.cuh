@@ -15,6 +15,7 @@ namespace act {
 using namespace ops;
 
 constexpr int kKinds = 3;
+constexpr char kWhich[] = "hidden_act must be 0 (ReLU), 1 (GELU) or 2 (SiLU)";
 
 struct Args {
     const void* z;

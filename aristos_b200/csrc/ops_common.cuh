@@ -120,6 +120,8 @@ inline size_t bytes_of(int torch_dtype) { return torch_dtype == 0 ? 4 : 2; }
 inline bool known_type(int torch_dtype) { return torch_dtype == 0 || torch_dtype == 2 || torch_dtype == 3; }
 constexpr int kMostRows = 0x7fff0000;  // launches count rows in ints, and round them up to whole blocks
 constexpr char kTypes[] = "torch_dtype must be 0 (float), 2 (bf16) or 3 (fp16)";
+constexpr char kNull[] = "null device pointer";
+constexpr char kNoDevice[] = "no current CUDA device";
 constexpr char kWhole[] = "a device pointer is no multiple of its element's size";
 constexpr long long kWaitCycles = 20000000000LL;  // about ten seconds: nothing but a copy or an MMA is waited for
 

@@ -5,7 +5,8 @@
 //
 //   f: 0 ReLU max(z, 0), 1 GELU z N(z) with N the normal distribution's sum, 2 SiLU z s(z) with s(z) = 1 / (1 + e^-z)
 //
-// Each element is read once and each result written once, in 32 bits with one rounding: bound by HBM.
+// Each element is read once and each result written once, in 32 bits with one rounding: bound by HBM (16384 rows, I = 2048, gated, bf16: 29.7 us
+// forward, 49.0 backward, 6.8 TB/s); rows that are loaded an element at a time by issue (2943 x 1087 floats, GELU: 14 and 16).
 #pragma once
 
 #include "ops_common.cuh"

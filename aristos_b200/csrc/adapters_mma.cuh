@@ -11,6 +11,11 @@
 // Where the summed direction is not the contiguous one (both products of the backward pass, the gradients' rows), 8 x 8 blocks change rows
 // and columns between lanes on their way (movmatrix); nothing is transposed in memory.
 //
+// What bounds them, alone: few rows latency (one row, N = K = 2048, rank 16: 5 us; 128 requests of a row each 11); prompts latency of loads
+// (7919 rows, N = 2880, K = 1088, rank 32, fp16: 44 us, 104 MB of HBM); many rows of a large rank shared memory, which the tensor cores' operands
+// cross four times (16384 rows, N = K = 4096, rank 64: 120 us forward and for dx, 402 MB each), and instructions beside it (gradients 93 us each for
+// 134 MB: the adapter with the most rows sets the time).
+//
 // u and v are factors of the second products as values of the element type: rounded once, as a projection's own input would be (both parts of
 // them would double those products' time on the tensor cores and halve the rounding error of a result).  fp16 has too little range for that:
 // a row is divided by a power of two first (in the gradients: all rows, by the largest so far).
@@ -96,6 +101,26 @@ __global__ void __launch_bounds__(256, RT == 64 && TR == 64 ? 1 : 2) rows_mma_ke
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) d[m][j][i] = 0.f;
+    // The matrix unit cuts its running sums off instead of rounding them, and u is a 32-bit result: every kWhole steps of 64 elements a warp's sums are
+    // added to those that it has in shared memory (columns of tile j in their own order; backward: as they were dealt).
+    constexpr int kWhole = 4;
+    bool begun = false;
+    auto put = [&] {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int col = !kBack ? j * 8 + t * 2 : RT == 16 ? t * 4 + j * 2 : j / 4 * 32 + t * 8 + j % 4 * 2;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float2* to = reinterpret_cast<float2*>(part + (ks * TR + (rg * MT + m) * 16 + h * 8 + quad) * S::kPitch + col);
+                    const float2 before = begun ? *to : make_float2(0.f, 0.f);
+                    *to = make_float2(before.x + d[m][j][2 * h], before.y + d[m][j][2 * h + 1]);
+                    d[m][j][2 * h] = d[m][j][2 * h + 1] = 0.f;
+                }
+            }
+        begun = true;
+    };
     // 32 elements at a time, two of those next to each other
     const int pieces = (a.len + 31) / 32, next = 2 * KS * blocks;
     const uint4 zero = make_uint4(0, 0, 0, 0);
@@ -112,6 +137,7 @@ __global__ void __launch_bounds__(256, RT == 64 && TR == 64 ? 1 : 2) rows_mma_ke
         uint4 x[2][MT][2];
         load_in(first, x[0]);
         load_in(first + 1, x[1]);
+        int taken = 0;
         for (int p0 = first; p0 < pieces; p0 += next) {
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
@@ -163,18 +189,10 @@ __global__ void __launch_bounds__(256, RT == 64 && TR == 64 ? 1 : 2) rows_mma_ke
                 }
                 load_in(p0 + next + half, x[half]);
             }
+            if (++taken % kWhole == 0) put();
         }
     }
-    // the warps' sums meet: columns of tile j in their own order (backward: as they were dealt)
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int col = !kBack ? j * 8 + t * 2 : RT == 16 ? t * 4 + j * 2 : j / 4 * 32 + t * 8 + j % 4 * 2;
-            float* to = part + (ks * TR + (rg * MT + m) * 16 + quad) * S::kPitch + col;
-            *reinterpret_cast<float2*>(to) = make_float2(d[m][j][0], d[m][j][1]);
-            *reinterpret_cast<float2*>(to + 8 * S::kPitch) = make_float2(d[m][j][2], d[m][j][3]);
-        }
+    put();  // the warps' sums meet
     __syncthreads();
     if (KS > 1 || kBack) {
         for (int i = threadIdx.x; i < n * RT; i += 256) {
@@ -460,7 +478,18 @@ __global__ void __launch_bounds__(kPipeThreads, 2) rows_pipe_kernel(Args a) {
         for (int j = 0; j < NT1; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) d[m][j][i] = 0.f;
+    float whole[MT][NT1][4] = {};  // as above: what the accumulators have had for kWhole steps is added up in registers
+    constexpr int kWhole = 4;
+    auto add_up = [&] {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < NT1; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) whole[m][j][i] += d[m][j][i], d[m][j][i] = 0.f;
+    };
     for (int step = 0; step < steps1; ++step) {
+        if (step % kWhole == 0) add_up();
         const uint32_t from = next();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -482,6 +511,7 @@ __global__ void __launch_bounds__(kPipeThreads, 2) rows_pipe_kernel(Args a) {
             }
         }
     }
+    add_up();
     float* sums = reinterpret_cast<float*>(memory + S::kSums);
     T* factors = reinterpret_cast<T*>(memory + S::kFactors);
     for (int part = 0; part < 2; ++part) {  // one half of the sums, and the other onto it
@@ -494,7 +524,7 @@ __global__ void __launch_bounds__(kPipeThreads, 2) rows_pipe_kernel(Args a) {
                     for (int h = 0; h < 2; ++h) {
                         float2* to = reinterpret_cast<float2*>(sums + ((rg * MT + m) * 16 + h * 8 + quad) * S::kSumPitch + (half * NT1 + j) * 8 + t * 2);
                         const float2 before = part ? *to : make_float2(0.f, 0.f);
-                        *to = make_float2(before.x + d[m][j][2 * h], before.y + d[m][j][2 * h + 1]);
+                        *to = make_float2(before.x + whole[m][j][2 * h], before.y + whole[m][j][2 * h + 1]);
                     }
         __syncthreads();
     }

@@ -1,21 +1,28 @@
-// The experts of a few tokens (moe_tokens.cuh) where rows begin on 16-byte boundaries: the chosen experts' weights are streamed once.
+// The experts of a few tokens (moe_tokens.cuh): the chosen experts' weights are streamed once.
 //
 //   stream_kernel<kUp>    h of every place, the second factor of a gated expert in the same pass
 //   stream_kernel<kDown>  out, all experts' shares of a column added up by the block that owns it
 //
-// One block a multiprocessor owns a share of the columns of EVERY expert, so the work is even however the tokens were sent, each sum is
-// finished where it began, and nothing is joined between blocks (where that would be too few columns at once, two to eight blocks share
-// columns and deal the experts among them: 23 tokens of 98 experts, I = 256, floats 291 -> SPREAD us).  Its eight warps are teams that take the experts in turn; each warp of
-// a team goes through its own 128 or 256 bytes of the weights' rows, and of the rows they are multiplied with, by 16-byte copies to
-// shared memory that are two or three steps ahead, across experts (copies of whole rows by the bulk engine took 90 cycles each of the
-// warp that issued them: 1480 us instead of 383 for 128 tokens).  A step is multiplied on the tensor cores (warp_mma.cuh), weights on the
-// instruction's 16 rows, up to 32 rows of an expert on its columns; floats by 32-bit multiply-adds, which up to 16 rows an expert are
-// fewer than the splitting that the tensor cores would want.  A team's partial sums meet in shared memory once an expert and tile.
+// One block a multiprocessor owns a share of the columns of EVERY expert, so the work is even however the tokens were sent and each sum is
+// finished where it began.  Where that would be too few columns at once, two to eight blocks share columns and deal the experts among them (kDown:
+// a cluster, which adds its results up; 23 tokens, 8 of 128 experts, H = 1280, I = 256, floats: 291 -> 139 us).  A block's eight warps are teams
+// that take the experts in turn; each warp of a team goes through its own 128 or 256 bytes of the weights' rows, and of the rows they are
+// multiplied with, by 16-byte copies to shared memory that are two or three steps ahead, across experts.  A step is multiplied on the tensor cores
+// (warp_mma.cuh), weights on the instruction's 16 rows, up to 32 rows of an expert on its columns; floats by 32-bit multiply-adds, which up to 16
+// rows an expert are fewer than the splitting that the tensor cores would want.  A team's partial sums meet in shared memory once an
+// expert and tile of columns.  (Copies of whole rows by the bulk engine took 90 cycles each of the warp that issued them: 1480 us for 128
+// tokens instead of 383 at that stage.)
 //
-// h goes from one kernel to the other rounded to the element type, as in the library's other layer.
+// h goes from one kernel to the other rounded to the element type, as in the library's other layer: a second value for what that leaves would
+// halve the rounding error of a result (2-norm 0.0024 to 0.0017, bf16) and read h twice.
 //
-// The second kernel's first weights are on their way before the first kernel has ended (common.cuh: which experts those are was
-// written by the kernel before both).
+// The second kernel's first weights are on their way before the first kernel has ended: which experts those are was written by the kernel
+// before both, and no kernel lets its successor begin before it has waited for its predecessor (common.cuh).
+//
+// Bound by HBM where rows are long and experts many: alone, kUp of 128 tokens (64 gated experts, H = I = 2048, bf16, 1.07 GB) 177 us = 6.0 TB/s,
+// 16 tokens of the large FFN (2.8 GB, both kernels) 427 us = 6.5 TB/s; by issue and latency where a block's share of an expert is small: kDown of
+// those 128 tokens (0.54 GB, 28 rows of 4 KB at a time) 107 us, 37 tokens with H = 1088, I = 2880 (135 MB each) 56 and 66.  One token: 22 us for all
+// three launches, of which the weights take 8 and an empty layer 12.
 #pragma once
 
 #include <cuda.h>

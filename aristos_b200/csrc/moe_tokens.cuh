@@ -5,7 +5,8 @@
 //   out = sum over k of w_k (W2[e_k] h_k + b2[e_k]),   h_k = f(z) or, gated, f(z) z',   z (and z') = W1[e_k] x + b1[e_k]
 //
 // Three launches: gate_kernel chooses, stream_kernel (moe_stream.cuh) makes h and then out.  A call reads the chosen experts' weights
-// once and little else: bound by HBM, and by latency for one token.
+// once and little else: bound by HBM, and by latency for one token.  The router is latency too: 8 us for one token alone, 14 for 128 (64 experts,
+// H = 2048; with rows straight from memory 12 and 28, in 64-bit arithmetic 14 and 43).
 //
 // The logits are sums of 46 bits: which expert is chosen does not hang on the order of a sum.  An expert whose logit is
 // minus infinity is never chosen: the place keeps -1 and a weight of 0, and a token all of whose experts are out gives zeros.

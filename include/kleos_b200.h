@@ -349,7 +349,8 @@ int kleos_activation_backward(const void* dh, long long lddh, const void* z, lon
  * x [T, H] and out [T, H] with row strides, gate [E, H], gate_bias [E] floats or NULL, W1 [E, I, H] (gated [E, 2 I, H]) and W2 [E, H, I]
  * as the products above take them, b1 and b2 or NULL; T from 0 to 128, K from 1 to 8.
  * topk [T, K] and weights [T, K] are written; with gate NULL they are what the caller's own router chose and are read: an id outside
- * 0 .. E - 1 is a place without an expert, and an expert may be named twice.  Logits are 64-bit sums of the elements.  An expert
+ * 0 .. E - 1 is a place without an expert, and an expert may be named twice.  Logits are exact to about 2^-46, h is rounded to
+ * torch_dtype between the products, everything else is 32 bits and one rounding.  An expert
  * whose logit is minus infinity (a gate_bias that takes it out of service) is never chosen: its place has topk -1 and weight 0, and a
  * token without any expert has zeros.  NaN counts as the largest logit and makes its token's weights and results NaN.
  * The workspace (16-byte aligned, kleos_moe_tokens_workspace(T, I, K) bytes, contents of no matter) belongs to the call while it runs:
@@ -364,7 +365,9 @@ int kleos_moe_tokens(const void* x, long long ldx, const void* gate, const float
  *   u = x A[l]^T,   y = base + scale[l] u B[l]^T
  * x [rows, K], base and y [rows, N], A [L, r, K], B [L, N, r], scale [L] floats or NULL for ones, u [rows, r] floats for the backward
  * pass, or NULL.  base (what the shared projection gave) may be y itself, or NULL for zeros.  offsets [R + 1] is ascending; rows before the
- * first request or behind the last, and those of requests whose adapter is outside 0 .. L - 1, have y = base and u = 0.
+ * first request or behind the last, and those of requests whose adapter is outside 0 .. L - 1, have y = base and u = 0.  On the tensor
+ * cores (16-bit rows on 16-byte boundaries, r a multiple of 8, or of 4 up to 16) u, and v below, enter the second products rounded to
+ * torch_dtype, fp16 after a division by a power of two that keeps them in its range.
  * R from 1 to 65536, L from 1 to 65535, r from 1 to 128. */
 int kleos_adapter_products(const void* x, long long ldx, const int32_t* offsets, const int32_t* adapter, const void* a, const void* b,
                            const float* scale, const void* base, long long ldb, int rows, int R, int L, int r, int N, int K,

@@ -229,3 +229,18 @@ def test_offsets_that_say_too_much():
     c.offsets.copy_(torch.tensor([-5, 30, 10 ** 9], dtype=torch.int32))
     c.of = torch.tensor([1] * 30 + [0] * 33, device="cuda")
     c.all().verify()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("lengths", [[1] * 20, [300, 200], [12000, 9000]])
+def test_long_sums(lengths, dtype):
+    """u is a 32-bit result: the matrix unit's running sums, which it cuts off (up to about 2^-27 of the sum of magnitudes a term), are
+    of at most 256 terms each, and of a warp's share of 8192 that are added up in 32 bits: 2^-19 of terms of one sign at worst."""
+    c = Case(lengths, [i % 2 for i in range(len(lengths))], 2, 16, 64, 8192, dtype)
+    c.x.copy_(c.x.abs())
+    c.a.copy_(c.a.abs())
+    c.forward()
+    for l in range(2):
+        mine = c.of == l
+        want = c.x[mine].double() @ c.a[l].double().t()
+        assert float(((c.u[mine].double() - want) / want).abs().max()) <= 2.0 ** -19

@@ -242,10 +242,13 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
 }
 
 // ---------------------------------------------------------------- gradients of the adapters
+// One of the two, or none (no strips).  Both are one launch where one kernel takes both.
 struct Grads {
     const void* in;      // x, or dy
     const float* c;      // v, or u
     void* out;           // dA [L, r, cols], or dB [L, cols, r]
+    bool db;             // which
+    int strips;          // of columns, a cluster each
     const int *offsets, *adapter;
     const float* scale;  // null: ones (dA: v has it already)
     long long ldi;
@@ -253,10 +256,10 @@ struct Grads {
     bool wide_out;       // results are floats
 };
 
-// dA (kDb false) or dB: a cluster takes 32 columns and 16 ranks of one adapter; its blocks take 64 rows of a request in turn, whose factors
+// dA and dB: a cluster takes 32 columns and 16 ranks of one adapter; its blocks take 64 rows of a request in turn, whose factors
 // are in shared memory, and a warp every eighth of those.
-template <typename T, bool kDb>
-__global__ void __launch_bounds__(256) grads_kernel(Grads a) {
+template <typename T>
+__global__ void __launch_bounds__(256) grads_kernel(Grads first_of_two, Grads second_of_two) {
     namespace cg = cooperative_groups;
     constexpr int J = 16, kRows = 64, kMine = kRows / 8;
     cg::cluster_group cluster = cg::this_cluster();
@@ -266,8 +269,11 @@ __global__ void __launch_bounds__(256) grads_kernel(Grads a) {
     const int blocks = (int)cluster.num_blocks(), block = (int)cluster.block_rank();
     pdl_wait();
     pdl_trigger();
+    const int strip = blockIdx.x / blocks;
+    const bool second = strip >= first_of_two.strips;
+    const Grads a = second ? second_of_two : first_of_two;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = blockIdx.y, j0 = blockIdx.z * J, n = min(J, a.r - j0);
-    const int first = blockIdx.x / blocks * 32, col = first + lane;
+    const int first = (strip - (second ? first_of_two.strips : 0)) * 32, col = first + lane;
     const bool there = col < a.cols;
     const T* in = static_cast<const T*>(a.in) + (there ? col : 0);
     float s[J];
@@ -319,11 +325,11 @@ __global__ void __launch_bounds__(256) grads_kernel(Grads a) {
     if (blocks > 1) cluster.sync();
     else __syncthreads();
     for (int i = block * 256 + threadIdx.x; i < n * 32; i += blocks * 256) {
-        const int j = kDb ? i % n : i / 32, cc = kDb ? i / n : i % 32;
+        const int j = a.db ? i % n : i / 32, cc = a.db ? i / n : i % 32;
         if (first + cc >= a.cols) continue;
         float v = 0.f;
         for (int k = 0; k < blocks; ++k) v += *cluster.map_shared_rank(&sums[j][cc], k);
-        const size_t at = kDb ? ((size_t)l * a.cols + first + cc) * a.r + j0 + j : ((size_t)l * a.r + j0 + j) * a.cols + first + cc;
+        const size_t at = a.db ? ((size_t)l * a.cols + first + cc) * a.r + j0 + j : ((size_t)l * a.r + j0 + j) * a.cols + first + cc;
         if (a.wide_out) static_cast<float*>(a.out)[at] = v;
         else static_cast<T*>(a.out)[at] = Elem<T>::from_f(v);
     }

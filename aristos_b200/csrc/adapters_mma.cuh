@@ -624,8 +624,8 @@ struct GradShape {
 
 // RT: columns of c (u or v) from blockIdx.z * RT on.  The cluster's blocks take kGradRows rows of a request in turn; both factors come through a
 // ring in shared memory, c a step before it is needed, when it is rounded to a factor of the products.
-template <typename T, bool kDb, int RT>
-__global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads a) {
+template <typename T, int RT>
+__global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, Grads second_of_two) {
     namespace cg = cooperative_groups;
     using S = GradShape<T, RT>;
     constexpr int MT = RT / 16;
@@ -635,7 +635,10 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads a) {
     cg::cluster_group cluster = cg::this_cluster();
     const int blocks = (int)cluster.num_blocks(), block = (int)cluster.block_rank();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, t = lane & 3;
-    const int l = blockIdx.y, j0 = blockIdx.z * RT, c0 = (int)(blockIdx.x / blocks) * kGradColumns;
+    const int strip = blockIdx.x / blocks;
+    const bool second = strip >= first_of_two.strips;
+    const Grads a = second ? second_of_two : first_of_two;
+    const int l = blockIdx.y, j0 = blockIdx.z * RT, c0 = (strip - (second ? first_of_two.strips : 0)) * kGradColumns;
     pdl_wait();
     pdl_trigger();
     float s[MT][4][4];
@@ -805,7 +808,7 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads a) {
     T* const out = static_cast<T*>(a.out);
     float* const wide_out = static_cast<float*>(a.out);
     auto store = [&](int j, int col, float v) {
-        const size_t to = kDb ? ((size_t)l * a.cols + c0 + first + col) * a.r + j0 + j : ((size_t)l * a.r + j0 + j) * a.cols + c0 + first + col;
+        const size_t to = a.db ? ((size_t)l * a.cols + c0 + first + col) * a.r + j0 + j : ((size_t)l * a.r + j0 + j) * a.cols + c0 + first + col;
         if (a.wide_out) wide_out[to] = v;
         else out[to] = Elem<T>::from_f(v);
     };
@@ -816,10 +819,10 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads a) {
         if (blocks == 1) v = *at;
         else
             for (int k = 0; k < blocks; ++k) v += *cluster.map_shared_rank(at, k);
-        if (kDb) *at = v;  // (nobody else reads this block's share of its own sums but itself)
+        if (a.db) *at = v;  // (nobody else reads this block's share of its own sums but itself)
         else if (col < columns) store(j, col, v);
     }
-    if constexpr (kDb) {
+    if (a.db) {
         __syncthreads();
         for (int i = threadIdx.x; i < width * columns; i += 256) store(i % width, i / width, sums[i % width * kPitch + first + i / width]);
     }

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "activation.cuh"
 #include "adapters.cuh"
@@ -125,27 +126,45 @@ cudaError_t adapter_rows(const adapters::Args& a, cudaStream_t st) {
     return launch(kernel, dim3((unsigned)(tiles * cluster)), 256, 0, cluster, st, a);
 }
 
-template <typename T, bool kDb>
-cudaError_t adapter_grads(const adapters::Grads& a, cudaStream_t st) {
+// Blocks of a cluster that share the rows of an adapter: until so many blocks a multiprocessor are there, while each has `rows` of them on average.
+int grads_cluster(long long groups, long long blocks, long long all, long long rows) {
+    int cluster = 1;
+    while (cluster < 8 && 2 * groups * cluster <= blocks * sm_count() && all > cluster * rows) cluster *= 2;
+    return cluster;
+}
+
+// One or both of them (no strips: not).
+template <typename T>
+cudaError_t adapter_grads(adapters::Grads a, adapters::Grads b, cudaStream_t st) {
     using namespace adapters;
+    auto tensor = [](const Grads& g) { return !g.out || (sizeof(T) == 2 && g.r % 2 == 0 && by_16(2, {g.in}, {g.ldi, g.cols}) && aligned(g.c, 8)); };
+    if (a.out && b.out && tensor(a) != tensor(b)) {
+        const cudaError_t rc = adapter_grads<T>(a, Grads{}, st);
+        return rc == cudaSuccess ? adapter_grads<T>(b, Grads{}, st) : rc;
+    }
+    if (!a.out) std::swap(a, b);
+    if (!a.out) return cudaSuccess;
+    auto cut = [&](int columns) {
+        a.strips = (a.cols + columns - 1) / columns;
+        b.strips = b.out ? (b.cols + columns - 1) / columns : 0;
+        return (long long)a.strips + b.strips;
+    };
     if constexpr (sizeof(T) == 2) {
-        if (a.r % 2 == 0 && by_16(2, {a.in}, {a.ldi, a.cols}) && aligned(a.c, 8))
+        if (tensor(a))
             return with_rank(std::min(a.r, 64), [&](auto rt) {
-                constexpr int RT = decltype(rt)::value, kBytes = GradShape<T, RT>::kBytes;
-                const auto kernel = grads_mma_kernel<T, kDb, RT>;
-                const long long strips = (a.cols + kGradColumns - 1) / kGradColumns, groups = strips * a.L * ((a.r + RT - 1) / RT);
-                int cluster = 1;
-                while (cluster < 8 && 2 * groups * cluster <= 2LL * sm_count() && a.rows > cluster * kGradRows * 4LL) cluster *= 2;
+                constexpr int RT = decltype(rt)::value <= 64 ? decltype(rt)::value : 64, kBytes = GradShape<T, RT>::kBytes;
+                const auto kernel = grads_mma_kernel<T, RT>;
+                const long long strips = cut(kGradColumns), parts = (a.r + RT - 1) / RT;
+                const int cluster = grads_cluster(strips * a.L * parts, 4, a.rows, kGradRows * 4LL);
                 static bool allowed[64];
                 cudaError_t rc = allow_smem(kernel, allowed, kBytes);
-                if (rc == cudaSuccess) rc = launch(kernel, dim3((unsigned)(strips * cluster), a.L, (a.r + RT - 1) / RT), 256, kBytes, cluster, st, a);
+                if (rc == cudaSuccess) rc = launch(kernel, dim3((unsigned)(strips * cluster), a.L, (unsigned)parts), 256, kBytes, cluster, st, a, b);
                 return rc;
             });
     }
-    const long long strips = (a.cols + 31) / 32, groups = strips * a.L * ((a.r + 15) / 16);
-    int cluster = 1;
-    while (cluster < 8 && 2 * groups * cluster <= 6LL * sm_count() && a.rows > cluster * 256) cluster *= 2;
-    return launch(grads_kernel<T, kDb>, dim3((unsigned)(strips * cluster), a.L, (a.r + 15) / 16), 256, 0, cluster, st, a);
+    const long long strips = cut(32), parts = (a.r + 15) / 16;
+    const int cluster = grads_cluster(strips * a.L * parts, 6, a.rows, 256);
+    return launch(grads_kernel<T>, dim3((unsigned)(strips * cluster), a.L, (unsigned)parts), 256, 0, cluster, st, a, b);
 }
 
 }  // namespace
@@ -234,16 +253,12 @@ int kleos_adapter_products_backward(const void* dy, long long lddy, const void* 
             g.adapter = adapter; g.scale = scale; g.ldi = lddy; g.ldb = ldb; g.ldo = lddx; g.rows = rows; g.R = R; g.L = L; g.r = r; g.len = N; g.cols = K;
             rc = adapter_rows<T, true>(g, st);
         }
-        adapters::Grads g{};
-        g.offsets = offsets; g.adapter = adapter; g.rows = rows; g.R = R; g.L = L; g.r = r; g.wide_out = grad_dtype == 0;
-        if (rc == cudaSuccess && da) {
-            g.in = x; g.c = static_cast<const float*>(workspace); g.out = da; g.ldi = ldx; g.cols = K;
-            rc = adapter_grads<T, false>(g, st);
-        }
-        if (rc == cudaSuccess && db) {
-            g.in = dy; g.c = u; g.out = db; g.scale = scale; g.ldi = lddy; g.cols = N;
-            rc = adapter_grads<T, true>(g, st);
-        }
+        adapters::Grads ga{}, gb{};
+        ga.offsets = offsets; ga.adapter = adapter; ga.rows = rows; ga.R = R; ga.L = L; ga.r = r; ga.wide_out = grad_dtype == 0;
+        gb = ga;
+        ga.in = x; ga.c = static_cast<const float*>(workspace); ga.out = da; ga.ldi = ldx; ga.cols = K;
+        gb.in = dy; gb.c = u; gb.out = db; gb.db = true; gb.scale = scale; gb.ldi = lddy; gb.cols = N;
+        if (rc == cudaSuccess) rc = adapter_grads<T>(ga, gb, st);
         return finish(call, rc);
     });
 }

@@ -37,6 +37,7 @@ struct Args {
     const float* scale;  // null: ones
     long long ldi, ldb, ldo;
     int rows, R, L, r, len, cols;  // len of `in`, columns of `out`
+    bool quads;                    // whether the adapters' elements can be read four at a time along the rank
 };
 
 struct Tile {
@@ -176,14 +177,25 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
             Vec<T, V> w[J], x[MW];
 #pragma unroll
             for (int m = 0; m < MW; ++m) x[m] = load_vec<T, V>(in[m] + k);
+            if (kBack && a.quads) {
 #pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const int jj = min(j0 + j, a.r - 1);
-                if constexpr (!kBack) {
-                    w[j] = load_vec<T, V>(p + (size_t)jj * a.len + k);
-                } else {
+                for (int j = 0; j < J; j += 4)
 #pragma unroll
-                    for (int v = 0; v < V; ++v) w[j].v[v] = p[(size_t)(k + v) * a.r + jj];
+                    for (int v = 0; v < V; ++v) {
+                        const Vec<T, 4> l = load_vec<T, 4>(p + (size_t)(k + v) * a.r + min(j0 + j, a.r - 4));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[j + i].v[v] = l.v[i];
+                    }
+            } else {
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    const int jj = min(j0 + j, a.r - 1);
+                    if constexpr (!kBack) {
+                        w[j] = load_vec<T, V>(p + (size_t)jj * a.len + k);
+                    } else {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) w[j].v[v] = p[(size_t)(k + v) * a.r + jj];
+                    }
                 }
             }
 #pragma unroll
@@ -229,6 +241,16 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
             s[m] = 0.f;
             before[m] = base && m < n ? Elem<T>::to_f(base[(long long)(t.begin + m) * a.ldb + c]) : 0.f;
         }
+        if (!kBack && a.quads) {
+#pragma unroll 4
+            for (int j = 0; j < a.r; j += 4) {
+                const Vec<T, 4> l = load_vec<T, 4>(q + (size_t)c * a.r + j);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int m = 0; m < M; ++m) s[m] = fmaf(u[m][j + i], Elem<T>::to_f(l.v[i]), s[m]);
+            }
+        } else
 #pragma unroll 8
         for (int j = 0; j < a.r; ++j) {
             const float w = Elem<T>::to_f(kBack ? q[(size_t)j * a.cols + c] : q[(size_t)c * a.r + j]);

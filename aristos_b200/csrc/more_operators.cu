@@ -123,7 +123,9 @@ cudaError_t adapter_rows(const adapters::Args& a, cudaStream_t st) {
     if (tiles * cluster > 0x7fffffff) return cudaErrorInvalidConfiguration;
     const bool wide = by_16(sizeof(T), {a.in, kBack ? nullptr : a.p}, {a.ldi, a.len});
     const auto kernel = wide ? rows_kernel<T, kBack ? 4 : W, kBack> : rows_kernel<T, 1, kBack>;
-    return launch(kernel, dim3((unsigned)(tiles * cluster)), 256, 0, cluster, st, a);
+    Args g = a;
+    g.quads = a.r % 4 == 0 && aligned(kBack ? a.p : a.q, 4 * sizeof(T));
+    return launch(kernel, dim3((unsigned)(tiles * cluster)), 256, 0, cluster, st, g);
 }
 
 // Blocks of a cluster that share the rows of an adapter: until so many blocks a multiprocessor are there, while each has `rows` of them on average.

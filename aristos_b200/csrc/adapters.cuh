@@ -11,7 +11,7 @@
 // A cluster of blocks takes some rows of a request: it shares the sums of u (of v), meets, and shares the columns of y
 // (of dx), so that u never leaves the chip between the two products.  Both passes over rows are one kernel: what differs is the
 // direction in which the adapters are read.  The kernels here take any element type and alignment, on the FP32 pipes, and are bound by
-// issue and latency (2943 rows, N = 1087, K = 1090, rank 12, floats: 49 us each way, gradients 27 each); those of adapters_mma.cuh take 16-bit rows on
+// issue and latency (2943 rows, N = 1087, K = 1090, rank 12, floats: 46 us each way, both gradients 35); those of adapters_mma.cuh take 16-bit rows on
 // 16-byte boundaries.
 #pragma once
 

@@ -13,8 +13,8 @@
 //
 // What bounds them, alone: few rows latency (one row, N = K = 2048, rank 16: 5 us; 128 requests of a row each 11); prompts latency of loads
 // (7919 rows, N = 2880, K = 1088, rank 32, fp16: 44 us, 104 MB of HBM); many rows of a large rank shared memory, which the tensor cores' operands
-// cross four times (16384 rows, N = K = 4096, rank 64: 120 us forward and for dx, 402 MB each), and instructions beside it (gradients 93 us each for
-// 134 MB: the adapter with the most rows sets the time).
+// cross four times (16384 rows, N = K = 4096, rank 64: 120 us forward and for dx, 402 MB each), and instructions beside it (both gradients 148 us for
+// 278 MB: the adapter with the most rows sets the time).
 //
 // u and v are factors of the second products as values of the element type: rounded once, as a projection's own input would be (both parts of
 // them would double those products' time on the tensor cores and halve the rounding error of a result).  fp16 has too little range for that:

@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
 
     // Copies: 8 lanes a line, 16 bytes each.  In odd rows the halves of a line change places: eight rows of 64 bytes are read without two of
     // them on one bank.
-    const int line = kUnit == 16 ? lane >> 3 : 0, sub = lane & 7, my_byte = part * kRowBytes + (kUnit == 16 ? sub * 16 : lane * kUnit);
+    const int line = kUnit == 16 ? lane >> 3 : 0, sub = lane & 7, my_byte = part * kRowBytes + (kUnit == 16 ? sub * 16 : lane * 4);
     const size_t next_set = (size_t)(kGated ? a.I : kTileColumns) * row_bytes;
     const uint32_t to_lane = tc::smem_u32(mine) + line * kRowBytes + ((sub ^ (line & 1) * 4) * 16);
     const char* const w_all = static_cast<const char*>(kIsDown ? a.w2 : a.w1);
@@ -258,34 +258,17 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
         }
         find();
     };
-    // Rows that do not begin on 16 bytes: a line at a time, each lane 4 bytes of it, or 2 and 2 by way of a register, sixteen lines on their way.
+    // Rows that do not begin on 16 bytes: a line at a time, each lane 4 bytes of it.  Where they do not begin on 4 either, by way of registers: a
+    // step's elements are loaded before the step at hand is multiplied and stored after it.
     const uint32_t mine_at = tc::smem_u32(mine);
-    auto place_of = [&](int row, int byte) { return mine_at + row * kRowBytes + (byte ^ (row & 1) * 64); };
-    auto copy_units = [&](int slot, bool take_weights, bool take_rows) {
+    auto place_of = [&](int row, int l) { return mine_at + row * kRowBytes + l * kLine + (lane * 4 ^ (row & 1) * 64); };
+    auto copy_words = [&](int slot, bool take_weights, bool take_rows) {
         const uint32_t at = slot * c.slot;
 #pragma unroll 1
         for (int l = 0; l < kLines; ++l) {
-            const int here = byte + l * kLine;  // this lane's byte of a row
+            const bool there = byte + l * kLine < row_bytes;
             auto lines = [&](int row0, int rows, auto from_of) {
-#pragma unroll 1
-                for (int r0 = 0; r0 < rows; r0 += 16) {
-                    if constexpr (kUnit == 4) {
-                        const bool there = here < row_bytes;
-                        for (int r = r0; r < min(rows, r0 + 16); ++r) copy_4(at + l * kLine + place_of(row0 + r, lane * 4), there ? from_of(r) + l * kLine : w_all, there);
-                    } else {
-                        uint16_t v[16][2];
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-#pragma unroll
-                            for (int k = 0; k < 2; ++k)
-                                v[r][k] = r0 + r < rows && here + k * 64 < row_bytes ? *reinterpret_cast<const uint16_t*>(from_of(r0 + r) + l * kLine + k * 64) : (uint16_t)0;
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-#pragma unroll
-                            for (int k = 0; k < 2; ++k)
-                                if (r0 + r < rows) asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + l * kLine + place_of(row0 + r0 + r, lane * 2 + k * 64)), "h"(v[r][k]) : "memory");
-                    }
-                }
+                for (int r = 0; r < rows; ++r) copy_4(at + place_of(row0 + r, l), there ? from_of(r) + l * kLine : w_all, there);
             };
             if (take_weights)
                 for (int m = 0; m < kSets; ++m)
@@ -293,9 +276,45 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
             if (take_rows) lines(kSets * kTileColumns, ahead.n, [&](int r) { return x_all + x_of[ahead.p0 + r] * x_row + byte; });
         }
     };
+    constexpr int kHeldRows = (kSets + 1) * kTileColumns;
+    uint16_t held[kUnit == 2 ? kLines * kHeldRows : 1][2];
+    int held_slot = -1, held_w = 0, held_n = 0;
+    bool held_weights = false, held_rows = false;
+    auto row_is_held = [&](int i) {  // row i of a slot
+        if (i >= kSets * kTileColumns) return held_rows && i - kSets * kTileColumns < held_n;
+        return held_weights && (kGated ? i % kTileColumns : i) < held_w;
+    };
+    auto fetch = [&](int slot, bool take_weights, bool take_rows) {
+        held_slot = slot, held_w = ahead.w, held_n = ahead.n, held_weights = take_weights, held_rows = take_rows;
+#pragma unroll
+        for (int l = 0; l < kLines; ++l)
+#pragma unroll
+            for (int i = 0; i < kHeldRows; ++i) {
+                const int here = byte + l * kLine, m = i / kTileColumns, r = i % kTileColumns;
+                const char* from = w_all;
+                if (row_is_held(i)) from = (m < kSets ? weights + (m ? next_set : 0) + (size_t)r * row_bytes : x_all + x_of[ahead.p0 + r] * x_row + byte) + l * kLine;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) held[l * kHeldRows + i][k] = row_is_held(i) && here + 2 * k < row_bytes ? reinterpret_cast<const uint16_t*>(from)[k] : (uint16_t)0;
+            }
+    };
+    auto stash = [&] {
+        if (held_slot < 0) return;
+#pragma unroll
+        for (int l = 0; l < kLines; ++l)
+#pragma unroll
+            for (int i = 0; i < kHeldRows; ++i)
+                if (row_is_held(i))
+                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(held_slot * c.slot + place_of(i, l)), "r"((uint32_t)held[l * kHeldRows + i][0] | (uint32_t)held[l * kHeldRows + i][1] << 16) : "memory");
+        held_slot = -1;
+    };
     // (a row may end inside a step: there the copies are of zeros.  A line ends in one too, or is whole: 128 bytes are eight lanes' 16.)
     auto copy = [&](int slot, bool take_weights, bool take_rows) {
-        if constexpr (kUnit < 16) return copy_units(slot, take_weights, take_rows);
+        if constexpr (kUnit == 4) return copy_words(slot, take_weights, take_rows);
+        if constexpr (kUnit == 2) {
+            stash();
+            fetch(slot, take_weights, take_rows);
+            return;
+        }
         const uint32_t to = to_lane + slot * c.slot;
 #pragma unroll
         for (int l = 0; l < kLines; ++l) {
@@ -352,6 +371,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
         }
         commit();
     }
+    if (kUnit == 2) stash();
 
     int slot = 0, turn = 0;
     const int lane_in_team = part * 32 + lane;
@@ -417,6 +437,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
                                 for (int m = 0; m < kSets; ++m) wm::multiply<T>(s[m][j], q[m], x);
                             }
                         }
+                        if (kUnit == 2) stash();
                         __syncwarp();
                     }
 #pragma unroll

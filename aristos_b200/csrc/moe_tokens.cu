@@ -66,7 +66,8 @@ cudaError_t moe_stream(const tokens::Args& a, cudaStream_t st) {
     }
     // rows of an expert at a time: as many as it has on average and some
     c.rows = std::min(a.T, a.T * a.K > 12 * a.E ? kMostRowsAtOnce : kMostRowsAtOnce / 2);
-    if (sizeof(T) == 4) c.rows = std::min(c.rows, kMode == kUpGated ? 8 : 16);  // (registers)
+    if (sizeof(T) == 4) c.rows = std::min(c.rows, kMode == kUpGated ? 8 : 16);  // (registers, here and next)
+    if (kUnit == 2) c.rows = std::min(c.rows, 16);
     // two sets of 16 columns where that takes fewer tiles (a gated expert's are its halves)
     const bool two = kMode != kUpGated && (sizeof(T) == 2 || c.rows <= 8) && (c.share + 31) / 32 < (c.share + 15) / 16;
     auto cut = [&](int most) {

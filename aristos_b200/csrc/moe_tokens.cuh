@@ -40,7 +40,8 @@ struct Args {
 constexpr int kGateBlocks = 8, kGateWarps = 8, kGateTokens = 4;
 
 // A sum that keeps what its additions round off (two floats at once): the total is exact to about 2^-46.  The multiprocessor's 64-bit
-// additions and conversions would take ten times as long (128 tokens, 64 experts: 41 us).
+// additions and conversions would take ten times as long (128 tokens, 64 experts: 41 us).  Once an infinity is in it, or a product or a
+// sum on the way is past the floats' range, the rest is no number: the kernel adds such a logit up anew in 64 bits.
 struct Kept {
     F2 s, rest;
     __device__ __forceinline__ Kept() : s(both(0.f)), rest(both(0.f)) {}
@@ -55,6 +56,12 @@ struct Kept {
         return ((double)a.x + (double)a.y) + ((double)b.x + (double)b.y);
     }
 };
+
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
 
 // A cluster takes up to kGateTokens tokens: its warps share the experts, its blocks the tokens that are then chosen for.  Rows on 16-byte
 // boundaries (V above 1) come a kilobyte at a time through shared memory, kGateStages steps of it.
@@ -135,9 +142,12 @@ __global__ void __launch_bounds__(32 * kGateWarps) gate_kernel(Args a) {
 #pragma unroll
         for (int t = 0; t < kGateTokens; ++t) {
             if (t >= n) break;
-            double v = s[t].total();
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            double v = warp_sum(s[t].total());
+            if (!isfinite(v)) {  // (of the whole warp alike)
+                v = 0.0;
+                for (int k = lane; k < a.H; k += 32) v += (double)Elem<T>::to_f(w[k]) * (double)Elem<T>::to_f(x[t * a.ldx + k]);
+                v = warp_sum(v);
+            }
             if (lane == 0 && e < a.E) *cluster.map_shared_rank(&logits[e], t) = a.gate_bias ? v + (double)a.gate_bias[e] : v;
         }
     }
@@ -169,9 +179,7 @@ __global__ void __launch_bounds__(32 * kGateWarps) gate_kernel(Args a) {
         if (lane == 0) logits[at] = -INFINITY;
         __syncwarp();
     }
-    double p = id < 0 ? 0.0 : exp(mine - top), sum = p;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const double p = id < 0 ? 0.0 : exp(mine - top), sum = warp_sum(p);
     if (lane < a.K) {
         a.topk[t * a.K + lane] = id;
         a.weights[t * a.K + lane] = id < 0 ? 0.f : (float)(p / sum);

@@ -349,9 +349,10 @@ int kleos_activation_backward(const void* dh, long long lddh, const void* z, lon
  * x [T, H] and out [T, H] with row strides, gate [E, H], gate_bias [E] floats or NULL, W1 [E, I, H] (gated [E, 2 I, H]) and W2 [E, H, I]
  * as the products above take them, b1 and b2 or NULL; T from 0 to 128, K from 1 to 8.
  * topk [T, K] and weights [T, K] are written; with gate NULL they are what the caller's own router chose and are read: an id outside
- * 0 .. E - 1 is a place without an expert, and an expert may be named twice.  Logits are exact to about 2^-46, h is rounded to
+ * 0 .. E - 1 is a place without an expert, and an expert may be named twice.  Logits are exact to about 2^-46 (those with
+ * infinities in them, or past the floats' range on the way, are sums of 64 bits), h is rounded to
  * torch_dtype between the products, everything else is 32 bits and one rounding.  An expert
- * whose logit is minus infinity (a gate_bias that takes it out of service) is never chosen: its place has topk -1 and weight 0, and a
+ * whose logit is minus infinity (a gate_bias that takes it out of service, a gate row, a token) is never chosen: its place has topk -1 and weight 0, and a
  * token without any expert has zeros.  NaN counts as the largest logit and makes its token's weights and results NaN.
  * The workspace (16-byte aligned, kleos_moe_tokens_workspace(T, I, K) bytes, contents of no matter) belongs to the call while it runs:
  * calls that may overlap have one each. */

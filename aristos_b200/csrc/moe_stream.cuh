@@ -14,7 +14,8 @@
 // tokens instead of 383 at that stage.)
 //
 // h goes from one kernel to the other rounded to the element type, as in the library's other layer: a second value for what that leaves would
-// halve the rounding error of a result (2-norm 0.0024 to 0.0017, bf16) and read h twice.
+// halve the rounding error of a result (2-norm 0.0024 to 0.0017, bf16) and read h twice.  A value past fp16's range is kept all the same
+// (PastRange): sums that it made no number are added up anew.
 //
 // The second kernel's first weights are on their way before the first kernel has ended: which experts those are was written by the kernel
 // before both, and no kernel lets its successor begin before it has waited for its predecessor (common.cuh).
@@ -158,6 +159,21 @@ __device__ __forceinline__ Groups group_places(const Args& a, char* memory, Coun
 // teams of eight 383 us, of four 355, of two 346; 37 tokens of 22: 186, 163, 158).
 __host__ __device__ __forceinline__ int team_size(int experts) { return experts >= kTeam2 ? 2 : experts >= kTeam4 ? 4 : 8; }
 
+// An fp16 value of h past the type's range.  In its place stands a number that is none, with the sign and ten bits of the value behind them; sixteen more are
+// as far behind the place as the workspace's first half is long: a float but for its last five bits.
+struct PastRange {
+    uint16_t first, second;
+    static __device__ __forceinline__ bool is(uint16_t v) { return (v & 0x7c00) == 0x7c00; }
+    __device__ __forceinline__ explicit PastRange(float h) {
+        const uint32_t v = ((h != h ? 0x7fc00000u : __float_as_uint(h)) + 16) >> 5;
+        first = (uint16_t)(v >> 26 << 15 | 0x7c00 | (v >> 16 & 0x3ff));
+        second = (uint16_t)v;
+    }
+    static __device__ __forceinline__ float value(uint16_t first, uint16_t second) {
+        return __uint_as_float((uint32_t)(first & 0x8000) << 16 | (uint32_t)(first & 0x3ff) << 21 | (uint32_t)second << 5);
+    }
+};
+
 __device__ __forceinline__ void copy_16(uint32_t to, const void* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
@@ -176,7 +192,7 @@ struct At {
 // may be copied in: 16 or 4, by the asynchronous copies, or 2.  kDepth: steps of a warp in shared memory.
 template <typename T, int kMode, int kLines, int kSets, int kUnit, int kDepth>
 __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
-    constexpr bool kGated = kMode == kUpGated, kIsDown = kMode == kDown, kMma = sizeof(T) == 2;
+    constexpr bool kGated = kMode == kUpGated, kIsDown = kMode == kDown, kMma = sizeof(T) == 2, kHalf = std::is_same<T, __half>::value;
     static_assert(!kGated || kSets == 2, "a set for each half");
     constexpr int kHalves = kGated ? 2 : 1;              // row sets of W1
     constexpr int kNTiles = kMostRowsAtOnce / 8;
@@ -207,6 +223,12 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
     float* const results = behind + 2 * meet_floats(kSets, c.rows);
     float* const sums = results + team * a.T * c.tile;
     auto team_sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(32 * size) : "memory"); };
+    auto team_any = [&](bool mine) {  // meets as well
+        int any;
+        asm volatile("{.reg .pred p, q; setp.ne.s32 p, %3, 0; bar.red.or.pred q, %1, %2, p; selp.s32 %0, 1, 0, q;}" : "=r"(any) : "r"(1 + team), "r"(32 * size), "r"((int)mine) : "memory");
+        return any != 0;
+    };
+    const size_t past = (size_t)a.T * a.K * a.ldh;  // elements to the second parts of h
 
     // Copies: 8 lanes a line, 16 bytes each.  In odd rows the halves of a line change places: eight rows of 64 bytes are read without two of
     // them on one bank.
@@ -405,8 +427,16 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
                     if constexpr (kGated) h *= a.b1 ? z2 + Elem<T>::to_f(b1[a.I]) : z2;
                     T* out = static_cast<T*>(a.h) + (size_t)g.of[p0 + row] * a.ldh + c0 + column;
                     *out = Elem<T>::from_f(h);
+                    if constexpr (kHalf) {
+                        uint16_t* bits = reinterpret_cast<uint16_t*>(out);
+                        if (PastRange::is(__half_as_ushort(Elem<T>::from_f(h)))) {
+                            const PastRange p(h);
+                            bits[0] = p.first, bits[past] = p.second;
+                        }
+                    }
                 };
                 // two buffers in turn, so that a team meets once a sum
+                bool odd = false;  // whether a sum of this lane is no number
                 float* meet = behind + (turn ? meet_floats(kSets, c.rows) : 0) + team * size * 16 * kSets * pitch;
                 turn ^= 1;
                 if constexpr (kMma) {
@@ -449,6 +479,11 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
                             float* to = meet + ((part * kSets + m) * 16 + quad) * pitch + j * 8 + t * 2;
                             *reinterpret_cast<float2*>(to) = make_float2(s[m][j][0], s[m][j][1]);
                             *reinterpret_cast<float2*>(to + 8 * pitch) = make_float2(s[m][j][2], s[m][j][3]);
+                            if constexpr (kIsDown && kHalf) {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (m * 16 + quad + i / 2 * 8 < w && j * 8 + t * 2 + i % 2 < n) odd |= !isfinite(s[m][j][i]);
+                            }
                         }
                 } else {
                     // floats: a lane multiplies its 16 bytes of two rows of each set with the same bytes of every row
@@ -489,13 +524,34 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
                         }
                     }
                 }
-                team_sync();
+                if constexpr (kIsDown && kHalf) odd = team_any(odd);
+                else team_sync();
                 auto sum_of = [&](int column, int row) {
                     const float* from = meet + column * pitch + row;
                     float v = *from;
                     for (int k = 1; k < size; ++k) v += *(from += 16 * kSets * pitch);
                     return v;
                 };
+                if constexpr (kIsDown && kHalf) {
+                    if (odd) {  // a warp a sum
+                        for (int i = part; i < w * n; i += size) {
+                            const int row = i / w, column = i - row * w;
+                            float v = sum_of(column, row);
+                            if (isfinite(v)) continue;
+                            const uint16_t* h = static_cast<const uint16_t*>(a.h) + (size_t)g.of[p0 + row] * a.ldh;
+                            const T* w2 = static_cast<const T*>(a.w2) + ((size_t)e * a.H + c0 + column) * a.I;
+                            v = 0.f;
+#pragma unroll 4
+                            for (int k = lane; k < a.I; k += 32) {
+                                const uint16_t bits = h[k];
+                                v = fmaf(Elem<T>::to_f(w2[k]), PastRange::is(bits) ? PastRange::value(bits, h[past + k]) : __half2float(__ushort_as_half(bits)), v);
+                            }
+                            v = ops::warp_sum(v);
+                            if (lane < size) meet[(lane * 16 * kSets + column) * pitch + row] = lane == 0 ? v : 0.f;
+                        }
+                        team_sync();
+                    }
+                }
                 for (int i = lane_in_team; i < w * n; i += 32 * size) {
                     const int row = i / w, column = i - row * w;
                     if constexpr (!kIsDown) {

@@ -14,6 +14,7 @@ using namespace ops;
 
 constexpr int kMostSize = 1 << 22;  // H and I
 
+// h: floats, or 16-bit values and (fp16) as many second parts (PastRange).  One size for all types.
 long long moe_workspace(int T, int I, int K) { return (long long)T * K * 4 * ((I + 7) / 8 * 8); }
 
 // Shared memory of a launch that takes `rows` of an expert at a time, and where what is in it lies.

@@ -18,7 +18,7 @@
 //
 // u and v are factors of the second products as values of the element type: rounded once, as a projection's own input would be (both parts of
 // them would double those products' time on the tensor cores and halve the rounding error of a result).  fp16 has too little range for that:
-// a row is divided by a power of two first (in the gradients: all rows, by the largest so far).
+// a row is divided by a power of two first (in the gradients: every rank by itself, all its rows by that of the largest so far).
 #pragma once
 
 #include "adapters.cuh"
@@ -40,6 +40,10 @@ __device__ __forceinline__ float shrink_of(float m) {
     const uint32_t e = __float_as_uint(m) >> 23 & 255;
     return e == 0 || e >= 254 ? 1.f : __uint_as_float((254 - e) << 23);
 }
+
+// The power of two that brings a largest value m to [2^14, 2^15), which leaves fp16 as much as it has below; 2^126 at most, which zero has too.
+__device__ __forceinline__ float top_of(float m) { return __uint_as_float(min(268u - (__float_as_uint(m) >> 23), 253u) << 23); }
+__device__ __forceinline__ float finite_size(float v) { return fabsf(v) < INFINITY ? fabsf(v) : 0.f; }
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -631,7 +635,9 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, G
     constexpr int MT = RT / 16;
     constexpr bool kShrink = std::is_same<T, __half>::value;
     extern __shared__ __align__(128) char memory[];
-    __shared__ float largest[kWarps];
+    constexpr int kRanks = kShrink ? RT : 2;
+    constexpr float kNoneYet = 0x1p127f;
+    __shared__ __align__(16) float largest[kWarps][kRanks], shrink[kRanks], change[kRanks];
     cg::cluster_group cluster = cg::this_cluster();
     const int blocks = (int)cluster.num_blocks(), block = (int)cluster.block_rank();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, t = lane & 3;
@@ -711,41 +717,49 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, G
         fill_c += S::kStage;
         if (fill >= ring_end) fill -= kGradStages * S::kStage, fill_c -= kGradStages * S::kStage;
     };
-    float shrink = 1.f;  // what the values of c are multiplied with (a power of two; the sums then have it too)
-    bool any = false;    // whether one of them was not zero
+    // shrink: what a rank's values of c are multiplied with (a power of two; its sums then have it too).  It goes by the rank's finite values alone: what
+    // is not a number stays so, in that rank's sums, and another rank's size costs this one no bits.
+    if (kShrink && threadIdx.x < RT) shrink[threadIdx.x] = kNoneYet;
     // the factors of a step whose copies are there, into one of two buffers
     auto round = [&](const char* stage, int which) {
-        float2 v[kMine];
-        float most = 0.f;
+        float2 v[kMine], most = make_float2(0.f, 0.f), by = make_float2(1.f, 1.f);
 #pragma unroll
         for (int k = 0; k < kMine; ++k) {
             v[k] = *reinterpret_cast<const float2*>(stage + S::kRows + c_at + k * kEvery * RT * 4);
-            most = fmaxf(most, fmaxf(fabsf(v[k].x), fabsf(v[k].y)));
+            if constexpr (kShrink) most = make_float2(fmaxf(most.x, finite_size(v[k].x)), fmaxf(most.y, finite_size(v[k].y)));
         }
         if constexpr (kShrink) {
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            __syncthreads();  // (all are through with the step before)
-            if (lane == 0) largest[warp] = most;
+            for (int o = RT / 2; o < 32; o *= 2)  // lanes with the same columns
+                most = make_float2(fmaxf(most.x, __shfl_xor_sync(0xffffffffu, most.x, o)), fmaxf(most.y, __shfl_xor_sync(0xffffffffu, most.y, o)));
+            if (lane < RT / 2) *reinterpret_cast<float2*>(&largest[warp][c_col]) = most;
             __syncthreads();
+            bool larger = false;
+            if (threadIdx.x < RT) {
+                float m = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) most = fmaxf(most, largest[w]);
-            const float want = shrink_of(most);
-            if (most > 0.f && (!any || want < shrink)) {  // (the first, or larger ones than before)
-                any = true;
-                const float by = want / shrink;
+                for (int w = 0; w < kWarps; ++w) m = fmaxf(m, largest[w][threadIdx.x]);
+                const float want = top_of(m), now = shrink[threadIdx.x];
+                larger = m > 0.f && want < now;
+                // (not zero: an infinity that is there already stays one)
+                change[threadIdx.x] = larger ? fmaxf(want / now, 0x1p-126f) : 1.f;
+                if (larger) shrink[threadIdx.x] = want;
+            }
+            if (__syncthreads_or(larger)) {
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                    for (int q = 0; q < 4; ++q) {
+                        const float f = change[m * 16 + q / 2 * 8 + quad];
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) s[m][j][q] *= by;
-                shrink = want;
+                        for (int j = 0; j < 4; ++j) s[m][j][q] *= f;
+                    }
             }
+            by = *reinterpret_cast<const float2*>(&shrink[c_col]);
         }
         T* to = c + which * kGradRows * S::kPitch + c_row * S::kPitch + c_col;
 #pragma unroll
-        for (int k = 0; k < kMine; ++k) *reinterpret_cast<uint32_t*>(to + k * kEvery * S::kPitch) = pack<T>(v[k].x * shrink, v[k].y * shrink);
+        for (int k = 0; k < kMine; ++k) *reinterpret_cast<uint32_t*>(to + k * kEvery * S::kPitch) = pack<T>(v[k].x * by.x, v[k].y * by.y);
     };
 
     // rows of this step and of those that are on their way
@@ -792,14 +806,16 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, G
     // the cluster's sums meet; the blocks share what is then to be stored
     float* sums = reinterpret_cast<float*>(memory);  // [RT][columns + 1]
     constexpr int kPitch = kGradColumns + 1;
-    const float scale = a.scale ? a.scale[l] : 1.f, grow = scale / shrink;
+    const float scale = a.scale ? a.scale[l] : 1.f;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            float* to = sums + (m * 16 + h * 8 + quad) * kPitch + warp * 32 + t * 2;
+            const int rank = m * 16 + h * 8 + quad;
+            const float grow = kShrink ? 1.f / shrink[rank] : 1.f;  // (exact; scale may not be)
+            float* to = sums + rank * kPitch + warp * 32 + t * 2;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) to[8 * j] = s[m][j][2 * h] * grow, to[8 * j + 1] = s[m][j][2 * h + 1] * grow;
+            for (int j = 0; j < 4; ++j) to[8 * j] = s[m][j][2 * h] * grow * scale, to[8 * j + 1] = s[m][j][2 * h + 1] * grow * scale;
         }
     if (blocks > 1) cluster.sync();
     else __syncthreads();

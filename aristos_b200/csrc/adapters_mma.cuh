@@ -35,13 +35,8 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     return r;
 }
 
-// The power of two that brings a largest value m to [1, 2); 1 for zero, infinities and NaN.
-__device__ __forceinline__ float shrink_of(float m) {
-    const uint32_t e = __float_as_uint(m) >> 23 & 255;
-    return e == 0 || e >= 254 ? 1.f : __uint_as_float((254 - e) << 23);
-}
-
-// The power of two that brings a largest value m to [2^14, 2^15), which leaves fp16 as much as it has below; 2^126 at most, which zero has too.
+// The power of two that brings a largest value m to [2^14, 2^15), which leaves fp16 as much as it has below: values down to 2^-28 of the largest keep all their
+// bits, those down to 2^-38 some.  2^126 at most, which zero has too.
 __device__ __forceinline__ float top_of(float m) { return __uint_as_float(min(268u - (__float_as_uint(m) >> 23), 253u) << 23); }
 __device__ __forceinline__ float finite_size(float v) { return fabsf(v) < INFINITY ? fabsf(v) : 0.f; }
 
@@ -224,13 +219,13 @@ __global__ void __launch_bounds__(256, RT == 64 && TR == 64 ? 1 : 2) rows_mma_ke
                     for (int k = 0; k < blocks; ++k) v[i] += *cluster.map_shared_rank(at, k);
                 if (a.u && block == 0 && j < a.r) a.u[(long long)(tile.begin + row) * a.r + j] = v[i];
             }
-            most = fmaxf(most, fabsf(v[i]));
+            most = fmaxf(most, finite_size(v[i]));
         }
         float shrink = 1.f;
         if constexpr (kShrink) {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            shrink = shrink_of(most);
+            shrink = top_of(most);
         }
 #pragma unroll
         for (int i = 0; i < V; ++i)
@@ -541,13 +536,13 @@ __global__ void __launch_bounds__(kPipeThreads, 2) rows_pipe_kernel(Args a) {
             const int j = i * 32 + lane;
             v[i] = j < RT && row < n ? sums[row * S::kSumPitch + j] * (kBack ? scale : 1.f) : 0.f;
             if (a.u && row < n && j < a.r) a.u[(long long)(tile.begin + row) * a.r + j] = v[i];
-            most = fmaxf(most, fabsf(v[i]));
+            most = fmaxf(most, finite_size(v[i]));
         }
         float shrink = 1.f;
         if constexpr (kShrink) {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            shrink = shrink_of(most);
+            shrink = top_of(most);
         }
 #pragma unroll
         for (int i = 0; i < V; ++i)

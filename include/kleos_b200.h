@@ -368,7 +368,8 @@ int kleos_moe_tokens(const void* x, long long ldx, const void* gate, const float
  * pass, or NULL.  base (what the shared projection gave) may be y itself, or NULL for zeros.  offsets [R + 1] is ascending; rows before the
  * first request or behind the last, and those of requests whose adapter is outside 0 .. L - 1, have y = base and u = 0.  On the tensor
  * cores (16-bit rows on 16-byte boundaries, r a multiple of 8, or of 4 up to 16) u, and v below, enter the second products rounded to
- * torch_dtype, fp16 after a division by a power of two that keeps them in its range.
+ * torch_dtype, fp16 after a division by a power of two: a row's values there, a rank's in the gradients.  Of those divided together the ones down
+ * to 2^-28 of the largest keep fp16's bits.
  * R from 1 to 65536, L from 1 to 65535, r from 1 to 128. */
 int kleos_adapter_products(const void* x, long long ldx, const int32_t* offsets, const int32_t* adapter, const void* a, const void* b,
                            const float* scale, const void* base, long long ldb, int rows, int R, int L, int r, int N, int K,

@@ -623,7 +623,11 @@ struct GradShape {
 
 // RT: columns of c (u or v) from blockIdx.z * RT on.  The cluster's blocks take kGradRows rows of a request in turn; both factors come through a
 // ring in shared memory, c a step before it is needed, when it is rounded to a factor of the products.
-template <typename T, int RT>
+//
+// The matrix unit cuts its running sums off instead of rounding them (expert_tc.cuh).  16-bit results' own rounding covers that; where results are floats
+// (kWide), every step's 32 rows are a sum of their own, which is added up in registers.  There is no room there for a second set of sums that would be
+// read back less often: 16384 rows, N = K = 4096, rank 64, bf16, 165 us instead of 149.
+template <typename T, int RT, bool kWide>
 __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, Grads second_of_two) {
     namespace cg = cooperative_groups;
     using S = GradShape<T, RT>;
@@ -778,18 +782,41 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, G
         take = take + S::kStage == ring_end ? ring : take + S::kStage;
         const uint32_t factors = static_cast<uint32_t>(__cvta_generic_to_shared(c + (step & 1) * kGradRows * S::kPitch));
         // 8 x 8 blocks: of c rows lane % 8 (+ 8 for lanes 16 on) and columns + 8 for every second eight lanes; of the other the other way round
-#pragma unroll
-        for (int k = 0; k < kGradRows / 16; ++k) {
-            if (k * 16 >= n[0]) break;
-            uint32_t b[2][4];
+        auto columns = [&](int k, uint32_t (&b)[2][4]) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) load_blocks<true>(b[j], from + (k * 16 + low + mid * 8) * S::kRowPitch + (warp * 32 + j * 16 + high * 8) * 2);
+        };
+        auto multiply = [&](int k, int m, const uint32_t (&b)[2][4], float (&d)[4][4]) {
+            uint32_t f[4];
+            load_blocks<true>(f, factors + ((k * 16 + low + high * 8) * S::kPitch + m * 16 + mid * 8) * 2);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) wm::mma16<T>(d[j], f[0], f[1], f[2], f[3], b[j / 2][j % 2 * 2], b[j / 2][j % 2 * 2 + 1]);
+        };
+        if constexpr (kWide) {
+            uint32_t b[2][2][4];
+            columns(0, b[0]);
+            columns(1, b[1]);
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                uint32_t f[4];
-                load_blocks<true>(f, factors + ((k * 16 + low + high * 8) * S::kPitch + m * 16 + mid * 8) * 2);
+                float d[4][4] = {};
+                multiply(0, m, b[0], d);
+                if (n[0] > 16) multiply(1, m, b[1], d);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) wm::mma16<T>(s[m][j], f[0], f[1], f[2], f[3], b[j / 2][j % 2 * 2], b[j / 2][j % 2 * 2 + 1]);
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; q += 2) {
+                        const float2 v = split(add2(pair(s[m][j][q], s[m][j][q + 1]), pair(d[j][q], d[j][q + 1])));
+                        s[m][j][q] = v.x, s[m][j][q + 1] = v.y;
+                    }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < kGradRows / 16; ++k) {
+                if (k * 16 >= n[0]) break;
+                uint32_t b[2][4];
+                columns(k, b);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) multiply(k, m, b, s[m]);
             }
         }
 #pragma unroll
@@ -820,7 +847,7 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, G
     float* const wide_out = static_cast<float*>(a.out);
     auto store = [&](int j, int col, float v) {
         const size_t to = a.db ? ((size_t)l * a.cols + c0 + first + col) * a.r + j0 + j : ((size_t)l * a.r + j0 + j) * a.cols + c0 + first + col;
-        if (a.wide_out) wide_out[to] = v;
+        if constexpr (kWide) wide_out[to] = v;
         else out[to] = Elem<T>::from_f(v);
     };
     for (int i = threadIdx.x; i < width * share; i += 256) {

@@ -155,13 +155,16 @@ cudaError_t adapter_grads(adapters::Grads a, adapters::Grads b, cudaStream_t st)
         if (tensor(a))
             return with_rank(std::min(a.r, 64), [&](auto rt) {
                 constexpr int RT = decltype(rt)::value <= 64 ? decltype(rt)::value : 64, kBytes = GradShape<T, RT>::kBytes;
-                const auto kernel = grads_mma_kernel<T, RT>;
                 const long long strips = cut(kGradColumns), parts = (a.r + RT - 1) / RT;
                 const int cluster = grads_cluster(strips * a.L * parts, 4, a.rows, kGradRows * 4LL);
-                static bool allowed[64];
-                cudaError_t rc = allow_smem(kernel, allowed, kBytes);
-                if (rc == cudaSuccess) rc = launch(kernel, dim3((unsigned)(strips * cluster), a.L, (unsigned)parts), 256, kBytes, cluster, st, a, b);
-                return rc;
+                auto run = [&](auto wide) {
+                    const auto kernel = grads_mma_kernel<T, RT, decltype(wide)::value>;
+                    static bool allowed[64];
+                    cudaError_t rc = allow_smem(kernel, allowed, kBytes);
+                    if (rc == cudaSuccess) rc = launch(kernel, dim3((unsigned)(strips * cluster), a.L, (unsigned)parts), 256, kBytes, cluster, st, a, b);
+                    return rc;
+                };
+                return a.wide_out ? run(std::true_type()) : run(std::false_type());
             });
     }
     const long long strips = cut(32), parts = (a.r + 15) / 16;

@@ -193,14 +193,12 @@ __global__ void __launch_bounds__(256, RT == 64 && TR == 64 ? 1 : 2) rows_mma_ke
     }
     put();  // the warps' sums meet
     __syncthreads();
-    if (KS > 1 || kBack) {
-        for (int i = threadIdx.x; i < n * RT; i += 256) {
-            float* at = part + i / RT * S::kPitch + i % RT;
-            float v = *at;
+    for (int i = threadIdx.x; i < n * RT; i += 256) {
+        float* at = part + i / RT * S::kPitch + i % RT;
+        float v = *at;
 #pragma unroll
-            for (int k = 1; k < KS; ++k) v += at[k * TR * S::kPitch];
-            *at = kBack ? v * scale : v;
-        }
+        for (int k = 1; k < KS; ++k) v += at[k * TR * S::kPitch];
+        *at = kBack ? v * scale : v;
     }
     if (blocks > 1) cluster.sync();
     else __syncthreads();
@@ -347,7 +345,6 @@ __device__ __forceinline__ int piece_at(int row, int piece) {
     if constexpr (kRowBytes == 64) return row * 64 + (piece ^ (row >> 1 & 3)) * 16;
     return row * 32 + (piece ^ (row >> 2 & 1)) * 16;
 }
-__device__ __forceinline__ void copy_16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
 __device__ __forceinline__ void copy_or_zero(uint32_t to, const void* from, bool there) {  // (nothing is read where it is not there)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }

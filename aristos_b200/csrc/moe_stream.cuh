@@ -174,9 +174,6 @@ struct PastRange {
     }
 };
 
-__device__ __forceinline__ void copy_16(uint32_t to, const void* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-}
 __device__ __forceinline__ void copy_4(uint32_t to, const void* from, bool there) {  // (zeros, and nothing is read, where it is not there)
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
 }

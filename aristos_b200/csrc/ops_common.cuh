@@ -28,6 +28,11 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& v) {
     *reinterpret_cast<Vec<T, N>*>(p) = v;
 }
 
+// 16 bytes to shared memory, asynchronously.
+__device__ __forceinline__ void copy_16(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

@@ -179,6 +179,12 @@ __device__ __forceinline__ void copy_4(uint32_t to, const void* from, bool there
 }
 __device__ __forceinline__ void zero_16(uint32_t to) { asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory"); }
 
+// The matrix unit cuts its running sums off instead of rounding them: by half a unit in 2^23 a step of 16 terms, about 2^-16 of 8192 terms of one sign.
+// That is a sixteenth and less of a 16-bit result's own rounding; a warp with more of a sum than that adds it up in the place where the team's sums meet, every kWhole
+// bytes.  (In all calls: one token 22.6 -> 24.8 us, 37 tokens with H = 1088, I = 2880 111 -> 117; every 256 terms, to registers, 128 tokens 279 -> 377.)
+constexpr int kWhole = 8192, kWholeAtMost = 16384;
+__host__ __device__ __forceinline__ bool longer_sums(int row_bytes, int experts) { return row_bytes > kWholeAtMost * team_size(experts); }
+
 // Where a warp's copies are in a launch's work: columns c0 .. c0 + w - 1 of expert e (number u of those that have a place), its places
 // p0 .. p0 + n - 1, step along the sum.
 struct At {
@@ -186,8 +192,9 @@ struct At {
 };
 
 // kLines: lines of a row in a warp's step.  kSets: sets of 16 rows of the weights (of a gated expert one a half).  kUnit: bytes that all rows
-// may be copied in: 16 or 4, by the asynchronous copies, or 2.  kDepth: steps of a warp in shared memory.
-template <typename T, int kMode, int kLines, int kSets, int kUnit, int kDepth>
+// may be copied in: 16 or 4, by the asynchronous copies, or 2.  kDepth: steps of a warp in shared memory.  kLong: sums leave the matrix unit
+// (longer_sums()).
+template <typename T, int kMode, int kLines, int kSets, int kUnit, int kDepth, bool kLong>
 __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
     constexpr bool kGated = kMode == kUpGated, kIsDown = kMode == kDown, kMma = sizeof(T) == 2, kHalf = std::is_same<T, __half>::value;
     static_assert(!kGated || kSets == 2, "a set for each half");
@@ -445,7 +452,25 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
                         for (int j = 0; j < kNTiles; ++j)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) s[m][j][i] = 0.f;
+                    auto place = [&](int m, int j, int h) { return reinterpret_cast<float2*>(meet + ((part * kSets + m) * 16 + quad + h * 8) * pitch + j * 8 + t * 2); };
+                    // the sums so far to their places, or all of them back
+                    auto keep = [&](bool first, bool back) {
+#pragma unroll
+                        for (int m = 0; m < kSets; ++m)
+#pragma unroll
+                            for (int j = 0; j < kNTiles; ++j)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    if (j >= tiles || j * 8 + t * 2 >= pitch) continue;
+                                    float2 v = make_float2(s[m][j][2 * h], s[m][j][2 * h + 1]);
+                                    if (!first) v.x += place(m, j, h)->x, v.y += place(m, j, h)->y;
+                                    if (!back) *place(m, j, h) = v;
+                                    s[m][j][2 * h] = back ? v.x : 0.f, s[m][j][2 * h + 1] = back ? v.y : 0.f;
+                                }
+                    };
+                    constexpr int kEvery = kWhole / kRowBytes;
                     for (int step = 0; step < steps; ++step) {
+                        if (kLong && step > 0 && step % kEvery == 0) keep(step == kEvery, false);
                         const char* in = next_slot();
 #pragma unroll
                         for (int b = 0; b < 2 * kLines; ++b) {
@@ -467,15 +492,15 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
                         if (kUnit == 2) stash();
                         __syncwarp();
                     }
+                    if (kLong && steps > kEvery) keep(false, true);
 #pragma unroll
                     for (int m = 0; m < kSets; ++m)
 #pragma unroll
                         for (int j = 0; j < kNTiles; ++j) {
                             if (j >= tiles) break;
                             if (j * 8 + t * 2 >= pitch) break;
-                            float* to = meet + ((part * kSets + m) * 16 + quad) * pitch + j * 8 + t * 2;
-                            *reinterpret_cast<float2*>(to) = make_float2(s[m][j][0], s[m][j][1]);
-                            *reinterpret_cast<float2*>(to + 8 * pitch) = make_float2(s[m][j][2], s[m][j][3]);
+                            *place(m, j, 0) = make_float2(s[m][j][0], s[m][j][1]);
+                            *place(m, j, 1) = make_float2(s[m][j][2], s[m][j][3]);
                             if constexpr (kIsDown && kHalf) {
 #pragma unroll
                                 for (int i = 0; i < 4; ++i)

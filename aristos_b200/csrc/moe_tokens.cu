@@ -29,7 +29,7 @@ int moe_smem(const tokens::Args& a, tokens::Cut& c, int rows) {
 }
 
 // False where not even `least` rows of an expert fit at a time.
-template <typename T, int kMode, int kLines, int kSets, int kUnit, int kDepth>
+template <typename T, int kMode, int kLines, int kSets, int kUnit, int kDepth, bool kLong = false>
 bool moe_stream_of(const tokens::Args& a, tokens::Cut c, int least, cudaStream_t st, cudaError_t* rc) {
     using namespace tokens;
     int rows = c.rows, smem;
@@ -39,7 +39,7 @@ bool moe_stream_of(const tokens::Args& a, tokens::Cut c, int least, cudaStream_t
         rows = std::max(least, (rows - 1) / 8 * 8);
     }
     const int cols = kMode == kDown ? a.H : a.I;
-    const auto kernel = stream_kernel<T, kMode, kLines, kSets, kUnit, kDepth>;
+    const auto kernel = stream_kernel<T, kMode, kLines, kSets, kUnit, kDepth, kLong>;
     static bool allowed[64];
     *rc = allow_smem(kernel, allowed, kMostSmem);
     if (*rc == cudaSuccess) *rc = launch(kernel, dim3((cols + c.share - 1) / c.share * c.spread), kStreamThreads, smem, kMode == kDown ? c.spread : 1, st, a, c);
@@ -79,6 +79,12 @@ cudaError_t moe_stream(const tokens::Args& a, cudaStream_t st) {
     // Three steps ahead where that leaves room for all but the fullest experts' rows (16 tokens of eight experts, four each on average: 453 us with
     // two steps, 427 with three).
     const int enough = std::min(c.rows, a.T * a.K <= 4 * a.E ? 8 : 16);
+    if constexpr (sizeof(T) == 2)
+        if (longer_sums((kMode == kDown ? a.I : a.H) * (int)sizeof(T), std::min(a.E, a.T * a.K) / c.spread)) {
+            if (kMode != kUpGated) cut(kTileColumns);
+            moe_stream_of<T, kMode, kMode == kUpGated ? 1 : 2, kMode == kUpGated ? 2 : 1, kUnit, 3, true>(a, c, 8, st, &rc);
+            return rc;
+        }
     if constexpr (kMode == kUpGated) {
         if constexpr (kUnit == 16)
             if (moe_stream_of<T, kMode, 1, 2, kUnit, 4>(a, c, enough, st, &rc)) return rc;

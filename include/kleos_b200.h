@@ -351,7 +351,8 @@ int kleos_activation_backward(const void* dh, long long lddh, const void* z, lon
  * topk [T, K] and weights [T, K] are written; with gate NULL they are what the caller's own router chose and are read: an id outside
  * 0 .. E - 1 is a place without an expert, and an expert may be named twice.  Logits are exact to about 2^-46 (those with
  * infinities in them, or past the floats' range on the way, are sums of 64 bits), h is rounded to
- * torch_dtype between the products (fp16: a value past 65504 is kept with 18 bits), everything else is 32 bits and one rounding.  An expert
+ * torch_dtype between the products (fp16: a value past 65504 is kept with 18 bits), everything else is 32 bits and one
+ * rounding (sums of 16-bit products stay on the matrix unit, see above, for 8192 terms at most).  An expert
  * whose logit is minus infinity (a gate_bias that takes it out of service, a gate row, a token) is never chosen: its place has topk -1 and weight 0, and a
  * token without any expert has zeros.  NaN counts as the largest logit and makes its token's weights and results NaN.
  * The workspace (16-byte aligned, kleos_moe_tokens_workspace(T, I, K) bytes, contents of no matter) belongs to the call while it runs:

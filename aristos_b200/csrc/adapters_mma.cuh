@@ -17,7 +17,8 @@
 // 278 MB: the adapter with the most rows sets the time).
 //
 // u and v are factors of the second products as values of the element type: rounded once, as a projection's own input would be (both parts of
-// them would double those products' time on the tensor cores and halve the rounding error of a result).  fp16 has too little range for that:
+// them would double those products' time on the tensor cores and halve the rounding error of a result).  Gradients in floats, which would show
+// that, are made of both parts.  fp16 has too little range for either:
 // a row is divided by a power of two first (in the gradients: every rank by itself, all its rows by that of the largest so far).
 #pragma once
 
@@ -38,6 +39,8 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
 // The power of two that brings a largest value m to [2^14, 2^15), which leaves fp16 as much as it has below: values down to 2^-28 of the largest keep all their
 // bits, those down to 2^-38 some.  2^126 at most, which zero has too.
 __device__ __forceinline__ float top_of(float m) { return __uint_as_float(min(268u - (__float_as_uint(m) >> 23), 253u) << 23); }
+// What a rounding left of a value; nothing of one that is no number or became an infinity.
+__device__ __forceinline__ float rest_of(float v, float rounded) { return fabsf(rounded) < INFINITY ? v - rounded : 0.f; }
 __device__ __forceinline__ float finite_size(float v) { return fabsf(v) < INFINITY ? fabsf(v) : 0.f; }
 
 template <typename T>
@@ -610,25 +613,25 @@ constexpr int kGradRows = 32, kGradColumns = 256, kGradStages = 4;
 
 template <typename T, int RT>
 struct GradShape {
-    static constexpr int kPitch = RT + 8;                          // elements of a row of c as a factor
     static constexpr int kRowPitch = kGradColumns * 2 + 16;        // bytes of a row of the other factor
-    static constexpr int kRows = kGradRows * kRowPitch, kStage = kRows + kGradRows * RT * 4;
-    static constexpr int kFactors = kGradStages * kStage;
-    static constexpr int kSums = RT * (kGradColumns + 1) * 4, kRing = kFactors + 2 * kGradRows * kPitch * 2;
+    static constexpr int kPitch = RT * 4 + 16;                     // bytes of a row of c: values, then both parts of every eight in their 32 bytes
+    static constexpr int kRows = kGradRows * kRowPitch, kStage = kRows + kGradRows * kPitch;
+    static constexpr int kSums = RT * (kGradColumns + 1) * 4, kRing = kGradStages * kStage;
     static constexpr int kBytes = kSums > kRing ? kSums : kRing;
 };
 
 // RT: columns of c (u or v) from blockIdx.z * RT on.  The cluster's blocks take kGradRows rows of a request in turn; both factors come through a
 // ring in shared memory, c a step before it is needed, when it is rounded to a factor of the products.
 //
-// The matrix unit cuts its running sums off instead of rounding them (expert_tc.cuh).  16-bit results' own rounding covers that; where results are floats
-// (kWide), every step's 32 rows are a sum of their own, which is added up in registers.  There is no room there for a second set of sums that would be
-// read back less often: 16384 rows, N = K = 4096, rank 64, bf16, 165 us instead of 149.
+// The matrix unit cuts its running sums off instead of rounding them (expert_tc.cuh), and u and v have 32 bits: 16-bit results' own rounding covers what is
+// lost of either.  Where results are floats (kWide), every 16 rows are a sum of their own, which is added up in registers (there is no room for a second
+// set of sums that would be read back less often), of both parts of c.  16384 rows, N = K = 4096, rank 64, bf16: 200 us instead of 149; the sums alone 166, and
+// 16-bit results of both parts 197.
 template <typename T, int RT, bool kWide>
 __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, Grads second_of_two) {
     namespace cg = cooperative_groups;
     using S = GradShape<T, RT>;
-    constexpr int MT = RT / 16;
+    constexpr int MT = RT / 16, kParts = kWide ? 2 : 1;
     constexpr bool kShrink = std::is_same<T, __half>::value;
     extern __shared__ __align__(128) char memory[];
     constexpr int kRanks = kShrink ? RT : 2;
@@ -650,7 +653,6 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, G
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[m][j][i] = 0.f;
-    T* c = reinterpret_cast<T*>(memory + S::kFactors);
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(memory));
 
     // This block's share of the adapter's rows, kGradRows of a request at a time.
@@ -693,8 +695,8 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, G
     const int c_row = (int)threadIdx.x * 2 / RT, c_col = (int)threadIdx.x * 2 % RT;
     const bool c_column = j0 + c_col < a.r;
     const float* const c_in = a.c + (long long)c_row * a.r + j0 + c_col;
-    const int c_at = (c_row * RT + c_col) * 4;
-    uint32_t fill_c = ring + S::kRows + c_at;
+    const int c_at = S::kRows + c_row * S::kPitch + c_col * 4;
+    uint32_t fill_c = ring + c_at;
     auto copy = [&](int row0, int n) {
         const T* from = in + row0 * a.ldi;
 #pragma unroll
@@ -706,7 +708,7 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, G
 #pragma unroll
         for (int k = 0; k < kMine; ++k, c_from += (long long)kEvery * a.r) {
             const bool there = c_column && c_row + k * kEvery < n;
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(fill_c + k * kEvery * RT * 4), "l"(there ? c_from : a.c), "r"(there ? 8 : 0) : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(fill_c + k * kEvery * S::kPitch), "l"(there ? c_from : a.c), "r"(there ? 8 : 0) : "memory");
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         fill += S::kStage;
@@ -716,15 +718,15 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, G
     // shrink: what a rank's values of c are multiplied with (a power of two; its sums then have it too).  It goes by the rank's finite values alone: what
     // is not a number stays so, in that rank's sums, and another rank's size costs this one no bits.
     if (kShrink && threadIdx.x < RT) shrink[threadIdx.x] = kNoneYet;
-    // the factors of a step whose copies are there, into one of two buffers
-    auto round = [&](const char* stage, int which) {
-        float2 v[kMine], most = make_float2(0.f, 0.f), by = make_float2(1.f, 1.f);
-#pragma unroll
-        for (int k = 0; k < kMine; ++k) {
-            v[k] = *reinterpret_cast<const float2*>(stage + S::kRows + c_at + k * kEvery * RT * 4);
-            if constexpr (kShrink) most = make_float2(fmaxf(most.x, finite_size(v[k].x)), fmaxf(most.y, finite_size(v[k].y)));
-        }
+    // The factors of a step whose copies are there, in the values' place: both parts of each.
+    auto round = [&](char* stage) {
         if constexpr (kShrink) {
+            float2 v[kMine], most = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < kMine; ++k) {
+                v[k] = *reinterpret_cast<const float2*>(stage + c_at + k * kEvery * S::kPitch);
+                most = make_float2(fmaxf(most.x, finite_size(v[k].x)), fmaxf(most.y, finite_size(v[k].y)));
+            }
 #pragma unroll
             for (int o = RT / 2; o < 32; o *= 2)  // lanes with the same columns
                 most = make_float2(fmaxf(most.x, __shfl_xor_sync(0xffffffffu, most.x, o)), fmaxf(most.y, __shfl_xor_sync(0xffffffffu, most.y, o)));
@@ -751,11 +753,36 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, G
                         for (int j = 0; j < 4; ++j) s[m][j][q] *= f;
                     }
             }
-            by = *reinterpret_cast<const float2*>(&shrink[c_col]);
-        }
-        T* to = c + which * kGradRows * S::kPitch + c_row * S::kPitch + c_col;
+            if constexpr (!kWide) {  // (all have read theirs)
+                const float2 by = *reinterpret_cast<const float2*>(shrink + c_col);
+                char* const to = stage + S::kRows + c_row * S::kPitch + c_col / 8 * 32 + c_col % 8 * 2;
 #pragma unroll
-        for (int k = 0; k < kMine; ++k) *reinterpret_cast<uint32_t*>(to + k * kEvery * S::kPitch) = pack<T>(v[k].x * by.x, v[k].y * by.y);
+                for (int k = 0; k < kMine; ++k) *reinterpret_cast<uint32_t*>(to + k * kEvery * S::kPitch) = pack<T>(v[k].x * by.x, v[k].y * by.y);
+                return;
+            }
+        }
+        if (threadIdx.x < 4 * RT) {  // eight values a thread
+            const int row = (int)threadIdx.x / (RT / 8), eight = (int)threadIdx.x % (RT / 8);
+            char* const c = stage + S::kRows + row * S::kPitch + eight * 32;
+            float v[8], by[8];
+            uint32_t part[2][4];
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+                *reinterpret_cast<float4*>(v + i) = *reinterpret_cast<const float4*>(c + i * 4);
+                if constexpr (kShrink) *reinterpret_cast<float4*>(by + i) = *reinterpret_cast<const float4*>(shrink + eight * 8 + i);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const float x = kShrink ? v[i] * by[i] : v[i], y = kShrink ? v[i + 1] * by[i + 1] : v[i + 1];
+                part[0][i / 2] = pack<T>(x, y);
+                if (!kWide) continue;
+                const float2 first = Pack2<T>::to_f2(*reinterpret_cast<const typename Pack2<T>::type*>(&part[0][i / 2]));
+                part[1][i / 2] = pack<T>(rest_of(x, first.x), rest_of(y, first.y));
+            }
+#pragma unroll
+            for (int p = 0; p < kParts; ++p)
+                *reinterpret_cast<uint4*>(c + p * 16) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
+        }
     };
 
     // rows of this step and of those that are on their way
@@ -768,43 +795,47 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, G
 #pragma unroll
     for (int i = 0; i < kGradStages - 1; ++i) one_more(i);
     asm volatile("cp.async.wait_group %0;" ::"n"(kGradStages - 2) : "memory");
-    // (a thread reads the values of c that it copied itself)
-    if (n[0] > 0) round(memory, 0);
+    __syncthreads();
+    if (n[0] > 0) round(memory);
     const int low = lane & 7, mid = lane >> 3 & 1, high = lane >> 4;
-    for (int step = 0; n[0] > 0; ++step) {
+    while (n[0] > 0) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kGradStages - 3) : "memory");
         __syncthreads();
         one_more(kGradStages - 1);
         const uint32_t from = take;
         take = take + S::kStage == ring_end ? ring : take + S::kStage;
-        const uint32_t factors = static_cast<uint32_t>(__cvta_generic_to_shared(c + (step & 1) * kGradRows * S::kPitch));
         // 8 x 8 blocks: of c rows lane % 8 (+ 8 for lanes 16 on) and columns + 8 for every second eight lanes; of the other the other way round
         auto columns = [&](int k, uint32_t (&b)[2][4]) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) load_blocks<true>(b[j], from + (k * 16 + low + mid * 8) * S::kRowPitch + (warp * 32 + j * 16 + high * 8) * 2);
         };
         auto multiply = [&](int k, int m, const uint32_t (&b)[2][4], float (&d)[4][4]) {
-            uint32_t f[4];
-            load_blocks<true>(f, factors + ((k * 16 + low + high * 8) * S::kPitch + m * 16 + mid * 8) * 2);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) wm::mma16<T>(d[j], f[0], f[1], f[2], f[3], b[j / 2][j % 2 * 2], b[j / 2][j % 2 * 2 + 1]);
+            for (int p = kParts - 1; p >= 0; --p) {
+                uint32_t f[4];
+                load_blocks<true>(f, from + S::kRows + (k * 16 + low + high * 8) * S::kPitch + ((m * 2 + mid) * 2 + p) * 16);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) wm::mma16<T>(d[j], f[0], f[1], f[2], f[3], b[j / 2][j % 2 * 2], b[j / 2][j % 2 * 2 + 1]);
+            }
         };
         if constexpr (kWide) {
-            uint32_t b[2][2][4];
-            columns(0, b[0]);
-            columns(1, b[1]);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                float d[4][4] = {};
-                multiply(0, m, b[0], d);
-                if (n[0] > 16) multiply(1, m, b[1], d);
+            for (int k = 0; k < kGradRows / 16; ++k) {
+                if (k * 16 >= n[0]) break;
+                uint32_t b[2][4];
+                columns(k, b);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int m = 0; m < MT; ++m) {
+                    float d[4][4] = {};
+                    multiply(k, m, b, d);
 #pragma unroll
-                    for (int q = 0; q < 4; q += 2) {
-                        const float2 v = split(add2(pair(s[m][j][q], s[m][j][q + 1]), pair(d[j][q], d[j][q + 1])));
-                        s[m][j][q] = v.x, s[m][j][q + 1] = v.y;
-                    }
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int q = 0; q < 4; q += 2) {
+                            const float2 v = split(add2(pair(s[m][j][q], s[m][j][q + 1]), pair(d[j][q], d[j][q + 1])));
+                            s[m][j][q] = v.x, s[m][j][q + 1] = v.y;
+                        }
+                }
             }
         } else {
 #pragma unroll
@@ -818,7 +849,7 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, G
         }
 #pragma unroll
         for (int i = 0; i < kGradStages - 1; ++i) n[i] = n[i + 1];
-        if (n[0] > 0) round(memory + (take - ring), step + 1 & 1);
+        if (n[0] > 0) round(memory + (take - ring));
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();

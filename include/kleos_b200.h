@@ -379,9 +379,9 @@ int kleos_adapter_products(const void* x, long long ldx, const int32_t* offsets,
 /* Gradients of kleos_adapter_products, from dy, x and the u of the forward pass:
  *   v = scale[l] dy B[l],   dx = dbase + v A[l],   dA[l] = sum of v^T x,   dB[l] = scale[l] sum of dy^T u
  * dbase (the shared projection's dx) may be dx itself, or NULL for zeros.  dA [L, r, K] and dB [L, N, r] of grad_dtype, 0 (float) or
- * torch_dtype, zeros for an adapter without rows, may be NULL; their factors u and v are rounded as above (in floats too, where rows are aligned as there and r
- * is even: up to half a unit of torch_dtype of each term).  Long sums of results in 16 bits stay on the matrix unit, as those of
- * kleos_expert_products_dw, an eighth of an adapter's rows and more at a time; those in floats are within 3e-6 of the 2-norm for these factors.  dA needs a 16-byte aligned workspace of
+ * torch_dtype, zeros for an adapter without rows, may be NULL.  On the tensor cores (as above, r even) results in 16 bits
+ * are of u and v rounded to torch_dtype, and their long sums stay on the matrix unit, as those of kleos_expert_products_dw; results in floats are of u
+ * and v in two parts (2^-16 of them in bf16, 2^-22 in fp16) and within 3e-6 of the 2-norm beside that.  dA needs a 16-byte aligned workspace of
  * kleos_adapter_products_workspace(rows, r) bytes, whose contents do not matter. */
 long long kleos_adapter_products_workspace(int rows, int r);
 int kleos_adapter_products_backward(const void* dy, long long lddy, const void* x, long long ldx, const float* u, const int32_t* offsets,

@@ -139,16 +139,24 @@ __global__ void __launch_bounds__(32 * kGateWarps) gate_kernel(Args a) {
                     if (t < n) add(s[t], p, pair(Elem<T>::to_f(x[t * a.ldx + k]), 0.f));
             }
         }
+        auto put = [&](int t, double v) {
+            if (lane == 0 && e < a.E) *cluster.map_shared_rank(&logits[e], t) = a.gate_bias ? v + (double)a.gate_bias[e] : v;
+        };
+        unsigned anew = 0;  // tokens, the same for the whole warp
 #pragma unroll
         for (int t = 0; t < kGateTokens; ++t) {
             if (t >= n) break;
-            double v = warp_sum(s[t].total());
-            if (!isfinite(v)) {  // (of the whole warp alike)
-                v = 0.0;
-                for (int k = lane; k < a.H; k += 32) v += (double)Elem<T>::to_f(w[k]) * (double)Elem<T>::to_f(x[t * a.ldx + k]);
-                v = warp_sum(v);
-            }
-            if (lane == 0 && e < a.E) *cluster.map_shared_rank(&logits[e], t) = a.gate_bias ? v + (double)a.gate_bias[e] : v;
+            const double v = warp_sum(s[t].total());
+            if (!isfinite(v)) anew |= 1u << t;
+            put(t, v);
+        }
+#pragma unroll 1
+        for (; anew; anew &= anew - 1) {
+            const int t = __ffs(anew) - 1;
+            double v = 0.0;
+#pragma unroll 1
+            for (int k = lane; k < a.H; k += 32) v += (double)Elem<T>::to_f(w[k]) * (double)Elem<T>::to_f(x[t * a.ldx + k]);
+            put(t, warp_sum(v));
         }
     }
     cluster.sync();

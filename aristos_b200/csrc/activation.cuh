@@ -5,8 +5,10 @@
 //
 //   f: 0 ReLU max(z, 0), 1 GELU z N(z) with N the normal distribution's sum, 2 SiLU z s(z) with s(z) = 1 / (1 + e^-z)
 //
-// Each element is read once and each result written once, in 32 bits with one rounding: bound by HBM (16384 rows, I = 2048, gated, bf16: 29.7 us
-// forward, 49.0 backward, 6.8 TB/s); rows that are loaded an element at a time by issue (2943 x 1087 floats, GELU: 14 and 16).
+// Each element is read once and each result written once, in 32 bits with one rounding.  16384 rows, I = 2048, one call after the other: ReLU and SiLU
+// are bound by HBM (gated, bf16: 32 us forward, 60 backward, 6.2 and 5.6 TB/s; floats 61 and 105, 6.5 and 6.4), GELU's erfc and exp of 32 bits
+// by issue (gated, bf16: 66 and 88 us, 3.0 and 3.8 TB/s; floats 86 and 107); so are rows that are loaded an element at a time (2943 x 1087
+// floats, GELU: 14 and 16).
 #pragma once
 
 #include "ops_common.cuh"

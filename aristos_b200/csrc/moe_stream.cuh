@@ -15,14 +15,15 @@
 //
 // h goes from one kernel to the other rounded to the element type, as in the library's other layer: a second value for what that leaves would
 // halve the rounding error of a result (2-norm 0.0024 to 0.0017, bf16) and read h twice.  A value past fp16's range is kept all the same
-// (PastRange): sums that it made no number are added up anew.
+// (PastRange): sums that it made no number are added up anew, by a warp each from memory (16 tokens of the large FFN 436 us; with a token that is no
+// number 492; with all of h past the range 11 ms).
 //
 // The second kernel's first weights are on their way before the first kernel has ended: which experts those are was written by the kernel
 // before both, and no kernel lets its successor begin before it has waited for its predecessor (common.cuh).
 //
-// Bound by HBM where rows are long and experts many: alone, kUp of 128 tokens (64 gated experts, H = I = 2048, bf16, 1.07 GB) 177 us = 6.0 TB/s,
+// Bound by HBM where rows are long and experts many: alone, kUp of 128 tokens (64 gated experts, H = I = 2048, bf16, 1.07 GB) 167 us = 6.4 TB/s,
 // 16 tokens of the large FFN (2.8 GB, both kernels) 427 us = 6.5 TB/s; by issue and latency where a block's share of an expert is small: kDown of
-// those 128 tokens (0.54 GB, 28 rows of 4 KB at a time) 107 us, 37 tokens with H = 1088, I = 2880 (135 MB each) 56 and 66.  One token: 22 us for all
+// those 128 tokens (0.54 GB, 28 rows of 4 KB at a time) 105 us, 37 tokens with H = 1088, I = 2880 (135 MB each) 57 and 65.  One token: 23 us for all
 // three launches, of which the weights take 8 and an empty layer 12.
 #pragma once
 
@@ -563,11 +564,12 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(Args a, Cut c) {
                             const uint16_t* h = static_cast<const uint16_t*>(a.h) + (size_t)g.of[p0 + row] * a.ldh;
                             const T* w2 = static_cast<const T*>(a.w2) + ((size_t)e * a.H + c0 + column) * a.I;
                             v = 0.f;
-#pragma unroll 4
-                            for (int k = lane; k < a.I; k += 32) {
-                                const uint16_t bits = h[k];
-                                v = fmaf(Elem<T>::to_f(w2[k]), PastRange::is(bits) ? PastRange::value(bits, h[past + k]) : __half2float(__ushort_as_half(bits)), v);
-                            }
+                            for (int k0 = 0; k0 < a.I && !__any_sync(0xffffffffu, v != v); k0 += 128)  // (a token that is no number is soon done)
+#pragma unroll
+                                for (int k = k0 + lane; k < min(a.I, k0 + 128); k += 32) {
+                                    const uint16_t bits = h[k];
+                                    v = fmaf(Elem<T>::to_f(w2[k]), PastRange::is(bits) ? PastRange::value(bits, h[past + k]) : __half2float(__ushort_as_half(bits)), v);
+                                }
                             v = ops::warp_sum(v);
                             if (lane < size) meet[(lane * 16 * kSets + column) * pitch + row] = lane == 0 ? v : 0.f;
                         }

@@ -609,6 +609,10 @@ __global__ void __launch_bounds__(kPipeThreads, 2) rows_pipe_kernel(Args a) {
 }
 
 // ---------------------------------------------------------------- gradients of the adapters
+// Up to so many rows results in 16 bits are made of both parts of u and v as well: a rank of a few rows is a few values, whose rounding shows in a whole row of
+// dA (column of dB) and is not evened out (four rows of one adapter, rank 32: 2-norm 0.0025 of dB, now 0.0017).  N = K = 4096, rank 64: 256 rows 25.9 us instead
+// of 24.9, 512 rows 35.8 instead of 33.5, 2048 rows 53 instead of 47.
+constexpr int kBothParts = 512;
 constexpr int kGradRows = 32, kGradColumns = 256, kGradStages = 4;
 
 template <typename T, int RT>
@@ -624,14 +628,14 @@ struct GradShape {
 // ring in shared memory, c a step before it is needed, when it is rounded to a factor of the products.
 //
 // The matrix unit cuts its running sums off instead of rounding them (expert_tc.cuh), and u and v have 32 bits: 16-bit results' own rounding covers what is
-// lost of either.  Where results are floats (kWide), every 16 rows are a sum of their own, which is added up in registers (there is no room for a second
+// lost of either from some rows on (kParts, kBothParts).  Where results are floats (kWide), every 16 rows are a sum of their own, which is added up in registers (there is no room for a second
 // set of sums that would be read back less often), of both parts of c.  16384 rows, N = K = 4096, rank 64, bf16: 200 us instead of 149; the sums alone 166, and
 // 16-bit results of both parts 197.
-template <typename T, int RT, bool kWide>
+template <typename T, int RT, bool kWide, int kParts>
 __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, Grads second_of_two) {
     namespace cg = cooperative_groups;
     using S = GradShape<T, RT>;
-    constexpr int MT = RT / 16, kParts = kWide ? 2 : 1;
+    constexpr int MT = RT / 16;
     constexpr bool kShrink = std::is_same<T, __half>::value;
     extern __shared__ __align__(128) char memory[];
     constexpr int kRanks = kShrink ? RT : 2;
@@ -753,7 +757,7 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, G
                         for (int j = 0; j < 4; ++j) s[m][j][q] *= f;
                     }
             }
-            if constexpr (!kWide) {  // (all have read theirs)
+            if constexpr (kParts == 1) {  // (all have read theirs)
                 const float2 by = *reinterpret_cast<const float2*>(shrink + c_col);
                 char* const to = stage + S::kRows + c_row * S::kPitch + c_col / 8 * 32 + c_col % 8 * 2;
 #pragma unroll
@@ -775,7 +779,7 @@ __global__ void __launch_bounds__(256, 2) grads_mma_kernel(Grads first_of_two, G
             for (int i = 0; i < 8; i += 2) {
                 const float x = kShrink ? v[i] * by[i] : v[i], y = kShrink ? v[i + 1] * by[i + 1] : v[i + 1];
                 part[0][i / 2] = pack<T>(x, y);
-                if (!kWide) continue;
+                if (kParts == 1) continue;
                 const float2 first = Pack2<T>::to_f2(*reinterpret_cast<const typename Pack2<T>::type*>(&part[0][i / 2]));
                 part[1][i / 2] = pack<T>(rest_of(x, first.x), rest_of(y, first.y));
             }

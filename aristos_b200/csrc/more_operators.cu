@@ -157,14 +157,15 @@ cudaError_t adapter_grads(adapters::Grads a, adapters::Grads b, cudaStream_t st)
                 constexpr int RT = decltype(rt)::value <= 64 ? decltype(rt)::value : 64, kBytes = GradShape<T, RT>::kBytes;
                 const long long strips = cut(kGradColumns), parts = (a.r + RT - 1) / RT;
                 const int cluster = grads_cluster(strips * a.L * parts, 4, a.rows, kGradRows * 4LL);
-                auto run = [&](auto wide) {
-                    const auto kernel = grads_mma_kernel<T, RT, decltype(wide)::value>;
+                auto run = [&](auto wide, auto both) {
+                    const auto kernel = grads_mma_kernel<T, RT, decltype(wide)::value, decltype(both)::value ? 2 : 1>;
                     static bool allowed[64];
                     cudaError_t rc = allow_smem(kernel, allowed, kBytes);
                     if (rc == cudaSuccess) rc = launch(kernel, dim3((unsigned)(strips * cluster), a.L, (unsigned)parts), 256, kBytes, cluster, st, a, b);
                     return rc;
                 };
-                return a.wide_out ? run(std::true_type()) : run(std::false_type());
+                if (a.wide_out) return run(std::true_type(), std::true_type());
+                return a.rows <= kBothParts ? run(std::false_type(), std::true_type()) : run(std::false_type(), std::false_type());
             });
     }
     const long long strips = cut(32), parts = (a.r + 15) / 16;

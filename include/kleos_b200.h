@@ -380,8 +380,8 @@ int kleos_adapter_products(const void* x, long long ldx, const int32_t* offsets,
  *   v = scale[l] dy B[l],   dx = dbase + v A[l],   dA[l] = sum of v^T x,   dB[l] = scale[l] sum of dy^T u
  * dbase (the shared projection's dx) may be dx itself, or NULL for zeros.  dA [L, r, K] and dB [L, N, r] of grad_dtype, 0 (float) or
  * torch_dtype, zeros for an adapter without rows, may be NULL.  On the tensor cores (as above, r even) results in 16 bits
- * are of u and v rounded to torch_dtype, and their long sums stay on the matrix unit, as those of kleos_expert_products_dw; results in floats are of u
- * and v in two parts (2^-16 of them in bf16, 2^-22 in fp16) and within 3e-6 of the 2-norm beside that.  dA needs a 16-byte aligned workspace of
+ * of more than 512 rows are of u and v rounded to torch_dtype, and their long sums stay on the matrix unit, as those of kleos_expert_products_dw; those of fewer rows and results in floats are of u
+ * and v in two parts (2^-16 of them in bf16, 2^-22 in fp16) and, floats, within 3e-6 of the 2-norm beside that.  dA needs a 16-byte aligned workspace of
  * kleos_adapter_products_workspace(rows, r) bytes, whose contents do not matter. */
 long long kleos_adapter_products_workspace(int rows, int r);
 int kleos_adapter_products_backward(const void* dy, long long lddy, const void* x, long long ldx, const float* u, const int32_t* offsets,

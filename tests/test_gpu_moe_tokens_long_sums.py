@@ -50,3 +50,15 @@ def test_long_rows_of_the_first_product(T, gated, dtype):
     layer.run()
     want = layer.x.double() @ layer.w1[0, :16].double().t()
     assert near(layer.out[:, :16], want, layer.x.dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,H,I,E,K,gated", [(16, 40, 70000, 8, 2, True), (40, 72, 20001, 64, 4, False), (128, 33, 34000, 9, 8, True), (5, 140002, 24, 6, 3, True),
+                                             (40, 40008, 56, 32, 2, True), (21, 50001, 40, 16, 2, False)])
+def test_layers_of_long_rows(T, H, I, E, K, gated, dtype):
+    """Several experts, tokens and blocks to a column, every alignment; the same bits again."""
+    layer = Layer(T, H, I, E, K, dtype, gated=gated, bias=True).run()
+    layer.verify()
+    first = layer.out.clone()
+    layer.workspace.fill_(0x7F)
+    assert torch.equal(layer.run().out, first)
